@@ -14,6 +14,7 @@ from typing import List
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libaps_moe.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "aps_moe.h")
+SERVE_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "aps_serve.h")
 
 APS_OK = 0
 APS_ERR_SHAPE = -1
@@ -26,6 +27,7 @@ APS_ERR_WORKSPACE = -6
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_E4M3 = 2
+KV_MXFP4 = 3
 
 _c_vp = ctypes.c_void_p
 _c_vpp = ctypes.POINTER(ctypes.c_void_p)
@@ -55,6 +57,20 @@ class WsLayout(ctypes.Structure):
         "tile_counts0", "slot1", "slot_rows", "slot_tokens")]
 
 
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("k", _c_vp), ("v", _c_vp), ("k_scale", _c_vp), ("v_scale", _c_vp), ("num_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
+
+
+class LogitsRules(ctypes.Structure):
+    _fields_ = [("history", _c_vp), ("history_lens", _c_vp), ("prompt_lens", _c_vp),
+                ("history_stride", ctypes.c_int64), ("repetition", _c_vp), ("frequency", _c_vp), ("presence", _c_vp),
+                ("bias_ids", _c_vp), ("bias_values", _c_vp), ("bias_lens", _c_vp), ("bias_stride", ctypes.c_int64),
+                ("mask", _c_vp), ("mask_rows", ctypes.c_int64), ("mask_stride", ctypes.c_int64),
+                ("mask_index", _c_vp)]
+
+
 class ApsError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"[{code}] {message}")
@@ -65,9 +81,9 @@ class ApsError(RuntimeError):
 _lib = None
 
 
-def declared_symbols() -> List[str]:
-    """Function names declared in include/aps_moe.h."""
-    text = open(HEADER_PATH).read()
+def declared_symbols(header: str = HEADER_PATH) -> List[str]:
+    """Function names declared in include/aps_moe.h (or another header)."""
+    text = open(header).read()
     return sorted(set(re.findall(r"^APS_API\s+[\w\s\*]+?\b(aps_\w+)\s*\(", text, flags=re.M)))
 
 
@@ -127,6 +143,17 @@ def lib():
     L.aps_moe_noalloc_scratch_bytes.restype = sz
     L.aps_prefix_dedup.argtypes = [_c_vp, _c_vp, i64, i64, i64, _c_vp, _c_vp, _c_vp, _c_vp, i64,
                                    ctypes.POINTER(i64)]
+    cache = ctypes.POINTER(KvCacheDesc)
+    L.aps_kv_append.argtypes = [cache, _c_vp, i64, _c_vp, i64, _c_vp, i64, _c_vp, i64, i32, i64, i32, _c_vp, _c_vp,
+                                _c_vp, _c_vp, i64, _c_vp]
+    L.aps_kv_gather.argtypes = [cache, _c_vp, i64, _c_vp, _c_vp, i32, _c_vp]
+    L.aps_attention_paged_workspace_size.argtypes = [cache, i64, i32, i64, i64, i64, i32, i32]
+    L.aps_attention_paged_workspace_size.restype = sz
+    L.aps_attention_paged.argtypes = [cache, _c_vp, i64, i32, i64, i32, _c_vp, _c_vp, _c_vp, i64, i64, i64, i64, i32,
+                                      i32, ctypes.c_float, _c_vp, _c_vp, sz, _c_vp]
+    L.aps_logits_process.argtypes = [_c_vp, i64, i32, i64, i64, ctypes.POINTER(LogitsRules), _c_vp, i64, _c_vp]
+    for name in ("aps_kv_append", "aps_kv_gather", "aps_attention_paged", "aps_logits_process"):
+        getattr(L, name).restype = ctypes.c_int
     for name in ("aps_moe_weights_register", "aps_moe_weights_release", "aps_moe_workspace_layout",
                  "aps_router_logits", "aps_moe_route_top2", "aps_moe_dispatch", "aps_moe_expert_ffn",
                  "aps_moe_combine", "aps_moe_forward_grouped", "aps_moe_forward", "aps_moe_ffn_up",

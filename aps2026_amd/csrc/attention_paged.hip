@@ -1,0 +1,616 @@
+// Attention of each sequence's newest tokens over its paged cache
+// (aps_attention_paged): a sliding window plus the first tokens, fp32, bf16
+// and 4-bit caches, any number of new tokens.
+//
+// The rows of a sequence under one key head are its (token, query head)
+// pairs, token-major; a tile is 16 of them, and a wave walks 32 (fp32 cache:
+// 16) keys a step with the products transposed:
+//   S^T = K Q^T    16 keys x 16 rows, A = K, B = Q^T
+//   O^T += V^T P^T  16 dims x 16 rows, A = V^T, B = P^T
+// In the MFMA's result a lane holds one row (lane % 16) and, of group g =
+// lane / 16, the keys 4 g + i; as B operand of the second product it has to
+// hold 8 (fp32: 1) keys of that row, any ones as long as A holds the same: so
+// the weights never leave their lane, the row's maximum and sum take two
+// exchanges, and scaling the accumulator is one factor a lane.  K is read in
+// MFMA layout; of V a lane reads head_dim / 16 neighbouring dims of 4 g + i's
+// rows and turns them in registers (v_perm), column c of dim tile t being dim
+// (head_dim / 16) c + t.  Nothing is staged in LDS: a key or value goes from
+// HBM to the registers that multiply it, once per tile of rows.
+//
+// Numbers: the running maximum and sum are fp32 in base 2 (scores times scale
+// log2 e).  fp32 queries against bf16 or 4-bit keys are split into three bf16
+// terms (24 bits: exact products on the bf16 MFMAs), fp32 weights likewise;
+// bf16 queries keep their weights to two terms (16 bits).  An fp32 cache runs
+// on the fp32 MFMAs.
+//
+// A value that a row does not see must not reach it.  Scores of such keys are
+// replaced; in the second product their weight is 0, but 0 times an infinity
+// or a NaN is a NaN: rows of V that no row of the tile sees are replaced by
+// zeros, and where rows differ in what they see, a row that ended in NaN is
+// computed again one key at a time (redo_row), from its own keys alone.
+//
+// Few rows and a long cache: the steps of a tile are split over the four waves
+// of a workgroup and over `splits` workgroups; the waves' (max, sum, O) meet
+// in LDS, the workgroups' in the workspace, joined by k_paged_join.
+#include <algorithm>
+
+#include "serve.hpp"
+
+namespace aps {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kRows = 16;      // rows of a tile
+constexpr int kMaxSplits = 64;  // one wave reads every split's maximum at once
+
+// What both kernels know of the launch.
+struct PagedDev {
+    PagedArgs a;
+    KvCache c;
+    int group;       // query heads per key head
+    int page_shift;
+    int splits;      // workgroups along the keys
+    int row_tiles;   // tiles of rows a sequence and key head can have
+    bool by_rows;    // the waves of a workgroup take a tile each (else a part of the keys each)
+    float scale_log2;
+};
+
+// Rows q0 .. q0 + len - 1 and the cached length of sequence b, inside the
+// arrays whatever the device values are.
+struct Seq {
+    int64_t q0;
+    int len, kv;
+};
+__device__ inline Seq sequence(const PagedDev& d, int64_t b) {
+    const int64_t lo = d.a.q_offsets[b], hi = d.a.q_offsets[b + 1];
+    Seq s;
+    s.q0 = lo < 0 ? 0 : lo > d.a.rows ? d.a.rows : lo;
+    int64_t n = (hi < d.a.rows ? hi : d.a.rows) - s.q0;
+    s.len = static_cast<int>(n < 0 ? 0 : n);
+    int64_t kv = d.a.kv_lens[b];
+    const int64_t held = d.a.table_stride << d.page_shift;
+    kv = kv < d.a.max_kv_len ? kv : d.a.max_kv_len;
+    kv = kv < held ? kv : held;
+    s.kv = static_cast<int>(kv < 0 ? 0 : kv);
+    return s;
+}
+
+// The keys that the rows at positions [pmin, pmax] see, in steps of STEP keys:
+// the first tokens' steps, then the window's.
+struct Keys {
+    int lo, hi, first;  // a key is seen by some row only if key < hi and (key >= lo or key < first)
+    int n1, t_lo, steps;
+};
+template <int STEP>
+__device__ inline Keys visible(const PagedDev& d, int pmin, int pmax) {
+    Keys k;
+    k.hi = pmax + 1 > 0 ? pmax + 1 : 0;
+    const int64_t lo = static_cast<int64_t>(pmin) + 1 - d.a.window;
+    k.lo = lo > 0 ? static_cast<int>(lo) : 0;
+    k.first = d.a.sinks < k.hi ? d.a.sinks : k.hi;
+    k.t_lo = k.lo / STEP;
+    const int t_hi = (k.hi + STEP - 1) / STEP;
+    k.n1 = (k.first + STEP - 1) / STEP;
+    if (k.n1 > k.t_lo) k.n1 = k.t_lo;
+    k.steps = k.n1 + (t_hi > k.t_lo ? t_hi - k.t_lo : 0);
+    return k;
+}
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline bool sees(const PagedDev& d, int pos, int key) {
+    return key <= pos && (static_cast<int64_t>(key) > static_cast<int64_t>(pos) - d.a.window || key < d.a.sinks);
+}
+__device__ inline float bf16_round(float x) { return __uint_as_float(pack2_bf16(x, 0.0f) << 16); }
+
+// One cached element as fp32 (redo_row).
+template <int D, Kv KV>
+__device__ inline float element(const void* base, const uint8_t* scales, int64_t head_row, int dim) {
+    if constexpr (KV == Kv::kF32) return static_cast<const float*>(base)[head_row * D + dim];
+    if constexpr (KV == Kv::kBf16)
+        return __uint_as_float(static_cast<uint32_t>(static_cast<const bf16_t*>(base)[head_row * D + dim]) << 16);
+    const uint32_t byte = static_cast<const uint8_t*>(base)[head_row * (D / 2) + dim / 2];
+    const uint32_t pair = mx_decode2<0>(byte, mx_scale(scales[head_row * (D / 32) + dim / 32]));
+    return dim & 1 ? bf16w_hi(pair) : bf16w_lo(pair);
+}
+
+// One row over the steps [t0, t1) from the keys it sees, one key at a time, by
+// a whole wave; o[dim], m and l in LDS.
+template <int D, bool Q32, Kv KV, int STEP>
+__device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const Keys& ks, int t0, int t1, int64_t qrow,
+                         int head, int pos, float* o, float* m_out, float* l_out) {
+    constexpr int PER = D / 64;
+    const int lane = threadIdx.x & 63;
+    float q[PER], acc[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int64_t at = qrow * d.a.q_stride + static_cast<int64_t>(head) * D + PER * lane + j;
+        q[j] = Q32 ? static_cast<const float*>(d.a.q)[at]
+                   : __uint_as_float(static_cast<uint32_t>(static_cast<const bf16_t*>(d.a.q)[at]) << 16);
+        acc[j] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int t = t0; t < t1; ++t) {
+        const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
+        for (int key = base; key < base + STEP; ++key) {
+            if (!sees(d, pos, key)) continue;
+            const int64_t page = table[key >> d.page_shift];
+            if (page < 0 || page >= d.c.num_pages) continue;
+            const int64_t hr = ((page * d.c.kv_heads + h) << d.page_shift) + (key & ((1 << d.page_shift) - 1));
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) s = fmaf(q[j], element<D, KV>(d.c.k, d.c.k_scale, hr, PER * lane + j), s);
+#pragma unroll
+            for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x);
+            s *= d.scale_log2;
+            const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = exp2_fast(m - ref), p = exp2_fast(s - ref);
+            m = mn;
+            l = l * f + p;
+            // a key whose weight is 0 counts for nothing even where its value is not finite
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                acc[j] = fmaf(p, element<D, KV>(d.c.v, d.c.v_scale, hr, PER * lane + j), acc[j] * f);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) o[PER * lane + j] = acc[j];
+    if (lane == 0) { *m_out = m; *l_out = l; }
+}
+
+template <int D, bool Q32, Kv KV>
+__global__ void __launch_bounds__(64 * kWaves, KV == Kv::kF32 ? 2 : 3)
+k_paged_rows(PagedDev d) {
+    constexpr bool FP = KV == Kv::kF32;
+    constexpr int HALVES = FP ? 1 : 2;
+    constexpr int STEP = 16 * HALVES;
+    constexpr int W = D / 16;          // dims of V a lane reads of a key, and dim tiles
+    constexpr int QT = Q32 ? 3 : 1;    // bf16 terms of a query
+    constexpr int PT = Q32 ? 3 : 2;    // bf16 terms of a weight
+    constexpr int KS = D / 32;         // MFMA steps over the dims
+    constexpr int OSTRIDE = D + 4;     // LDS row, off the banks' period
+    __shared__ float sm_o[kWaves][kRows][OSTRIDE];
+    __shared__ float sm_m[kWaves][kRows], sm_l[kWaves][kRows];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    uint32_t id = blockIdx.x;
+    const int split = id % d.splits;
+    id /= d.splits;
+    const int per = d.by_rows ? kWaves : 1;
+    const uint32_t row_blocks = (d.row_tiles + per - 1) / per;
+    // the last rows see the most keys: they start first
+    const int rb = static_cast<int>(row_blocks - 1 - id % row_blocks);
+    id /= row_blocks;
+    const int h = id % d.c.kv_heads;
+    const int64_t b = id / d.c.kv_heads;
+    const Seq sq = sequence(d, b);
+    const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
+    const int nrows = static_cast<int>(qlen * d.group);
+    const int r0 = (d.by_rows ? rb * kWaves + wave : rb) * kRows;
+    const bool any = r0 < nrows;
+    if (!d.by_rows && !any) return;  // the whole workgroup
+    const int32_t* table = d.a.page_table + b * d.a.table_stride;
+
+    const int p0 = sq.kv - sq.len;  // position of the first new token
+    const int r_last = r0 + kRows - 1 < nrows ? r0 + kRows - 1 : nrows - 1;
+    const int pmin = p0 + r0 / d.group, pmax = any ? p0 + r_last / d.group : -1;
+    const int row = r0 + c;
+    const bool live = row < nrows;
+    const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
+    const int pos = live ? p0 + tok : -1;
+    const Keys ks = visible<STEP>(d, pmin, pmax);
+    const int parts = d.splits * (d.by_rows ? 1 : kWaves), part = d.by_rows ? split : split * kWaves + wave;
+    const int each = (ks.steps + parts - 1) / parts;
+    const int t0 = part * each < ks.steps ? part * each : ks.steps;
+    const int t1 = t0 + each < ks.steps ? t0 + each : ks.steps;
+
+    // the queries, in the order of dims that the cache's loads give
+    f32x4 qf[FP ? D / 16 : 1];
+    bf16x8 qb[FP ? 1 : QT][FP ? 1 : KS];
+    if (any) {
+        const int64_t qat = (sq.q0 + tok) * d.a.q_stride + static_cast<int64_t>(qh) * D;
+        if constexpr (FP) {
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s)
+                qf[s] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(d.a.q) + qat + 16 * s + 4 * g);
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int dim = KV == Kv::kMx ? (D / 4) * g + 8 * s : 32 * s + 8 * g;
+                if constexpr (Q32) {
+                    const float* p = static_cast<const float*>(d.a.q) + qat + dim;
+                    const f32x4 x0 = *reinterpret_cast<const f32x4*>(p), x1 = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float x = j < 4 ? x0[j & 3] : x1[j & 3];
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) {
+                            const float hi = bf16_round(x);
+                            qb[t][s][j] = static_cast<__bf16>(hi);
+                            x -= hi;
+                        }
+                    }
+                } else {
+                    qb[0][s] = *reinterpret_cast<const bf16x8*>(static_cast<const bf16_t*>(d.a.q) + qat + dim);
+                }
+            }
+        }
+    }
+
+    f32x4 acc[W];
+#pragma unroll
+    for (int t = 0; t < W; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+
+    for (int t = t0; t < t1; ++t) {
+        const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
+        bool dead[HALVES];
+        int64_t hrow[HALVES];  // (page, head, offset) row of the half's first key
+#pragma unroll
+        for (int a = 0; a < HALVES; ++a) {
+            const int key = base + 16 * a;
+            // past the last position there may be no table entry either
+            const int page = key < ks.hi ? table[key >> d.page_shift] : -1;
+            dead[a] = page < 0 || page >= d.c.num_pages;
+            hrow[a] = ((static_cast<int64_t>(dead[a] ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
+                      (key & ((1 << d.page_shift) - 1));
+        }
+        f32x4 s4[HALVES];
+        float vf[FP ? 4 : 1][W];
+        uint32_t vw[FP ? 1 : 8][FP ? 1 : W / 2];  // two dims of a key to a word
+        if constexpr (FP) {
+            const float* kp = static_cast<const float*>(d.c.k) + (hrow[0] + c) * D + 4 * g;
+            f32x4 kf[D / 16];
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) kf[s] = *reinterpret_cast<const f32x4*>(kp + 16 * s);
+            const float* vp = static_cast<const float*>(d.c.v) + (hrow[0] + 4 * g) * D + W * c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x = 0; x < W; x += 4) {
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(vp + i * D + x);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) vf[i][x + y] = w[y];
+                }
+            s4[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s4[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[s][e], qf[s][e], s4[0], 0, 0, 0);
+        } else {
+            bf16x8 kb[HALVES][KS];
+            if constexpr (KV == Kv::kBf16) {
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const bf16_t* kp = static_cast<const bf16_t*>(d.c.k) + (hrow[a] + c) * D + 8 * g;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) kb[a][s] = *reinterpret_cast<const bf16x8*>(kp + 32 * s);
+                }
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const bf16_t* vp = static_cast<const bf16_t*>(d.c.v) + (hrow[a] + 4 * g) * D + W * c;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (W == 8) {
+                            const u32x4 w = *reinterpret_cast<const u32x4*>(vp + i * D);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) vw[4 * a + i][x] = w[x];
+                        } else {
+                            const u32x2 w = *reinterpret_cast<const u32x2*>(vp + i * D);
+                            vw[4 * a + i][0] = w[0];
+                            vw[4 * a + i][1] = w[1];
+                        }
+                    }
+                }
+            } else {
+                // a lane reads D / 4 neighbouring dims of a key: one block's, or half a block's
+                uint32_t kw[2][KS], ksc[2], vc[8], vsc[8];
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const uint8_t* kp = static_cast<const uint8_t*>(d.c.k) + (hrow[a] + c) * (D / 2) + (D / 8) * g;
+                    if constexpr (KS == 4) {
+                        const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) kw[a][s] = w[s];
+                    } else {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
+                        kw[a][0] = w[0];
+                        kw[a][1] = w[1];
+                    }
+                    ksc[a] = d.c.k_scale[(hrow[a] + c) * (D / 32) + (D / 4) * g / 32];
+                }
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const uint8_t* vp = static_cast<const uint8_t*>(d.c.v) + (hrow[a] + 4 * g) * (D / 2) + (W / 2) * c;
+                    const uint8_t* sp = d.c.v_scale + (hrow[a] + 4 * g) * (D / 32) + W * c / 32;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (W == 8) vc[4 * a + i] = *reinterpret_cast<const uint32_t*>(vp + i * (D / 2));
+                        else vc[4 * a + i] = *reinterpret_cast<const uint16_t*>(vp + i * (D / 2));
+                        vsc[4 * a + i] = sp[i * (D / 32)];
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const float sc = mx_scale(ksc[a]);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const u32x4 w = {mx_decode2<0>(kw[a][s], sc), mx_decode2<1>(kw[a][s], sc),
+                                         mx_decode2<2>(kw[a][s], sc), mx_decode2<3>(kw[a][s], sc)};
+                        kb[a][s] = __builtin_bit_cast(bf16x8, w);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float sc = mx_scale(vsc[j]);
+                    vw[j][0] = mx_decode2<0>(vc[j], sc);
+                    vw[j][1] = mx_decode2<1>(vc[j], sc);
+                    if constexpr (W == 8) {
+                        vw[j][2] = mx_decode2<2>(vc[j], sc);
+                        vw[j][3] = mx_decode2<3>(vc[j], sc);
+                    }
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                s4[a] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t3 = QT - 1; t3 >= 0; --t3)
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)
+                        s4[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[a][s], qb[t3][s], s4[a], 0, 0, 0);
+            }
+        }
+
+        bool full = base + STEP - 1 <= pmin &&
+                    (static_cast<int64_t>(base) > static_cast<int64_t>(pmax) - d.a.window ||
+                     base + STEP - 1 < d.a.sinks);
+#pragma unroll
+        for (int a = 0; a < HALVES; ++a) full = full && !dead[a];
+#pragma unroll
+        for (int a = 0; a < HALVES; ++a) s4[a] *= d.scale_log2;
+        if (!full) {
+#pragma unroll
+            for (int a = 0; a < HALVES; ++a)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = base + 16 * a + 4 * g + i;
+                    if (dead[a] || !sees(d, pos, key)) s4[a][i] = -INFINITY;
+                    const bool some = !dead[a] && key < ks.hi && (key >= ks.lo || key < ks.first);
+                    if constexpr (FP) {
+#pragma unroll
+                        for (int x = 0; x < W; ++x) vf[i][x] = some ? vf[i][x] : 0.0f;
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < W / 2; ++x) vw[4 * a + i][x] = some ? vw[4 * a + i][x] : 0u;
+                    }
+                }
+        }
+        float top = fmaxf(fmaxf(s4[0][0], s4[0][1]), fmaxf(s4[0][2], s4[0][3]));
+        if constexpr (HALVES == 2)
+            top = fmaxf(top, fmaxf(fmaxf(s4[1][0], s4[1][1]), fmaxf(s4[1][2], s4[1][3])));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float f = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int x = 0; x < W; ++x) acc[x] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int a = 0; a < HALVES; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s4[a][i] = exp2_fast(s4[a][i] - ref);
+                l += s4[a][i];
+            }
+        if constexpr (FP) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x = 0; x < W; ++x)
+                    acc[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[i][x], s4[0][i], acc[x], 0, 0, 0);
+        } else {
+            u32x4 pb[PT];  // the weights' terms, 8 bf16 each
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x0 = s4[j / 2][2 * (j & 1)], x1 = s4[j / 2][2 * (j & 1) + 1];
+#pragma unroll
+                for (int t3 = 0; t3 < PT; ++t3) {
+                    pb[t3][j] = pack2_bf16(x0, x1);
+                    x0 -= bf16w_lo(pb[t3][j]);
+                    x1 -= bf16w_hi(pb[t3][j]);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < W; ++x) {
+                u32x4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[j] = __builtin_amdgcn_perm(vw[2 * j + 1][x / 2], vw[2 * j][x / 2],
+                                                 x & 1 ? 0x07060302u : 0x05040100u);
+                const bf16x8 va = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+                for (int t3 = PT - 1; t3 >= 0; --t3)
+                    acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pb[t3]), acc[x],
+                                                                      0, 0, 0);
+            }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // the wave's part to LDS: row c, dims W (4 g + i) + t
+    bool nan = l != l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < W; t += 4) {
+            const f32x4 v = {acc[t][i], acc[t + 1][i], acc[t + 2][i], acc[t + 3][i]};
+            nan = nan || v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3];
+            *reinterpret_cast<f32x4*>(&sm_o[wave][c][W * (4 * g + i) + t]) = v;
+        }
+    if (g == 0) { sm_m[wave][c] = m; sm_l[wave][c] = l; }
+    if (any && pmin != pmax) {
+        const uint64_t bad = __ballot(nan && live);
+        uint32_t rows = static_cast<uint32_t>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu);
+        while (rows) {
+            const int x = __builtin_ctz(rows);
+            rows &= rows - 1;
+            const int rr = r0 + x;
+            redo_row<D, Q32, KV, STEP>(d, table, h, ks, t0, t1, sq.q0 + rr / d.group, h * d.group + rr % d.group,
+                                       p0 + rr / d.group, sm_o[wave][x], &sm_m[wave][x], &sm_l[wave][x]);
+        }
+    }
+    __syncthreads();
+
+    // join the waves' parts (by_rows: each wave has rows of its own) and write
+    // the result, or the workgroup's part of it
+    constexpr int TPR = D / 8;                 // threads of a row, 8 dims each
+    const int tiles = d.by_rows ? kWaves : 1, parts_w = d.by_rows ? 1 : kWaves;
+    for (int x = threadIdx.x; x < tiles * kRows * TPR; x += 64 * kWaves) {
+        const int dim = 8 * (x % TPR), rt = x / TPR / kRows, rc = x / TPR % kRows;
+        const int rr = (d.by_rows ? rb * kWaves + rt : rb) * kRows + rc;
+        if (rr >= nrows) continue;
+        float mm = -INFINITY;
+        for (int w = 0; w < parts_w; ++w) mm = fmaxf(mm, sm_m[d.by_rows ? rt : w][rc]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float ll = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < parts_w; ++w) {
+            const int sl = d.by_rows ? rt : w;
+            const float f = exp2_fast(sm_m[sl][rc] - ref);
+            ll = fmaf(sm_l[sl][rc], f, ll);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = fmaf(sm_o[sl][rc][dim + j], f, o[j]);
+        }
+        const int64_t orow = (sq.q0 + rr / d.group) * d.a.q_heads + h * d.group + rr % d.group;
+        if (d.splits > 1) {
+            const int64_t at = orow * d.splits + split;
+            float* po = d.a.part + at * D + dim;
+            *reinterpret_cast<f32x4*>(po) = f32x4{o[0], o[1], o[2], o[3]};
+            *reinterpret_cast<f32x4*>(po + 4) = f32x4{o[4], o[5], o[6], o[7]};
+            if (dim == 0) {
+                float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+                ml[0] = mm;
+                ml[1] = ll;
+            }
+        } else {
+            const float inv = ll == 0.0f ? 0.0f : __fdiv_rn(1.0f, ll);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = ll == 0.0f ? 0.0f : o[j] * inv;
+            if constexpr (Q32) {
+                float* out = static_cast<float*>(d.a.out) + orow * D + dim;
+                *reinterpret_cast<f32x4*>(out) = f32x4{o[0], o[1], o[2], o[3]};
+                *reinterpret_cast<f32x4*>(out + 4) = f32x4{o[4], o[5], o[6], o[7]};
+            } else {
+                *reinterpret_cast<u32x4*>(static_cast<bf16_t*>(d.a.out) + orow * D + dim) =
+                    u32x4{pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3]), pack2_bf16(o[4], o[5]),
+                          pack2_bf16(o[6], o[7])};
+            }
+        }
+    }
+}
+
+// out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits of one
+// (row, head), a wave each.  Rows that no sequence names are not touched: the
+// grid walks the sequences.
+template <int D, bool Q32>
+__global__ void __launch_bounds__(64)
+k_paged_join(PagedDev d) {
+    constexpr int PER = D / 64;
+    const int lane = threadIdx.x;
+    uint32_t id = blockIdx.x;
+    const int head = id % d.a.q_heads;
+    id /= d.a.q_heads;
+    const int tok = id % static_cast<uint32_t>(d.a.max_q_len);
+    const Seq sq = sequence(d, id / static_cast<uint32_t>(d.a.max_q_len));
+    if (tok >= sq.len) return;
+    const int64_t orow = (sq.q0 + tok) * d.a.q_heads + head, at = orow * d.splits;
+    const float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+    const float m = lane < d.splits ? ml[2 * lane] : -INFINITY, l = lane < d.splits ? ml[2 * lane + 1] : 0.0f;
+    float top = m;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float w = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
+    float sum = w * l;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
+    float o[PER] = {};
+    const float* po = d.a.part + at * D + PER * lane;
+    for (int s = 0; s < d.splits; ++s) {
+        const float ws = __shfl(w, s);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) o[j] = fmaf(ws, po[static_cast<int64_t>(s) * D + j], o[j]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const float v = sum == 0.0f ? 0.0f : o[j] * inv;
+        if constexpr (Q32) static_cast<float*>(d.a.out)[orow * D + PER * lane + j] = v;
+        else static_cast<bf16_t*>(d.a.out)[orow * D + PER * lane + j] = static_cast<bf16_t>(pack2_bf16(v, 0.0f) & 0xFFFFu);
+    }
+}
+
+PagedDev plan(const KvCache& c, const PagedArgs& a) {
+    PagedDev d;
+    d.a = a;
+    d.c = c;
+    d.page_shift = c.page_shift;
+    d.group = a.q_heads / c.kv_heads;
+    d.scale_log2 = a.scale * 1.4426950408889634f;
+    const int64_t rows = a.max_q_len * d.group;
+    d.row_tiles = static_cast<int>(ceil_div(rows, kRows));
+    const int64_t heads = a.batch * c.kv_heads;
+    d.by_rows = d.row_tiles >= kWaves;
+    const int64_t blocks = heads * ceil_div(d.row_tiles, d.by_rows ? kWaves : 1);
+    // keys one tile can see, and workgroups for 256 CUs of four
+    const int64_t keys = std::min<int64_t>(a.max_kv_len, static_cast<int64_t>(a.window) + a.sinks + 16);
+    const int64_t steps = ceil_div(keys, 32);
+    int64_t splits = d.by_rows ? 1 : ceil_div(1024, blocks);
+    splits = std::min<int64_t>(splits, ceil_div(steps, 2 * kWaves));
+    d.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
+    return d;
+}
+
+template <int D, bool Q32, Kv KV>
+hipError_t launch(const PagedDev& d, hipStream_t s) {
+    const int64_t blocks = d.a.batch * d.c.kv_heads * d.splits * ceil_div(d.row_tiles, d.by_rows ? kWaves : 1);
+    const int64_t joins = d.a.batch * d.a.max_q_len * d.a.q_heads;
+    if (blocks > 0x7FFFFFFF || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, d);
+    if (d.splits > 1)
+        hipLaunchKernelGGL((k_paged_join<D, Q32>), dim3(static_cast<unsigned>(joins)), dim3(64), 0, s, d);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_d(const PagedDev& d, bool q_f32, hipStream_t s) {
+    if (d.c.type == Kv::kF32) return launch<D, true, Kv::kF32>(d, s);
+    if (d.c.type == Kv::kBf16)
+        return q_f32 ? launch<D, true, Kv::kBf16>(d, s) : launch<D, false, Kv::kBf16>(d, s);
+    return q_f32 ? launch<D, true, Kv::kMx>(d, s) : launch<D, false, Kv::kMx>(d, s);
+}
+
+}  // namespace
+
+size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a) {
+    const PagedDev d = plan(cache, a);
+    return d.splits > 1 ? static_cast<size_t>(a.rows) * a.q_heads * d.splits * (cache.head_dim + 2) * 4 : 0;
+}
+
+hipError_t launch_attention_paged(const KvCache& cache, const PagedArgs& a, bool q_f32, hipStream_t s) {
+    if (a.rows <= 0 || a.batch <= 0 || a.max_q_len <= 0) return hipSuccess;
+    const PagedDev d = plan(cache, a);
+    return cache.head_dim == 128 ? launch_d<128>(d, q_f32, s) : launch_d<64>(d, q_f32, s);
+}
+
+}  // namespace aps

@@ -23,10 +23,10 @@
 #include "common.hpp"
 
 namespace {
-
 thread_local std::string g_error;
+}
 
-int fail(int code, const char* fmt, ...) {
+int aps::fail(int code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -35,6 +35,10 @@ int fail(int code, const char* fmt, ...) {
     g_error = buf;
     return code;
 }
+
+namespace {
+
+using aps::fail;
 
 int hip_fail(hipError_t err, const char* what) {
     return fail(APS_ERR_HIP, "%s: %s", what, hipGetErrorString(err));

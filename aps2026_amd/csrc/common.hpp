@@ -216,6 +216,9 @@ __host__ __device__ inline int64_t max_row_tiles(int64_t n, int64_t bm, int64_t 
     return ceil_div(n, bm) + E;
 }
 
+// Sets the thread's aps_moe_last_error message; returns code (capi.hip).
+int fail(int code, const char* fmt, ...);
+
 // ---- launchers (defined in the .hip files) --------------------------------
 
 // Router GEMM; with routes != nullptr also the top-2 routes and the tile

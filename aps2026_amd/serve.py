@@ -1,0 +1,299 @@
+"""Serving operators over the C ABI (include/aps_serve.h): a paged key/value
+cache, attention over it, and the rules on the logits of the next token.
+
+The reference has no counterpart: its generate_decode computes the whole
+prefix again for every token (src/model.cu:163-204).  decoder.Model.decode
+runs on these.
+
+A decode step of a batch, on torch's current stream:
+
+    plan = PagedBatch(q_lens, kv_lens, pages, cache.page_size, device)
+    q = kv_append_gpu(cache, k, v, plan.positions, plan.slots, cos, sin, q=q)
+    out = attention_paged_gpu(q, cache, plan.q_offsets, plan.kv_lens, plan.page_table, plan.max_q_len,
+                              plan.max_kv_len, q_heads=16, window=2047, sinks=4)
+
+Calls launch kernels and read nothing back, so they can be captured into a
+graph; index arrays are read on the device (PagedBatch checks its own on the
+host).  Wrong shapes, types and layouts raise ValueError.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import capi
+from .moe import _call, _require, _stream
+
+MXFP4 = capi.KV_MXFP4
+_CODE = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16}
+
+
+def _p(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+class _on:
+    """The tensors' device as the current one, for a launch on its stream."""
+
+    def __init__(self, device: torch.device):
+        self.index, self.before = device.index, torch.cuda.current_device()
+
+    def __enter__(self):
+        if self.index != self.before:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)
+
+
+def _dev(t: torch.Tensor, device: torch.device, dtype: torch.dtype, what: str) -> torch.Tensor:
+    if t.dtype is not dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what}: expects a contiguous {dtype} tensor on {device}")
+    return t
+
+
+class PagedKvCache:
+    """One layer's cache: k and v [pages][kv_heads][page][head_dim], fp32 or
+    bf16; or, given k_scale and v_scale, 4-bit codes [..][head_dim / 2] (uint8)
+    with scale bytes [..][head_dim / 32] (uint8).  The tensors stay the
+    caller's; allocate() makes them."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None):
+        mx = k_scale is not None or v_scale is not None
+        _require(k.dim() == 4 and k.shape == v.shape and k.dtype is v.dtype and k.is_cuda and v.device == k.device
+                 and k.is_contiguous() and v.is_contiguous(), "paged cache: k and v [pages, kv_heads, page, head_dim]")
+        self.pages, self.kv_heads, self.page_size, width = k.shape
+        self.device = k.device
+        if mx:
+            _require(k.dtype is torch.uint8 and k_scale is not None and v_scale is not None,
+                     "paged cache: 4-bit codes are uint8 with k_scale and v_scale")
+            self.head_dim, self.dtype = 2 * width, MXFP4
+            want = (self.pages, self.kv_heads, self.page_size, self.head_dim // 32)
+            for s in (k_scale, v_scale):
+                _require(tuple(s.shape) == want and s.dtype is torch.uint8 and s.device == self.device
+                         and s.is_contiguous(), f"paged cache: scales {want}")
+        else:
+            _require(k.dtype in _CODE, f"paged cache: dtype {k.dtype}")
+            self.head_dim, self.dtype = width, _CODE[k.dtype]
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._desc = capi.KvCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), self.pages, self.page_size,
+                                      self.kv_heads, self.head_dim, self.dtype)
+        self._ref = ctypes.byref(self._desc)
+
+    @staticmethod
+    def allocate(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype, device) -> "PagedKvCache":
+        """dtype: torch.float32, torch.bfloat16 or "mxfp4" (4 bits)."""
+        shape = (pages, kv_heads, page_size)
+        if dtype in ("mxfp4", MXFP4):
+            z = lambda n: torch.zeros((*shape, n), dtype=torch.uint8, device=device)  # noqa: E731
+            return PagedKvCache(z(head_dim // 2), z(head_dim // 2), z(head_dim // 32), z(head_dim // 32))
+        z = lambda: torch.zeros((*shape, head_dim), dtype=dtype, device=device)  # noqa: E731
+        return PagedKvCache(z(), z())
+
+
+class PagedBatch:
+    """A batch's index arrays on the device, checked on the host: q_lens[b] new
+    tokens of sequence b, kv_lens[b] cached positions with them, pages[b] its
+    page ids.  positions and slots of the new tokens' rows, for the append;
+    q_offsets, kv_lens, page_table and the two maxima, for the attention."""
+
+    def __init__(self, q_lens: Sequence[int], kv_lens: Sequence[int], pages: Sequence[Sequence[int]], page_size: int,
+                 device, num_pages: Optional[int] = None):
+        q, kv = np.asarray(q_lens, np.int64).reshape(-1), np.asarray(kv_lens, np.int64).reshape(-1)
+        _require(q.size == kv.size == len(pages), "paged batch: one length and page list a sequence")
+        _require(bool(np.all(q >= 0)) and bool(np.all(kv >= q)) and bool(np.all(kv < 1 << 30)) and int(q.sum()) < 1 << 30,
+                 "paged batch: 0 <= q_lens <= kv_lens")
+        ids = [np.asarray(p, np.int64).reshape(-1) for p in pages]
+        for n, p in zip(kv, ids):
+            _require(p.size * page_size >= n, "paged batch: too few pages")
+            _require(p.size == 0 or (p.min() >= 0 and p.max() < (num_pages if num_pages is not None else 1 << 31)),
+                     "paged batch: page id")
+        table = np.full((q.size, max([p.size for p in ids], default=0) or 1), -1, np.int32)
+        for b, p in enumerate(ids):
+            table[b, :p.size] = p
+        seq = np.repeat(np.arange(q.size), q)
+        pos = np.arange(seq.size) - np.repeat(np.cumsum(q) - q, q) + (kv - q)[seq]
+        slots = table[seq, pos // page_size].astype(np.int64) * page_size + pos % page_size
+        _require(np.unique(slots).size == slots.size, "paged batch: two new tokens share a slot")
+        up = lambda a, t: torch.from_numpy(np.ascontiguousarray(a.astype(t))).to(device)  # noqa: E731
+        self.rows, self.batch = int(q.sum()), int(q.size)
+        self.max_q_len, self.max_kv_len = int(q.max(initial=0)), int(kv.max(initial=0))
+        self.positions, self.slots = up(pos, np.int32), up(slots, np.int64)
+        self.q_offsets = up(np.concatenate([[0], np.cumsum(q)]), np.int32)
+        self.kv_lens, self.page_table = up(kv, np.int32), up(table, np.int32)
+
+
+def _rows_of(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
+    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
+        raise ValueError(f"{what}: expects rows of {width} neighbouring values")
+    return t
+
+
+def _stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def kv_append_gpu(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
+                  cos: torch.Tensor, sin: torch.Tensor, q: Optional[torch.Tensor] = None,
+                  q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Writes k (rotated by positions) and v, [rows, kv_heads * head_dim] with
+    any row stride, into the cache's slots; returns q [rows, q_heads *
+    head_dim] rotated (into q_out; q itself rotates in place).  cos and sin:
+    [positions, head_dim / 2] fp32 (rope_table).  slots int64, -1 for padding
+    rows, otherwise distinct; positions int32."""
+    rows, dev = k.shape[0], cache.device
+    width = cache.kv_heads * cache.head_dim
+    _rows_of(k, width, "kv_append")
+    _rows_of(v, width, "kv_append")
+    code = _CODE.get(k.dtype)
+    if code is None or v.dtype is not k.dtype or v.shape[0] != rows or k.device != dev or v.device != dev:
+        raise ValueError("kv_append: k and v of one fp32 or bf16 type on the cache's device")
+    _dev(positions, dev, torch.int32, "kv_append positions")
+    _dev(slots, dev, torch.int64, "kv_append slots")
+    _dev(cos, dev, torch.float32, "kv_append cos")
+    _dev(sin, dev, torch.float32, "kv_append sin")
+    if positions.numel() != rows or slots.numel() != rows or cos.shape != sin.shape or cos.dim() != 2 or \
+            cos.shape[1] * 2 != cache.head_dim:
+        raise ValueError("kv_append shape")
+    q_heads = q_stride = o_stride = 0
+    if q is not None:
+        if q.dim() != 2 or q.shape[0] != rows or q.shape[1] % cache.head_dim or q.dtype is not k.dtype or \
+                q.device != dev:
+            raise ValueError("kv_append: q [rows, q_heads * head_dim] of k's type")
+        _rows_of(q, q.shape[1], "kv_append")
+        q_heads = q.shape[1] // cache.head_dim
+        if q_out is None:
+            q_out = torch.empty((rows, q.shape[1]), dtype=q.dtype, device=dev)
+        elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.device != dev:
+            raise ValueError("kv_append: q_out of q's shape and type")
+        else:
+            _rows_of(q_out, q.shape[1], "kv_append")
+        q_stride, o_stride = _stride(q), _stride(q_out)
+    with _on(dev):
+        _call(capi.lib().aps_kv_append(cache._ref, _p(k), _stride(k), _p(v), _stride(v), _p(q), q_stride, _p(q_out),
+                                       o_stride, code, rows, q_heads, _p(positions), _p(slots), _p(cos), _p(sin),
+                                       cos.shape[0], _stream(dev)))
+    return q_out if q is not None else None
+
+
+def kv_gather_gpu(cache: PagedKvCache, slots: torch.Tensor, out_dtype: torch.dtype = torch.float32
+                  ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [rows, kv_heads * head_dim] of the slots (int64; zeros for one
+    outside the cache), the values of the codes for a 4-bit cache."""
+    _require(out_dtype in _CODE, f"kv_gather: dtype {out_dtype}")
+    _dev(slots, cache.device, torch.int64, "kv_gather slots")
+    rows = slots.numel()
+    k = torch.empty((rows, cache.kv_heads * cache.head_dim), dtype=out_dtype, device=cache.device)
+    v = torch.empty_like(k)
+    with _on(cache.device):
+        _call(capi.lib().aps_kv_gather(cache._ref, _p(slots), rows, _p(k), _p(v), _CODE[out_dtype],
+                                       _stream(cache.device)))
+    return k, v
+
+
+def attention_paged_gpu(q: torch.Tensor, cache: PagedKvCache, q_offsets: torch.Tensor, kv_lens: torch.Tensor,
+                        page_table: torch.Tensor, max_q_len: int, max_kv_len: int, q_heads: int, window: int,
+                        sinks: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                        workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Softmax attention of the batch's new tokens (rows of q) over the cached
+    keys they see: the last `window` up to their own and the first `sinks`.
+    scale: 1 / sqrt(head_dim) unless given.  The workspace is torch's, taken
+    on the current stream, unless one is given (uint8).  Rows of a given `out`
+    that no sequence names are left as they were."""
+    dev, width = cache.device, q_heads * cache.head_dim
+    _rows_of(q, width, "attention_paged")
+    code = _CODE.get(q.dtype)
+    if code is None or q.device != dev:
+        raise ValueError("attention_paged: fp32 or bf16 queries on the cache's device")
+    _dev(q_offsets, dev, torch.int32, "attention_paged q_offsets")
+    _dev(kv_lens, dev, torch.int32, "attention_paged kv_lens")
+    _dev(page_table, dev, torch.int32, "attention_paged page_table")
+    batch, rows = kv_lens.numel(), q.shape[0]
+    if q_offsets.numel() != batch + 1 or page_table.dim() != 2 or page_table.shape[0] != batch:
+        raise ValueError("attention_paged shape")
+    if out is None:
+        out = torch.empty((rows, width), dtype=q.dtype, device=dev)
+    elif tuple(out.shape) != (rows, width) or out.dtype is not q.dtype or out.device != dev or \
+            not out.is_contiguous():
+        raise ValueError("attention_paged: out of q's shape and type, contiguous")
+    if scale is None:
+        scale = 1.0 / math.sqrt(cache.head_dim)
+    lib = capi.lib()
+    window = min(window, 0x7FFFFFFF)
+    need = lib.aps_attention_paged_workspace_size(cache._ref, rows, q_heads, batch, max_q_len, max_kv_len, window,
+                                                  sinks)
+    if need and workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        _call(lib.aps_attention_paged(cache._ref, _p(q), _stride(q), code, rows, q_heads, _p(q_offsets), _p(kv_lens),
+                                      _p(page_table), page_table.shape[1], batch, max_q_len, max_kv_len, window,
+                                      sinks, scale, _p(out), _p(workspace),
+                                      workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                                      _stream(dev)))
+    return out
+
+
+def logits_process_gpu(logits: torch.Tensor, history: Optional[torch.Tensor] = None,
+                       history_lens: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
+                       repetition: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None,
+                       presence: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                       bias_values: Optional[torch.Tensor] = None, bias_lens: Optional[torch.Tensor] = None,
+                       mask: Optional[torch.Tensor] = None, mask_index: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The logits [rows, vocab] after the rules (aps_logits_process): penalties
+    by each row's history [rows, n] (int32, the first history_lens of it, the
+    first prompt_lens of those the prompt), biases of the first bias_lens ids
+    of bias_ids [rows, n], and a bit mask [masks, words] (int32 words, bit t %
+    32 of word t / 32 allows token t; row r's is mask_index[r], or r).  A rule
+    without its arrays is off.  out may be logits itself."""
+    _require(logits.dim() == 2, "logits_process: logits [rows, vocab]")
+    rows, vocab = logits.shape
+    dev, code = logits.device, _CODE.get(logits.dtype)
+    _rows_of(logits, vocab, "logits_process")
+    if code is None or not logits.is_cuda:
+        raise ValueError("logits_process: fp32 or bf16 logits on a GPU")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    elif out.shape != logits.shape or out.dtype is not logits.dtype or out.device != dev:
+        raise ValueError("logits_process: out of the logits' shape and type")
+    else:
+        _rows_of(out, vocab, "logits_process")
+
+    def per_row(t, dtype):
+        if t is not None:
+            _dev(t, dev, dtype, "logits_process")
+            _require(t.numel() == rows, "logits_process: one value a row")
+
+    for t in (history_lens, prompt_lens, bias_lens, mask_index):
+        per_row(t, torch.int32)
+    for t in (repetition, frequency, presence):
+        per_row(t, torch.float32)
+    for t, other in ((history, None), (bias_ids, bias_values)):
+        if t is not None:
+            _dev(t, dev, torch.int32, "logits_process")
+            _require(t.dim() == 2 and t.shape[0] == rows, "logits_process: lists [rows, n]")
+    if bias_ids is not None:
+        _require(bias_values is not None and bias_values.shape == bias_ids.shape and bias_lens is not None,
+                 "logits_process: biases need bias_values of their shape and bias_lens")
+        _dev(bias_values, dev, torch.float32, "logits_process")
+    _require(history_lens is not None if history is not None else repetition is frequency is presence is None,
+             "logits_process: penalties need a history, a history its history_lens")
+    if mask is not None:
+        _dev(mask, dev, torch.int32, "logits_process")
+        _require(mask.dim() == 2 and mask.shape[1] * 32 >= vocab and (mask_index is not None or mask.shape[0] >= rows),
+                 "logits_process: mask [masks, words] with a word for every 32 logits")
+    rules = capi.LogitsRules(
+        _p(history), _p(history_lens), _p(prompt_lens), history.shape[1] if history is not None else 0,
+        _p(repetition), _p(frequency), _p(presence), _p(bias_ids), _p(bias_values), _p(bias_lens),
+        bias_ids.shape[1] if bias_ids is not None else 0, _p(mask), mask.shape[0] if mask is not None else 0,
+        mask.shape[1] if mask is not None else 0, _p(mask_index))
+    with _on(dev):
+        _call(capi.lib().aps_logits_process(_p(logits), _stride(logits), code, rows, vocab, ctypes.byref(rules),
+                                            _p(out), _stride(out), _stream(dev)))
+    return out

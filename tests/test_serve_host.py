@@ -1,0 +1,210 @@
+"""Host-side checks of the serving operators that need no GPU: the exports, the
+refusals of bad arguments before anything touches the device, and the batch
+plan's own checks."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from aps2026_amd import capi, serve
+from tests import serve_oracle
+
+P = 1 << 20   # an aligned address that is never read: every call here is refused or empty
+
+
+def cache(**kw):
+    d = dict(k=P, v=P, k_scale=None, v_scale=None, num_pages=8, page_size=16, kv_heads=4, head_dim=128,
+             dtype=capi.DTYPE_BF16)
+    d.update(kw)
+    return ctypes.byref(capi.KvCacheDesc(*[d[n] for n, _ in capi.KvCacheDesc._fields_]))
+
+
+def append(c=None, rows=0, **kw):
+    d = dict(k=P, ks=512, v=P, vs=512, q=None, qs=0, qo=None, qos=0, dt=capi.DTYPE_F32, qh=0, pos=P, slots=P, cos=P,
+             sin=P, mp=4)
+    d.update(kw)
+    return capi.lib().aps_kv_append(c if c is not None else cache(), d["k"], d["ks"], d["v"], d["vs"], d["q"],
+                                    d["qs"], d["qo"], d["qos"], d["dt"], rows, d["qh"], d["pos"], d["slots"],
+                                    d["cos"], d["sin"], d["mp"], None)
+
+
+def attend(c=None, rows=4, **kw):
+    d = dict(q=P, qs=2048, dt=capi.DTYPE_BF16, qh=16, qo=P, kl=P, tab=P, ts=4, batch=2, mq=1, mk=64, window=2047,
+             sinks=4, scale=0.1, out=P, ws=None, wb=0)
+    d.update(kw)
+    return capi.lib().aps_attention_paged(c if c is not None else cache(), d["q"], d["qs"], d["dt"], rows, d["qh"],
+                                          d["qo"], d["kl"], d["tab"], d["ts"], d["batch"], d["mq"], d["mk"],
+                                          d["window"], d["sinks"], d["scale"], d["out"], d["ws"], d["wb"], None)
+
+
+def test_exports():
+    names = capi.declared_symbols(capi.SERVE_HEADER_PATH)
+    assert len(names) == 5
+    for n in names:
+        assert hasattr(capi.lib(), n), n
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(page_size=8), capi.APS_ERR_SHAPE), (dict(page_size=48), capi.APS_ERR_SHAPE),
+    (dict(page_size=512), capi.APS_ERR_SHAPE), (dict(page_size=0), capi.APS_ERR_SHAPE),
+    (dict(head_dim=96), capi.APS_ERR_SHAPE), (dict(kv_heads=0), capi.APS_ERR_SHAPE),
+    (dict(num_pages=0), capi.APS_ERR_SHAPE), (dict(num_pages=1 << 37), capi.APS_ERR_SHAPE),
+    (dict(dtype=capi.DTYPE_E4M3), capi.APS_ERR_DTYPE),
+    (dict(k=None), capi.APS_ERR_ARG), (dict(v=P + 8), capi.APS_ERR_ARG),
+    (dict(dtype=capi.KV_MXFP4), capi.APS_ERR_ARG),
+    (dict(dtype=capi.KV_MXFP4, k_scale=P, v_scale=P + 1), capi.APS_ERR_ARG),
+])
+def test_bad_caches(kw, code):
+    assert append(cache(**kw), rows=1) == code, capi.last_error()
+    assert capi.lib().aps_kv_gather(cache(**kw), P, 1, P, P, capi.DTYPE_F32, None) == code
+    assert attend(cache(**kw)) == code
+    assert capi.last_error()
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dt=capi.DTYPE_E4M3), capi.APS_ERR_DTYPE), (dict(rows=-1), capi.APS_ERR_SHAPE),
+    (dict(rows=(1 << 30) + 1), capi.APS_ERR_SHAPE), (dict(ks=511), capi.APS_ERR_SHAPE),
+    (dict(vs=0), capi.APS_ERR_SHAPE), (dict(mp=-1), capi.APS_ERR_SHAPE),
+    (dict(q=P, qo=P, qh=6, qs=768, qos=768), capi.APS_ERR_SHAPE),
+    (dict(q=P, qo=P, qh=16, qs=2047, qos=2048), capi.APS_ERR_SHAPE),
+    (dict(q=P, qo=P, qh=16, qs=2048, qos=4096), capi.APS_ERR_ARG),
+    (dict(rows=1, q=P, qo=None, qh=16, qs=2048, qos=2048), capi.APS_ERR_ARG),
+    (dict(rows=1, k=None), capi.APS_ERR_ARG), (dict(rows=1, pos=None), capi.APS_ERR_ARG),
+    (dict(rows=1, slots=P + 4), capi.APS_ERR_ARG), (dict(rows=1, cos=None), capi.APS_ERR_ARG),
+    (dict(rows=1, k=P + 2), capi.APS_ERR_ARG),
+])
+def test_append_refusals(kw, code):
+    assert append(**kw) == code, capi.last_error()
+
+
+def test_append_of_nothing_and_types():
+    assert append() == capi.APS_OK
+    assert append(cache(dtype=capi.DTYPE_F32), dt=capi.DTYPE_BF16) == capi.APS_ERR_DTYPE
+    assert append(cache(dtype=capi.DTYPE_F32)) == capi.APS_OK
+    assert capi.lib().aps_kv_append(None, P, 512, P, 512, None, 0, None, 0, 0, 0, 0, P, P, P, P, 4,
+                                    None) == capi.APS_ERR_ARG
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(rows=-1), capi.APS_ERR_SHAPE), (dict(dt=7), capi.APS_ERR_DTYPE), (dict(dtype=7), capi.APS_ERR_DTYPE),
+])
+def test_gather_refusals(kw, code):
+    dt = kw.get("dt", kw.get("dtype", capi.DTYPE_F32))
+    assert capi.lib().aps_kv_gather(cache(), P, kw.get("rows", 1), P, P, dt, None) == code
+
+
+def test_gather_of_nothing():
+    L = capi.lib()
+    assert L.aps_kv_gather(cache(), None, 0, None, None, capi.DTYPE_F32, None) == capi.APS_OK
+    assert L.aps_kv_gather(cache(), P, 3, None, None, capi.DTYPE_F32, None) == capi.APS_OK
+    assert L.aps_kv_gather(cache(), None, 3, P, P, capi.DTYPE_F32, None) == capi.APS_ERR_ARG
+    assert L.aps_kv_gather(cache(), P, 3, P + 4, P, capi.DTYPE_F32, None) == capi.APS_ERR_ARG
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(qh=15), capi.APS_ERR_SHAPE), (dict(qh=0), capi.APS_ERR_SHAPE), (dict(qs=2040), capi.APS_ERR_SHAPE),
+    (dict(qs=2052), capi.APS_ERR_SHAPE), (dict(window=0), capi.APS_ERR_SHAPE), (dict(sinks=-1), capi.APS_ERR_SHAPE),
+    (dict(rows=-1), capi.APS_ERR_SHAPE), (dict(batch=-1), capi.APS_ERR_SHAPE), (dict(mq=-1), capi.APS_ERR_SHAPE),
+    (dict(mk=-1), capi.APS_ERR_SHAPE), (dict(mk=1 << 31), capi.APS_ERR_SHAPE), (dict(ts=-1), capi.APS_ERR_SHAPE),
+    (dict(dt=capi.DTYPE_E4M3), capi.APS_ERR_DTYPE), (dict(scale=float("nan")), capi.APS_ERR_ARG),
+    (dict(scale=float("inf")), capi.APS_ERR_ARG), (dict(q=None), capi.APS_ERR_ARG), (dict(out=None), capi.APS_ERR_ARG),
+    (dict(qo=None), capi.APS_ERR_ARG), (dict(kl=None), capi.APS_ERR_ARG), (dict(tab=None), capi.APS_ERR_ARG),
+    (dict(q=P + 8), capi.APS_ERR_ARG), (dict(out=P + 4), capi.APS_ERR_ARG), (dict(kl=P + 1), capi.APS_ERR_ARG),
+])
+def test_attention_refusals(kw, code):
+    assert attend(**kw) == code, capi.last_error()
+    assert capi.last_error()
+
+
+def test_attention_of_nothing_and_workspace():
+    assert attend(rows=0, q=None, out=None) == capi.APS_OK
+    assert attend(batch=0, q=None) == capi.APS_OK
+    assert attend(mq=0, q=None) == capi.APS_OK
+    assert attend(cache(dtype=capi.DTYPE_F32)) == capi.APS_ERR_DTYPE       # bf16 queries on an fp32 cache
+    size = capi.lib().aps_attention_paged_workspace_size
+    need = size(cache(num_pages=9000), 1, 16, 1, 1, 131072, 131072, 0)
+    assert need > 0 and need % 4 == 0                                      # one long sequence is split
+    assert size(cache(), 0, 16, 1, 1, 64, 64, 0) == 0
+    assert size(cache(), 1, 15, 1, 1, 64, 64, 0) == 0
+    long = dict(rows=1, batch=1, mk=131072, window=131072, sinks=0)
+    assert attend(**long) == capi.APS_ERR_WORKSPACE
+    assert attend(**long, ws=P, wb=need - 1) == capi.APS_ERR_WORKSPACE
+    assert attend(**long, ws=P + 16, wb=need) == capi.APS_ERR_WORKSPACE
+
+
+def logits(rules=None, rows=1, **kw):
+    d = dict(x=P, xs=100, dt=capi.DTYPE_F32, vocab=100, out=P, os=100)
+    d.update(kw)
+    r = capi.LogitsRules(**(rules or {}))
+    return capi.lib().aps_logits_process(d["x"], d["xs"], d["dt"], rows, d["vocab"], ctypes.byref(r), d["out"],
+                                         d["os"], None)
+
+
+@pytest.mark.parametrize("rules,kw,code", [
+    ({}, dict(dt=capi.DTYPE_E4M3), capi.APS_ERR_DTYPE), ({}, dict(rows=-1), capi.APS_ERR_SHAPE),
+    ({}, dict(vocab=-1), capi.APS_ERR_SHAPE), ({}, dict(xs=99), capi.APS_ERR_SHAPE),
+    ({}, dict(os=99), capi.APS_ERR_SHAPE), ({}, dict(x=None), capi.APS_ERR_ARG), ({}, dict(out=None), capi.APS_ERR_ARG),
+    ({}, dict(os=104), capi.APS_ERR_ARG), ({}, dict(x=P + 1, out=P + 2), capi.APS_ERR_ARG),
+    (dict(history=P), {}, capi.APS_ERR_ARG),
+    (dict(bias_ids=P, bias_stride=3), {}, capi.APS_ERR_ARG),
+    (dict(mask=P, mask_rows=1, mask_stride=3), {}, capi.APS_ERR_SHAPE),
+    (dict(mask=P, mask_rows=1, mask_stride=4), dict(rows=2), capi.APS_ERR_SHAPE),
+])
+def test_logits_refusals(rules, kw, code):
+    assert logits(rules, **kw) == code, capi.last_error()
+
+
+def test_logits_of_nothing():
+    assert logits(rows=0, x=None, out=None) == capi.APS_OK
+    assert logits(vocab=0, x=None, out=None) == capi.APS_OK
+    assert capi.lib().aps_logits_process(P, 1, 0, 1, 1, None, P, 1, None) == capi.APS_ERR_ARG
+
+
+def test_batch_plan():
+    b = serve.PagedBatch([2, 0, 1], [3, 0, 18], [[5], [], [2, 7]], 16, "cpu", num_pages=8)
+    assert b.positions.tolist() == [1, 2, 17] and b.slots.tolist() == [81, 82, 113]
+    assert b.q_offsets.tolist() == [0, 2, 2, 3] and b.kv_lens.tolist() == [3, 0, 18]
+    assert b.page_table.tolist() == [[5, -1], [-1, -1], [2, 7]]
+    assert (b.rows, b.batch, b.max_q_len, b.max_kv_len) == (3, 3, 2, 18)
+    empty = serve.PagedBatch([], [], [], 16, "cpu")
+    assert empty.rows == 0 and empty.q_offsets.tolist() == [0]
+
+
+@pytest.mark.parametrize("args,message", [
+    (([2], [1], [[0]]), "0 <= q_lens <= kv_lens"), (([1], [17], [[0]]), "too few pages"),
+    (([1], [1], [[8]]), "page id"), (([1], [1], [[-1]]), "page id"), (([1, 1], [1, 1], [[3], [3]]), "share a slot"),
+    (([1], [1, 2], [[0]]), "one length"),
+])
+def test_batch_plan_refusals(args, message):
+    with pytest.raises(ValueError, match=message):
+        serve.PagedBatch(*args, 16, "cpu", num_pages=8)
+
+
+def test_python_mirror_refuses_cpu_tensors():
+    with pytest.raises(ValueError, match="paged cache"):
+        serve.PagedKvCache(torch.zeros(2, 1, 16, 64), torch.zeros(2, 1, 16, 64))
+    with pytest.raises(ValueError, match="logits_process"):
+        serve.logits_process_gpu(torch.zeros(2, 5))
+
+
+def test_oracle_blocks_of_four_bits():
+    """The oracle's own 4-bit blocks: nearest magnitudes, ties to the even
+    code, the smallest scale without saturation."""
+    x = np.zeros((1, 32), np.float32)
+    x[0, :10] = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.26, 6.0, -5.01]
+    codes, byte = serve_oracle.mx_encode(x)
+    assert byte.tolist() == [[127]]
+    val = serve_oracle.mx_values(codes, byte)[0, :10]
+    assert val.tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, -0.5, 6.0, -6.0]
+    x[0, 8] = 6.5
+    assert serve_oracle.mx_encode(x)[1].tolist() == [[128]]
+    x[0, 8] = np.inf
+    assert np.isnan(serve_oracle.mx_values(*serve_oracle.mx_encode(x))).all()
+    rng = np.random.default_rng(0)
+    y = (rng.standard_normal((50, 64)) * np.exp2(rng.integers(-20, 20, (50, 1)))).astype(np.float32)
+    c, b = serve_oracle.mx_encode(y)
+    top = np.abs(y.reshape(50, 2, 32)).max(-1)
+    assert np.all(top <= 6 * np.exp2(b - 127.0)) and np.all(top > 3 * np.exp2(b - 127.0))
+    off = np.abs(serve_oracle.mx_values(c, b) - y).reshape(50, 2, 32)
+    assert np.all(off <= np.exp2(b - 127.0)[..., None])   # half of the widest step, 2
