@@ -31,10 +31,11 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
-from . import capi, prefix
+from . import capi, prefix, serve
 from .attention import HEAD_DIM, NUM_ATTENTION_HEADS, NUM_KV_HEADS, ROPE_THETA, SLIDING_WINDOW, _device_table
 from .moe import NORM_EPS, MoeWeights, _call, register_moe_weights_gpu
 
+EOS_TOKEN_ID = 32000                  # reference include/config.h:25
 QD = NUM_ATTENTION_HEADS * HEAD_DIM   # 2048: q and attention-output width
 KD = NUM_KV_HEADS * HEAD_DIM          # 512: k and v width
 
@@ -147,6 +148,22 @@ class RowPlan:
                        last_rows=to_dev(last), prompt_tokens=rows)
 
 
+@dataclass
+class CachedRows:
+    """The rows of one step over paged caches: new tokens of each sequence,
+    packed, and where their keys and values go (one page table for every
+    layer's cache)."""
+    batch: serve.PagedBatch
+    node_token: torch.Tensor   # int32 [rows]: token id of each row
+    last_rows: torch.Tensor    # int32 [batch]: each sequence's last row
+    window: int = SLIDING_WINDOW
+    sinks: int = 0
+
+    @property
+    def rows(self) -> int:
+        return self.batch.rows
+
+
 def routes_view(b: "Buffers", moe: MoeWeights) -> torch.Tensor:
     """The routes [rows][2] (u8) the last MoE block wrote into b.ws."""
     off = moe.layout(b.rows).routes
@@ -246,10 +263,21 @@ class DecoderLayer:
         _call(L.aps_attention_tree(_p(b.q), _p(b.k), _p(b.v), _p(b.att), _p(plan.pos), _p(plan.anc), plan.max_len,
                                    T, NUM_ATTENTION_HEADS, NUM_KV_HEADS, HEAD_DIM, SLIDING_WINDOW, stream))
 
-    def forward_carry(self, b: Buffers, plan: RowPlan, has_carry: bool, stream) -> None:
+    def attention_cached(self, b: Buffers, plan: CachedRows, cache: serve.PagedKvCache, stream) -> None:
+        """normed -> att over the paged cache: projections, q and k rotated as
+        k and v go into the cache, attention over what is there."""
+        self._project(b, b.normed, (("q_proj", b.q, QD), ("k_proj", b.k, KD), ("v_proj", b.v, KD)), stream)
+        p = plan.batch
+        c, s = _device_table(b.q.device, p.max_kv_len, HEAD_DIM, ROPE_THETA)
+        serve.kv_append_gpu(cache, b.k, b.v, p.positions, p.slots, c, s, q=b.q, q_out=b.q)
+        serve.attention_paged_gpu(b.q, cache, p.q_offsets, p.kv_lens, p.page_table, p.max_q_len, p.max_kv_len,
+                                  q_heads=NUM_ATTENTION_HEADS, window=plan.window, sinks=plan.sinks, out=b.att)
+
+    def forward_carry(self, b: Buffers, plan, has_carry: bool, stream, cache: Optional[serve.PagedKvCache] = None
+                      ) -> None:
         """In place on b: on entry the layer input is b.x (+ b.carry when
         has_carry); on exit b.x is the MoE output and b.carry the attention
-        residual."""
+        residual.  plan: a RowPlan, or with this layer's cache CachedRows."""
         L, T, H, w = capi.lib(), b.rows, self.H, self.w
         if has_carry:
             _call(L.aps_add_layer_norm(_p(b.x), _p(b.carry), _p(w.in_w), _p(w.in_b), T, H, ctypes.c_float(NORM_EPS),
@@ -257,7 +285,10 @@ class DecoderLayer:
         else:
             _call(L.aps_layer_norm(_p(b.x), _p(w.in_w), _p(w.in_b), T, H, ctypes.c_float(NORM_EPS), _p(b.normed),
                                    stream))
-        self.attention(b, plan, stream)
+        if cache is None:
+            self.attention(b, plan, stream)
+        else:
+            self.attention_cached(b, plan, cache, stream)
         # attn = att W_o^T + b_o into carry, then carry += x and post = LN(carry)
         self._project(b, b.att, (("o_proj", b.carry, H),), stream)
         _call(L.aps_add_layer_norm(_p(b.carry), _p(b.x), _p(w.post_w), _p(w.post_b), T, H, ctypes.c_float(NORM_EPS),
@@ -300,18 +331,20 @@ class Model:
             self._bufs[rows] = b
         return b
 
-    def prefill(self, plan: RowPlan, on_layer=None) -> torch.Tensor:
+    def prefill(self, plan, on_layer=None, caches: Optional[Sequence[serve.PagedKvCache]] = None) -> torch.Tensor:
         """logits [batch][vocab] of each prompt's last token; launches only
         (the outputs come from torch's caching allocator).  on_layer(i, b),
         when given, runs after layer i's launches (for example to copy its
-        routes out of the shared workspace on the same stream)."""
+        routes out of the shared workspace on the same stream).  With caches
+        (one a layer) plan is CachedRows: its tokens join the sequences that
+        the caches hold."""
         L, dev = capi.lib(), self.emb.device
         stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
         b = self.buffers(plan.rows)
         T, H = plan.rows, self.H
         _call(L.aps_gather_rows(_p(self.emb), self.emb.shape[0], H, _p(plan.node_token), T, _p(b.x), stream))
         for i, layer in enumerate(self.layers):
-            layer.forward_carry(b, plan, i > 0, stream)
+            layer.forward_carry(b, plan, i > 0, stream, caches[i] if caches is not None else None)
             if on_layer is not None:
                 on_layer(i, b)
         if self.layers:
@@ -336,3 +369,88 @@ class Model:
 
     def generate(self, prompts: Sequence[Sequence[int]]) -> torch.Tensor:
         return self.prefill(RowPlan.from_prompts(prompts, self.emb.device))
+
+    def generate_decode(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, kv_dtype=torch.float32,
+                        page_size: int = 16, window: int = SLIDING_WINDOW, sinks: int = 0,
+                        repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
+                        bias: Optional[Dict[int, float]] = None, mask: Optional[torch.Tensor] = None,
+                        eos: int = EOS_TOKEN_ID) -> Tuple[List[List[int]], torch.Tensor]:
+        """Greedy decoding of a prompt batch on paged caches (kv_dtype:
+        torch.float32, torch.bfloat16 or "mxfp4"): each token is computed once,
+        where the reference's generate_decode runs the whole prefix again for
+        each (src/model.cu:163-204).  Returns the new ids of each prompt, up to
+        and with eos, and the logits [batch][max_new_tokens][vocab] they were
+        chosen from: after the penalties, the biases {id: value} and the mask
+        ([1] or [batch] rows of int32 words, bit t % 32 of word t / 32 allows
+        token t).  Of equal logits the lowest id wins.  One host wait, at the
+        end."""
+        if len(prompts) == 0:
+            raise RuntimeError("generate_decode received an empty input batch")
+        if max_new_tokens < 1:
+            raise ValueError("max_new_tokens must be positive")
+        dev, n_seq = self.emb.device, len(prompts)
+        V = self.head_w.shape[0]
+        lens = [len(p) for p in prompts]
+        flat = np.concatenate([np.asarray(p, np.int64).reshape(-1) for p in prompts])
+        if min(lens) == 0:
+            raise ValueError("empty input")
+        if max(lens) + max_new_tokens - 1 > prefix.MAX_POSITION_EMBEDDINGS:
+            raise ValueError("sequence is too long")
+        if flat.min() < 0 or flat.max() >= self.emb.shape[0]:
+            raise ValueError("token out of vocabulary")
+        # pages for the whole answer, consecutive for each sequence
+        need = [-(-(n + max_new_tokens - 1) // page_size) for n in lens]
+        first = np.cumsum([0] + need)
+        pages = [range(first[b], first[b + 1]) for b in range(n_seq)]
+        caches = [serve.PagedKvCache.allocate(int(first[-1]), page_size, NUM_KV_HEADS, HEAD_DIM, kv_dtype, dev)
+                  for _ in self.layers]
+        plan = serve.PagedBatch(lens, lens, pages, page_size, dev, num_pages=int(first[-1]))
+        last = np.cumsum(lens) - 1
+        i32 = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+        rows = CachedRows(plan, i32(flat), i32(last), window, sinks)
+        # one new token a sequence from here on: the same arrays, advanced on the device
+        step = serve.PagedBatch([1] * n_seq, [n + max_new_tokens - 1 for n in lens], pages, page_size, dev)
+        kv_lens, seq = i32(lens), torch.arange(n_seq, device=dev)
+        rules = {}
+        history = None
+        if repetition != 1.0 or frequency != 0.0 or presence != 0.0:
+            history = torch.full((n_seq, max(lens) + max_new_tokens), -1, dtype=torch.int32, device=dev)
+            for b, p in enumerate(prompts):
+                history[b, :lens[b]] = i32(p)
+            full = lambda v: torch.full((n_seq,), v, dtype=torch.float32, device=dev)  # noqa: E731
+            rules.update(history=history, prompt_lens=i32(lens), repetition=full(repetition),
+                         frequency=full(frequency), presence=full(presence))
+        if bias:
+            rules.update(bias_ids=i32([list(bias)] * n_seq), bias_lens=i32([len(bias)] * n_seq),
+                         bias_values=torch.tensor([list(bias.values())] * n_seq, dtype=torch.float32, device=dev))
+        if mask is not None:
+            rules.update(mask=mask.to(dev).contiguous())
+            if mask.shape[0] == 1:
+                rules.update(mask_index=torch.zeros(n_seq, dtype=torch.int32, device=dev))
+        out = torch.empty((n_seq, max_new_tokens, V), dtype=torch.float32, device=dev)
+        ids = torch.empty((n_seq, max_new_tokens), dtype=torch.int32, device=dev)
+        for t in range(max_new_tokens):
+            logits = self.prefill(rows, caches=caches)
+            if rules:
+                if history is not None:
+                    rules["history_lens"] = kv_lens
+                serve.logits_process_gpu(logits, out=logits, **rules)
+            out[:, t] = logits
+            # argmax leaves open which of equal logits it takes
+            top = torch.where(logits == logits.amax(1, keepdim=True), torch.arange(V, device=dev), V).amin(1)
+            token = top.clamp(max=V - 1).to(torch.int32)
+            ids[:, t] = token
+            if t + 1 == max_new_tokens:
+                break
+            if history is not None:
+                history[seq, kv_lens.long()] = token
+            step.positions = kv_lens.clone()
+            kv_lens = kv_lens + 1
+            at = step.positions.long()
+            page = step.page_table[seq, at // page_size].long()
+            step.slots, step.kv_lens = page * page_size + at % page_size, kv_lens
+            rows = CachedRows(step, token, seq.to(torch.int32), window, sinks)
+        done = []
+        for row in ids.cpu().tolist():
+            done.append(row[:row.index(eos) + 1] if eos in row else row)
+        return done, out
