@@ -47,6 +47,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kRows = 16;      // rows of a tile
 constexpr int kMaxSplits = 64;  // one wave reads every split's maximum at once
+constexpr int64_t kTiledRows = 64;  // rows of a sequence under a key head from which k_paged_tiles takes them
 
 // What both kernels know of the launch.
 struct PagedDev {
@@ -55,8 +56,10 @@ struct PagedDev {
     int group;       // query heads per key head
     int page_shift;
     int splits;      // workgroups along the keys
-    int row_tiles;   // tiles of rows a sequence and key head can have
+    int row_tiles;   // tiles (tiled: blocks) of rows a sequence and key head can have
+    bool tiled;      // k_paged_tiles, else k_paged_rows
     bool by_rows;    // the waves of a workgroup take a tile each (else a part of the keys each)
+    int64_t blocks;  // workgroups
     float scale_log2;
 };
 
@@ -520,6 +523,369 @@ k_paged_rows(PagedDev d) {
     }
 }
 
+// ---- many rows ----------------------------------------------------------------
+//
+// The same products on 32 x 32 MFMAs for chunks: a workgroup takes 128 rows (32
+// a wave) under one key head and walks 64 keys a step, K and V staged in LDS
+// (bf16: global_load_lds straight from the pages; 4 bits: decoded on the way)
+// one step ahead in two buffers.
+//   S^T = K Q^T     32 keys x 32 rows; a lane holds row lane % 32 and keys
+//                   8 (i / 4) + 4 (lane / 32) + i % 4
+//   O^T += V^T P^T   32 dims x 32 rows; the 8 weights a lane holds of 16 keys are
+//                   the B operand as they are, and V^T comes transposed out of
+//                   LDS (ds_read_b64_tr_b16: 4 keys of one dim) in that order.
+// The running reference m of a row follows its maximum only when that has grown
+// by more than 2^8: weights are then below 256, which neither their bf16 nor the
+// fp32 sums feel, and most steps leave the accumulator alone.
+// LDS rows are one key's D values; 16-byte chunks are permuted so that the lanes
+// served together (16 keys' same chunk for K, 4 keys' 64 bytes for V) lie in
+// different banks.
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTileRows = 32;            // rows of a wave
+constexpr int kBlockRows = kWaves * kTileRows;
+constexpr int kTileKeys = 64;            // keys of a step
+constexpr float kLag = 8.0f;
+
+template <int D>
+__device__ inline int k_swizzle(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
+template <int D>
+__device__ inline int v_swizzle(int key) { return D == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
+
+#define APS_AGP(p) ((const __attribute__((address_space(1))) void*)(p))
+#define APS_ALP(p) ((__attribute__((address_space(3))) void*)(p))
+
+template <int D, bool Q32, Kv KV>
+__global__ void __launch_bounds__(64 * kWaves, 2)
+k_paged_tiles(PagedDev d) {
+    constexpr int ROW = 2 * D;                 // LDS bytes of a key
+    constexpr int CH = ROW / 16;               // 16-byte chunks of a key
+    constexpr int QT = Q32 ? 3 : 1, PT = Q32 ? 3 : 1;
+    constexpr int KS = D / 16, DT = D / 32;
+    __shared__ __align__(1024) uint8_t sm[2][2][kTileKeys * ROW];  // [buffer][k, v]
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
+    // workgroups of one key head are neighbours in one XCD's share of the grid:
+    // they read the same keys through one L2
+    const uint32_t share = (gridDim.x + 7) / 8;
+    uint32_t id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+    const uint32_t row_blocks = d.row_tiles;
+    if (id >= static_cast<uint32_t>(d.blocks)) return;
+    const int split = id % d.splits;
+    id /= d.splits;
+    const int rb = static_cast<int>(row_blocks - 1 - id % row_blocks);
+    id /= row_blocks;
+    const int h = id % d.c.kv_heads;
+    const int64_t b = id / d.c.kv_heads;
+    const Seq sq = sequence(d, b);
+    const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
+    const int nrows = static_cast<int>(qlen * d.group);
+    const int rb0 = rb * kBlockRows;
+    if (rb0 >= nrows) return;
+    const int32_t* table = d.a.page_table + b * d.a.table_stride;
+    const int p0 = sq.kv - sq.len;
+    const int rb1 = (rb0 + kBlockRows < nrows ? rb0 + kBlockRows : nrows) - 1;
+    const Keys ks = visible<kTileKeys>(d, p0 + rb0 / d.group, p0 + rb1 / d.group);
+    const int each = (ks.steps + d.splits - 1) / d.splits;
+    const int t0 = split * each < ks.steps ? split * each : ks.steps;
+    const int t1 = t0 + each < ks.steps ? t0 + each : ks.steps;
+
+    const int r0 = rb0 + wave * kTileRows;
+    const bool any = r0 < nrows;
+    const int r_last = r0 + kTileRows - 1 < nrows ? r0 + kTileRows - 1 : nrows - 1;
+    const int pmin = p0 + r0 / d.group, pmax = any ? p0 + r_last / d.group : -1;
+    const int row = r0 + c;
+    const bool live = row < nrows;
+    const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
+    const int pos = live ? p0 + tok : -1;
+
+    // queries: a lane holds dims 16 s + 8 hf + j of its row; the sign of the
+    // scale goes into them, so that the largest product is the largest score
+    bf16x8 qb[QT][KS];
+    const float cs = d.scale_log2 == 0.0f ? 1.0f : fabsf(d.scale_log2);
+    const uint32_t flip = d.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = d.scale_log2 == 0.0f ? 0u : ~0u;
+    {
+        const int64_t qat = (sq.q0 + tok) * d.a.q_stride + static_cast<int64_t>(qh) * D;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int dim = 16 * s + 8 * hf;
+            if constexpr (Q32) {
+                const float* p = static_cast<const float*>(d.a.q) + qat + dim;
+                const f32x4 x0 = *reinterpret_cast<const f32x4*>(p), x1 = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float x = j < 4 ? x0[j & 3] : x1[j & 3];
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        const float hi = bf16_round(x);
+                        qb[t][s][j] = static_cast<__bf16>(hi);
+                        x -= hi;
+                    }
+                }
+            } else {
+                qb[0][s] = *reinterpret_cast<const bf16x8*>(static_cast<const bf16_t*>(d.a.q) + qat + dim);
+            }
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                u32x4 w = __builtin_bit_cast(u32x4, qb[t][s]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
+                qb[t][s] = __builtin_bit_cast(bf16x8, w);
+            }
+        }
+    }
+
+    // ---- staging: a wave takes the step's keys 16 wave .. 16 wave + 15
+    auto base_of = [&](int t) { return (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * kTileKeys; };
+    auto page_of = [&](int key) {   // the page of 16 keys, -1 where there is none
+        const int page = key < ks.hi ? table[key >> d.page_shift] : -1;
+        return page >= 0 && page < d.c.num_pages ? page : -1;
+    };
+    u32x4 mk{}, mv{};
+    uint32_t mks = 0, mvs = 0;
+    auto fetch = [&](int t, int buf) {
+        const int key = base_of(t) + 16 * wave;
+        const int page = page_of(key);
+        const int64_t hrow = ((static_cast<int64_t>(page < 0 ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
+                             (key & ((1 << d.page_shift) - 1));
+        if constexpr (KV == Kv::kBf16) {
+            constexpr int RPI = 1024 / ROW;  // keys of one copy
+            const uint8_t* kp = static_cast<const uint8_t*>(d.c.k) + hrow * ROW;
+            const uint8_t* vp = static_cast<const uint8_t*>(d.c.v) + hrow * ROW;
+#pragma unroll
+            for (int i = 0; i < 16 / RPI; ++i) {
+                const int r = RPI * i + lane / CH, ph = lane % CH;
+                __builtin_amdgcn_global_load_lds(APS_AGP(kp + r * ROW + ((ph ^ k_swizzle<D>(r)) << 4)),
+                                                 APS_ALP(&sm[buf][0][(16 * wave + RPI * i) * ROW]), 16, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 16 / RPI; ++i) {
+                const int r = RPI * i + lane / CH, ph = lane % CH;
+                __builtin_amdgcn_global_load_lds(APS_AGP(vp + r * ROW + ((ph ^ v_swizzle<D>(r)) << 4)),
+                                                 APS_ALP(&sm[buf][1][(16 * wave + RPI * i) * ROW]), 16, 0, 0);
+            }
+        } else {
+            const int64_t at = hrow + lane / 4;  // four lanes a key
+            const uint8_t* kp = static_cast<const uint8_t*>(d.c.k) + at * (D / 2) + (lane & 3) * (D / 8);
+            const uint8_t* vp = static_cast<const uint8_t*>(d.c.v) + at * (D / 2) + (lane & 3) * (D / 8);
+            if constexpr (D == 128) {
+                mk = *reinterpret_cast<const u32x4*>(kp);
+                mv = *reinterpret_cast<const u32x4*>(vp);
+            } else {
+                const u32x2 a = *reinterpret_cast<const u32x2*>(kp), w = *reinterpret_cast<const u32x2*>(vp);
+                mk = u32x4{a[0], a[1], 0u, 0u};
+                mv = u32x4{w[0], w[1], 0u, 0u};
+            }
+            mks = d.c.k_scale[at * (D / 32) + (lane & 3) * (D / 4) / 32];
+            mvs = d.c.v_scale[at * (D / 32) + (lane & 3) * (D / 4) / 32];
+        }
+    };
+    auto commit = [&](int t, int buf) {
+        const int key0 = base_of(t) + 16 * wave;
+        if constexpr (KV == Kv::kMx) {
+            const int r = lane / 4;
+            const float sk = mx_scale(mks), sv = mx_scale(mvs);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const int chunk = (lane & 3) * (D / 32) + j;
+                uint8_t* at = &sm[buf][0][(16 * wave + r) * ROW];
+                *reinterpret_cast<u32x4*>(at + ((chunk ^ k_swizzle<D>(r)) << 4)) =
+                    u32x4{mx_decode2<0>(mk[j], sk), mx_decode2<1>(mk[j], sk), mx_decode2<2>(mk[j], sk),
+                          mx_decode2<3>(mk[j], sk)};
+                at = &sm[buf][1][(16 * wave + r) * ROW];
+                *reinterpret_cast<u32x4*>(at + ((chunk ^ v_swizzle<D>(r)) << 4)) =
+                    u32x4{mx_decode2<0>(mv[j], sv), mx_decode2<1>(mv[j], sv), mx_decode2<2>(mv[j], sv),
+                          mx_decode2<3>(mv[j], sv)};
+            }
+        } else {
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies are in LDS
+        }
+        // values that no row of the block sees become zeros
+        const bool whole = page_of(key0) >= 0 && key0 + 15 < ks.hi && (key0 >= ks.lo || key0 + 15 < ks.first);
+        if (!whole) {
+            const int r = lane / 4, key = key0 + r;
+            if (page_of(key0) < 0 || key >= ks.hi || (key < ks.lo && key >= ks.first)) {
+                u32x4* at = reinterpret_cast<u32x4*>(&sm[buf][1][(16 * wave + r) * ROW + (lane & 3) * (ROW / 4)]);
+#pragma unroll
+                for (int j = 0; j < ROW / 64; ++j) at[j] = u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+    };
+
+    // LDS offsets of a lane's operands
+    int k_off[KS], v_off[DT];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) k_off[s] = c * ROW + (((2 * s + hf) ^ k_swizzle<D>(c)) << 4);
+    {
+        const int i = lane & 15, r = i >> 2, dh = (lane >> 4) & 1;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            v_off[t] = (4 * hf + r) * ROW + (((4 * t + 2 * dh + ((i & 3) >> 1)) ^ v_swizzle<D>(r)) << 4) + 8 * (i & 1);
+    }
+
+    f32x16 acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    if (t0 < t1) {
+        fetch(t0, 0);
+        commit(t0, 0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1, base = base_of(t);
+        if (t + 1 < t1) fetch(t + 1, buf ^ 1);
+        // a step that no row of this wave sees is left out
+        const bool none = base > pmax ||
+                          (static_cast<int64_t>(base) + kTileKeys - 1 <= static_cast<int64_t>(pmin) - d.a.window &&
+                           base >= d.a.sinks);
+        if (!none) {
+            const uint8_t* kt = sm[buf][0];
+            const uint8_t* vt = sm[buf][1];
+            f32x16 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < KS; ++x) {
+                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + k_off[x] + u * 32 * ROW);
+#pragma unroll
+                    for (int q3 = QT - 1; q3 >= 0; --q3)
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[q3][x], s[u], 0, 0, 0);
+                }
+            }
+            uint32_t dead = 0;
+#pragma unroll
+            for (int a = 0; a < 4; ++a) dead |= page_of(base + 16 * a) < 0 ? 1u << a : 0u;
+            const bool full = dead == 0 && base + kTileKeys - 1 <= pmin &&
+                              (static_cast<int64_t>(base) > static_cast<int64_t>(pmax) - d.a.window ||
+                               base + kTileKeys - 1 < d.a.sinks);
+            if (!full) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = 32 * u + 8 * (i / 4) + 4 * hf + i % 4;
+                        if ((dead >> (at / 16) & 1u) || !sees(d, pos, base + at)) s[u][i] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+            top = fmaxf(top, __shfl_xor(top, 32)) * cs;
+            if (__any(top > m + kLag)) {
+                const float mn = top > m + kLag ? top : m;
+                const float f = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int x = 0; x < DT; ++x) acc[x] *= f;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[u][i] = exp2_fast(fmaf(s[u][i], cs, -ref));
+                    l += s[u][i];
+                }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {   // 16 keys each
+                u32x4 pb[PT];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float a0 = s[x / 2][8 * (x & 1) + 2 * j], a1 = s[x / 2][8 * (x & 1) + 2 * j + 1];
+#pragma unroll
+                    for (int p3 = 0; p3 < PT; ++p3) {
+                        pb[p3][j] = pack2_bf16(a0, a1);
+                        a0 -= bf16w_lo(pb[p3][j]);
+                        a1 -= bf16w_hi(pb[p3][j]);
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < DT; ++y) {
+                    typedef __attribute__((address_space(3))) s16x4* lds_s4;
+                    const uint8_t* at = vt + v_off[y] + 16 * x * ROW;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 8 * ROW));
+                    const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
+                    const bf16x8 va = __builtin_bit_cast(bf16x8, u32x4{wl[0], wl[1], wh[0], wh[1]});
+#pragma unroll
+                    for (int p3 = PT - 1; p3 >= 0; --p3)
+                        acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8, pb[p3]), acc[y],
+                                                                          0, 0, 0);
+                }
+            }
+        }
+        if (t + 1 < t1) commit(t + 1, buf ^ 1);
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32);
+
+    bool nan = l != l;
+#pragma unroll
+    for (int y = 0; y < DT; ++y)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) nan = nan || acc[y][i] != acc[y][i];
+    const uint64_t bad = __ballot(nan && live);
+    uint32_t rows = static_cast<uint32_t>(bad | bad >> 32);
+    if (any && pmin != pmax) {
+        // every wave is past the last step's barrier: the staging buffers are free
+        float* red = reinterpret_cast<float*>(&sm[0][0][0]) + wave * (D + 2);
+        while (rows) {
+            const int x = __builtin_ctz(rows);
+            rows &= rows - 1;
+            const int rr = r0 + x;
+            redo_row<D, Q32, KV, kTileKeys>(d, table, h, ks, t0, t1, sq.q0 + rr / d.group,
+                                            h * d.group + rr % d.group, p0 + rr / d.group, red, red + D, red + D + 1);
+            __builtin_amdgcn_wave_barrier();
+            if (c == x) {
+                m = red[D];
+                l = red[D + 1];
+#pragma unroll
+                for (int y = 0; y < DT; ++y)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[y][i] = red[32 * y + 8 * (i / 4) + 4 * hf + i % 4];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    if (!live) return;
+    const int64_t orow = (sq.q0 + tok) * d.a.q_heads + qh;
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    const int64_t at = orow * d.splits + split;
+    if (d.splits > 1 && hf == 0) {
+        float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+        ml[0] = m;
+        ml[1] = l;
+    }
+#pragma unroll
+    for (int y = 0; y < DT; ++y)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int dim = 32 * y + 2 * i + 4 * hf;
+            f32x4 v = {acc[y][i], acc[y][i + 1], acc[y][i + 2], acc[y][i + 3]};
+            if (d.splits > 1) {
+                *reinterpret_cast<f32x4*>(d.a.part + at * D + dim) = v;
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = l == 0.0f ? 0.0f : v[j] * inv;
+            if constexpr (Q32)
+                *reinterpret_cast<f32x4*>(static_cast<float*>(d.a.out) + orow * D + dim) = v;
+            else
+                *reinterpret_cast<u32x2*>(static_cast<bf16_t*>(d.a.out) + orow * D + dim) =
+                    u32x2{pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3])};
+        }
+}
+
 // out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits of one
 // (row, head), a wave each.  Rows that no sequence names are not touched: the
 // grid walks the sequences.
@@ -567,26 +933,39 @@ PagedDev plan(const KvCache& c, const PagedArgs& a) {
     d.page_shift = c.page_shift;
     d.group = a.q_heads / c.kv_heads;
     d.scale_log2 = a.scale * 1.4426950408889634f;
-    const int64_t rows = a.max_q_len * d.group;
-    d.row_tiles = static_cast<int>(ceil_div(rows, kRows));
-    const int64_t heads = a.batch * c.kv_heads;
-    d.by_rows = d.row_tiles >= kWaves;
-    const int64_t blocks = heads * ceil_div(d.row_tiles, d.by_rows ? kWaves : 1);
-    // keys one tile can see, and workgroups for 256 CUs of four
+    const int64_t rows = a.max_q_len * d.group, heads = a.batch * c.kv_heads;
+    // keys one tile can see, in steps of 32
     const int64_t keys = std::min<int64_t>(a.max_kv_len, static_cast<int64_t>(a.window) + a.sinks + 16);
     const int64_t steps = ceil_div(keys, 32);
-    int64_t splits = d.by_rows ? 1 : ceil_div(1024, blocks);
-    splits = std::min<int64_t>(splits, ceil_div(steps, 2 * kWaves));
+    d.tiled = c.type != Kv::kF32 && rows >= kTiledRows;
+    int64_t splits;
+    if (d.tiled) {
+        d.by_rows = false;
+        d.row_tiles = static_cast<int>(ceil_div(rows, kBlockRows));
+        splits = std::min<int64_t>(ceil_div(512, heads * d.row_tiles), ceil_div(steps, 8));
+    } else {
+        d.row_tiles = static_cast<int>(ceil_div(rows, kRows));
+        d.by_rows = d.row_tiles >= kWaves;
+        const int64_t blocks = heads * ceil_div(d.row_tiles, d.by_rows ? kWaves : 1);
+        splits = std::min<int64_t>(ceil_div(1024, blocks), ceil_div(steps, d.by_rows ? 8 : 2 * kWaves));
+    }
     d.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
+    d.blocks = heads * d.splits * (d.tiled || !d.by_rows ? d.row_tiles : ceil_div(d.row_tiles, kWaves));
     return d;
 }
 
 template <int D, bool Q32, Kv KV>
 hipError_t launch(const PagedDev& d, hipStream_t s) {
-    const int64_t blocks = d.a.batch * d.c.kv_heads * d.splits * ceil_div(d.row_tiles, d.by_rows ? kWaves : 1);
     const int64_t joins = d.a.batch * d.a.max_q_len * d.a.q_heads;
-    if (blocks > 0x7FFFFFFF || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, d);
+    if (d.blocks > 0x7FFFFFF0 || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
+    const dim3 block(64 * kWaves);
+    if constexpr (KV != Kv::kF32) {
+        if (d.tiled)
+            hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), dim3(static_cast<unsigned>(ceil_div(d.blocks, 8) * 8)),
+                               block, 0, s, d);
+    }
+    if (!d.tiled)
+        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)), block, 0, s, d);
     if (d.splits > 1)
         hipLaunchKernelGGL((k_paged_join<D, Q32>), dim3(static_cast<unsigned>(joins)), dim3(64), 0, s, d);
     return hipGetLastError();

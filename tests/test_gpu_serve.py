@@ -314,9 +314,11 @@ def test_rows_left_alone_and_pages_left_out(gpu_device, qt, kind):
         c.check(got, 2047, 1)
         short = torch.full_like(out, 5.0)
         c.run(2047, 1, out=short, max_q_len=2)
-        keep = np.concatenate([[True, True] + [False] * (n - 2) for n in q_lens] + [[False] * 4])
-        same = (short == out).all(1).cpu().numpy()
-        assert same[keep].all() and bool((short[torch.from_numpy(~keep)] == 5.0).all())
+        keep = torch.from_numpy(np.concatenate([[True, True] + [False] * (n - 2) for n in q_lens] + [[False] * 4]))
+        keep = keep.to(gpu_device)
+        assert bool((short[~keep] == 5.0).all())
+        # fewer queries may take another kernel: its rows are held to the same bound
+        c.check(torch.where(keep[:, None], short, out), 2047, 1)
 
 
 def test_lengths_past_the_bounds_are_cut(gpu_device):
