@@ -104,9 +104,36 @@ __device__ inline Keys visible(const PagedDev& d, int pmin, int pmax) {
     return k;
 }
 
+// The page of the 16 keys 16 a .. of step t, -1 where there is none: behind the
+// last key that is seen, past t1, or an id outside the cache.  A wave reads the
+// pages of many steps at once, a lane each.
+template <int STEP>
+__device__ inline int page_of(const PagedDev& d, const int32_t* table, const Keys& ks, int t, int t1, int a) {
+    const int key = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP + 16 * a;
+    const int page = t < t1 && key < ks.hi ? table[key >> d.page_shift] : -1;
+    return page >= 0 && page < d.c.num_pages ? page : -1;
+}
+
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ inline bool sees(const PagedDev& d, int pos, int key) {
-    return key <= pos && (static_cast<int64_t>(key) > static_cast<int64_t>(pos) - d.a.window || key < d.a.sinks);
+// A row's view of the keys: key <= pos and (key > low or key < sinks).
+struct View {
+    int pos, low;
+};
+__device__ inline View view(const PagedDev& d, int pos) {
+    const int64_t low = static_cast<int64_t>(pos) - d.a.window;
+    return View{pos, low > -1 ? static_cast<int>(low) : -1};
+}
+__device__ inline bool sees(const PagedDev& d, const View& v, int key) {
+    return (key <= v.pos) & ((key > v.low) | (key < d.a.sinks));
+}
+// Maximum and sum over the lanes l, l ^ 16 and l, l ^ 32.
+__device__ inline float max_x32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float max_x16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ inline float bf16_round(float x) { return __uint_as_float(pack2_bf16(x, 0.0f) << 16); }
 
@@ -127,6 +154,7 @@ template <int D, bool Q32, Kv KV, int STEP>
 __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const Keys& ks, int t0, int t1, int64_t qrow,
                          int head, int pos, float* o, float* m_out, float* l_out) {
     constexpr int PER = D / 64;
+    const View vis = view(d, pos);
     const int lane = threadIdx.x & 63;
     float q[PER], acc[PER];
 #pragma unroll
@@ -140,7 +168,7 @@ __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const K
     for (int t = t0; t < t1; ++t) {
         const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
         for (int key = base; key < base + STEP; ++key) {
-            if (!sees(d, pos, key)) continue;
+            if (!sees(d, vis, key)) continue;
             const int64_t page = table[key >> d.page_shift];
             if (page < 0 || page >= d.c.num_pages) continue;
             const int64_t hr = ((page * d.c.kv_heads + h) << d.page_shift) + (key & ((1 << d.page_shift) - 1));
@@ -250,18 +278,21 @@ k_paged_rows(PagedDev d) {
     for (int t = 0; t < W; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
 
+    const View vis = view(d, pos);
+    constexpr int AHEAD = 64 / HALVES;  // steps whose pages the lanes hold
+    int pages = -1;
     for (int t = t0; t < t1; ++t) {
         const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
+        const int slot = (t - t0) % AHEAD;
+        if (slot == 0) pages = page_of<STEP>(d, table, ks, t + lane / HALVES, t1, lane % HALVES);
         bool dead[HALVES];
         int64_t hrow[HALVES];  // (page, head, offset) row of the half's first key
 #pragma unroll
         for (int a = 0; a < HALVES; ++a) {
-            const int key = base + 16 * a;
-            // past the last position there may be no table entry either
-            const int page = key < ks.hi ? table[key >> d.page_shift] : -1;
-            dead[a] = page < 0 || page >= d.c.num_pages;
+            const int page = __builtin_amdgcn_readlane(pages, slot * HALVES + a);
+            dead[a] = page < 0;
             hrow[a] = ((static_cast<int64_t>(dead[a] ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
-                      (key & ((1 << d.page_shift) - 1));
+                      ((base + 16 * a) & ((1 << d.page_shift) - 1));
         }
         f32x4 s4[HALVES];
         float vf[FP ? 4 : 1][W];
@@ -384,8 +415,8 @@ k_paged_rows(PagedDev d) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = base + 16 * a + 4 * g + i;
-                    if (dead[a] || !sees(d, pos, key)) s4[a][i] = -INFINITY;
-                    const bool some = !dead[a] && key < ks.hi && (key >= ks.lo || key < ks.first);
+                    s4[a][i] = (dead[a] | !sees(d, vis, key)) ? -INFINITY : s4[a][i];
+                    const bool some = !dead[a] & (key < ks.hi) & ((key >= ks.lo) | (key < ks.first));
                     if constexpr (FP) {
 #pragma unroll
                         for (int x = 0; x < W; ++x) vf[i][x] = some ? vf[i][x] : 0.0f;
@@ -398,8 +429,7 @@ k_paged_rows(PagedDev d) {
         float top = fmaxf(fmaxf(s4[0][0], s4[0][1]), fmaxf(s4[0][2], s4[0][3]));
         if constexpr (HALVES == 2)
             top = fmaxf(top, fmaxf(fmaxf(s4[1][0], s4[1][1]), fmaxf(s4[1][2], s4[1][3])));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = max_x32(max_x16(top));
         if (__any(top > m)) {
             const float mn = fmaxf(m, top);
             const float f = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
@@ -600,7 +630,7 @@ k_paged_tiles(PagedDev d) {
     const int row = r0 + c;
     const bool live = row < nrows;
     const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
-    const int pos = live ? p0 + tok : -1;
+    const View vis = view(d, live ? p0 + tok : -1);
 
     // queries: a lane holds dims 16 s + 8 hf + j of its row; the sign of the
     // scale goes into them, so that the largest product is the largest score
@@ -640,15 +670,16 @@ k_paged_tiles(PagedDev d) {
 
     // ---- staging: a wave takes the step's keys 16 wave .. 16 wave + 15
     auto base_of = [&](int t) { return (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * kTileKeys; };
-    auto page_of = [&](int key) {   // the page of 16 keys, -1 where there is none
-        const int page = key < ks.hi ? table[key >> d.page_shift] : -1;
-        return page >= 0 && page < d.c.num_pages ? page : -1;
-    };
     u32x4 mk{}, mv{};
     uint32_t mks = 0, mvs = 0;
+    int pages = -1;         // lane 4 i + a: the page of 16 keys a of step i of sixteen
+    uint32_t dead_next = 0;  // bit a: 16 keys a of the step that was fetched have no page
     auto fetch = [&](int t, int buf) {
+        const int slot = (t - t0) & 15;
+        if (slot == 0) pages = page_of<kTileKeys>(d, table, ks, t + lane / 4, t1, lane & 3);
+        dead_next = static_cast<uint32_t>(__ballot(pages < 0) >> (4 * slot)) & 15u;
         const int key = base_of(t) + 16 * wave;
-        const int page = page_of(key);
+        const int page = __builtin_amdgcn_readlane(pages, 4 * slot + wave);
         const int64_t hrow = ((static_cast<int64_t>(page < 0 ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
                              (key & ((1 << d.page_shift) - 1));
         if constexpr (KV == Kv::kBf16) {
@@ -704,10 +735,11 @@ k_paged_tiles(PagedDev d) {
             __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies are in LDS
         }
         // values that no row of the block sees become zeros
-        const bool whole = page_of(key0) >= 0 && key0 + 15 < ks.hi && (key0 >= ks.lo || key0 + 15 < ks.first);
+        const bool gone = dead_next >> wave & 1u;
+        const bool whole = !gone && key0 + 15 < ks.hi && (key0 >= ks.lo || key0 + 15 < ks.first);
         if (!whole) {
             const int r = lane / 4, key = key0 + r;
-            if (page_of(key0) < 0 || key >= ks.hi || (key < ks.lo && key >= ks.first)) {
+            if (gone || key >= ks.hi || (key < ks.lo && key >= ks.first)) {
                 u32x4* at = reinterpret_cast<u32x4*>(&sm[buf][1][(16 * wave + r) * ROW + (lane & 3) * (ROW / 4)]);
 #pragma unroll
                 for (int j = 0; j < ROW / 64; ++j) at[j] = u32x4{0u, 0u, 0u, 0u};
@@ -740,6 +772,7 @@ k_paged_tiles(PagedDev d) {
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1, base = base_of(t);
+        const uint32_t dead = dead_next;
         if (t + 1 < t1) fetch(t + 1, buf ^ 1);
         // a step that no row of this wave sees is left out
         const bool none = base > pmax ||
@@ -761,9 +794,6 @@ k_paged_tiles(PagedDev d) {
                         s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[q3][x], s[u], 0, 0, 0);
                 }
             }
-            uint32_t dead = 0;
-#pragma unroll
-            for (int a = 0; a < 4; ++a) dead |= page_of(base + 16 * a) < 0 ? 1u << a : 0u;
             const bool full = dead == 0 && base + kTileKeys - 1 <= pmin &&
                               (static_cast<int64_t>(base) > static_cast<int64_t>(pmax) - d.a.window ||
                                base + kTileKeys - 1 < d.a.sinks);
@@ -773,13 +803,14 @@ k_paged_tiles(PagedDev d) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int at = 32 * u + 8 * (i / 4) + 4 * hf + i % 4;
-                        if ((dead >> (at / 16) & 1u) || !sees(d, pos, base + at)) s[u][i] = -INFINITY;
+                        const bool out = (dead >> (2 * u + i / 8) & 1u) | !sees(d, vis, base + at);
+                        s[u][i] = out ? -INFINITY : s[u][i];
                     }
             }
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
-            top = fmaxf(top, __shfl_xor(top, 32)) * cs;
+            top = max_x32(top) * cs;
             if (__any(top > m + kLag)) {
                 const float mn = top > m + kLag ? top : m;
                 const float f = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
