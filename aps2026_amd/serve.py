@@ -26,7 +26,7 @@ import numpy as np
 import torch
 
 from . import capi
-from .moe import _call, _require, _stream
+from .moe import _call, _require
 
 MXFP4 = capi.KV_MXFP4
 _CODE = {torch.float32: capi.DTYPE_F32, torch.bfloat16: capi.DTYPE_BF16}
@@ -36,25 +36,28 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """The tensors' device as the current one, for a launch on its stream."""
-
-    def __init__(self, device: torch.device):
-        self.index, self.before = device.index, torch.cuda.current_device()
-
-    def __enter__(self):
-        if self.index != self.before:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.index != self.before:
-            torch.cuda.set_device(self.before)
+# A decode step is a row of short launches, so what Python does around them
+# counts: the stream's handle without an object for it, checks on plain numbers.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _dev(t: torch.Tensor, device: torch.device, dtype: torch.dtype, what: str) -> torch.Tensor:
+def _launch(fn, device: torch.device, *args) -> None:
+    """fn(*args, the current stream of device), with device current."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _call(rc)
+
+
+def _dev(t: torch.Tensor, device: torch.device, dtype: torch.dtype, what: str) -> int:
+    """The address of a contiguous tensor of that type on that device."""
     if t.dtype is not dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: expects a contiguous {dtype} tensor on {device}")
-    return t
+    return t.data_ptr()
 
 
 class PagedKvCache:
@@ -65,25 +68,26 @@ class PagedKvCache:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
-        mx = k_scale is not None or v_scale is not None
-        _require(k.dim() == 4 and k.shape == v.shape and k.dtype is v.dtype and k.is_cuda and v.device == k.device
-                 and k.is_contiguous() and v.is_contiguous(), "paged cache: k and v [pages, kv_heads, page, head_dim]")
-        self.pages, self.kv_heads, self.page_size, width = k.shape
-        self.device = k.device
-        if mx:
-            _require(k.dtype is torch.uint8 and k_scale is not None and v_scale is not None,
+        shape, dt, dev = k.shape, k.dtype, k.device
+        if len(shape) != 4 or v.shape != shape or v.dtype is not dt or dev.type != "cuda" or v.device != dev or \
+                not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("paged cache: k and v [pages, kv_heads, page, head_dim] on a GPU")
+        self.pages, self.kv_heads, self.page_size, self.head_dim = shape
+        if k_scale is not None or v_scale is not None:
+            _require(dt is torch.uint8 and k_scale is not None and v_scale is not None,
                      "paged cache: 4-bit codes are uint8 with k_scale and v_scale")
-            self.head_dim, self.dtype = 2 * width, MXFP4
-            want = (self.pages, self.kv_heads, self.page_size, self.head_dim // 32)
+            self.head_dim *= 2
+            self.dtype = MXFP4
+            want = (*shape[:3], self.head_dim // 32)
             for s in (k_scale, v_scale):
-                _require(tuple(s.shape) == want and s.dtype is torch.uint8 and s.device == self.device
-                         and s.is_contiguous(), f"paged cache: scales {want}")
+                _require(s.shape == want and s.dtype is torch.uint8 and s.device == dev and s.is_contiguous(),
+                         f"paged cache: scales {want}")
         else:
-            _require(k.dtype in _CODE, f"paged cache: dtype {k.dtype}")
-            self.head_dim, self.dtype = width, _CODE[k.dtype]
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self._desc = capi.KvCacheDesc(_p(k), _p(v), _p(k_scale), _p(v_scale), self.pages, self.page_size,
-                                      self.kv_heads, self.head_dim, self.dtype)
+            _require(dt in _CODE, f"paged cache: dtype {dt}")
+            self.dtype = _CODE[dt]
+        self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, dev
+        self._desc = capi.KvCacheDesc(k.data_ptr(), v.data_ptr(), _p(k_scale), _p(v_scale), self.pages,
+                                      self.page_size, self.kv_heads, self.head_dim, self.dtype)
         self._ref = ctypes.byref(self._desc)
 
     @staticmethod
@@ -129,14 +133,14 @@ class PagedBatch:
         self.kv_lens, self.page_table = up(kv, np.int32), up(table, np.int32)
 
 
-def _rows_of(t: torch.Tensor, width: int, what: str) -> torch.Tensor:
-    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
-        raise ValueError(f"{what}: expects rows of {width} neighbouring values")
-    return t
-
-
-def _stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _rows_of(t: torch.Tensor, width: int, what: str) -> int:
+    """The row stride of a matrix whose rows are `width` neighbouring values."""
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == width:
+        row, col = t.stride()
+        if col == 1 or width == 1:
+            return row if shape[0] > 1 or row > width else width
+    raise ValueError(f"{what}: expects rows of {width} neighbouring values")
 
 
 def kv_append_gpu(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
@@ -147,38 +151,36 @@ def kv_append_gpu(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, positio
     head_dim] rotated (into q_out; q itself rotates in place).  cos and sin:
     [positions, head_dim / 2] fp32 (rope_table).  slots int64, -1 for padding
     rows, otherwise distinct; positions int32."""
-    rows, dev = k.shape[0], cache.device
-    width = cache.kv_heads * cache.head_dim
-    _rows_of(k, width, "kv_append")
-    _rows_of(v, width, "kv_append")
-    code = _CODE.get(k.dtype)
-    if code is None or v.dtype is not k.dtype or v.shape[0] != rows or k.device != dev or v.device != dev:
+    what, dev, dim, dt = "kv_append", cache.device, cache.head_dim, k.dtype
+    width, rows = cache.kv_heads * dim, k.shape[0]
+    k_stride, v_stride = _rows_of(k, width, what), _rows_of(v, width, what)
+    code = _CODE.get(dt)
+    if code is None or v.dtype is not dt or v.shape[0] != rows or k.device != dev or v.device != dev:
         raise ValueError("kv_append: k and v of one fp32 or bf16 type on the cache's device")
-    _dev(positions, dev, torch.int32, "kv_append positions")
-    _dev(slots, dev, torch.int64, "kv_append slots")
-    _dev(cos, dev, torch.float32, "kv_append cos")
-    _dev(sin, dev, torch.float32, "kv_append sin")
+    max_pos = cos.shape[0]
     if positions.numel() != rows or slots.numel() != rows or cos.shape != sin.shape or cos.dim() != 2 or \
-            cos.shape[1] * 2 != cache.head_dim:
+            cos.shape[1] * 2 != dim:
         raise ValueError("kv_append shape")
     q_heads = q_stride = o_stride = 0
+    qp = op = None
     if q is not None:
-        if q.dim() != 2 or q.shape[0] != rows or q.shape[1] % cache.head_dim or q.dtype is not k.dtype or \
-                q.device != dev:
+        q_width = q.shape[-1]
+        q_stride = _rows_of(q, q_width, what)
+        if q.shape[0] != rows or q_width % dim or q.dtype is not dt or q.device != dev:
             raise ValueError("kv_append: q [rows, q_heads * head_dim] of k's type")
-        _rows_of(q, q.shape[1], "kv_append")
-        q_heads = q.shape[1] // cache.head_dim
+        q_heads = q_width // dim
         if q_out is None:
-            q_out = torch.empty((rows, q.shape[1]), dtype=q.dtype, device=dev)
-        elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.device != dev:
+            q_out = torch.empty((rows, q_width), dtype=dt, device=dev)
+            o_stride = q_width
+        elif q_out.shape != q.shape or q_out.dtype is not dt or q_out.device != dev:
             raise ValueError("kv_append: q_out of q's shape and type")
         else:
-            _rows_of(q_out, q.shape[1], "kv_append")
-        q_stride, o_stride = _stride(q), _stride(q_out)
-    with _on(dev):
-        _call(capi.lib().aps_kv_append(cache._ref, _p(k), _stride(k), _p(v), _stride(v), _p(q), q_stride, _p(q_out),
-                                       o_stride, code, rows, q_heads, _p(positions), _p(slots), _p(cos), _p(sin),
-                                       cos.shape[0], _stream(dev)))
+            o_stride = _rows_of(q_out, q_width, what)
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    _launch(capi.lib().aps_kv_append, dev, cache._ref, k.data_ptr(), k_stride, v.data_ptr(), v_stride, qp, q_stride,
+            op, o_stride, code, rows, q_heads, _dev(positions, dev, torch.int32, what),
+            _dev(slots, dev, torch.int64, what), _dev(cos, dev, torch.float32, what),
+            _dev(sin, dev, torch.float32, what), max_pos)
     return q_out if q is not None else None
 
 
@@ -187,13 +189,11 @@ def kv_gather_gpu(cache: PagedKvCache, slots: torch.Tensor, out_dtype: torch.dty
     """(k, v) [rows, kv_heads * head_dim] of the slots (int64; zeros for one
     outside the cache), the values of the codes for a 4-bit cache."""
     _require(out_dtype in _CODE, f"kv_gather: dtype {out_dtype}")
-    _dev(slots, cache.device, torch.int64, "kv_gather slots")
-    rows = slots.numel()
+    at, rows = _dev(slots, cache.device, torch.int64, "kv_gather"), slots.numel()
     k = torch.empty((rows, cache.kv_heads * cache.head_dim), dtype=out_dtype, device=cache.device)
     v = torch.empty_like(k)
-    with _on(cache.device):
-        _call(capi.lib().aps_kv_gather(cache._ref, _p(slots), rows, _p(k), _p(v), _CODE[out_dtype],
-                                       _stream(cache.device)))
+    _launch(capi.lib().aps_kv_gather, cache.device, cache._ref, at, rows, k.data_ptr(), v.data_ptr(),
+            _CODE[out_dtype])
     return k, v
 
 
@@ -206,36 +206,37 @@ def attention_paged_gpu(q: torch.Tensor, cache: PagedKvCache, q_offsets: torch.T
     scale: 1 / sqrt(head_dim) unless given.  The workspace is torch's, taken
     on the current stream, unless one is given (uint8).  Rows of a given `out`
     that no sequence names are left as they were."""
-    dev, width = cache.device, q_heads * cache.head_dim
-    _rows_of(q, width, "attention_paged")
-    code = _CODE.get(q.dtype)
+    what, dev, dim = "attention_paged", cache.device, cache.head_dim
+    width = q_heads * dim
+    q_stride = _rows_of(q, width, what)
+    dt = q.dtype
+    code = _CODE.get(dt)
     if code is None or q.device != dev:
         raise ValueError("attention_paged: fp32 or bf16 queries on the cache's device")
-    _dev(q_offsets, dev, torch.int32, "attention_paged q_offsets")
-    _dev(kv_lens, dev, torch.int32, "attention_paged kv_lens")
-    _dev(page_table, dev, torch.int32, "attention_paged page_table")
-    batch, rows = kv_lens.numel(), q.shape[0]
-    if q_offsets.numel() != batch + 1 or page_table.dim() != 2 or page_table.shape[0] != batch:
+    batch, rows, table = kv_lens.numel(), q.shape[0], page_table.shape
+    if q_offsets.numel() != batch + 1 or len(table) != 2 or table[0] != batch:
         raise ValueError("attention_paged shape")
     if out is None:
-        out = torch.empty((rows, width), dtype=q.dtype, device=dev)
-    elif tuple(out.shape) != (rows, width) or out.dtype is not q.dtype or out.device != dev or \
-            not out.is_contiguous():
+        out = torch.empty((rows, width), dtype=dt, device=dev)
+    elif out.shape != (rows, width) or out.dtype is not dt or out.device != dev or not out.is_contiguous():
         raise ValueError("attention_paged: out of q's shape and type, contiguous")
     if scale is None:
-        scale = 1.0 / math.sqrt(cache.head_dim)
-    lib = capi.lib()
+        scale = 1.0 / math.sqrt(dim)
     window = min(window, 0x7FFFFFFF)
+    lib = capi.lib()
     need = lib.aps_attention_paged_workspace_size(cache._ref, rows, q_heads, batch, max_q_len, max_kv_len, window,
                                                   sinks)
-    if need and workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        _call(lib.aps_attention_paged(cache._ref, _p(q), _stride(q), code, rows, q_heads, _p(q_offsets), _p(kv_lens),
-                                      _p(page_table), page_table.shape[1], batch, max_q_len, max_kv_len, window,
-                                      sinks, scale, _p(out), _p(workspace),
-                                      workspace.numel() * workspace.element_size() if workspace is not None else 0,
-                                      _stream(dev)))
+    wp, wn = None, 0
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        elif workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("attention_paged: a contiguous workspace on the cache's device")
+        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch(lib.aps_attention_paged, dev, cache._ref, q.data_ptr(), q_stride, code, rows, q_heads,
+            _dev(q_offsets, dev, torch.int32, what), _dev(kv_lens, dev, torch.int32, what),
+            _dev(page_table, dev, torch.int32, what), table[1], batch, max_q_len, max_kv_len, window, sinks, scale,
+            out.data_ptr(), wp, wn)
     return out
 
 
@@ -252,48 +253,54 @@ def logits_process_gpu(logits: torch.Tensor, history: Optional[torch.Tensor] = N
     of bias_ids [rows, n], and a bit mask [masks, words] (int32 words, bit t %
     32 of word t / 32 allows token t; row r's is mask_index[r], or r).  A rule
     without its arrays is off.  out may be logits itself."""
+    what = "logits_process"
     _require(logits.dim() == 2, "logits_process: logits [rows, vocab]")
     rows, vocab = logits.shape
-    dev, code = logits.device, _CODE.get(logits.dtype)
-    _rows_of(logits, vocab, "logits_process")
-    if code is None or not logits.is_cuda:
+    dev, dt = logits.device, logits.dtype
+    code = _CODE.get(dt)
+    if code is None or dev.type != "cuda":
         raise ValueError("logits_process: fp32 or bf16 logits on a GPU")
+    stride = _rows_of(logits, vocab, what)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
-    elif out.shape != logits.shape or out.dtype is not logits.dtype or out.device != dev:
+        out = torch.empty((rows, vocab), dtype=dt, device=dev)
+    elif out.shape != logits.shape or out.dtype is not dt or out.device != dev:
         raise ValueError("logits_process: out of the logits' shape and type")
+    rules = capi.LogitsRules()
+
+    def each(t, dtype):  # one value a row
+        if t.numel() != rows:
+            raise ValueError("logits_process: one value a row")
+        return _dev(t, dev, dtype, what)
+
+    i32, f32 = torch.int32, torch.float32
+    if history is not None:
+        _require(history.dim() == 2 and history.shape[0] == rows and history_lens is not None,
+                 "logits_process: a history [rows, n] and its history_lens")
+        rules.history, rules.history_lens = _dev(history, dev, i32, what), each(history_lens, i32)
+        rules.history_stride = history.shape[1]
+        if prompt_lens is not None:
+            rules.prompt_lens = each(prompt_lens, i32)
+        if repetition is not None:
+            rules.repetition = each(repetition, f32)
+        if frequency is not None:
+            rules.frequency = each(frequency, f32)
+        if presence is not None:
+            rules.presence = each(presence, f32)
     else:
-        _rows_of(out, vocab, "logits_process")
-
-    def per_row(t, dtype):
-        if t is not None:
-            _dev(t, dev, dtype, "logits_process")
-            _require(t.numel() == rows, "logits_process: one value a row")
-
-    for t in (history_lens, prompt_lens, bias_lens, mask_index):
-        per_row(t, torch.int32)
-    for t in (repetition, frequency, presence):
-        per_row(t, torch.float32)
-    for t, other in ((history, None), (bias_ids, bias_values)):
-        if t is not None:
-            _dev(t, dev, torch.int32, "logits_process")
-            _require(t.dim() == 2 and t.shape[0] == rows, "logits_process: lists [rows, n]")
+        _require(repetition is frequency is presence is None, "logits_process: penalties need a history")
     if bias_ids is not None:
-        _require(bias_values is not None and bias_values.shape == bias_ids.shape and bias_lens is not None,
-                 "logits_process: biases need bias_values of their shape and bias_lens")
-        _dev(bias_values, dev, torch.float32, "logits_process")
-    _require(history_lens is not None if history is not None else repetition is frequency is presence is None,
-             "logits_process: penalties need a history, a history its history_lens")
+        _require(bias_ids.dim() == 2 and bias_ids.shape[0] == rows and bias_lens is not None and
+                 bias_values is not None and bias_values.shape == bias_ids.shape,
+                 "logits_process: biases are bias_ids and bias_values [rows, n] and bias_lens")
+        rules.bias_ids, rules.bias_values = _dev(bias_ids, dev, i32, what), _dev(bias_values, dev, f32, what)
+        rules.bias_lens, rules.bias_stride = each(bias_lens, i32), bias_ids.shape[1]
     if mask is not None:
-        _dev(mask, dev, torch.int32, "logits_process")
         _require(mask.dim() == 2 and mask.shape[1] * 32 >= vocab and (mask_index is not None or mask.shape[0] >= rows),
                  "logits_process: mask [masks, words] with a word for every 32 logits")
-    rules = capi.LogitsRules(
-        _p(history), _p(history_lens), _p(prompt_lens), history.shape[1] if history is not None else 0,
-        _p(repetition), _p(frequency), _p(presence), _p(bias_ids), _p(bias_values), _p(bias_lens),
-        bias_ids.shape[1] if bias_ids is not None else 0, _p(mask), mask.shape[0] if mask is not None else 0,
-        mask.shape[1] if mask is not None else 0, _p(mask_index))
-    with _on(dev):
-        _call(capi.lib().aps_logits_process(_p(logits), _stride(logits), code, rows, vocab, ctypes.byref(rules),
-                                            _p(out), _stride(out), _stream(dev)))
+        rules.mask = _dev(mask, dev, i32, what)
+        rules.mask_rows, rules.mask_stride = mask.shape
+        if mask_index is not None:
+            rules.mask_index = each(mask_index, i32)
+    _launch(capi.lib().aps_logits_process, dev, logits.data_ptr(), stride, code, rows, vocab, ctypes.byref(rules),
+            out.data_ptr(), _rows_of(out, vocab, what))
     return out
