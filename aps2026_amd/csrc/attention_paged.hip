@@ -29,10 +29,11 @@
 // zeros, and where rows differ in what they see, a row that ended in NaN is
 // computed again one key at a time (redo_row), from its own keys alone.
 //
-// Few rows and a long cache: the steps of a tile are split over the four waves
-// of a workgroup and over `splits` workgroups; the waves' (max, sum, O) meet
-// in LDS, the workgroups' in the workspace, joined by k_paged_join.
+// Few rows and a long cache: the steps of a tile are split over the 4 to 8 waves
+// of a workgroup and, past that, over `splits` workgroups; the waves' (max, sum,
+// O) meet in LDS, the workgroups' in the workspace, joined by k_paged_join.
 #include <algorithm>
+#include <type_traits>
 
 #include "serve.hpp"
 
@@ -45,8 +46,10 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
+constexpr int kMostWaves = 8;  // 256 registers a wave
 constexpr int kRows = 16;      // rows of a tile
-constexpr int kMaxSplits = 64;  // one wave reads every split's maximum at once
+constexpr int kMaxSplits = 64;  // k_paged_join: one wave reads every split's maximum at once
+constexpr unsigned kPlainLds = 62 * 1024;  // dynamic LDS that needs no leave: 64 KB less the static part
 constexpr int64_t kTiledRows = 64;  // rows of a sequence under a key head from which k_paged_tiles takes them
 
 // What both kernels know of the launch.
@@ -59,6 +62,8 @@ struct PagedDev {
     int row_tiles;   // tiles (tiled: blocks) of rows a sequence and key head can have
     bool tiled;      // k_paged_tiles, else k_paged_rows
     bool by_rows;    // the waves of a workgroup take a tile each (else a part of the keys each)
+    int waves;       // of a workgroup
+    int lds_rows;    // rows of a tile that can be live: LDS keeps those
     int64_t blocks;  // workgroups
     float scale_log2;
 };
@@ -194,7 +199,7 @@ __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const K
 }
 
 template <int D, bool Q32, Kv KV>
-__global__ void __launch_bounds__(64 * kWaves, KV == Kv::kF32 ? 2 : 3)
+__global__ void __launch_bounds__(64 * kMostWaves, 2)
 k_paged_rows(PagedDev d) {
     constexpr bool FP = KV == Kv::kF32;
     constexpr int HALVES = FP ? 1 : 2;
@@ -204,15 +209,16 @@ k_paged_rows(PagedDev d) {
     constexpr int PT = Q32 ? 3 : 2;    // bf16 terms of a weight
     constexpr int KS = D / 32;         // MFMA steps over the dims
     constexpr int OSTRIDE = D + 4;     // LDS row, off the banks' period
-    __shared__ float sm_o[kWaves][kRows][OSTRIDE];
-    __shared__ float sm_m[kWaves][kRows], sm_l[kWaves][kRows];
+    __shared__ float sm_m[kMostWaves][kRows], sm_l[kMostWaves][kRows];
+    extern __shared__ __align__(16) float sm_o[];  // [waves][lds_rows][OSTRIDE]
+    auto o_row = [&](int w, int r) { return sm_o + (w * d.lds_rows + r) * OSTRIDE; };
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     uint32_t id = blockIdx.x;
     const int split = id % d.splits;
     id /= d.splits;
-    const int per = d.by_rows ? kWaves : 1;
+    const int per = d.by_rows ? d.waves : 1;
     const uint32_t row_blocks = (d.row_tiles + per - 1) / per;
     // the last rows see the most keys: they start first
     const int rb = static_cast<int>(row_blocks - 1 - id % row_blocks);
@@ -222,7 +228,7 @@ k_paged_rows(PagedDev d) {
     const Seq sq = sequence(d, b);
     const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
     const int nrows = static_cast<int>(qlen * d.group);
-    const int r0 = (d.by_rows ? rb * kWaves + wave : rb) * kRows;
+    const int r0 = (d.by_rows ? rb * d.waves + wave : rb) * kRows;
     const bool any = r0 < nrows;
     if (!d.by_rows && !any) return;  // the whole workgroup
     const int32_t* table = d.a.page_table + b * d.a.table_stride;
@@ -235,7 +241,7 @@ k_paged_rows(PagedDev d) {
     const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
     const int pos = live ? p0 + tok : -1;
     const Keys ks = visible<STEP>(d, pmin, pmax);
-    const int parts = d.splits * (d.by_rows ? 1 : kWaves), part = d.by_rows ? split : split * kWaves + wave;
+    const int parts = d.splits * (d.by_rows ? 1 : d.waves), part = d.by_rows ? split : split * d.waves + wave;
     const int each = (ks.steps + parts - 1) / parts;
     const int t0 = part * each < ks.steps ? part * each : ks.steps;
     const int t1 = t0 + each < ks.steps ? t0 + each : ks.steps;
@@ -281,114 +287,135 @@ k_paged_rows(PagedDev d) {
     const View vis = view(d, pos);
     constexpr int AHEAD = 64 / HALVES;  // steps whose pages the lanes hold
     int pages = -1;
-    for (int t = t0; t < t1; ++t) {
+    // what a lane reads of a step: its part of K, of V, and 4-bit scale bytes
+    constexpr bool MX = KV == Kv::kMx;
+    constexpr int KW = FP ? D / 4 : MX ? 2 * KS : 8 * KS;   // words
+    constexpr int VW = FP ? 4 * W : MX ? 8 : 4 * W;
+    struct Step {
+        bool dead[HALVES];  // no page
+        uint32_t k[KW], v[VW], ks[MX ? 2 : 1], vs[MX ? 8 : 1];
+    };
+    auto words = [](const void* p, auto n, uint32_t* to) {
+        constexpr int N = decltype(n)::value;
+        if constexpr (N == 4) {
+            const u32x4 w = *static_cast<const u32x4*>(p);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) to[x] = w[x];
+        } else {
+            const u32x2 w = *static_cast<const u32x2*>(p);
+            to[0] = w[0];
+            to[1] = w[1];
+        }
+    };
+    using Four = std::integral_constant<int, 4>;
+    auto load = [&](int t, Step& st) {
         const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
         const int slot = (t - t0) % AHEAD;
         if (slot == 0) pages = page_of<STEP>(d, table, ks, t + lane / HALVES, t1, lane % HALVES);
-        bool dead[HALVES];
-        int64_t hrow[HALVES];  // (page, head, offset) row of the half's first key
+        const auto* kb = static_cast<const uint8_t*>(d.c.k);
+        const auto* vb = static_cast<const uint8_t*>(d.c.v);
 #pragma unroll
         for (int a = 0; a < HALVES; ++a) {
             const int page = __builtin_amdgcn_readlane(pages, slot * HALVES + a);
-            dead[a] = page < 0;
-            hrow[a] = ((static_cast<int64_t>(dead[a] ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
-                      ((base + 16 * a) & ((1 << d.page_shift) - 1));
+            st.dead[a] = page < 0;
+            // (page, head, offset) row of the half's first key
+            const int64_t hrow = ((static_cast<int64_t>(page < 0 ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
+                                 ((base + 16 * a) & ((1 << d.page_shift) - 1));
+            if constexpr (FP) {
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s) words(kb + (hrow + c) * (4 * D) + 64 * s + 16 * g, Four(), st.k + 4 * s);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int x = 0; x < W; x += 4)
+                        words(vb + (hrow + 4 * g + i) * (4 * D) + 4 * (W * c + x), Four(), st.v + W * i + x);
+            } else if constexpr (!MX) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    words(kb + (hrow + c) * (2 * D) + 64 * s + 16 * g, Four(), st.k + 4 * (KS * a + s));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    words(vb + (hrow + 4 * g + i) * (2 * D) + 2 * W * c,
+                          std::integral_constant<int, W / 2>(), st.v + (W / 2) * (4 * a + i));
+            } else {
+                // D / 4 neighbouring dims of a key of K: one block's, or half a block's
+                words(kb + (hrow + c) * (D / 2) + (D / 8) * g, std::integral_constant<int, KS>(), st.k + KS * a);
+                st.ks[a] = d.c.k_scale[(hrow + c) * (D / 32) + (D / 4) * g / 32];
+                const uint8_t* vp = vb + (hrow + 4 * g) * (D / 2) + (W / 2) * c;
+                const uint8_t* sp = d.c.v_scale + (hrow + 4 * g) * (D / 32) + W * c / 32;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (W == 8) st.v[4 * a + i] = *reinterpret_cast<const uint32_t*>(vp + i * (D / 2));
+                    else st.v[4 * a + i] = *reinterpret_cast<const uint16_t*>(vp + i * (D / 2));
+                    st.vs[4 * a + i] = sp[i * (D / 32)];
+                }
+            }
         }
+    };
+
+    // A step is read one ahead (37 x 2051 fp32 keys 80 -> 63 us, 64 x 8192 bf16 154
+    // -> 148), except of a 4-bit cache, whose steps are short and whose decoding
+    // wants the registers for a third or fourth wave (64 x 16384 keys 92, read
+    // ahead 96).
+    constexpr bool EARLY = !MX;
+    Step next;
+    if (EARLY && t0 < t1) load(t0, next);
+    for (int t = t0; t < t1; ++t) {
+        const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
+        Step st;
+        if constexpr (EARLY) {
+            st = next;
+            if (t + 1 < t1) load(t + 1, next);
+        } else {
+            load(t, st);
+        }
+        const auto& dead = st.dead;
         f32x4 s4[HALVES];
         float vf[FP ? 4 : 1][W];
         uint32_t vw[FP ? 1 : 8][FP ? 1 : W / 2];  // two dims of a key to a word
         if constexpr (FP) {
-            const float* kp = static_cast<const float*>(d.c.k) + (hrow[0] + c) * D + 4 * g;
-            f32x4 kf[D / 16];
-#pragma unroll
-            for (int s = 0; s < D / 16; ++s) kf[s] = *reinterpret_cast<const f32x4*>(kp + 16 * s);
-            const float* vp = static_cast<const float*>(d.c.v) + (hrow[0] + 4 * g) * D + W * c;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int x = 0; x < W; x += 4) {
-                    const f32x4 w = *reinterpret_cast<const f32x4*>(vp + i * D + x);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) vf[i][x + y] = w[y];
-                }
+                for (int x = 0; x < W; ++x) vf[i][x] = __uint_as_float(st.v[W * i + x]);
             s4[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < D / 16; ++s)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    s4[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[s][e], qf[s][e], s4[0], 0, 0, 0);
+                    s4[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(st.k[4 * s + e]), qf[s][e], s4[0], 0,
+                                                                  0, 0);
         } else {
             bf16x8 kb[HALVES][KS];
-            if constexpr (KV == Kv::kBf16) {
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const bf16_t* kp = static_cast<const bf16_t*>(d.c.k) + (hrow[a] + c) * D + 8 * g;
+            for (int a = 0; a < 2; ++a)
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) kb[a][s] = *reinterpret_cast<const bf16x8*>(kp + 32 * s);
-                }
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const bf16_t* vp = static_cast<const bf16_t*>(d.c.v) + (hrow[a] + 4 * g) * D + W * c;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (W == 8) {
-                            const u32x4 w = *reinterpret_cast<const u32x4*>(vp + i * D);
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) vw[4 * a + i][x] = w[x];
-                        } else {
-                            const u32x2 w = *reinterpret_cast<const u32x2*>(vp + i * D);
-                            vw[4 * a + i][0] = w[0];
-                            vw[4 * a + i][1] = w[1];
-                        }
-                    }
-                }
-            } else {
-                // a lane reads D / 4 neighbouring dims of a key: one block's, or half a block's
-                uint32_t kw[2][KS], ksc[2], vc[8], vsc[8];
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const uint8_t* kp = static_cast<const uint8_t*>(d.c.k) + (hrow[a] + c) * (D / 2) + (D / 8) * g;
-                    if constexpr (KS == 4) {
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) kw[a][s] = w[s];
+                for (int s = 0; s < KS; ++s) {
+                    u32x4 w;
+                    if constexpr (MX) {
+                        const float sc = mx_scale(st.ks[a]);
+                        const uint32_t code = st.k[KS * a + s];
+                        w = u32x4{mx_decode2<0>(code, sc), mx_decode2<1>(code, sc), mx_decode2<2>(code, sc),
+                                  mx_decode2<3>(code, sc)};
                     } else {
-                        const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
-                        kw[a][0] = w[0];
-                        kw[a][1] = w[1];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) w[x] = st.k[4 * (KS * a + s) + x];
                     }
-                    ksc[a] = d.c.k_scale[(hrow[a] + c) * (D / 32) + (D / 4) * g / 32];
+                    kb[a][s] = __builtin_bit_cast(bf16x8, w);
                 }
 #pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const uint8_t* vp = static_cast<const uint8_t*>(d.c.v) + (hrow[a] + 4 * g) * (D / 2) + (W / 2) * c;
-                    const uint8_t* sp = d.c.v_scale + (hrow[a] + 4 * g) * (D / 32) + W * c / 32;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if constexpr (W == 8) vc[4 * a + i] = *reinterpret_cast<const uint32_t*>(vp + i * (D / 2));
-                        else vc[4 * a + i] = *reinterpret_cast<const uint16_t*>(vp + i * (D / 2));
-                        vsc[4 * a + i] = sp[i * (D / 32)];
-                    }
-                }
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const float sc = mx_scale(ksc[a]);
-#pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        const u32x4 w = {mx_decode2<0>(kw[a][s], sc), mx_decode2<1>(kw[a][s], sc),
-                                         mx_decode2<2>(kw[a][s], sc), mx_decode2<3>(kw[a][s], sc)};
-                        kb[a][s] = __builtin_bit_cast(bf16x8, w);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float sc = mx_scale(vsc[j]);
-                    vw[j][0] = mx_decode2<0>(vc[j], sc);
-                    vw[j][1] = mx_decode2<1>(vc[j], sc);
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (MX) {
+                    const float sc = mx_scale(st.vs[j]);
+                    vw[j][0] = mx_decode2<0>(st.v[j], sc);
+                    vw[j][1] = mx_decode2<1>(st.v[j], sc);
                     if constexpr (W == 8) {
-                        vw[j][2] = mx_decode2<2>(vc[j], sc);
-                        vw[j][3] = mx_decode2<3>(vc[j], sc);
+                        vw[j][2] = mx_decode2<2>(st.v[j], sc);
+                        vw[j][3] = mx_decode2<3>(st.v[j], sc);
                     }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < W / 2; ++x) vw[j][x] = st.v[(W / 2) * j + x];
                 }
             }
 #pragma unroll
@@ -490,7 +517,7 @@ k_paged_rows(PagedDev d) {
         for (int t = 0; t < W; t += 4) {
             const f32x4 v = {acc[t][i], acc[t + 1][i], acc[t + 2][i], acc[t + 3][i]};
             nan = nan || v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3];
-            *reinterpret_cast<f32x4*>(&sm_o[wave][c][W * (4 * g + i) + t]) = v;
+            if (c < d.lds_rows) *reinterpret_cast<f32x4*>(o_row(wave, c) + W * (4 * g + i) + t) = v;
         }
     if (g == 0) { sm_m[wave][c] = m; sm_l[wave][c] = l; }
     if (any && pmin != pmax) {
@@ -501,7 +528,7 @@ k_paged_rows(PagedDev d) {
             rows &= rows - 1;
             const int rr = r0 + x;
             redo_row<D, Q32, KV, STEP>(d, table, h, ks, t0, t1, sq.q0 + rr / d.group, h * d.group + rr % d.group,
-                                       p0 + rr / d.group, sm_o[wave][x], &sm_m[wave][x], &sm_l[wave][x]);
+                                       p0 + rr / d.group, o_row(wave, x), &sm_m[wave][x], &sm_l[wave][x]);
         }
     }
     __syncthreads();
@@ -509,10 +536,10 @@ k_paged_rows(PagedDev d) {
     // join the waves' parts (by_rows: each wave has rows of its own) and write
     // the result, or the workgroup's part of it
     constexpr int TPR = D / 8;                 // threads of a row, 8 dims each
-    const int tiles = d.by_rows ? kWaves : 1, parts_w = d.by_rows ? 1 : kWaves;
-    for (int x = threadIdx.x; x < tiles * kRows * TPR; x += 64 * kWaves) {
+    const int tiles = d.by_rows ? d.waves : 1, parts_w = d.by_rows ? 1 : d.waves;
+    for (int x = threadIdx.x; x < tiles * kRows * TPR; x += 64 * d.waves) {
         const int dim = 8 * (x % TPR), rt = x / TPR / kRows, rc = x / TPR % kRows;
-        const int rr = (d.by_rows ? rb * kWaves + rt : rb) * kRows + rc;
+        const int rr = (d.by_rows ? rb * d.waves + rt : rb) * kRows + rc;
         if (rr >= nrows) continue;
         float mm = -INFINITY;
         for (int w = 0; w < parts_w; ++w) mm = fmaxf(mm, sm_m[d.by_rows ? rt : w][rc]);
@@ -523,7 +550,7 @@ k_paged_rows(PagedDev d) {
             const float f = exp2_fast(sm_m[sl][rc] - ref);
             ll = fmaf(sm_l[sl][rc], f, ll);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = fmaf(sm_o[sl][rc][dim + j], f, o[j]);
+            for (int j = 0; j < 8; ++j) o[j] = fmaf(o_row(sl, rc)[dim + j], f, o[j]);
         }
         const int64_t orow = (sq.q0 + rr / d.group) * d.a.q_heads + h * d.group + rr % d.group;
         if (d.splits > 1) {
@@ -920,13 +947,14 @@ k_paged_tiles(PagedDev d) {
 }
 
 // out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits of one
-// (row, head), a wave each.  Rows that no sequence names are not touched: the
+// (row, head), a workgroup each.  Rows that no sequence names are not touched: the
 // grid walks the sequences.
-template <int D, bool Q32>
-__global__ void __launch_bounds__(64)
+template <int D, bool Q32, int JW>
+__global__ void __launch_bounds__(64 * JW)
 k_paged_join(PagedDev d) {
     constexpr int PER = D / 64;
-    const int lane = threadIdx.x;
+    __shared__ float part[JW][D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t id = blockIdx.x;
     const int head = id % d.a.q_heads;
     id /= d.a.q_heads;
@@ -936,6 +964,8 @@ k_paged_join(PagedDev d) {
     const int64_t orow = (sq.q0 + tok) * d.a.q_heads + head, at = orow * d.splits;
     const float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
     const float m = lane < d.splits ? ml[2 * lane] : -INFINITY, l = lane < d.splits ? ml[2 * lane + 1] : 0.0f;
+    const float* po = d.a.part + at * D + PER * lane;
+    float o[PER] = {};
     float top = m;
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
@@ -943,12 +973,20 @@ k_paged_join(PagedDev d) {
     float sum = w * l;
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
-    float o[PER] = {};
-    const float* po = d.a.part + at * D + PER * lane;
-    for (int s = 0; s < d.splits; ++s) {
-        const float ws = __shfl(w, s);
+    for (int s = wave; s < d.splits; s += JW) {
+        const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
 #pragma unroll
         for (int j = 0; j < PER; ++j) o[j] = fmaf(ws, po[static_cast<int64_t>(s) * D + j], o[j]);
+    }
+    if constexpr (JW > 1) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) part[wave][PER * lane + j] = o[j];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int x = 1; x < JW; ++x)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) o[j] += part[x][PER * lane + j];
     }
     const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
@@ -959,7 +997,7 @@ k_paged_join(PagedDev d) {
     }
 }
 
-PagedDev plan(const KvCache& c, const PagedArgs& a) {
+PagedDev plan(const KvCache& c, const PagedArgs& a, bool q_f32) {
     PagedDev d;
     d.a = a;
     d.c = c;
@@ -971,16 +1009,31 @@ PagedDev plan(const KvCache& c, const PagedArgs& a) {
     const int64_t keys = std::min<int64_t>(a.max_kv_len, static_cast<int64_t>(a.window) + a.sinks + 16);
     const int64_t steps = ceil_div(keys, 32);
     d.tiled = c.type != Kv::kF32 && rows >= kTiledRows;
-    int64_t splits;
+    int64_t splits = 1;
+    d.by_rows = false;
+    d.waves = kWaves;
+    d.lds_rows = kRows;
     if (d.tiled) {
-        d.by_rows = false;
         d.row_tiles = static_cast<int>(ceil_div(rows, kBlockRows));
         splits = std::min<int64_t>(ceil_div(512, heads * d.row_tiles), ceil_div(steps, 8));
     } else {
         d.row_tiles = static_cast<int>(ceil_div(rows, kRows));
         d.by_rows = d.row_tiles >= kWaves;
-        const int64_t blocks = heads * ceil_div(d.row_tiles, d.by_rows ? kWaves : 1);
-        splits = std::min<int64_t>(ceil_div(1024, blocks), ceil_div(steps, d.by_rows ? 8 : 2 * kWaves));
+        if (d.by_rows) {
+            splits = std::min<int64_t>(ceil_div(1024, heads * ceil_div(d.row_tiles, kWaves)), ceil_div(steps, 8));
+        } else {
+            const int64_t tiles = heads * d.row_tiles;
+            splits = std::min<int64_t>(ceil_div(1024, tiles), ceil_div(steps, 2 * kWaves));
+            if (splits > 1 && steps <= 4 * kMostWaves) {
+                // short: one larger workgroup instead of a second launch
+                d.waves = kMostWaves;
+                splits = 1;
+            } else if (splits > kMaxSplits) {
+                d.waves = kMostWaves;
+                splits = kMaxSplits;
+            }
+            d.lds_rows = static_cast<int>(std::min<int64_t>(kRows, rows));
+        }
     }
     d.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
     d.blocks = heads * d.splits * (d.tiled || !d.by_rows ? d.row_tiles : ceil_div(d.row_tiles, kWaves));
@@ -997,10 +1050,20 @@ hipError_t launch(const PagedDev& d, hipStream_t s) {
             hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)),
                                block, 0, s, d);
     }
-    if (!d.tiled)
-        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)), block, 0, s, d);
-    if (d.splits > 1)
-        hipLaunchKernelGGL((k_paged_join<D, Q32>), dim3(static_cast<unsigned>(joins)), dim3(64), 0, s, d);
+    if (!d.tiled) {
+        const unsigned lds = static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4;
+        if (lds > kPlainLds) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_rows<D, Q32, KV>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                     static_cast<int>(lds));
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)), dim3(64 * d.waves), lds,
+                           s, d);
+    }
+    const dim3 grid(static_cast<unsigned>(joins));
+    if (d.splits > 16) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
+    else if (d.splits > 1) hipLaunchKernelGGL((k_paged_join<D, Q32, 1>), grid, dim3(64), 0, s, d);
     return hipGetLastError();
 }
 
@@ -1014,14 +1077,14 @@ hipError_t launch_d(const PagedDev& d, bool q_f32, hipStream_t s) {
 
 }  // namespace
 
-size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a) {
-    const PagedDev d = plan(cache, a);
+size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a, bool q_f32) {
+    const PagedDev d = plan(cache, a, q_f32);
     return d.splits > 1 ? static_cast<size_t>(a.rows) * a.q_heads * d.splits * (cache.head_dim + 2) * 4 : 0;
 }
 
 hipError_t launch_attention_paged(const KvCache& cache, const PagedArgs& a, bool q_f32, hipStream_t s) {
     if (a.rows <= 0 || a.batch <= 0 || a.max_q_len <= 0) return hipSuccess;
-    const PagedDev d = plan(cache, a);
+    const PagedDev d = plan(cache, a, q_f32);
     return cache.head_dim == 128 ? launch_d<128>(d, q_f32, s) : launch_d<64>(d, q_f32, s);
 }
 
