@@ -50,7 +50,7 @@ constexpr int kMostWaves = 8;  // 256 registers a wave
 constexpr int kRows = 16;      // rows of a tile
 constexpr int kMaxSplits = 64;  // k_paged_join: one wave reads every split's maximum at once
 constexpr unsigned kPlainLds = 62 * 1024;  // dynamic LDS that needs no leave: 64 KB less the static part
-constexpr int64_t kTiledRows = 64;  // rows of a sequence under a key head from which k_paged_tiles takes them
+constexpr int64_t kTiledRows = 33;  // rows of a sequence under a key head from which k_paged_tiles takes them
 
 // What both kernels know of the launch.
 struct PagedDev {
@@ -603,13 +603,12 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTileRows = 32;            // rows of a wave
 constexpr int kBlockRows = kWaves * kTileRows;
-constexpr int kTileKeys = 64;            // keys of a step
 constexpr float kLag = 8.0f;
 
-template <int D>
-__device__ inline int k_swizzle(int key) { return D == 128 ? key & 15 : (key >> 1) & 7; }
-template <int D>
-__device__ inline int v_swizzle(int key) { return D == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
+template <int D, bool FP>
+__device__ inline int k_swizzle(int key) { return FP || D == 128 ? key & 15 : (key >> 1) & 7; }
+template <int D, bool FP>
+__device__ inline int v_swizzle(int key) { return FP ? 0 : D == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2; }
 
 #define APS_AGP(p) ((const __attribute__((address_space(1))) void*)(p))
 #define APS_ALP(p) ((__attribute__((address_space(3))) void*)(p))
@@ -617,11 +616,16 @@ __device__ inline int v_swizzle(int key) { return D == 128 ? (key & 3) << 2 : ((
 template <int D, bool Q32, Kv KV>
 __global__ void __launch_bounds__(64 * kWaves, 2)
 k_paged_tiles(PagedDev d) {
-    constexpr int ROW = 2 * D;                 // LDS bytes of a key
+    constexpr bool FP = KV == Kv::kF32;
+    constexpr int KEYS = FP ? 32 : 64;         // keys of a step
+    constexpr int U = KEYS / 32;               // 32-key halves of it
+    constexpr int GROUPS = KEYS / 16;          // 16-key groups, each of one page
+    constexpr int ROW = (FP ? 4 : 2) * D;      // LDS bytes of a key
     constexpr int CH = ROW / 16;               // 16-byte chunks of a key
     constexpr int QT = Q32 ? 3 : 1, PT = Q32 ? 3 : 1;
-    constexpr int KS = D / 16, DT = D / 32;
-    __shared__ __align__(1024) uint8_t sm[2][2][kTileKeys * ROW];  // [buffer][k, v]
+    constexpr int KS = D / (FP ? 8 : 16);      // chunks of a lane: its half of a key's dims
+    constexpr int DT = D / 32;
+    __shared__ __align__(1024) uint8_t sm[2][2][KEYS * ROW];  // [k, v][buffer]
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
@@ -643,7 +647,7 @@ k_paged_tiles(PagedDev d) {
     const int32_t* table = d.a.page_table + b * d.a.table_stride;
     const int p0 = sq.kv - sq.len;
     const int rb1 = (rb0 + kBlockRows < nrows ? rb0 + kBlockRows : nrows) - 1;
-    const Keys ks = visible<kTileKeys>(d, p0 + rb0 / d.group, p0 + rb1 / d.group);
+    const Keys ks = visible<KEYS>(d, p0 + rb0 / d.group, p0 + rb1 / d.group);
     const int each = (ks.steps + d.splits - 1) / d.splits;
     const int t0 = split * each < ks.steps ? split * each : ks.steps;
     const int t1 = t0 + each < ks.steps ? t0 + each : ks.steps;
@@ -659,15 +663,25 @@ k_paged_tiles(PagedDev d) {
 
     // queries: a lane holds dims 16 s + 8 hf + j of its row; the sign of the
     // scale goes into them, so that the largest product is the largest score
-    bf16x8 qb[QT][KS];
+    bf16x8 qb[FP ? 1 : QT][FP ? 1 : KS];
+    f32x4 qf[FP ? KS : 1];
     const float cs = d.scale_log2 == 0.0f ? 1.0f : fabsf(d.scale_log2);
-    const uint32_t flip = d.scale_log2 < 0.0f ? 0x80008000u : 0u, keep = d.scale_log2 == 0.0f ? 0u : ~0u;
+    const uint32_t flip = d.scale_log2 < 0.0f ? (FP ? 0x80000000u : 0x80008000u) : 0u;
+    const uint32_t keep = d.scale_log2 == 0.0f ? 0u : ~0u;
     {
         const int64_t qat = (sq.q0 + tok) * d.a.q_stride + static_cast<int64_t>(qh) * D;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const int dim = 16 * s + 8 * hf;
-            if constexpr (Q32) {
+            const int dim = (FP ? 8 : 16) * s + (FP ? 4 : 8) * hf;
+            if constexpr (FP) {
+                u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const float*>(d.a.q) + qat + dim);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
+                qf[s] = __builtin_bit_cast(f32x4, w);
+                continue;
+            }
+            if constexpr (FP) {
+            } else if constexpr (Q32) {
                 const float* p = static_cast<const float*>(d.a.q) + qat + dim;
                 const f32x4 x0 = *reinterpret_cast<const f32x4*>(p), x1 = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
@@ -693,79 +707,77 @@ k_paged_tiles(PagedDev d) {
         }
     }
 
-    // ---- staging: a wave takes the step's keys 16 wave .. 16 wave + 15
-    auto base_of = [&](int t) { return (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * kTileKeys; };
+    // ---- staging, one step ahead.  64 keys: a wave copies 16 keys of K and of V;
+    // 32 keys: two waves copy K, two V.
+    const int grp = wave % GROUPS;
+    const bool with_k = GROUPS == kWaves || wave < GROUPS, with_v = GROUPS == kWaves || wave >= GROUPS;
+    auto base_of = [&](int t) { return (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * KEYS; };
     u32x4 mk{}, mv{};
     uint32_t mks = 0, mvs = 0;
-    int pages = -1;         // lane 4 i + a: the page of 16 keys a of step i of sixteen
+    int pages = -1;          // lane GROUPS i + a: the page of 16 keys a of step i of 64 / GROUPS
     uint32_t dead_next = 0;  // bit a: 16 keys a of the step that was fetched have no page
-    auto fetch = [&](int t, int buf) {
-        const int slot = (t - t0) & 15;
-        if (slot == 0) pages = page_of<kTileKeys>(d, table, ks, t + lane / 4, t1, lane & 3);
-        dead_next = static_cast<uint32_t>(__ballot(pages < 0) >> (4 * slot)) & 15u;
-        const int key = base_of(t) + 16 * wave;
-        const int page = __builtin_amdgcn_readlane(pages, 4 * slot + wave);
-        const int64_t hrow = ((static_cast<int64_t>(page < 0 ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
-                             (key & ((1 << d.page_shift) - 1));
-        if constexpr (KV == Kv::kBf16) {
+    auto fetch1 = [&](int which, int64_t hrow, int buf) {  // one operand's 16 keys, to LDS or (4 bits) to registers
+        const uint8_t* src = static_cast<const uint8_t*>(which ? d.c.v : d.c.k);
+        if constexpr (KV != Kv::kMx) {
+            src += hrow * ROW;
             constexpr int RPI = 1024 / ROW;  // keys of one copy
-            const uint8_t* kp = static_cast<const uint8_t*>(d.c.k) + hrow * ROW;
-            const uint8_t* vp = static_cast<const uint8_t*>(d.c.v) + hrow * ROW;
 #pragma unroll
             for (int i = 0; i < 16 / RPI; ++i) {
-                const int r = RPI * i + lane / CH, ph = lane % CH;
-                __builtin_amdgcn_global_load_lds(APS_AGP(kp + r * ROW + ((ph ^ k_swizzle<D>(r)) << 4)),
-                                                 APS_ALP(&sm[buf][0][(16 * wave + RPI * i) * ROW]), 16, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 16 / RPI; ++i) {
-                const int r = RPI * i + lane / CH, ph = lane % CH;
-                __builtin_amdgcn_global_load_lds(APS_AGP(vp + r * ROW + ((ph ^ v_swizzle<D>(r)) << 4)),
-                                                 APS_ALP(&sm[buf][1][(16 * wave + RPI * i) * ROW]), 16, 0, 0);
+                const int r = RPI * i + lane / CH;
+                const int chunk = (lane % CH) ^ (which ? v_swizzle<D, FP>(r) : k_swizzle<D, FP>(r));
+                __builtin_amdgcn_global_load_lds(APS_AGP(src + r * ROW + 16 * chunk),
+                                                 APS_ALP(&sm[which][buf][(16 * grp + RPI * i) * ROW]), 16, 0, 0);
             }
         } else {
             const int64_t at = hrow + lane / 4;  // four lanes a key
-            const uint8_t* kp = static_cast<const uint8_t*>(d.c.k) + at * (D / 2) + (lane & 3) * (D / 8);
-            const uint8_t* vp = static_cast<const uint8_t*>(d.c.v) + at * (D / 2) + (lane & 3) * (D / 8);
+            src += at * (D / 2) + (lane & 3) * (D / 8);
+            u32x4& w = which ? mv : mk;
             if constexpr (D == 128) {
-                mk = *reinterpret_cast<const u32x4*>(kp);
-                mv = *reinterpret_cast<const u32x4*>(vp);
+                w = *reinterpret_cast<const u32x4*>(src);
             } else {
-                const u32x2 a = *reinterpret_cast<const u32x2*>(kp), w = *reinterpret_cast<const u32x2*>(vp);
-                mk = u32x4{a[0], a[1], 0u, 0u};
-                mv = u32x4{w[0], w[1], 0u, 0u};
+                const u32x2 half = *reinterpret_cast<const u32x2*>(src);
+                w = u32x4{half[0], half[1], 0u, 0u};
             }
-            mks = d.c.k_scale[at * (D / 32) + (lane & 3) * (D / 4) / 32];
-            mvs = d.c.v_scale[at * (D / 32) + (lane & 3) * (D / 4) / 32];
+            (which ? mvs : mks) = (which ? d.c.v_scale : d.c.k_scale)[at * (D / 32) + (lane & 3) * (D / 4) / 32];
+        }
+    };
+    auto fetch = [&](int t, int buf) {
+        const int slot = (t - t0) % (64 / GROUPS);
+        if (slot == 0) pages = page_of<KEYS>(d, table, ks, t + lane / GROUPS, t1, lane % GROUPS);
+        dead_next = static_cast<uint32_t>(__ballot(pages < 0) >> (GROUPS * slot)) & ((1u << GROUPS) - 1);
+        const int page = __builtin_amdgcn_readlane(pages, GROUPS * slot + grp);
+        const int64_t hrow = ((static_cast<int64_t>(page < 0 ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
+                             ((base_of(t) + 16 * grp) & ((1 << d.page_shift) - 1));
+        if (with_k) fetch1(0, hrow, buf);
+        if (with_v) fetch1(1, hrow, buf);
+    };
+    auto decode1 = [&](int which, int buf) {
+        const int r = lane / 4;
+        const u32x4 w = which ? mv : mk;
+        const float sc = mx_scale(which ? mvs : mks);
+        uint8_t* at = &sm[which][buf][(16 * grp + r) * ROW];
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            const int chunk = ((lane & 3) * (D / 32) + j) ^ (which ? v_swizzle<D, FP>(r) : k_swizzle<D, FP>(r));
+            *reinterpret_cast<u32x4*>(at + 16 * chunk) = u32x4{mx_decode2<0>(w[j], sc), mx_decode2<1>(w[j], sc),
+                                                               mx_decode2<2>(w[j], sc), mx_decode2<3>(w[j], sc)};
         }
     };
     auto commit = [&](int t, int buf) {
-        const int key0 = base_of(t) + 16 * wave;
         if constexpr (KV == Kv::kMx) {
-            const int r = lane / 4;
-            const float sk = mx_scale(mks), sv = mx_scale(mvs);
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-                const int chunk = (lane & 3) * (D / 32) + j;
-                uint8_t* at = &sm[buf][0][(16 * wave + r) * ROW];
-                *reinterpret_cast<u32x4*>(at + ((chunk ^ k_swizzle<D>(r)) << 4)) =
-                    u32x4{mx_decode2<0>(mk[j], sk), mx_decode2<1>(mk[j], sk), mx_decode2<2>(mk[j], sk),
-                          mx_decode2<3>(mk[j], sk)};
-                at = &sm[buf][1][(16 * wave + r) * ROW];
-                *reinterpret_cast<u32x4*>(at + ((chunk ^ v_swizzle<D>(r)) << 4)) =
-                    u32x4{mx_decode2<0>(mv[j], sv), mx_decode2<1>(mv[j], sv), mx_decode2<2>(mv[j], sv),
-                          mx_decode2<3>(mv[j], sv)};
-            }
+            if (with_k) decode1(0, buf);
+            if (with_v) decode1(1, buf);
         } else {
             __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies are in LDS
         }
         // values that no row of the block sees become zeros
-        const bool gone = dead_next >> wave & 1u;
+        const int key0 = base_of(t) + 16 * grp;
+        const bool gone = dead_next >> grp & 1u;
         const bool whole = !gone && key0 + 15 < ks.hi && (key0 >= ks.lo || key0 + 15 < ks.first);
-        if (!whole) {
+        if (with_v && !whole) {
             const int r = lane / 4, key = key0 + r;
             if (gone || key >= ks.hi || (key < ks.lo && key >= ks.first)) {
-                u32x4* at = reinterpret_cast<u32x4*>(&sm[buf][1][(16 * wave + r) * ROW + (lane & 3) * (ROW / 4)]);
+                u32x4* at = reinterpret_cast<u32x4*>(&sm[1][buf][(16 * grp + r) * ROW + (lane & 3) * (ROW / 4)]);
 #pragma unroll
                 for (int j = 0; j < ROW / 64; ++j) at[j] = u32x4{0u, 0u, 0u, 0u};
             }
@@ -775,12 +787,12 @@ k_paged_tiles(PagedDev d) {
     // LDS offsets of a lane's operands
     int k_off[KS], v_off[DT];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k_off[s] = c * ROW + (((2 * s + hf) ^ k_swizzle<D>(c)) << 4);
+    for (int s = 0; s < KS; ++s) k_off[s] = c * ROW + (((2 * s + hf) ^ k_swizzle<D, FP>(c)) << 4);
     {
         const int i = lane & 15, r = i >> 2, dh = (lane >> 4) & 1;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
-            v_off[t] = (4 * hf + r) * ROW + (((4 * t + 2 * dh + ((i & 3) >> 1)) ^ v_swizzle<D>(r)) << 4) + 8 * (i & 1);
+            v_off[t] = (4 * hf + r) * ROW + (((4 * t + 2 * dh + ((i & 3) >> 1)) ^ v_swizzle<D, FP>(r)) << 4) + 8 * (i & 1);
     }
 
     f32x16 acc[DT];
@@ -801,34 +813,41 @@ k_paged_tiles(PagedDev d) {
         if (t + 1 < t1) fetch(t + 1, buf ^ 1);
         // a step that no row of this wave sees is left out
         const bool none = base > pmax ||
-                          (static_cast<int64_t>(base) + kTileKeys - 1 <= static_cast<int64_t>(pmin) - d.a.window &&
+                          (static_cast<int64_t>(base) + KEYS - 1 <= static_cast<int64_t>(pmin) - d.a.window &&
                            base >= d.a.sinks);
         if (!none) {
-            const uint8_t* kt = sm[buf][0];
-            const uint8_t* vt = sm[buf][1];
-            f32x16 s[2];
+            const uint8_t* kt = sm[0][buf];
+            const uint8_t* vt = sm[1][buf];
+            f32x16 s[U];
             // the other wave of the SIMD does its softmax meanwhile (391 -> 378 us at 4 x
             // 2048 tokens on 8192 keys; with the second product too, no gain)
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
 #pragma unroll
                 for (int x = 0; x < KS; ++x) {
-                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + k_off[x] + u * 32 * ROW);
+                    if constexpr (FP) {
+                        const f32x4 kf = *reinterpret_cast<const f32x4*>(kt + k_off[x]);
 #pragma unroll
-                    for (int q3 = QT - 1; q3 >= 0; --q3)
-                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[q3][x], s[u], 0, 0, 0);
+                        for (int j = 0; j < 4; ++j)
+                            s[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[x][j], s[u], 0, 0, 0);
+                    } else {
+                        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + k_off[x] + u * 32 * ROW);
+#pragma unroll
+                        for (int q3 = QT - 1; q3 >= 0; --q3)
+                            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[q3][x], s[u], 0, 0, 0);
+                    }
                 }
             }
             __builtin_amdgcn_s_setprio(0);
-            const bool full = dead == 0 && base + kTileKeys - 1 <= pmin &&
+            const bool full = dead == 0 && base + KEYS - 1 <= pmin &&
                               (static_cast<int64_t>(base) > static_cast<int64_t>(pmax) - d.a.window ||
-                               base + kTileKeys - 1 < d.a.sinks);
+                               base + KEYS - 1 < d.a.sinks);
             if (!full) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < U; ++u)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int at = 32 * u + 8 * (i / 4) + 4 * hf + i % 4;
@@ -838,7 +857,7 @@ k_paged_tiles(PagedDev d) {
             }
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+            for (int i = 0; i < 16; ++i) top = fmaxf(fmaxf(top, s[0][i]), s[U - 1][i]);
             top = max_x32(top) * cs;
             if (__any(top > m + kLag)) {
                 const float mn = top > m + kLag ? top : m;
@@ -850,37 +869,58 @@ k_paged_tiles(PagedDev d) {
             }
             const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     s[u][i] = exp2_fast(fmaf(s[u][i], cs, -ref));
                     l += s[u][i];
                 }
+            if constexpr (FP) {
+                // key 8 (i / 4) + 4 hf + i % 4 of V, dims DT c .. DT c + DT - 1
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {   // 16 keys each
-                u32x4 pb[PT];
+                for (int i = 0; i < 16; ++i) {
+                    const uint8_t* at = vt + (8 * (i / 4) + 4 * hf + i % 4) * ROW + 4 * DT * c;
+                    float v[DT];
+                    if constexpr (DT == 4) {
+                        const f32x4 w = *reinterpret_cast<const f32x4*>(at);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float a0 = s[x / 2][8 * (x & 1) + 2 * j], a1 = s[x / 2][8 * (x & 1) + 2 * j + 1];
-#pragma unroll
-                    for (int p3 = 0; p3 < PT; ++p3) {
-                        pb[p3][j] = pack2_bf16(a0, a1);
-                        a0 -= bf16w_lo(pb[p3][j]);
-                        a1 -= bf16w_hi(pb[p3][j]);
+                        for (int y = 0; y < 4; ++y) v[y] = w[y];
+                    } else {
+                        const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+                        v[0] = __uint_as_float(w[0]);
+                        v[1] = __uint_as_float(w[1]);
                     }
+#pragma unroll
+                    for (int y = 0; y < DT; ++y)
+                        acc[y] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[y], s[0][i], acc[y], 0, 0, 0);
                 }
+            } else {
 #pragma unroll
-                for (int y = 0; y < DT; ++y) {
-                    typedef __attribute__((address_space(3))) s16x4* lds_s4;
-                    const uint8_t* at = vt + v_off[y] + 16 * x * ROW;
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at));
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 8 * ROW));
-                    const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
-                    const bf16x8 va = __builtin_bit_cast(bf16x8, u32x4{wl[0], wl[1], wh[0], wh[1]});
+                for (int x = 0; x < 4; ++x) {   // 16 keys each
+                    u32x4 pb[PT];
 #pragma unroll
-                    for (int p3 = PT - 1; p3 >= 0; --p3)
-                        acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8, pb[p3]), acc[y],
-                                                                          0, 0, 0);
+                    for (int j = 0; j < 4; ++j) {
+                        float a0 = s[x / 2][8 * (x & 1) + 2 * j], a1 = s[x / 2][8 * (x & 1) + 2 * j + 1];
+#pragma unroll
+                        for (int p3 = 0; p3 < PT; ++p3) {
+                            pb[p3][j] = pack2_bf16(a0, a1);
+                            a0 -= bf16w_lo(pb[p3][j]);
+                            a1 -= bf16w_hi(pb[p3][j]);
+                        }
+                    }
+#pragma unroll
+                    for (int y = 0; y < DT; ++y) {
+                        typedef __attribute__((address_space(3))) s16x4* lds_s4;
+                        const uint8_t* at = vt + v_off[y] + 16 * x * ROW;
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at));
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 8 * ROW));
+                        const u32x2 wl = __builtin_bit_cast(u32x2, lo), wh = __builtin_bit_cast(u32x2, hi);
+                        const bf16x8 va = __builtin_bit_cast(bf16x8, u32x4{wl[0], wl[1], wh[0], wh[1]});
+#pragma unroll
+                        for (int p3 = PT - 1; p3 >= 0; --p3)
+                            acc[y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8, pb[p3]), acc[y],
+                                                                              0, 0, 0);
+                    }
                 }
             }
         }
@@ -889,6 +929,11 @@ k_paged_tiles(PagedDev d) {
     }
     l += __shfl_xor(l, 32);
 
+    // the dim that a lane holds in acc[y][i]
+    auto dim_of = [&](int y, int i) {
+        const int m = 8 * (i / 4) + 4 * hf + i % 4;
+        return FP ? DT * m + y : 32 * y + m;
+    };
     bool nan = l != l;
 #pragma unroll
     for (int y = 0; y < DT; ++y)
@@ -903,7 +948,7 @@ k_paged_tiles(PagedDev d) {
             const int x = __builtin_ctz(rows);
             rows &= rows - 1;
             const int rr = r0 + x;
-            redo_row<D, Q32, KV, kTileKeys>(d, table, h, ks, t0, t1, sq.q0 + rr / d.group,
+            redo_row<D, Q32, KV, KEYS>(d, table, h, ks, t0, t1, sq.q0 + rr / d.group,
                                             h * d.group + rr % d.group, p0 + rr / d.group, red, red + D, red + D + 1);
             __builtin_amdgcn_wave_barrier();
             if (c == x) {
@@ -912,7 +957,7 @@ k_paged_tiles(PagedDev d) {
 #pragma unroll
                 for (int y = 0; y < DT; ++y)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[y][i] = red[32 * y + 8 * (i / 4) + 4 * hf + i % 4];
+                    for (int i = 0; i < 16; ++i) acc[y][i] = red[dim_of(y, i)];
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -925,6 +970,19 @@ k_paged_tiles(PagedDev d) {
         float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
         ml[0] = m;
         ml[1] = l;
+    }
+    if constexpr (FP) {
+        float* to = d.splits > 1 ? d.a.part + at * D : static_cast<float*>(d.a.out) + orow * D;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float v[DT];
+#pragma unroll
+            for (int y = 0; y < DT; ++y)
+                v[y] = d.splits > 1 ? acc[y][i] : l == 0.0f ? 0.0f : acc[y][i] * inv;
+            if constexpr (DT == 4) *reinterpret_cast<f32x4*>(to + dim_of(0, i)) = f32x4{v[0], v[1], v[2], v[3]};
+            else *reinterpret_cast<u32x2*>(to + dim_of(0, i)) = u32x2{__float_as_uint(v[0]), __float_as_uint(v[1])};
+        }
+        return;
     }
 #pragma unroll
     for (int y = 0; y < DT; ++y)
@@ -1008,7 +1066,7 @@ PagedDev plan(const KvCache& c, const PagedArgs& a, bool q_f32) {
     // keys one tile can see, in steps of 32
     const int64_t keys = std::min<int64_t>(a.max_kv_len, static_cast<int64_t>(a.window) + a.sinks + 16);
     const int64_t steps = ceil_div(keys, 32);
-    d.tiled = c.type != Kv::kF32 && rows >= kTiledRows;
+    d.tiled = rows >= kTiledRows;
     int64_t splits = 1;
     d.by_rows = false;
     d.waves = kWaves;
@@ -1045,11 +1103,8 @@ hipError_t launch(const PagedDev& d, hipStream_t s) {
     const int64_t joins = d.a.batch * d.a.max_q_len * d.a.q_heads;
     if (d.blocks > 0x7FFFFFF0 || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
     const dim3 block(64 * kWaves);
-    if constexpr (KV != Kv::kF32) {
-        if (d.tiled)
-            hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)),
-                               block, 0, s, d);
-    }
+    if (d.tiled)
+        hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)), block, 0, s, d);
     if (!d.tiled) {
         const unsigned lds = static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4;
         if (lds > kPlainLds) {
