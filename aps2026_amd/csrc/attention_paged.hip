@@ -48,7 +48,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kMostWaves = 8;  // 256 registers a wave
 constexpr int kRows = 16;      // rows of a tile
-constexpr int kMaxSplits = 64;  // k_paged_join: one wave reads every split's maximum at once
+constexpr int kMaxSplits = 256;
 constexpr unsigned kPlainLds = 62 * 1024;  // dynamic LDS that needs no leave: 64 KB less the static part
 constexpr int64_t kTiledRows = 33;  // rows of a sequence under a key head from which k_paged_tiles takes them
 
@@ -61,7 +61,6 @@ struct PagedDev {
     int splits;      // workgroups along the keys
     int row_tiles;   // tiles (tiled: blocks) of rows a sequence and key head can have
     bool tiled;      // k_paged_tiles, else k_paged_rows
-    bool by_rows;    // the waves of a workgroup take a tile each (else a part of the keys each)
     int waves;       // of a workgroup
     int lds_rows;    // rows of a tile that can be live: LDS keeps those
     int64_t blocks;  // workgroups
@@ -218,30 +217,26 @@ k_paged_rows(PagedDev d) {
     uint32_t id = blockIdx.x;
     const int split = id % d.splits;
     id /= d.splits;
-    const int per = d.by_rows ? d.waves : 1;
-    const uint32_t row_blocks = (d.row_tiles + per - 1) / per;
-    // the last rows see the most keys: they start first
-    const int rb = static_cast<int>(row_blocks - 1 - id % row_blocks);
-    id /= row_blocks;
+    const int rt = id % d.row_tiles;
+    id /= d.row_tiles;
     const int h = id % d.c.kv_heads;
     const int64_t b = id / d.c.kv_heads;
     const Seq sq = sequence(d, b);
     const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
     const int nrows = static_cast<int>(qlen * d.group);
-    const int r0 = (d.by_rows ? rb * d.waves + wave : rb) * kRows;
-    const bool any = r0 < nrows;
-    if (!d.by_rows && !any) return;  // the whole workgroup
+    const int r0 = rt * kRows;
+    if (r0 >= nrows) return;  // the whole workgroup
     const int32_t* table = d.a.page_table + b * d.a.table_stride;
 
     const int p0 = sq.kv - sq.len;  // position of the first new token
     const int r_last = r0 + kRows - 1 < nrows ? r0 + kRows - 1 : nrows - 1;
-    const int pmin = p0 + r0 / d.group, pmax = any ? p0 + r_last / d.group : -1;
+    const int pmin = p0 + r0 / d.group, pmax = p0 + r_last / d.group;
     const int row = r0 + c;
     const bool live = row < nrows;
     const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
     const int pos = live ? p0 + tok : -1;
     const Keys ks = visible<STEP>(d, pmin, pmax);
-    const int parts = d.splits * (d.by_rows ? 1 : d.waves), part = d.by_rows ? split : split * d.waves + wave;
+    const int parts = d.splits * d.waves, part = split * d.waves + wave;
     const int each = (ks.steps + parts - 1) / parts;
     const int t0 = part * each < ks.steps ? part * each : ks.steps;
     const int t1 = t0 + each < ks.steps ? t0 + each : ks.steps;
@@ -249,7 +244,7 @@ k_paged_rows(PagedDev d) {
     // the queries, in the order of dims that the cache's loads give
     f32x4 qf[FP ? D / 16 : 1];
     bf16x8 qb[FP ? 1 : QT][FP ? 1 : KS];
-    if (any) {
+    {
         const int64_t qat = (sq.q0 + tok) * d.a.q_stride + static_cast<int64_t>(qh) * D;
         if constexpr (FP) {
 #pragma unroll
@@ -520,7 +515,7 @@ k_paged_rows(PagedDev d) {
             if (c < d.lds_rows) *reinterpret_cast<f32x4*>(o_row(wave, c) + W * (4 * g + i) + t) = v;
         }
     if (g == 0) { sm_m[wave][c] = m; sm_l[wave][c] = l; }
-    if (any && pmin != pmax) {
+    if (pmin != pmax) {
         const uint64_t bad = __ballot(nan && live);
         uint32_t rows = static_cast<uint32_t>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu);
         while (rows) {
@@ -533,24 +528,21 @@ k_paged_rows(PagedDev d) {
     }
     __syncthreads();
 
-    // join the waves' parts (by_rows: each wave has rows of its own) and write
-    // the result, or the workgroup's part of it
-    constexpr int TPR = D / 8;                 // threads of a row, 8 dims each
-    const int tiles = d.by_rows ? d.waves : 1, parts_w = d.by_rows ? 1 : d.waves;
-    for (int x = threadIdx.x; x < tiles * kRows * TPR; x += 64 * d.waves) {
-        const int dim = 8 * (x % TPR), rt = x / TPR / kRows, rc = x / TPR % kRows;
-        const int rr = (d.by_rows ? rb * d.waves + rt : rb) * kRows + rc;
+    // join the waves' parts and write the result, or the workgroup's part of it
+    constexpr int TPR = D / 8;  // threads of a row, 8 dims each
+    for (int x = threadIdx.x; x < kRows * TPR; x += 64 * d.waves) {
+        const int dim = 8 * (x % TPR), rc = x / TPR;
+        const int rr = r0 + rc;
         if (rr >= nrows) continue;
         float mm = -INFINITY;
-        for (int w = 0; w < parts_w; ++w) mm = fmaxf(mm, sm_m[d.by_rows ? rt : w][rc]);
+        for (int w = 0; w < d.waves; ++w) mm = fmaxf(mm, sm_m[w][rc]);
         const float ref = mm == -INFINITY ? 0.0f : mm;
         float ll = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        for (int w = 0; w < parts_w; ++w) {
-            const int sl = d.by_rows ? rt : w;
-            const float f = exp2_fast(sm_m[sl][rc] - ref);
-            ll = fmaf(sm_l[sl][rc], f, ll);
+        for (int w = 0; w < d.waves; ++w) {
+            const float f = exp2_fast(sm_m[w][rc] - ref);
+            ll = fmaf(sm_l[w][rc], f, ll);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = fmaf(o_row(sl, rc)[dim + j], f, o[j]);
+            for (int j = 0; j < 8; ++j) o[j] = fmaf(o_row(w, rc)[dim + j], f, o[j]);
         }
         const int64_t orow = (sq.q0 + rr / d.group) * d.a.q_heads + h * d.group + rr % d.group;
         if (d.splits > 1) {
@@ -1012,6 +1004,7 @@ __global__ void __launch_bounds__(64 * JW)
 k_paged_join(PagedDev d) {
     constexpr int PER = D / 64;
     __shared__ float part[JW][D];
+    __shared__ float weight[JW][kMaxSplits];  // a wave's own copy
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t id = blockIdx.x;
     const int head = id % d.a.q_heads;
@@ -1021,20 +1014,34 @@ k_paged_join(PagedDev d) {
     if (tok >= sq.len) return;
     const int64_t orow = (sq.q0 + tok) * d.a.q_heads + head, at = orow * d.splits;
     const float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
-    const float m = lane < d.splits ? ml[2 * lane] : -INFINITY, l = lane < d.splits ? ml[2 * lane + 1] : 0.0f;
-    const float* po = d.a.part + at * D + PER * lane;
-    float o[PER] = {};
-    float top = m;
+    float m[kMaxSplits / 64], l[kMaxSplits / 64], top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kMaxSplits / 64; ++x) {
+        const int s = 64 * x + lane;
+        m[x] = s < d.splits ? ml[2 * s] : -INFINITY;
+        l[x] = s < d.splits ? ml[2 * s + 1] : 0.0f;
+        top = fmaxf(top, m[x]);
+    }
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-    const float w = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
-    float sum = w * l;
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kMaxSplits / 64; ++x) {
+        const float w = exp2_fast(m[x] - ref);
+        weight[wave][64 * x + lane] = w;
+        sum = fmaf(w, l[x], sum);
+    }
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
+    __builtin_amdgcn_wave_barrier();
+    const float* po = d.a.part + at * D + PER * lane;
+    float o[PER] = {};
+#pragma unroll 4
     for (int s = wave; s < d.splits; s += JW) {
-        const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
+        const float w = weight[wave][s];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] = fmaf(ws, po[static_cast<int64_t>(s) * D + j], o[j]);
+        for (int j = 0; j < PER; ++j) o[j] = fmaf(w, po[static_cast<int64_t>(s) * D + j], o[j]);
     }
     if constexpr (JW > 1) {
 #pragma unroll
@@ -1067,34 +1074,26 @@ PagedDev plan(const KvCache& c, const PagedArgs& a, bool q_f32) {
     const int64_t keys = std::min<int64_t>(a.max_kv_len, static_cast<int64_t>(a.window) + a.sinks + 16);
     const int64_t steps = ceil_div(keys, 32);
     d.tiled = rows >= kTiledRows;
-    int64_t splits = 1;
-    d.by_rows = false;
+    int64_t splits;
     d.waves = kWaves;
-    d.lds_rows = kRows;
+    d.lds_rows = static_cast<int>(std::min<int64_t>(kRows, rows));
+    d.row_tiles = static_cast<int>(ceil_div(rows, d.tiled ? kBlockRows : kRows));
+    const int64_t tiles = heads * d.row_tiles;
     if (d.tiled) {
-        d.row_tiles = static_cast<int>(ceil_div(rows, kBlockRows));
-        splits = std::min<int64_t>(ceil_div(512, heads * d.row_tiles), ceil_div(steps, 8));
+        splits = std::min<int64_t>(ceil_div(512, tiles), ceil_div(steps, 8));
     } else {
-        d.row_tiles = static_cast<int>(ceil_div(rows, kRows));
-        d.by_rows = d.row_tiles >= kWaves;
-        if (d.by_rows) {
-            splits = std::min<int64_t>(ceil_div(1024, heads * ceil_div(d.row_tiles, kWaves)), ceil_div(steps, 8));
-        } else {
-            const int64_t tiles = heads * d.row_tiles;
-            splits = std::min<int64_t>(ceil_div(1024, tiles), ceil_div(steps, 2 * kWaves));
-            if (splits > 1 && steps <= 4 * kMostWaves) {
-                // short: one larger workgroup instead of a second launch
-                d.waves = kMostWaves;
-                splits = 1;
-            } else if (splits > kMaxSplits) {
-                d.waves = kMostWaves;
-                splits = kMaxSplits;
-            }
-            d.lds_rows = static_cast<int>(std::min<int64_t>(kRows, rows));
+        // four workgroups a CU of a large batch, two where there are few tiles and
+        // the parts to join weigh more (us with two / four: 64 x 8192 keys 148 /
+        // 145, in 4 bits 99 / 89; 32 x 2051 27 / 31, 1 x 100000 39 / 42)
+        splits = std::min<int64_t>(ceil_div(tiles > 128 ? 1024 : 512, tiles), ceil_div(steps, 2 * kWaves));
+        if (splits > 1 && steps <= 4 * kMostWaves) {
+            // short: one larger workgroup instead of a second launch
+            d.waves = kMostWaves;
+            splits = 1;
         }
     }
     d.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
-    d.blocks = heads * d.splits * (d.tiled || !d.by_rows ? d.row_tiles : ceil_div(d.row_tiles, kWaves));
+    d.blocks = tiles * d.splits;
     return d;
 }
 
@@ -1117,7 +1116,8 @@ hipError_t launch(const PagedDev& d, hipStream_t s) {
                            s, d);
     }
     const dim3 grid(static_cast<unsigned>(joins));
-    if (d.splits > 16) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
+    if (d.splits > 64) hipLaunchKernelGGL((k_paged_join<D, Q32, 16>), grid, dim3(1024), 0, s, d);
+    else if (d.splits > 8) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
     else if (d.splits > 1) hipLaunchKernelGGL((k_paged_join<D, Q32, 1>), grid, dim3(64), 0, s, d);
     return hipGetLastError();
 }
