@@ -67,24 +67,29 @@ struct PagedDev {
     float scale_log2;
 };
 
-// Rows q0 .. q0 + len - 1 and the cached length of sequence b, inside the
-// arrays whatever the device values are.
+// Rows q0 .. q0 + len - 1 and the cached length of a sequence, inside the arrays
+// whatever the device values are.
 struct Seq {
     int64_t q0;
     int len, kv;
 };
-__device__ inline Seq sequence(const PagedDev& d, int64_t b) {
-    const int64_t lo = d.a.q_offsets[b], hi = d.a.q_offsets[b + 1];
+__device__ inline Seq clipped(const PagedDev& d, int64_t lo, int64_t hi, int64_t kv) {
     Seq s;
     s.q0 = lo < 0 ? 0 : lo > d.a.rows ? d.a.rows : lo;
-    int64_t n = (hi < d.a.rows ? hi : d.a.rows) - s.q0;
+    const int64_t n = (hi < d.a.rows ? hi : d.a.rows) - s.q0;
     s.len = static_cast<int>(n < 0 ? 0 : n);
-    int64_t kv = d.a.kv_lens[b];
     const int64_t held = d.a.table_stride << d.page_shift;
     kv = kv < d.a.max_kv_len ? kv : d.a.max_kv_len;
     kv = kv < held ? kv : held;
     s.kv = static_cast<int>(kv < 0 ? 0 : kv);
     return s;
+}
+// Sequence b, the same in every lane (in scalar registers, and with it the
+// places that loads start from).
+__device__ inline Seq sequence(const PagedDev& d, int64_t b) {
+    return clipped(d, __builtin_amdgcn_readfirstlane(d.a.q_offsets[b]),
+                   __builtin_amdgcn_readfirstlane(d.a.q_offsets[b + 1]),
+                   __builtin_amdgcn_readfirstlane(d.a.kv_lens[b]));
 }
 
 // The keys that the rows at positions [pmin, pmax] see, in steps of STEP keys:
@@ -96,6 +101,9 @@ struct Keys {
 template <int STEP>
 __device__ inline Keys visible(const PagedDev& d, int pmin, int pmax) {
     Keys k;
+    // (the division behind a position leaves scalar registers)
+    pmin = __builtin_amdgcn_readfirstlane(pmin);
+    pmax = __builtin_amdgcn_readfirstlane(pmax);
     k.hi = pmax + 1 > 0 ? pmax + 1 : 0;
     const int64_t lo = static_cast<int64_t>(pmin) + 1 - d.a.window;
     k.lo = lo > 0 ? static_cast<int>(lo) : 0;
@@ -215,12 +223,12 @@ k_paged_rows(PagedDev d) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     uint32_t id = blockIdx.x;
-    const int split = id % d.splits;
+    const int split = __builtin_amdgcn_readfirstlane(id % d.splits);
     id /= d.splits;
-    const int rt = id % d.row_tiles;
+    const int rt = __builtin_amdgcn_readfirstlane(id % d.row_tiles);
     id /= d.row_tiles;
-    const int h = id % d.c.kv_heads;
-    const int64_t b = id / d.c.kv_heads;
+    const int h = __builtin_amdgcn_readfirstlane(id % d.c.kv_heads);
+    const int64_t b = __builtin_amdgcn_readfirstlane(id / d.c.kv_heads);
     const Seq sq = sequence(d, b);
     const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
     const int nrows = static_cast<int>(qlen * d.group);
@@ -230,14 +238,15 @@ k_paged_rows(PagedDev d) {
 
     const int p0 = sq.kv - sq.len;  // position of the first new token
     const int r_last = r0 + kRows - 1 < nrows ? r0 + kRows - 1 : nrows - 1;
-    const int pmin = p0 + r0 / d.group, pmax = p0 + r_last / d.group;
+    const int pmin = __builtin_amdgcn_readfirstlane(p0 + r0 / d.group);
+    const int pmax = __builtin_amdgcn_readfirstlane(p0 + r_last / d.group);
     const int row = r0 + c;
     const bool live = row < nrows;
     const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
     const int pos = live ? p0 + tok : -1;
     const Keys ks = visible<STEP>(d, pmin, pmax);
     const int parts = d.splits * d.waves, part = split * d.waves + wave;
-    const int each = (ks.steps + parts - 1) / parts;
+    const int each = __builtin_amdgcn_readfirstlane((ks.steps + parts - 1) / parts);
     const int t0 = part * each < ks.steps ? part * each : ks.steps;
     const int t1 = t0 + each < ks.steps ? t0 + each : ks.steps;
 
@@ -303,12 +312,16 @@ k_paged_rows(PagedDev d) {
         }
     };
     using Four = std::integral_constant<int, 4>;
+    // a lane's bytes past the (uniform) place of 16 keys: a 32-bit offset and a
+    // constant for each load
+    const uint32_t k_lane = FP ? c * (4 * D) + 16 * g : MX ? c * (D / 2) + (D / 8) * g : c * (2 * D) + 16 * g;
+    const uint32_t v_lane = FP ? 4 * g * (4 * D) + 4 * W * c : MX ? 4 * g * (D / 2) + (W / 2) * c
+                                                                  : 4 * g * (2 * D) + 2 * W * c;
+    const uint32_t ks_lane = c * (D / 32) + (D / 4) * g / 32, vs_lane = 4 * g * (D / 32) + W * c / 32;
     auto load = [&](int t, Step& st) {
         const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
         const int slot = (t - t0) % AHEAD;
         if (slot == 0) pages = page_of<STEP>(d, table, ks, t + lane / HALVES, t1, lane % HALVES);
-        const auto* kb = static_cast<const uint8_t*>(d.c.k);
-        const auto* vb = static_cast<const uint8_t*>(d.c.v);
 #pragma unroll
         for (int a = 0; a < HALVES; ++a) {
             const int page = __builtin_amdgcn_readlane(pages, slot * HALVES + a);
@@ -316,33 +329,32 @@ k_paged_rows(PagedDev d) {
             // (page, head, offset) row of the half's first key
             const int64_t hrow = ((static_cast<int64_t>(page < 0 ? 0 : page) * d.c.kv_heads + h) << d.page_shift) +
                                  ((base + 16 * a) & ((1 << d.page_shift) - 1));
+            constexpr int BYTES = FP ? 4 * D : MX ? D / 2 : 2 * D;  // of a key
+            const uint8_t* kp = static_cast<const uint8_t*>(d.c.k) + hrow * BYTES;
+            const uint8_t* vp = static_cast<const uint8_t*>(d.c.v) + hrow * BYTES;
             if constexpr (FP) {
 #pragma unroll
-                for (int s = 0; s < D / 16; ++s) words(kb + (hrow + c) * (4 * D) + 64 * s + 16 * g, Four(), st.k + 4 * s);
+                for (int s = 0; s < D / 16; ++s) words(kp + k_lane + 64 * s, Four(), st.k + 4 * s);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int x = 0; x < W; x += 4)
-                        words(vb + (hrow + 4 * g + i) * (4 * D) + 4 * (W * c + x), Four(), st.v + W * i + x);
+                    for (int x = 0; x < W; x += 4) words(vp + v_lane + BYTES * i + 4 * x, Four(), st.v + W * i + x);
             } else if constexpr (!MX) {
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    words(kb + (hrow + c) * (2 * D) + 64 * s + 16 * g, Four(), st.k + 4 * (KS * a + s));
+                for (int s = 0; s < KS; ++s) words(kp + k_lane + 64 * s, Four(), st.k + 4 * (KS * a + s));
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    words(vb + (hrow + 4 * g + i) * (2 * D) + 2 * W * c,
-                          std::integral_constant<int, W / 2>(), st.v + (W / 2) * (4 * a + i));
+                    words(vp + v_lane + BYTES * i, std::integral_constant<int, W / 2>(), st.v + (W / 2) * (4 * a + i));
             } else {
                 // D / 4 neighbouring dims of a key of K: one block's, or half a block's
-                words(kb + (hrow + c) * (D / 2) + (D / 8) * g, std::integral_constant<int, KS>(), st.k + KS * a);
-                st.ks[a] = d.c.k_scale[(hrow + c) * (D / 32) + (D / 4) * g / 32];
-                const uint8_t* vp = vb + (hrow + 4 * g) * (D / 2) + (W / 2) * c;
-                const uint8_t* sp = d.c.v_scale + (hrow + 4 * g) * (D / 32) + W * c / 32;
+                words(kp + k_lane, std::integral_constant<int, KS>(), st.k + KS * a);
+                st.ks[a] = (d.c.k_scale + hrow * (D / 32))[ks_lane];
+                const uint8_t* sp = d.c.v_scale + hrow * (D / 32);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if constexpr (W == 8) st.v[4 * a + i] = *reinterpret_cast<const uint32_t*>(vp + i * (D / 2));
-                    else st.v[4 * a + i] = *reinterpret_cast<const uint16_t*>(vp + i * (D / 2));
-                    st.vs[4 * a + i] = sp[i * (D / 32)];
+                    if constexpr (W == 8) st.v[4 * a + i] = *reinterpret_cast<const uint32_t*>(vp + v_lane + BYTES * i);
+                    else st.v[4 * a + i] = *reinterpret_cast<const uint16_t*>(vp + v_lane + BYTES * i);
+                    st.vs[4 * a + i] = (sp + vs_lane)[i * (D / 32)];
                 }
             }
         }
@@ -608,6 +620,7 @@ __device__ inline int v_swizzle(int key) { return FP ? 0 : D == 128 ? (key & 3) 
 template <int D, bool Q32, Kv KV>
 __global__ void __launch_bounds__(64 * kWaves, 2)
 k_paged_tiles(PagedDev d) {
+    constexpr int BLOCK = kBlockRows;
     constexpr bool FP = KV == Kv::kF32;
     constexpr int KEYS = FP ? 32 : 64;         // keys of a step
     constexpr int U = KEYS / 32;               // 32-key halves of it
@@ -621,33 +634,60 @@ k_paged_tiles(PagedDev d) {
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
-    // row blocks of one key head go round the XCDs: each L2 reads every
-    // sequence's keys, but no XCD is left with the long ones
+    // Workgroups take the row blocks that there are, sequence by sequence, so
+    // that those without one are the last of the grid (left between, they
+    // take their XCD's share: 3 ragged chunks of 500 tokens 59 us, closed up
+    // 35).  Row blocks of one key head go round the XCDs: each L2 reads every
+    // sequence's keys, but no XCD is left with the long ones.
     uint32_t id = blockIdx.x;
-    const uint32_t row_blocks = d.row_tiles;
-    const int split = id % d.splits;
+    const uint32_t per = static_cast<uint32_t>(d.c.kv_heads * d.splits);
+    int64_t b = -1;
+    uint32_t row_blocks = 0;
+    for (int64_t b0 = 0; b0 < d.a.batch; b0 += 64) {
+        uint32_t n = 0;
+        if (b0 + lane < d.a.batch) {
+            const int64_t len = clipped(d, d.a.q_offsets[b0 + lane], d.a.q_offsets[b0 + lane + 1], 0).len;
+            n = static_cast<uint32_t>(((len < d.a.max_q_len ? len : d.a.max_q_len) * d.group + BLOCK - 1) / BLOCK);
+        }
+        uint32_t upto = n;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) {
+            const uint32_t v = __shfl_up(upto, x);
+            upto += lane >= x ? v : 0u;
+        }
+        const uint64_t past = __ballot(id < upto * per);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            row_blocks = __builtin_amdgcn_readlane(n, at);
+            id -= (__builtin_amdgcn_readlane(upto, at) - row_blocks) * per;
+            b = b0 + at;
+            break;
+        }
+        id -= __builtin_amdgcn_readlane(upto, 63) * per;
+    }
+    if (b < 0) return;
+    const int split = __builtin_amdgcn_readfirstlane(id % d.splits);
     id /= d.splits;
-    const int rb = static_cast<int>(row_blocks - 1 - id % row_blocks);
-    id /= row_blocks;
-    const int h = id % d.c.kv_heads;
-    const int64_t b = id / d.c.kv_heads;
+    // the last rows see the most keys: they start first
+    const int rb = __builtin_amdgcn_readfirstlane(row_blocks - 1 - id % row_blocks);
+    const int h = __builtin_amdgcn_readfirstlane(id / row_blocks);
     const Seq sq = sequence(d, b);
     const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
     const int nrows = static_cast<int>(qlen * d.group);
-    const int rb0 = rb * kBlockRows;
-    if (rb0 >= nrows) return;
+    const int rb0 = rb * BLOCK;
     const int32_t* table = d.a.page_table + b * d.a.table_stride;
     const int p0 = sq.kv - sq.len;
-    const int rb1 = (rb0 + kBlockRows < nrows ? rb0 + kBlockRows : nrows) - 1;
+    const int rb1 = (rb0 + BLOCK < nrows ? rb0 + BLOCK : nrows) - 1;
     const Keys ks = visible<KEYS>(d, p0 + rb0 / d.group, p0 + rb1 / d.group);
-    const int each = (ks.steps + d.splits - 1) / d.splits;
+    const int each = __builtin_amdgcn_readfirstlane((ks.steps + d.splits - 1) / d.splits);
     const int t0 = split * each < ks.steps ? split * each : ks.steps;
     const int t1 = t0 + each < ks.steps ? t0 + each : ks.steps;
 
     const int r0 = rb0 + wave * kTileRows;
     const bool any = r0 < nrows;
     const int r_last = r0 + kTileRows - 1 < nrows ? r0 + kTileRows - 1 : nrows - 1;
-    const int pmin = p0 + r0 / d.group, pmax = any ? p0 + r_last / d.group : -1;
+    const int pmin = __builtin_amdgcn_readfirstlane(p0 + r0 / d.group);
+    const int pmax = __builtin_amdgcn_readfirstlane(any ? p0 + r_last / d.group : -1);
     const int row = r0 + c;
     const bool live = row < nrows;
     const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
@@ -708,29 +748,38 @@ k_paged_tiles(PagedDev d) {
     uint32_t mks = 0, mvs = 0;
     int pages = -1;          // lane GROUPS i + a: the page of 16 keys a of step i of 64 / GROUPS
     uint32_t dead_next = 0;  // bit a: 16 keys a of the step that was fetched have no page
+    // where a lane's 16 bytes of each copy come from, past the (uniform) place of
+    // the 16 keys: 32-bit offsets, one add in the load (4 bits: four lanes a key,
+    // codes and scales)
+    constexpr bool MX = KV == Kv::kMx;
+    constexpr int RPI = MX ? 16 : 1024 / ROW;  // keys of one copy
+    uint32_t k_src[16 / RPI], v_src[16 / RPI];
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+        const int r = RPI * i + lane / CH;
+        k_src[i] = MX ? lane / 4 * (D / 2) + (lane & 3) * (D / 8) : r * ROW + 16 * ((lane % CH) ^ k_swizzle<D, FP>(r));
+        v_src[i] = MX ? lane / 4 * (D / 32) + (lane & 3) * (D / 4) / 32
+                      : r * ROW + 16 * ((lane % CH) ^ v_swizzle<D, FP>(r));
+    }
     auto fetch1 = [&](int which, int64_t hrow, int buf) {  // one operand's 16 keys, to LDS or (4 bits) to registers
         const uint8_t* src = static_cast<const uint8_t*>(which ? d.c.v : d.c.k);
         if constexpr (KV != Kv::kMx) {
             src += hrow * ROW;
-            constexpr int RPI = 1024 / ROW;  // keys of one copy
 #pragma unroll
-            for (int i = 0; i < 16 / RPI; ++i) {
-                const int r = RPI * i + lane / CH;
-                const int chunk = (lane % CH) ^ (which ? v_swizzle<D, FP>(r) : k_swizzle<D, FP>(r));
-                __builtin_amdgcn_global_load_lds(APS_AGP(src + r * ROW + 16 * chunk),
+            for (int i = 0; i < 16 / RPI; ++i)
+                __builtin_amdgcn_global_load_lds(APS_AGP(src + (which ? v_src : k_src)[i]),
                                                  APS_ALP(&sm[which][buf][(16 * grp + RPI * i) * ROW]), 16, 0, 0);
-            }
         } else {
-            const int64_t at = hrow + lane / 4;  // four lanes a key
-            src += at * (D / 2) + (lane & 3) * (D / 8);
+            src += hrow * (D / 2);
             u32x4& w = which ? mv : mk;
             if constexpr (D == 128) {
-                w = *reinterpret_cast<const u32x4*>(src);
+                w = *reinterpret_cast<const u32x4*>(src + k_src[0]);
             } else {
-                const u32x2 half = *reinterpret_cast<const u32x2*>(src);
+                const u32x2 half = *reinterpret_cast<const u32x2*>(src + k_src[0]);
                 w = u32x4{half[0], half[1], 0u, 0u};
             }
-            (which ? mvs : mks) = (which ? d.c.v_scale : d.c.k_scale)[at * (D / 32) + (lane & 3) * (D / 4) / 32];
+            const uint8_t* sc = (which ? d.c.v_scale : d.c.k_scale) + hrow * (D / 32);
+            (which ? mvs : mks) = sc[v_src[0]];
         }
     };
     auto fetch = [&](int t, int buf) {
