@@ -48,7 +48,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kMostWaves = 8;  // 256 registers a wave
 constexpr int kRows = 16;      // rows of a tile
-constexpr int kMaxSplits = 256;
+constexpr int kMaxSplits = 256, kFewSplits = 8;
 constexpr unsigned kPlainLds = 62 * 1024;  // dynamic LDS that needs no leave: 64 KB less the static part
 constexpr int64_t kTiledRows = 33;  // rows of a sequence under a key head from which k_paged_tiles takes them
 
@@ -1053,7 +1053,7 @@ __global__ void __launch_bounds__(64 * JW)
 k_paged_join(PagedDev d) {
     constexpr int PER = D / 64;
     __shared__ float part[JW][D];
-    __shared__ float weight[JW][kMaxSplits];  // a wave's own copy
+    __shared__ float weight[JW][JW == 1 ? 1 : kMaxSplits];  // a wave's own copy
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t id = blockIdx.x;
     const int head = id % d.a.q_heads;
@@ -1063,9 +1063,21 @@ k_paged_join(PagedDev d) {
     if (tok >= sq.len) return;
     const int64_t orow = (sq.q0 + tok) * d.a.q_heads + head, at = orow * d.splits;
     const float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
-    float m[kMaxSplits / 64], l[kMaxSplits / 64], top = -INFINITY;
+    const float* po = d.a.part + at * D + PER * lane;
+    constexpr int MOST = JW == 1 ? kFewSplits : kMaxSplits, MX = (MOST + 63) / 64;
+    // few splits: everything is on its way before the first wait
+    float few[JW == 1 ? kFewSplits : 1][PER];
+    if constexpr (JW == 1) {
 #pragma unroll
-    for (int x = 0; x < kMaxSplits / 64; ++x) {
+        for (int s = 0; s < kFewSplits; ++s)
+            if (s < d.splits) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) few[s][j] = po[static_cast<int64_t>(s) * D + j];
+            }
+    }
+    float m[MX], l[MX], top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < MX; ++x) {
         const int s = 64 * x + lane;
         m[x] = s < d.splits ? ml[2 * s] : -INFINITY;
         l[x] = s < d.splits ? ml[2 * s + 1] : 0.0f;
@@ -1074,23 +1086,33 @@ k_paged_join(PagedDev d) {
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    float sum = 0.0f, w[MX];
 #pragma unroll
-    for (int x = 0; x < kMaxSplits / 64; ++x) {
-        const float w = exp2_fast(m[x] - ref);
-        weight[wave][64 * x + lane] = w;
-        sum = fmaf(w, l[x], sum);
+    for (int x = 0; x < MX; ++x) {
+        w[x] = exp2_fast(m[x] - ref);
+        sum = fmaf(w[x], l[x], sum);
     }
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
-    __builtin_amdgcn_wave_barrier();
-    const float* po = d.a.part + at * D + PER * lane;
     float o[PER] = {};
-#pragma unroll 4
-    for (int s = wave; s < d.splits; s += JW) {
-        const float w = weight[wave][s];
+    if constexpr (JW == 1) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] = fmaf(w, po[static_cast<int64_t>(s) * D + j], o[j]);
+        for (int s = 0; s < kFewSplits; ++s)
+            if (s < d.splits) {
+                const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w[0]), s));
+#pragma unroll
+                for (int j = 0; j < PER; ++j) o[j] = fmaf(ws, few[s][j], o[j]);
+            }
+    } else {
+#pragma unroll
+        for (int x = 0; x < MX; ++x) weight[wave][64 * x + lane] = w[x];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+        for (int s = wave; s < d.splits; s += JW) {
+            const float ws = weight[wave][s];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) o[j] = fmaf(ws, po[static_cast<int64_t>(s) * D + j], o[j]);
+        }
     }
     if constexpr (JW > 1) {
 #pragma unroll
@@ -1166,7 +1188,7 @@ hipError_t launch(const PagedDev& d, hipStream_t s) {
     }
     const dim3 grid(static_cast<unsigned>(joins));
     if (d.splits > 64) hipLaunchKernelGGL((k_paged_join<D, Q32, 16>), grid, dim3(1024), 0, s, d);
-    else if (d.splits > 8) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
+    else if (d.splits > kFewSplits) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
     else if (d.splits > 1) hipLaunchKernelGGL((k_paged_join<D, Q32, 1>), grid, dim3(64), 0, s, d);
     return hipGetLastError();
 }
