@@ -49,7 +49,7 @@ constexpr int kWaves = 4;
 constexpr int kMostWaves = 8;  // 256 registers a wave
 constexpr int kRows = 16;      // rows of a tile
 constexpr int kMaxSplits = 256, kFewSplits = 8;
-constexpr unsigned kPlainLds = 62 * 1024;  // dynamic LDS that needs no leave: 64 KB less the static part
+constexpr int kPlainLds = 62 * 1024;  // dynamic LDS that needs no leave: 64 KB less the static part
 constexpr int64_t kTiledRows = 33;  // rows of a sequence under a key head from which k_paged_tiles takes them
 
 // What both kernels know of the launch.
@@ -61,11 +61,20 @@ struct PagedDev {
     int splits;      // workgroups along the keys
     int row_tiles;   // tiles (tiled: blocks) of rows a sequence and key head can have
     bool tiled;      // k_paged_tiles, else k_paged_rows
+    int least, most;  // rows of the sequences that this launch serves
+    int64_t max_q;    // the most tokens of one
     int waves;       // of a workgroup
     int lds_rows;    // rows of a tile that can be live: LDS keeps those
     int64_t blocks;  // workgroups
+    float* part;     // of the splits
     float scale_log2;
 };
+// The rows under one key head that a sequence has in this launch, 0 if it is
+// another's.
+__device__ inline int rows_of(const PagedDev& d, int len) {
+    const int64_t n = (len < d.a.max_q_len ? len : d.a.max_q_len) * d.group;
+    return n >= d.least && n <= d.most ? static_cast<int>(n) : 0;
+}
 
 // Rows q0 .. q0 + len - 1 and the cached length of a sequence, inside the arrays
 // whatever the device values are.
@@ -230,8 +239,7 @@ k_paged_rows(PagedDev d) {
     const int h = __builtin_amdgcn_readfirstlane(id % d.c.kv_heads);
     const int64_t b = __builtin_amdgcn_readfirstlane(id / d.c.kv_heads);
     const Seq sq = sequence(d, b);
-    const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
-    const int nrows = static_cast<int>(qlen * d.group);
+    const int nrows = rows_of(d, sq.len);
     const int r0 = rt * kRows;
     if (r0 >= nrows) return;  // the whole workgroup
     const int32_t* table = d.a.page_table + b * d.a.table_stride;
@@ -517,7 +525,8 @@ k_paged_rows(PagedDev d) {
     l += __shfl_xor(l, 32);
 
     // the wave's part to LDS: row c, dims W (4 g + i) + t
-    bool nan = l != l;
+    // (a NaN total is the row's own: scores that it does not see are replaced)
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -528,7 +537,7 @@ k_paged_rows(PagedDev d) {
         }
     if (g == 0) { sm_m[wave][c] = m; sm_l[wave][c] = l; }
     if (pmin != pmax) {
-        const uint64_t bad = __ballot(nan && live);
+        const uint64_t bad = __ballot(nan && live && l == l);
         uint32_t rows = static_cast<uint32_t>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu);
         while (rows) {
             const int x = __builtin_ctz(rows);
@@ -559,11 +568,11 @@ k_paged_rows(PagedDev d) {
         const int64_t orow = (sq.q0 + rr / d.group) * d.a.q_heads + h * d.group + rr % d.group;
         if (d.splits > 1) {
             const int64_t at = orow * d.splits + split;
-            float* po = d.a.part + at * D + dim;
+            float* po = d.part + at * D + dim;
             *reinterpret_cast<f32x4*>(po) = f32x4{o[0], o[1], o[2], o[3]};
             *reinterpret_cast<f32x4*>(po + 4) = f32x4{o[4], o[5], o[6], o[7]};
             if (dim == 0) {
-                float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+                float* ml = d.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
                 ml[0] = mm;
                 ml[1] = ll;
             }
@@ -646,8 +655,8 @@ k_paged_tiles(PagedDev d) {
     for (int64_t b0 = 0; b0 < d.a.batch; b0 += 64) {
         uint32_t n = 0;
         if (b0 + lane < d.a.batch) {
-            const int64_t len = clipped(d, d.a.q_offsets[b0 + lane], d.a.q_offsets[b0 + lane + 1], 0).len;
-            n = static_cast<uint32_t>(((len < d.a.max_q_len ? len : d.a.max_q_len) * d.group + BLOCK - 1) / BLOCK);
+            const Seq one = clipped(d, d.a.q_offsets[b0 + lane], d.a.q_offsets[b0 + lane + 1], 0);
+            n = static_cast<uint32_t>((rows_of(d, one.len) + BLOCK - 1) / BLOCK);
         }
         uint32_t upto = n;
 #pragma unroll
@@ -672,8 +681,7 @@ k_paged_tiles(PagedDev d) {
     const int rb = __builtin_amdgcn_readfirstlane(row_blocks - 1 - id % row_blocks);
     const int h = __builtin_amdgcn_readfirstlane(id / row_blocks);
     const Seq sq = sequence(d, b);
-    const int64_t qlen = sq.len < d.a.max_q_len ? sq.len : d.a.max_q_len;
-    const int nrows = static_cast<int>(qlen * d.group);
+    const int nrows = rows_of(d, sq.len);
     const int rb0 = rb * BLOCK;
     const int32_t* table = d.a.page_table + b * d.a.table_stride;
     const int p0 = sq.kv - sq.len;
@@ -975,12 +983,12 @@ k_paged_tiles(PagedDev d) {
         const int m = 8 * (i / 4) + 4 * hf + i % 4;
         return FP ? DT * m + y : 32 * y + m;
     };
-    bool nan = l != l;
+    bool nan = false;  // a NaN total is the row's own: scores that it does not see are replaced
 #pragma unroll
     for (int y = 0; y < DT; ++y)
 #pragma unroll
         for (int i = 0; i < 16; ++i) nan = nan || acc[y][i] != acc[y][i];
-    const uint64_t bad = __ballot(nan && live);
+    const uint64_t bad = __ballot(nan && live && l == l);
     uint32_t rows = static_cast<uint32_t>(bad | bad >> 32);
     if (any && pmin != pmax) {
         // every wave is past the last step's barrier: the staging buffers are free
@@ -1008,12 +1016,12 @@ k_paged_tiles(PagedDev d) {
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
     const int64_t at = orow * d.splits + split;
     if (d.splits > 1 && hf == 0) {
-        float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+        float* ml = d.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
         ml[0] = m;
         ml[1] = l;
     }
     if constexpr (FP) {
-        float* to = d.splits > 1 ? d.a.part + at * D : static_cast<float*>(d.a.out) + orow * D;
+        float* to = d.splits > 1 ? d.part + at * D : static_cast<float*>(d.a.out) + orow * D;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float v[DT];
@@ -1032,7 +1040,7 @@ k_paged_tiles(PagedDev d) {
             const int dim = 32 * y + 2 * i + 4 * hf;
             f32x4 v = {acc[y][i], acc[y][i + 1], acc[y][i + 2], acc[y][i + 3]};
             if (d.splits > 1) {
-                *reinterpret_cast<f32x4*>(d.a.part + at * D + dim) = v;
+                *reinterpret_cast<f32x4*>(d.part + at * D + dim) = v;
                 continue;
             }
 #pragma unroll
@@ -1046,8 +1054,9 @@ k_paged_tiles(PagedDev d) {
 }
 
 // out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits of one
-// (row, head), a workgroup each.  Rows that no sequence names are not touched: the
-// grid walks the sequences.
+// (row, head), a workgroup each.  The row's sequence is looked up, 64 at a time,
+// while its parts are on their way: rows that no sequence of this launch names
+// are left as they were.
 template <int D, bool Q32, int JW>
 __global__ void __launch_bounds__(64 * JW)
 k_paged_join(PagedDev d) {
@@ -1055,15 +1064,10 @@ k_paged_join(PagedDev d) {
     __shared__ float part[JW][D];
     __shared__ float weight[JW][JW == 1 ? 1 : kMaxSplits];  // a wave's own copy
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t id = blockIdx.x;
-    const int head = id % d.a.q_heads;
-    id /= d.a.q_heads;
-    const int tok = id % static_cast<uint32_t>(d.a.max_q_len);
-    const Seq sq = sequence(d, id / static_cast<uint32_t>(d.a.max_q_len));
-    if (tok >= sq.len) return;
-    const int64_t orow = (sq.q0 + tok) * d.a.q_heads + head, at = orow * d.splits;
-    const float* ml = d.a.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
-    const float* po = d.a.part + at * D + PER * lane;
+    const int64_t orow = blockIdx.x, at = orow * d.splits;
+    const int64_t row = blockIdx.x / static_cast<uint32_t>(d.a.q_heads);
+    const float* ml = d.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+    const float* po = d.part + at * D + PER * lane;
     constexpr int MOST = JW == 1 ? kFewSplits : kMaxSplits, MX = (MOST + 63) / 64;
     // few splits: everything is on its way before the first wait
     float few[JW == 1 ? kFewSplits : 1][PER];
@@ -1083,6 +1087,16 @@ k_paged_join(PagedDev d) {
         l[x] = s < d.splits ? ml[2 * s + 1] : 0.0f;
         top = fmaxf(top, m[x]);
     }
+    bool named = false;
+    for (int64_t b0 = 0; b0 < d.a.batch && !named; b0 += 64) {
+        bool mine = false;
+        if (b0 + lane < d.a.batch) {
+            const Seq one = clipped(d, d.a.q_offsets[b0 + lane], d.a.q_offsets[b0 + lane + 1], 0);
+            mine = row >= one.q0 && (row - one.q0) * d.group < rows_of(d, one.len);
+        }
+        named = __ballot(mine) != 0;
+    }
+    if (!named) return;
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -1133,31 +1147,36 @@ k_paged_join(PagedDev d) {
     }
 }
 
-PagedDev plan(const KvCache& c, const PagedArgs& a, bool q_f32) {
+// One launch over the sequences of least .. most rows under a key head.
+PagedDev plan_one(const KvCache& c, const PagedArgs& a, int64_t least, int64_t most) {
     PagedDev d;
     d.a = a;
     d.c = c;
     d.page_shift = c.page_shift;
     d.group = a.q_heads / c.kv_heads;
     d.scale_log2 = a.scale * 1.4426950408889634f;
-    const int64_t rows = a.max_q_len * d.group, heads = a.batch * c.kv_heads;
+    d.least = static_cast<int>(least);
+    d.most = static_cast<int>(most);
+    d.max_q = std::min<int64_t>(a.max_q_len, std::max<int64_t>(most / d.group, 1));
+    const int64_t rows = d.max_q * d.group, heads = a.batch * c.kv_heads;
     // keys one tile can see, in steps of 32
     const int64_t keys = std::min<int64_t>(a.max_kv_len, static_cast<int64_t>(a.window) + a.sinks + 16);
     const int64_t steps = ceil_div(keys, 32);
-    d.tiled = rows >= kTiledRows;
-    int64_t splits;
+    d.tiled = most >= kTiledRows;
     d.waves = kWaves;
     d.lds_rows = static_cast<int>(std::min<int64_t>(kRows, rows));
     d.row_tiles = static_cast<int>(ceil_div(rows, d.tiled ? kBlockRows : kRows));
-    const int64_t tiles = heads * d.row_tiles;
+    int64_t tiles = heads * d.row_tiles, splits;
     if (d.tiled) {
-        splits = std::min<int64_t>(ceil_div(512, tiles), ceil_div(steps, 8));
+        // two workgroups a CU; blocks of rows there can be, and about how many there are
+        tiles = std::min<int64_t>(tiles, c.kv_heads * (a.rows * d.group / kBlockRows + a.batch));
+        splits = std::min<int64_t>(512 / ceil_div(a.rows * a.q_heads, kBlockRows), ceil_div(steps, 8));
     } else {
         // four workgroups a CU of a large batch, two where there are few tiles and
         // the parts to join weigh more (us with two / four: 64 x 8192 keys 148 /
         // 145, in 4 bits 99 / 89; 32 x 2051 27 / 31, 1 x 100000 39 / 42)
         splits = std::min<int64_t>(ceil_div(tiles > 128 ? 1024 : 512, tiles), ceil_div(steps, 2 * kWaves));
-        if (splits > 1 && steps <= 4 * kMostWaves) {
+        if (splits > 1 && steps <= 4 * kMostWaves && kMostWaves * d.lds_rows * (c.head_dim + 4) * 4 <= kPlainLds) {
             // short: one larger workgroup instead of a second launch
             d.waves = kMostWaves;
             splits = 1;
@@ -1168,25 +1187,39 @@ PagedDev plan(const KvCache& c, const PagedArgs& a, bool q_f32) {
     return d;
 }
 
+int64_t part_floats(const PagedDev& d) {
+    return d.splits > 1 ? ceil_div(d.a.rows * d.a.q_heads * d.splits * (d.c.head_dim + 2), 64) * 64 : 0;
+}
+
+// The launches of a call: long chunks to k_paged_tiles, the rest to
+// k_paged_rows.  Which sequence is which stands on the device; the host goes by
+// the lengths' bound and mean: where all but the longest can only be short, a
+// batch may mix chunks with steps and both are launched, else one serves all.
+struct Plan {
+    PagedDev d[2];
+    int n;
+};
+Plan plan(const KvCache& c, const PagedArgs& a) {
+    Plan p;
+    const int64_t group = a.q_heads / c.kv_heads, longest = a.max_q_len * group;
+    const bool mixed = longest >= kTiledRows && a.batch > 1 &&
+                       (a.rows - a.max_q_len) * group < kTiledRows * (a.batch - 1);
+    p.n = mixed ? 2 : 1;
+    p.d[0] = plan_one(c, a, mixed ? kTiledRows : 1, longest);
+    if (mixed) p.d[1] = plan_one(c, a, 1, kTiledRows - 1);
+    return p;
+}
+
 template <int D, bool Q32, Kv KV>
 hipError_t launch(const PagedDev& d, hipStream_t s) {
-    const int64_t joins = d.a.batch * d.a.max_q_len * d.a.q_heads;
-    if (d.blocks > 0x7FFFFFF0 || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
-    const dim3 block(64 * kWaves);
+    const int64_t joins = d.a.rows * d.a.q_heads;
+    if (d.blocks > 0x7FFFFFFF || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
+    const dim3 blocks(static_cast<unsigned>(d.blocks)), grid(static_cast<unsigned>(joins));
     if (d.tiled)
-        hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)), block, 0, s, d);
-    if (!d.tiled) {
-        const unsigned lds = static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4;
-        if (lds > kPlainLds) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_paged_rows<D, Q32, KV>),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                     static_cast<int>(lds));
-            if (e != hipSuccess) return e;
-        }
-        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), dim3(static_cast<unsigned>(d.blocks)), dim3(64 * d.waves), lds,
-                           s, d);
-    }
-    const dim3 grid(static_cast<unsigned>(joins));
+        hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), blocks, dim3(64 * kWaves), 0, s, d);
+    else
+        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), blocks, dim3(64 * d.waves),
+                           static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4, s, d);
     if (d.splits > 64) hipLaunchKernelGGL((k_paged_join<D, Q32, 16>), grid, dim3(1024), 0, s, d);
     else if (d.splits > kFewSplits) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
     else if (d.splits > 1) hipLaunchKernelGGL((k_paged_join<D, Q32, 1>), grid, dim3(64), 0, s, d);
@@ -1203,15 +1236,24 @@ hipError_t launch_d(const PagedDev& d, bool q_f32, hipStream_t s) {
 
 }  // namespace
 
-size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a, bool q_f32) {
-    const PagedDev d = plan(cache, a, q_f32);
-    return d.splits > 1 ? static_cast<size_t>(a.rows) * a.q_heads * d.splits * (cache.head_dim + 2) * 4 : 0;
+size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a) {
+    const Plan p = plan(cache, a);
+    int64_t n = 0;
+    for (int i = 0; i < p.n; ++i) n += part_floats(p.d[i]);
+    return static_cast<size_t>(n) * 4;
 }
 
 hipError_t launch_attention_paged(const KvCache& cache, const PagedArgs& a, bool q_f32, hipStream_t s) {
     if (a.rows <= 0 || a.batch <= 0 || a.max_q_len <= 0) return hipSuccess;
-    const PagedDev d = plan(cache, a, q_f32);
-    return cache.head_dim == 128 ? launch_d<128>(d, q_f32, s) : launch_d<64>(d, q_f32, s);
+    Plan p = plan(cache, a);
+    float* part = a.part;
+    for (int i = 0; i < p.n; ++i) {
+        p.d[i].part = part;
+        part += part_floats(p.d[i]);
+        const hipError_t e = cache.head_dim == 128 ? launch_d<128>(p.d[i], q_f32, s) : launch_d<64>(p.d[i], q_f32, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace aps

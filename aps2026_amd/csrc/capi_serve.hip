@@ -1,7 +1,5 @@
 // C ABI of the serving operators (declared in include/aps_serve.h): argument
 // checks, then the launches.
-#include <algorithm>
-
 #include "../../include/aps_serve.h"
 #include "serve.hpp"
 
@@ -151,8 +149,7 @@ size_t aps_attention_paged_workspace_size(const aps_kv_cache* cache, int64_t row
     if (check_cache(cache, "attention_paged", false, &c)) return 0;
     if (check_paged(c, rows, q_heads, batch, max_q_len, max_kv_len, window, sinks, &a)) return 0;
     if (rows == 0 || batch == 0 || a.max_q_len == 0) return 0;
-    // enough for queries of either type
-    return std::max(aps::attention_paged_part_bytes(c, a, true), aps::attention_paged_part_bytes(c, a, false));
+    return aps::attention_paged_part_bytes(c, a);
 }
 
 int aps_attention_paged(const aps_kv_cache* cache, const void* q, int64_t q_stride, int32_t q_dtype, int64_t rows,
@@ -179,7 +176,7 @@ int aps_attention_paged(const aps_kv_cache* cache, const void* q, int64_t q_stri
     if (mis(q, 16) || mis(out, 16)) return fail(APS_ERR_ARG, "%s: q and out must be 16-byte aligned", what);
     if (mis(q_offsets, 4) || mis(kv_lens, 4) || mis(page_table, 4))
         return fail(APS_ERR_ARG, "%s: index arrays must be 4-byte aligned", what);
-    const size_t need = aps::attention_paged_part_bytes(c, a, q_dtype == APS_DTYPE_F32);
+    const size_t need = aps::attention_paged_part_bytes(c, a);
     if (need && (!workspace || workspace_bytes < need))
         return fail(APS_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
     if (need && mis(workspace, 256)) return fail(APS_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", what);

@@ -45,7 +45,7 @@ struct PagedArgs {
     float* part;  // partial results of a split key axis
 };
 // Bytes of `part`, and the launch; both follow one plan of the sizes.
-size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a, bool q_f32);
+size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a);
 hipError_t launch_attention_paged(const KvCache& cache, const PagedArgs& a, bool q_f32, hipStream_t s);
 
 struct LogitsArgs {

@@ -170,6 +170,7 @@ SHAPES = {
     "guesses": ([5, 3, 9], [90, 3, 161], 64, 4),
     "empty": ([0, 2, 0, 4, 1], [0, 5, 31, 2, 0], 16, 2),      # more queries than keys, no keys, no queries
     "chunk": ([77, 40], [77, 200], 2047, 0),
+    "mixed": ([1, 90, 0, 2, 1, 1, 3, 1, 1, 1], [70, 90, 4, 2, 300, 33, 3, 1, 0, 64], 2047, 1),
     "chunk_window": ([100, 33, 1], [150, 33, 90], 30, 7),
 }
 
