@@ -1168,9 +1168,12 @@ PagedDev plan_one(const KvCache& c, const PagedArgs& a, int64_t least, int64_t m
     d.row_tiles = static_cast<int>(ceil_div(rows, d.tiled ? kBlockRows : kRows));
     int64_t tiles = heads * d.row_tiles, splits;
     if (d.tiled) {
-        // two workgroups a CU; blocks of rows there can be, and about how many there are
+        // the blocks of rows that there can be, and about how many there are; two
+        // workgroups a CU and no more (a third round costs what a split saves)
         tiles = std::min<int64_t>(tiles, c.kv_heads * (a.rows * d.group / kBlockRows + a.batch));
-        splits = std::min<int64_t>(512 / ceil_div(a.rows * a.q_heads, kBlockRows), ceil_div(steps, 8));
+        const int64_t about = std::max<int64_t>(ceil_div(a.rows * a.q_heads, kBlockRows),
+                                                c.kv_heads * (least > 1 ? 1 : a.batch));
+        splits = std::min<int64_t>(512 / about, ceil_div(steps, 8));
     } else {
         // four workgroups a CU of a large batch, two where there are few tiles and
         // the parts to join weigh more (us with two / four: 64 x 8192 keys 148 /
