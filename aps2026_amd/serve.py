@@ -41,16 +41,24 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _launch(fn, device: torch.device, *args) -> None:
     """fn(*args, the current stream of device), with device current."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
     if rc:
         _call(rc)
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An unset contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _dev(t: torch.Tensor, device: torch.device, dtype: torch.dtype, what: str) -> int:
@@ -65,6 +73,9 @@ class PagedKvCache:
     bf16; or, given k_scale and v_scale, 4-bit codes [..][head_dim / 2] (uint8)
     with scale bytes [..][head_dim / 32] (uint8).  The tensors stay the
     caller's; allocate() makes them."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "pages", "kv_heads", "page_size", "head_dim", "dtype", "device",
+                 "_desc", "_ref")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
@@ -170,8 +181,7 @@ def kv_append_gpu(cache: PagedKvCache, k: torch.Tensor, v: torch.Tensor, positio
             raise ValueError("kv_append: q [rows, q_heads * head_dim] of k's type")
         q_heads = q_width // dim
         if q_out is None:
-            q_out = torch.empty((rows, q_width), dtype=dt, device=dev)
-            o_stride = q_width
+            q_out, o_stride = _like(q), q_width
         elif q_out.shape != q.shape or q_out.dtype is not dt or q_out.device != dev:
             raise ValueError("kv_append: q_out of q's shape and type")
         else:
@@ -217,7 +227,7 @@ def attention_paged_gpu(q: torch.Tensor, cache: PagedKvCache, q_offsets: torch.T
     if q_offsets.numel() != batch + 1 or len(table) != 2 or table[0] != batch:
         raise ValueError("attention_paged shape")
     if out is None:
-        out = torch.empty((rows, width), dtype=dt, device=dev)
+        out = _like(q)
     elif out.shape != (rows, width) or out.dtype is not dt or out.device != dev or not out.is_contiguous():
         raise ValueError("attention_paged: out of q's shape and type, contiguous")
     if scale is None:
@@ -262,7 +272,7 @@ def logits_process_gpu(logits: torch.Tensor, history: Optional[torch.Tensor] = N
         raise ValueError("logits_process: fp32 or bf16 logits on a GPU")
     stride = _rows_of(logits, vocab, what)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=dt, device=dev)
+        out = _like(logits)
     elif out.shape != logits.shape or out.dtype is not dt or out.device != dev:
         raise ValueError("logits_process: out of the logits' shape and type")
     rules = capi.LogitsRules()

@@ -420,6 +420,72 @@ def test_step_in_a_graph_and_on_another_stream(gpu_device, qt, kind):
         assert torch.equal(bits(other), bits(want)), n
 
 
+@pytest.mark.parametrize("qt,kind", [(F32, "bf16"), (BF16, "mxfp4"), (F32, "f32")])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1] * 70 + [2], [7 + 3 * i for i in range(71)]),
+                                            ([11] * 66, [20 + 2 * i for i in range(66)]),
+                                            ([1, 40] * 35, [50 + i for i in range(70)])])
+def test_many_sequences(gpu_device, qt, kind, q_lens, kv_lens):
+    """More sequences than a wave has lanes."""
+    note(f"many sequences {qt} {kind} {len(q_lens)}")
+    c = Case(gpu_device, qt, kind, 4, 1, 64, 16, q_lens, kv_lens, seed=12)
+    c.check(c.run(40, 2), 40, 2)
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 2], [1800, 1500]), ([40], [1700]), ([50, 1], [1300, 1900])])
+def test_split_rows_left_alone(gpu_device, q_lens, kv_lens):
+    """The join of a split key axis writes the rows of the sequences alone."""
+    for qt, kind in ((BF16, "bf16"), (F32, "mxfp4")):
+        note(f"split rows left alone {qt} {kind} {q_lens}")
+        c = Case(gpu_device, qt, kind, 4, 1, 128, 16, q_lens, kv_lens, extra_rows=5, seed=9)
+        c.offs[:] = c.offs + 2                       # two rows before the first sequence, three behind the last
+        out = torch.full((c.rows, 4 * 128), 3.0, dtype=qt, device=gpu_device)
+        c.run(1 << 30, 0, out=out)
+        n = sum(q_lens)
+        assert bool((out[:2] == 3.0).all()) and bool((out[2 + n:] == 3.0).all())
+        c.q, c.offs, c.rows = c.q[2:2 + n].contiguous(), c.offs - 2, n
+        c.check(out[2:2 + n], 1 << 30, 0)
+
+
+@pytest.mark.parametrize("qt,kind", [(F32, "f32"), (F32, "bf16"), (BF16, "mxfp4")])
+@pytest.mark.parametrize("q_lens,kv_lens", [([3, 1], [40, 50]), ([60, 2], [90, 64])])
+def test_a_row_that_is_nan_stays_alone(gpu_device, qt, kind, q_lens, kv_lens):
+    c = Case(gpu_device, qt, kind, 4, 2, 64, 16, q_lens, kv_lens, seed=21)
+    clean = f64(c.run(64, 1))
+    c.q[1] = float("nan")
+    got = f64(c.run(64, 1))
+    assert np.isnan(got[1]).all()
+    keep = np.arange(c.rows) != 1
+    assert np.array_equal(got[keep], clean[keep])
+
+
+def test_two_graphs_at_once(gpu_device):
+    """Two recorded calls replayed together on two streams share nothing."""
+    dev = gpu_device
+    cases = [Case(dev, BF16, "bf16", 8, 2, 128, 16, [1, 1], [1900, 1500], seed=31),
+             Case(dev, F32, "mxfp4", 8, 2, 128, 16, [2, 40], [1200, 300], seed=32)]
+    side = [torch.cuda.Stream(dev), torch.cuda.Stream(dev)]
+    graphs, outs, want = [], [], []
+    for c in cases:
+        args = (c.up(c.offs), c.up(c.kv_lens), c.up(c.table), c.max_q, c.max_kv)
+        call = lambda c=c, args=args: serve.attention_paged_gpu(c.q, c.cache, *args, q_heads=8, window=1 << 30)  # noqa: E731
+        want.append(call().clone())
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call())
+        graphs.append((g, args))
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for (g, _a), st in zip(graphs, side):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(bits(o), bits(w))
+
+
 def test_attention_of_nothing(gpu_device):
     c = Case(gpu_device, BF16, "bf16", 4, 1, 64, 16, [1, 1], [5, 7], seed=2)
     e = torch.empty(0, dtype=torch.int32, device=gpu_device)
@@ -517,6 +583,33 @@ def test_logits_rules_alone(gpu_device):
     for other in ("bias_ids", "bias_values", "bias_lens"):
         q.pop(other)
     assert torch.equal(bits(got), bits(_logit_want(x, q)))
+
+
+def test_logits_in_a_graph_and_on_another_stream(gpu_device):
+    dev = gpu_device
+    x, r = _logit_case(dev, F32, 3, 5000, 90, 7, True, seed=2)
+    t = {n: torch.from_numpy(a).to(dev) for n, a in r.items()}
+    want = bits(_logit_want(x, r))
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        got = serve.logits_process_gpu(x, **t)
+    side.synchronize()
+    assert torch.equal(bits(got), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = serve.logits_process_gpu(x, **t)
+    for _ in range(4):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(bits(out), want)
+        serve.logits_process_gpu(x)
+        t["history_lens"].add_(0)
+    t["history_lens"].zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(bits(out), bits(_logit_want(x, {**r, "history_lens": np.zeros(3, np.int32)})))
 
 
 def test_logits_that_are_not_finite(gpu_device):
