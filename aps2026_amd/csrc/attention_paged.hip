@@ -701,52 +701,6 @@ k_paged_tiles(PagedDev d) {
     const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
     const View vis = view(d, live ? p0 + tok : -1);
 
-    // queries: a lane holds dims 16 s + 8 hf + j of its row; the sign of the
-    // scale goes into them, so that the largest product is the largest score
-    bf16x8 qb[FP ? 1 : QT][FP ? 1 : KS];
-    f32x4 qf[FP ? KS : 1];
-    const float cs = d.scale_log2 == 0.0f ? 1.0f : fabsf(d.scale_log2);
-    const uint32_t flip = d.scale_log2 < 0.0f ? (FP ? 0x80000000u : 0x80008000u) : 0u;
-    const uint32_t keep = d.scale_log2 == 0.0f ? 0u : ~0u;
-    {
-        const int64_t qat = (sq.q0 + tok) * d.a.q_stride + static_cast<int64_t>(qh) * D;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int dim = (FP ? 8 : 16) * s + (FP ? 4 : 8) * hf;
-            if constexpr (FP) {
-                u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const float*>(d.a.q) + qat + dim);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
-                qf[s] = __builtin_bit_cast(f32x4, w);
-                continue;
-            }
-            if constexpr (FP) {
-            } else if constexpr (Q32) {
-                const float* p = static_cast<const float*>(d.a.q) + qat + dim;
-                const f32x4 x0 = *reinterpret_cast<const f32x4*>(p), x1 = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float x = j < 4 ? x0[j & 3] : x1[j & 3];
-#pragma unroll
-                    for (int t = 0; t < QT; ++t) {
-                        const float hi = bf16_round(x);
-                        qb[t][s][j] = static_cast<__bf16>(hi);
-                        x -= hi;
-                    }
-                }
-            } else {
-                qb[0][s] = *reinterpret_cast<const bf16x8*>(static_cast<const bf16_t*>(d.a.q) + qat + dim);
-            }
-#pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                u32x4 w = __builtin_bit_cast(u32x4, qb[t][s]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
-                qb[t][s] = __builtin_bit_cast(bf16x8, w);
-            }
-        }
-    }
-
     // ---- staging, one step ahead.  64 keys: a wave copies 16 keys of K and of V;
     // 32 keys: two waves copy K, two V.
     const int grp = wave % GROUPS;
@@ -833,6 +787,54 @@ k_paged_tiles(PagedDev d) {
         }
     };
 
+    if (t0 < t1) fetch(t0, 0);  // on its way while the queries are read
+
+    // queries: a lane holds dims 16 s + 8 hf + j of its row; the sign of the
+    // scale goes into them, so that the largest product is the largest score
+    bf16x8 qb[FP ? 1 : QT][FP ? 1 : KS];
+    f32x4 qf[FP ? KS : 1];
+    const float cs = d.scale_log2 == 0.0f ? 1.0f : fabsf(d.scale_log2);
+    const uint32_t flip = d.scale_log2 < 0.0f ? (FP ? 0x80000000u : 0x80008000u) : 0u;
+    const uint32_t keep = d.scale_log2 == 0.0f ? 0u : ~0u;
+    {
+        const int64_t qat = (sq.q0 + tok) * d.a.q_stride + static_cast<int64_t>(qh) * D;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int dim = (FP ? 8 : 16) * s + (FP ? 4 : 8) * hf;
+            if constexpr (FP) {
+                u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const float*>(d.a.q) + qat + dim);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
+                qf[s] = __builtin_bit_cast(f32x4, w);
+                continue;
+            }
+            if constexpr (FP) {
+            } else if constexpr (Q32) {
+                const float* p = static_cast<const float*>(d.a.q) + qat + dim;
+                const f32x4 x0 = *reinterpret_cast<const f32x4*>(p), x1 = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float x = j < 4 ? x0[j & 3] : x1[j & 3];
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        const float hi = bf16_round(x);
+                        qb[t][s][j] = static_cast<__bf16>(hi);
+                        x -= hi;
+                    }
+                }
+            } else {
+                qb[0][s] = *reinterpret_cast<const bf16x8*>(static_cast<const bf16_t*>(d.a.q) + qat + dim);
+            }
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                u32x4 w = __builtin_bit_cast(u32x4, qb[t][s]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
+                qb[t][s] = __builtin_bit_cast(bf16x8, w);
+            }
+        }
+    }
+
     // LDS offsets of a lane's operands
     int k_off[KS], v_off[DT];
 #pragma unroll
@@ -851,10 +853,7 @@ k_paged_tiles(PagedDev d) {
         for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    if (t0 < t1) {
-        fetch(t0, 0);
-        commit(t0, 0);
-    }
+    if (t0 < t1) commit(t0, 0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1, base = base_of(t);
