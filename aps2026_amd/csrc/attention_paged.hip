@@ -369,10 +369,11 @@ k_paged_rows(PagedDev d) {
     };
 
     // A step is read one ahead (37 x 2051 fp32 keys 80 -> 63 us, 64 x 8192 bf16 154
-    // -> 148), except of a 4-bit cache, whose steps are short and whose decoding
+    // -> 148; of a 4-bit cache with fp32 queries 64 x 16384 keys 132 -> 111), except
+    // of a 4-bit cache with BF16 queries, whose steps are short and whose decoding
     // wants the registers for a third or fourth wave (64 x 16384 keys 92, read
-    // ahead 96).
-    constexpr bool EARLY = !MX;
+    // ahead 98).
+    constexpr bool EARLY = !MX || Q32;
     Step next;
     if (EARLY && t0 < t1) load(t0, next);
     for (int t = t0; t < t1; ++t) {

@@ -85,8 +85,9 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * [q_heads][head_dim] contiguous, of q's type.  q_heads is a multiple of
  * kv_heads; query head h reads key head h / (q_heads / kv_heads).
  * q_dtype F32 takes every cache type, BF16 the BF16 and MXFP4 ones.  Products
- * are exact and sums are fp32; with BF16 queries the softmax weights are
- * rounded to bf16 for their product with v where a sequence has many rows.
+ * are exact and sums are fp32; with BF16 queries the softmax weights of a
+ * sequence with more than 32 rows (tokens times q_heads / kv_heads) are rounded
+ * to bf16 for their product with v, other sequences' to 16 bits.
  *
  * All arrays in device memory.  max_q_len and max_kv_len bound the batch's
  * lengths on the host (they shape the launch, so a recorded graph serves any
@@ -94,12 +95,12 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * were, lengths past max_kv_len or past table_stride pages are cut.
  * Rows of out that no sequence names are left as they were.  A query that sees
  * no key (kv_lens[b] below its queries' number, or 0), or whose every score is
- * -inf, gives zeros.  A page id outside the cache leaves its keys out; ids of
- * pages that no query sees are not read from.  Values and keys that a row does
+ * -inf, gives zeros.  A page id outside the cache leaves its keys out; entries
+ * for pages that no query sees may hold anything.  Values and keys that a row does
  * not see do not reach it, infinities and NaN among them.
  * workspace: aps_attention_paged_workspace_size bytes (0: none), 256-byte
  * aligned; calls that overlap need one each.  q, out 16-byte aligned, q_stride
- * a multiple of 16 bytes. */
+ * a multiple of 16 bytes.  out and workspace overlap nothing else of the call. */
 APS_API size_t aps_attention_paged_workspace_size(const aps_kv_cache* cache, int64_t rows, int32_t q_heads,
                                                   int64_t batch, int64_t max_q_len, int64_t max_kv_len,
                                                   int32_t window, int32_t sinks);
