@@ -203,7 +203,6 @@ __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const K
             const float f = exp2_fast(m - ref), p = exp2_fast(s - ref);
             m = mn;
             l = l * f + p;
-            // a key whose weight is 0 counts for nothing even where its value is not finite
 #pragma unroll
             for (int j = 0; j < PER; ++j)
                 acc[j] = fmaf(p, element<D, KV>(d.c.v, d.c.v_scale, hr, PER * lane + j), acc[j] * f);
@@ -990,7 +989,9 @@ k_paged_tiles(PagedDev d) {
         for (int i = 0; i < 16; ++i) nan = nan || acc[y][i] != acc[y][i];
     const uint64_t bad = __ballot(nan && live && l == l);
     uint32_t rows = static_cast<uint32_t>(bad | bad >> 32);
-    if (any && pmin != pmax) {
+    // (values are set to zero where no row of the block sees them: a wave's rows may
+    // all be one token's that does not see what another wave's do)
+    if (any && rb0 / d.group != rb1 / d.group) {
         // every wave is past the last step's barrier: the staging buffers are free
         float* red = reinterpret_cast<float*>(&sm[0][0][0]) + wave * (D + 2);
         while (rows) {

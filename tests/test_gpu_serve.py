@@ -298,6 +298,28 @@ def test_unseen_values_do_not_reach_a_row(gpu_device, qt, kind, q_lens, kv_lens)
     assert (np.abs(got - want.reshape(c.rows, -1)) <= bound)[~hit].all()
 
 
+@pytest.mark.parametrize("qt,kind", [(F32, "f32"), (F32, "bf16"), (F32, "mxfp4"), (BF16, "bf16"), (BF16, "mxfp4")])
+@pytest.mark.parametrize("qh,kvh,n,kv,window,back", [(32, 1, 4, 60, 2047, 0),    # 32 rows a token
+                                                     (32, 1, 4, 60, 3, 4), (64, 1, 2, 1500, 2047, 0),
+                                                     (8, 2, 41, 97, 3, 8)])       # one token behind full ones
+def test_unseen_values_of_other_tokens(gpu_device, qt, kind, qh, kvh, n, kv, window, back):
+    """A value that is not finite, `back` keys before the last, and groups of
+    rows that are one token's, whose neighbours' keys it does not see."""
+    note(f"other tokens {qt} {kind} {qh}/{kvh} {n} {kv} {window}")
+    c = Case(gpu_device, qt, kind, qh, kvh, 64, 16, [n], [kv], seed=5)
+    j = kv - 1 - back
+    page, off = c.table[0, j // 16], j % 16
+    if kind == "mxfp4":
+        c.cache.v_scale[page, :, off] = 255
+    else:
+        c.cache.v[page, :, off] = float("inf")
+    got = f64(c.run(window, 0)).reshape(n, -1)
+    at = np.arange(kv - n, kv)
+    hit = (j <= at) & (j > at - window)
+    assert hit.any() and not hit.all()
+    assert np.isfinite(got[~hit]).all() and not np.isfinite(got[hit]).any()
+
+
 @pytest.mark.parametrize("qt,kind", [(F32, "bf16"), (BF16, "mxfp4")])
 def test_rows_left_alone_and_pages_left_out(gpu_device, qt, kind):
     """Rows behind the last sequence and past max_q_len keep their bytes; page
