@@ -8,8 +8,14 @@ namespace {
 using aps::fail;
 
 constexpr int64_t kMaxRows = int64_t(1) << 30;
+constexpr int64_t kMaxBatch = int64_t(1) << 20;  // workgroups look their sequence up among all of them
 
 bool mis(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+bool overlap(const void* p, size_t np, const void* q, size_t nq) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return np && nq && a < b + nq && b < a + np;
+}
 
 int launched(hipError_t err, const char* what) {
     if (err == hipSuccess) return APS_OK;
@@ -66,7 +72,7 @@ int check_paged(const aps::KvCache& c, int64_t rows, int32_t q_heads, int64_t ba
                 int64_t max_kv_len, int32_t window, int32_t sinks, aps::PagedArgs* a) {
     const char* what = "attention_paged";
     if (int rc = check_heads(c, q_heads, what)) return rc;
-    if (rows < 0 || rows > kMaxRows || batch < 0 || batch > kMaxRows || max_q_len < 0 || max_kv_len < 0 ||
+    if (rows < 0 || rows > kMaxRows || batch < 0 || batch > kMaxBatch || max_q_len < 0 || max_kv_len < 0 ||
         max_kv_len > kMaxRows)
         return fail(APS_ERR_SHAPE, "%s: rows %lld, batch %lld, max_q_len %lld, max_kv_len %lld", what, (long long)rows,
                     (long long)batch, (long long)max_q_len, (long long)max_kv_len);
@@ -180,6 +186,12 @@ int aps_attention_paged(const aps_kv_cache* cache, const void* q, int64_t q_stri
     if (need && (!workspace || workspace_bytes < need))
         return fail(APS_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
     if (need && mis(workspace, 256)) return fail(APS_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", what);
+    // rows are read after others were written: nothing in place
+    const size_t elt = q_dtype == APS_DTYPE_F32 ? 4 : 2, out_bytes = static_cast<size_t>(rows * qd) * elt;
+    const size_t q_bytes = static_cast<size_t>((rows - 1) * q_stride + qd) * elt;
+    if (overlap(out, out_bytes, q, q_bytes) || overlap(workspace, need, out, out_bytes) ||
+        overlap(workspace, need, q, q_bytes))
+        return fail(APS_ERR_ARG, "%s: q, out and workspace overlap", what);
     a.q = q;
     a.q_stride = q_stride;
     a.q_offsets = q_offsets;

@@ -398,6 +398,10 @@ class Model:
             raise ValueError("sequence is too long")
         if flat.min() < 0 or flat.max() >= self.emb.shape[0]:
             raise ValueError("token out of vocabulary")
+        if not repetition > 0.0:
+            raise ValueError("repetition must be positive")
+        if mask is not None and (mask.dim() != 2 or mask.shape[0] not in (1, n_seq)):
+            raise ValueError("mask: one row of words, or one a prompt")
         # pages for the whole answer, consecutive for each sequence
         need = [-(-(n + max_new_tokens - 1) // page_size) for n in lens]
         first = np.cumsum([0] + need)

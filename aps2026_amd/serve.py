@@ -39,8 +39,6 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 # A decode step is a row of short launches, so what Python does around them
 # counts: the stream's handle without an object for it, checks on plain numbers.
 _raw_stream = torch._C._cuda_getCurrentRawStream
-
-
 _current_device = torch._C._cuda_getDevice
 
 
@@ -215,7 +213,7 @@ def attention_paged_gpu(q: torch.Tensor, cache: PagedKvCache, q_offsets: torch.T
     keys they see: the last `window` up to their own and the first `sinks`.
     scale: 1 / sqrt(head_dim) unless given.  The workspace is torch's, taken
     on the current stream, unless one is given (uint8).  Rows of a given `out`
-    that no sequence names are left as they were."""
+    (not q) that no sequence names are left as they were, of a new one unset."""
     what, dev, dim = "attention_paged", cache.device, cache.head_dim
     width = q_heads * dim
     q_stride = _rows_of(q, width, what)
@@ -232,7 +230,9 @@ def attention_paged_gpu(q: torch.Tensor, cache: PagedKvCache, q_offsets: torch.T
         raise ValueError("attention_paged: out of q's shape and type, contiguous")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    window = min(window, 0x7FFFFFFF)
+    if window < 1 or sinks < 0:
+        raise ValueError("attention_paged: window >= 1 and sinks >= 0")
+    window, sinks = min(window, 0x7FFFFFFF), min(sinks, 0x7FFFFFFF)
     lib = capi.lib()
     need = lib.aps_attention_paged_workspace_size(cache._ref, rows, q_heads, batch, max_q_len, max_kv_len, window,
                                                   sinks)

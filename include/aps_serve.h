@@ -85,11 +85,12 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * [q_heads][head_dim] contiguous, of q's type.  q_heads is a multiple of
  * kv_heads; query head h reads key head h / (q_heads / kv_heads).
  * q_dtype F32 takes every cache type, BF16 the BF16 and MXFP4 ones.  Products
- * are exact and sums are fp32; with BF16 queries the softmax weights of a
- * sequence with more than 32 rows (tokens times q_heads / kv_heads) are rounded
- * to bf16 for their product with v, other sequences' to 16 bits.
+ * are exact and sums are fp32; with BF16 queries the softmax weights are held
+ * to 16 bits for their product with v, and to bf16's 8 in a call whose longest
+ * sequence may have more than 32 rows (max_q_len times q_heads / kv_heads).
  *
- * All arrays in device memory.  max_q_len and max_kv_len bound the batch's
+ * All arrays in device memory; q_offsets ascend; batch up to 2^20, max_kv_len up
+ * to 2^30.  max_q_len and max_kv_len bound the batch's
  * lengths on the host (they shape the launch, so a recorded graph serves any
  * lengths within them): queries past max_q_len of a sequence are left as they
  * were, lengths past max_kv_len or past table_stride pages are cut.
@@ -97,10 +98,12 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * no key (kv_lens[b] below its queries' number, or 0), or whose every score is
  * -inf, gives zeros.  A page id outside the cache leaves its keys out; entries
  * for pages that no query sees may hold anything.  Values and keys that a row does
- * not see do not reach it, infinities and NaN among them.
+ * not see do not reach it, infinities and NaN among them; of those that it does
+ * see, NaN may stand where the formula has an infinity.
  * workspace: aps_attention_paged_workspace_size bytes (0: none), 256-byte
  * aligned; calls that overlap need one each.  q, out 16-byte aligned, q_stride
- * a multiple of 16 bytes.  out and workspace overlap nothing else of the call. */
+ * a multiple of 16 bytes.  out and workspace overlap nothing else of the call (refused
+ * for q, out and workspace). */
 APS_API size_t aps_attention_paged_workspace_size(const aps_kv_cache* cache, int64_t rows, int32_t q_heads,
                                                   int64_t batch, int64_t max_q_len, int64_t max_kv_len,
                                                   int32_t window, int32_t sinks);

@@ -133,3 +133,9 @@ def test_decode_refusals(model, gpu_device):
         model.generate_decode([[1] * 4000], 98)
     with pytest.raises(ValueError, match="token out of vocabulary"):
         model.generate_decode([[V]], 1)
+    with pytest.raises(ValueError, match="repetition must be positive"):
+        model.generate_decode([[1]], 1, repetition=0.0)
+    with pytest.raises(ValueError, match="one row of words"):
+        model.generate_decode([[1], [2]], 1, mask=torch.full((3, V // 32 + 1), -1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="window >= 1"):
+        model.generate_decode([[1]], 1, window=1 << 33, sinks=-1)

@@ -133,6 +133,27 @@ def test_attention_of_nothing_and_workspace():
     assert attend(**long, ws=P + 16, wb=need) == capi.APS_ERR_WORKSPACE
 
 
+@pytest.mark.parametrize("kw", [
+    dict(out=P), dict(out=P + 2048 * 2 * 4 - 16), dict(out=P - 2048 * 2 * 4 + 16),
+    dict(qs=4096, out=P + 4096 * 2 * 3 + 2048 * 2 - 16),
+])
+def test_attention_in_place_is_refused(kw):
+    assert attend(**kw) == capi.APS_ERR_ARG
+    assert "overlap" in capi.last_error()
+
+
+def test_attention_workspace_overlap_is_refused():
+    long = dict(rows=1, batch=1, mk=131072, window=131072, sinks=0)
+    need = capi.lib().aps_attention_paged_workspace_size(cache(), 1, 16, 1, 1, 131072, 131072, 0)
+    for q, out in ((P, 16 * P), (16 * P, P), (16 * P, P + need - 16)):
+        assert attend(**long, q=q, out=out, ws=P, wb=need) == capi.APS_ERR_ARG
+        assert "overlap" in capi.last_error()
+
+
+def test_attention_of_too_many_sequences():
+    assert attend(batch=(1 << 20) + 1) == capi.APS_ERR_SHAPE
+
+
 def logits(rules=None, rows=1, **kw):
     d = dict(x=P, xs=100, dt=capi.DTYPE_F32, vocab=100, out=P, os=100)
     d.update(kw)
