@@ -156,6 +156,14 @@ __device__ inline float max_x16(float x) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// x and the lanes c ^ 7 (row_half_mirror) or c ^ 8 (row_ror:8) of the 16: sums of
+// the same two numbers in either lane.
+template <int CTRL>
+__device__ inline float plus_dpp(float x) {
+    return x + __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+constexpr int kHalfMirror = 0x141, kRor8 = 0x128;
+__device__ inline float less_bits(float x, uint32_t mask) { return x - __uint_as_float(__float_as_uint(x) & mask); }
 __device__ inline float bf16_round(float x) { return __uint_as_float(pack2_bf16(x, 0.0f) << 16); }
 
 // One cached element as fp32 (redo_row).
@@ -213,15 +221,20 @@ __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const K
     if (lane == 0) { *m_out = m; *l_out = l; }
 }
 
-template <int D, bool Q32, Kv KV>
+// SIDE: few rows (side_rows), whose terms stand side by side in the 16 columns of
+// the MFMAs: column c holds term c / 4 of row c % 4 (mirrored where c & 4, for the
+// sums over lanes c ^ 7), with BF16 queries term c / 8 of row c % 8.
+constexpr int side_rows(bool q32) { return q32 ? 4 : 8; }
+
+template <int D, bool Q32, Kv KV, bool SIDE>
 __global__ void __launch_bounds__(64 * kMostWaves, 2)
 k_paged_rows(PagedDev d) {
     constexpr bool FP = KV == Kv::kF32;
     constexpr int HALVES = FP ? 1 : 2;
     constexpr int STEP = 16 * HALVES;
     constexpr int W = D / 16;          // dims of V a lane reads of a key, and dim tiles
-    constexpr int QT = Q32 ? 3 : 1;    // bf16 terms of a query
-    constexpr int PT = Q32 ? 3 : 2;    // bf16 terms of a weight
+    constexpr int QT = Q32 && !SIDE ? 3 : 1;        // products a query's bf16 terms take
+    constexpr int PT = SIDE ? 1 : Q32 ? 3 : 2;      // and a weight's
     constexpr int KS = D / 32;         // MFMA steps over the dims
     constexpr int OSTRIDE = D + 4;     // LDS row, off the banks' period
     __shared__ float sm_m[kMostWaves][kRows], sm_l[kMostWaves][kRows];
@@ -247,10 +260,13 @@ k_paged_rows(PagedDev d) {
     const int r_last = r0 + kRows - 1 < nrows ? r0 + kRows - 1 : nrows - 1;
     const int pmin = __builtin_amdgcn_readfirstlane(p0 + r0 / d.group);
     const int pmax = __builtin_amdgcn_readfirstlane(p0 + r_last / d.group);
-    const int row = r0 + c;
+    const int term = !SIDE ? 0 : Q32 ? c >> 2 : c >> 3;
+    const int row = r0 + (!SIDE ? c : !Q32 ? c & 7 : c & 4 ? 3 - (c & 3) : c & 3);
     const bool live = row < nrows;
     const int tok = live ? row / d.group : 0, qh = h * d.group + (live ? row % d.group : 0);
     const int pos = live ? p0 + tok : -1;
+    // what of a weight a term leaves out: 8 leading bits a term before it
+    const uint32_t out1 = term == 0 ? 0u : term == 3 ? ~0u : 0xFFFF0000u, out2 = term == 2 ? 0xFFFF0000u : 0u;
     const Keys ks = visible<STEP>(d, pmin, pmax);
     const int parts = d.splits * d.waves, part = split * d.waves + wave;
     const int each = __builtin_amdgcn_readfirstlane((ks.steps + parts - 1) / parts);
@@ -276,6 +292,11 @@ k_paged_rows(PagedDev d) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         float x = j < 4 ? x0[j & 3] : x1[j & 3];
+                        if constexpr (SIDE) {
+                            const float t0 = bf16_round(x), t1 = bf16_round(x - t0), t2 = bf16_round(x - t0 - t1);
+                            qb[0][s][j] = static_cast<__bf16>(term == 0 ? t0 : term == 1 ? t1 : term == 2 ? t2 : 0.0f);
+                            continue;
+                        }
 #pragma unroll
                         for (int t = 0; t < QT; ++t) {
                             const float hi = bf16_round(x);
@@ -441,6 +462,10 @@ k_paged_rows(PagedDev d) {
 #pragma unroll
                     for (int s = 0; s < KS; ++s)
                         s4[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[a][s], qb[t3][s], s4[a], 0, 0, 0);
+                if constexpr (SIDE && Q32) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s4[a][i] = plus_dpp<kRor8>(plus_dpp<kHalfMirror>(s4[a][i]));
+                }
             }
         }
 
@@ -499,6 +524,16 @@ k_paged_rows(PagedDev d) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float x0 = s4[j / 2][2 * (j & 1)], x1 = s4[j / 2][2 * (j & 1) + 1];
+                if constexpr (SIDE) {
+                    x0 = less_bits(x0, out1);
+                    x1 = less_bits(x1, out1);
+                    if constexpr (Q32) {
+                        x0 = less_bits(x0, out2);
+                        x1 = less_bits(x1, out2);
+                    }
+                    pb[0][j] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302u);
+                    continue;
+                }
 #pragma unroll
                 for (int t3 = 0; t3 < PT; ++t3) {
                     pb[t3][j] = pack2_bf16(x0, x1);
@@ -523,6 +558,15 @@ k_paged_rows(PagedDev d) {
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    if constexpr (SIDE) {
+#pragma unroll
+        for (int x = 0; x < W; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (Q32) acc[x][i] = plus_dpp<kHalfMirror>(acc[x][i]);
+                acc[x][i] = plus_dpp<kRor8>(acc[x][i]);
+            }
+    }
 
     // the wave's part to LDS: row c, dims W (4 g + i) + t
     // (a NaN total is the row's own: scores that it does not see are replaced)
@@ -538,7 +582,8 @@ k_paged_rows(PagedDev d) {
     if (g == 0) { sm_m[wave][c] = m; sm_l[wave][c] = l; }
     if (pmin != pmax) {
         const uint64_t bad = __ballot(nan && live && l == l);
-        uint32_t rows = static_cast<uint32_t>((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu);
+        constexpr uint32_t COLUMNS = SIDE ? (1u << side_rows(Q32)) - 1 : 0xFFFFu;
+        uint32_t rows = static_cast<uint32_t>(bad | bad >> 16 | bad >> 32 | bad >> 48) & COLUMNS;
         while (rows) {
             const int x = __builtin_ctz(rows);
             rows &= rows - 1;
@@ -1221,8 +1266,11 @@ hipError_t launch(const PagedDev& d, hipStream_t s) {
     const dim3 blocks(static_cast<unsigned>(d.blocks)), grid(static_cast<unsigned>(joins));
     if (d.tiled)
         hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), blocks, dim3(64 * kWaves), 0, s, d);
+    else if (KV != Kv::kF32 && d.lds_rows <= side_rows(Q32))
+        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV, KV != Kv::kF32>), blocks, dim3(64 * d.waves),
+                           static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4, s, d);
     else
-        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV>), blocks, dim3(64 * d.waves),
+        hipLaunchKernelGGL((k_paged_rows<D, Q32, KV, false>), blocks, dim3(64 * d.waves),
                            static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4, s, d);
     if (d.splits > 64) hipLaunchKernelGGL((k_paged_join<D, Q32, 16>), grid, dim3(1024), 0, s, d);
     else if (d.splits > kFewSplits) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);

@@ -256,6 +256,35 @@ def test_attention_split(gpu_device, qt, kind, dim, q_lens, kv_lens):
     c.check(c.run(300, 9), 300, 9)
 
 
+@pytest.mark.parametrize("qt,kind", [(F32, "bf16"), (F32, "mxfp4"), (BF16, "bf16"), (BF16, "mxfp4")])
+@pytest.mark.parametrize("qh,kvh,dim,q_lens", [(3, 3, 64, [4, 1, 3]), (4, 2, 128, [2, 0, 1]), (6, 2, 128, [1, 1, 1]),
+                                               (4, 1, 64, [1, 2, 1]), (7, 1, 128, [1, 1, 1]), (2, 1, 64, [4, 3, 1]),
+                                               (5, 1, 64, [1, 1, 1]), (1, 1, 128, [8, 5, 2]), (9, 1, 64, [1, 1, 1])])
+def test_attention_of_few_rows(gpu_device, qt, kind, qh, kvh, dim, q_lens):
+    """1 to 9 rows under a key head, where terms of numbers stand beside rows;
+    short, long and windowed, queries and keys of very different sizes."""
+    note(f"few rows {qt} {kind} {qh}/{kvh} {dim} {q_lens}")
+    c = Case(gpu_device, qt, kind, qh, kvh, dim, 16, q_lens, [9, 70, 1100], seed=12)
+    c.check(c.run(1 << 30, 0), 1 << 30, 0)
+    c.check(c.run(37, 3), 37, 3)
+    c.q *= torch.exp2(torch.randint(-6, 3, c.q.shape, device=c.dev).float()).to(qt)
+    c.check(c.run(1 << 30, 0), 1 << 30, 0)
+
+
+@pytest.mark.parametrize("qt,kind", [(F32, "bf16"), (F32, "mxfp4"), (BF16, "bf16"), (BF16, "mxfp4")])
+@pytest.mark.parametrize("n,kv", [(4, 40), (3, 1500)])
+def test_unseen_values_of_few_rows(gpu_device, qt, kind, n, kv):
+    note(f"unseen by few rows {qt} {kind} {n} {kv}")
+    c = Case(gpu_device, qt, kind, 2, 2, 64, 16, [n], [kv], seed=4)
+    page, off = c.table[0, (kv - 2) // 16], (kv - 2) % 16
+    if kind == "mxfp4":
+        c.cache.v_scale[page, :, off] = 255
+    else:
+        c.cache.v[page, :, off] = float("inf")
+    got = f64(c.run(1 << 30, 0)).reshape(n, -1)
+    assert np.isfinite(got[:n - 2]).all() and not np.isfinite(got[n - 2:]).any()
+
+
 @pytest.mark.parametrize("qt,kind", [(F32, "f32"), (F32, "bf16"), (F32, "mxfp4"), (BF16, "bf16"), (BF16, "mxfp4")])
 @pytest.mark.parametrize("q_lens,kv_lens", [([4, 20], [60, 20]), ([100], [130])])
 def test_unseen_values_do_not_reach_a_row(gpu_device, qt, kind, q_lens, kv_lens):
