@@ -222,8 +222,12 @@ __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const K
 }
 
 // SIDE: few rows (side_rows), whose terms stand side by side in the 16 columns of
-// the MFMAs: column c holds term c / 4 of row c % 4 (mirrored where c & 4, for the
-// sums over lanes c ^ 7), with BF16 queries term c / 8 of row c % 8.
+// the MFMAs instead of one product after the other: column c holds term c / 4 of
+// row c % 4 (mirrored where c & 4, for the sums over lanes c ^ 7), with BF16
+// queries term c / 8 of row c % 8.  Scores are summed over a row's columns, which
+// then hold the same weight and take their term of it; O is summed at the end.
+// (One sequence of 131072 4-bit keys, fp32 queries: 27.0 -> 24.7 us; 64 of 16384:
+// 113 -> 94, with BF16 queries 91 -> 89; a bf16 cache is bound by its bytes.)
 constexpr int side_rows(bool q32) { return q32 ? 4 : 8; }
 
 template <int D, bool Q32, Kv KV, bool SIDE>
@@ -389,11 +393,12 @@ k_paged_rows(PagedDev d) {
     };
 
     // A step is read one ahead (37 x 2051 fp32 keys 80 -> 63 us, 64 x 8192 bf16 154
-    // -> 148; of a 4-bit cache with fp32 queries 64 x 16384 keys 132 -> 111), except
-    // of a 4-bit cache with BF16 queries, whose steps are short and whose decoding
-    // wants the registers for a third or fourth wave (64 x 16384 keys 92, read
-    // ahead 98).
-    constexpr bool EARLY = !MX || Q32;
+    // -> 148; 64 x 16384 4-bit keys under fp32 rows 132 -> 111), except of a
+    // 4-bit cache in the leaner variants, whose decoding wants the registers for a
+    // third or fourth wave (the same keys under 4 bf16 rows 92, read ahead 98, under
+    // 4 fp32 rows 95, read ahead 101).  Two steps in turn instead of the copy of one:
+    // no faster, and spills.
+    constexpr bool EARLY = !MX || (Q32 && !SIDE);
     Step next;
     if (EARLY && t0 < t1) load(t0, next);
     for (int t = t0; t < t1; ++t) {
@@ -651,7 +656,13 @@ k_paged_rows(PagedDev d) {
 //                   LDS (ds_read_b64_tr_b16: 4 keys of one dim) in that order.
 // The running reference m of a row follows its maximum only when that has grown
 // by more than 2^8: weights are then below 256, which neither their bf16 nor the
-// fp32 sums feel, and most steps leave the accumulator alone.
+// fp32 sums feel, and most steps leave the accumulator alone.  With bf16 queries a
+// weight is rounded to bf16 for its product with V (half a step, 2^-9, of either
+// sign on each of many keys, against 2^-9 in the bf16 output itself; the sum of the
+// weights keeps 32 bits): a second term would cost half as many MFMAs again.  fp32
+// queries keep three.
+// Bound by the matrix cores and what feeds them: 4 x 2048 tokens on 8192 keys, 16
+// heads of 128, bf16, 358 us = 0.91 PFLOP/s (the library's 8192^3 product 1.16).
 // LDS rows are one key's D values; 16-byte chunks are permuted so that the lanes
 // served together (16 keys' same chunk for K, 4 keys' 64 bytes for V) lie in
 // different banks.
