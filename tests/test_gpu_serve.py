@@ -373,6 +373,37 @@ def test_rows_left_alone_and_pages_left_out(gpu_device, qt, kind):
         c.check(torch.where(keep[:, None], short, out), 2047, 1)
 
 
+@pytest.mark.parametrize("qt,kind", [(F32, "f32"), (F32, "mxfp4"), (BF16, "bf16")])
+def test_pages_that_sequences_share(gpu_device, qt, kind):
+    """A common prefix held once: sequences whose tables name the same pages,
+    one of them twice the same sequence, and slots read back more than once."""
+    note(f"shared pages {qt} {kind}")
+    c = Case(gpu_device, qt, kind, 8, 2, 64, 16, [1, 40, 1, 2], [70, 70, 70, 66], seed=6)
+    c.table[1:] = c.table[0]
+    c.check(c.run(1 << 30, 0), 1 << 30, 0)
+    c.check(c.run(20, 3), 20, 3)
+    slots = torch.tensor([int(c.table[0, 1]) * 16 + 3] * 5, device=c.dev)
+    for t in serve.kv_gather_gpu(c.cache, slots):
+        assert torch.equal(t, t[:1].expand_as(t)) and t.isfinite().all()
+
+
+@pytest.mark.parametrize("qt,kind", [(F32, "f32"), (F32, "bf16"), (BF16, "mxfp4")])
+def test_table_entries_that_no_query_sees(gpu_device, qt, kind):
+    """Entries past the length and before the window hold anything."""
+    note(f"unseen entries {qt} {kind}")
+    for q_lens, kv_lens in (([1, 2], [150, 90]), ([50, 3], [170, 40])):
+        c = Case(gpu_device, qt, kind, 8, 2, 64, 16, q_lens, kv_lens, seed=9)
+        want = c.run(30, 2)
+        wide = np.full((2, c.table.shape[1] + 5), 0x7FFFFFFF, np.int32)
+        wide[:, :c.table.shape[1]] = c.table
+        for b, n in enumerate(kv_lens):
+            first = max((n - q_lens[b] + 1 - 30) // 16, 1)
+            wide[b, 1:first] = -0x80000000
+            wide[b, -(-n // 16):] = 0x7FFFFFFF
+        c.table = wide
+        assert torch.equal(bits(c.run(30, 2)), bits(want))
+
+
 def test_lengths_past_the_bounds_are_cut(gpu_device):
     """kv_lens past max_kv_len or the table, offsets past the rows: nothing is
     read or written outside the arrays."""
