@@ -646,6 +646,12 @@ def test_logits(gpu_device, dtype, rows, vocab, hist, bias, mask):
     assert bool((wide[:, 0] == 9.0).all()) and bool((wide[:, vocab + 1:] == 9.0).all())
 
 
+@pytest.mark.parametrize("rows,vocab", [(64, 2049), (67, 1030), (131, 6100)])
+def test_logits_of_many_rows(gpu_device, rows, vocab):
+    """Rows dealt to the XCDs, their number no multiple of 8 among them."""
+    test_logits(gpu_device, BF16, rows, vocab, 60, 3, True)
+
+
 def test_logits_rules_alone(gpu_device):
     """Each rule without the others; no rule at all copies the logits."""
     x, r = _logit_case(gpu_device, F32, 4, 777, 50, 6, True, seed=11)
