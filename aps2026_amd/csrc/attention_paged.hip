@@ -27,7 +27,8 @@
 // replaced; in the second product their weight is 0, but 0 times an infinity
 // or a NaN is a NaN: rows of V that no row of the tile sees are replaced by
 // zeros, and where rows differ in what they see, a row that ended in NaN is
-// computed again one key at a time (redo_row), from its own keys alone.
+// computed again from its own keys alone (redo_row) if a value that it does not
+// see may be why (stray).
 //
 // Few rows and a long cache: the steps of a tile are split over the 4 to 8 waves
 // of a workgroup and, past that, over `splits` workgroups; the waves' (max, sum,
@@ -177,8 +178,40 @@ __device__ inline float element(const void* base, const uint8_t* scales, int64_t
     return dim & 1 ? bf16w_hi(pair) : bf16w_lo(pair);
 }
 
-// One row over the steps [t0, t1) from the keys it sees, one key at a time, by
-// a whole wave; o[dim], m and l in LDS.
+// True if a value that is not finite may have reached a row that does not see it:
+// one of a key that other rows see, in a step of [t0, t1) that rows at positions
+// [pmin, pmax] do not all see whole.  (Where they do, it is the row's own.)
+template <int D, Kv KV, int STEP>
+__device__ bool stray(const PagedDev& d, const int32_t* table, int h, const Keys& ks, int t0, int t1, int pmin,
+                      int pmax, int pos) {
+    const View vis = view(d, pos);
+    const int lane = threadIdx.x & 63;
+    bool found = false;
+    for (int t = t0; t < t1 && !found; ++t) {
+        const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
+        if (base + STEP - 1 <= pmin && (static_cast<int64_t>(base) > static_cast<int64_t>(pmax) - d.a.window ||
+                                        base + STEP - 1 < d.a.sinks))
+            continue;
+        bool bad = false;
+        for (int key = base; key < base + STEP && key < ks.hi; ++key) {
+            if ((key < ks.lo && key >= ks.first) || sees(d, vis, key)) continue;
+            const int64_t page = table[key >> d.page_shift];
+            if (page < 0 || page >= d.c.num_pages) continue;
+            const int64_t hr = ((page * d.c.kv_heads + h) << d.page_shift) + (key & ((1 << d.page_shift) - 1));
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+                const float x = element<D, KV>(d.c.v, d.c.v_scale, hr, D / 64 * lane + j);
+                bad |= x - x != 0.0f;
+            }
+        }
+        found = __any(bad);
+    }
+    return found;
+}
+
+// One row over the steps [t0, t1) from the keys it sees alone, by a whole wave:
+// 64 keys at a time, a lane the score of each, then the values one key after the
+// other; o[dim], m and l in LDS.
 template <int D, bool Q32, Kv KV, int STEP>
 __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const Keys& ks, int t0, int t1, int64_t qrow,
                          int head, int pos, float* o, float* m_out, float* l_out) {
@@ -194,26 +227,45 @@ __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const K
         acc[j] = 0.0f;
     }
     float m = -INFINITY, l = 0.0f;
-    for (int t = t0; t < t1; ++t) {
-        const int base = (t < ks.n1 ? t : t - ks.n1 + ks.t_lo) * STEP;
-        for (int key = base; key < base + STEP; ++key) {
-            if (!sees(d, vis, key)) continue;
-            const int64_t page = table[key >> d.page_shift];
-            if (page < 0 || page >= d.c.num_pages) continue;
-            const int64_t hr = ((page * d.c.kv_heads + h) << d.page_shift) + (key & ((1 << d.page_shift) - 1));
-            float s = 0.0f;
+    for (int t = t0; t < t1; t += 64 / STEP) {
+        const int mine = t + lane / STEP;
+        const int key = (mine < ks.n1 ? mine : mine - ks.n1 + ks.t_lo) * STEP + lane % STEP;
+        const bool seen = mine < t1 && sees(d, vis, key);
+        const int64_t page = seen ? table[key >> d.page_shift] : -1;
+        const bool held = page >= 0 && page < d.c.num_pages;
+        const int64_t hr =
+            held ? ((page * d.c.kv_heads + h) << d.page_shift) + (key & ((1 << d.page_shift) - 1)) : 0;
+        float s = 0.0f;
+        for (int x = 0; x < 64; ++x)
 #pragma unroll
-            for (int j = 0; j < PER; ++j) s = fmaf(q[j], element<D, KV>(d.c.k, d.c.k_scale, hr, PER * lane + j), s);
+            for (int j = 0; j < PER; ++j) {
+                const float qx = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q[j]), x));
+                s = fmaf(qx, held ? element<D, KV>(d.c.k, d.c.k_scale, hr, PER * x + j) : 0.0f, s);
+            }
+        s = held ? s * d.scale_log2 : -INFINITY;
+        float top = s;
 #pragma unroll
-            for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x);
-            s *= d.scale_log2;
-            const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
-            const float f = exp2_fast(m - ref), p = exp2_fast(s - ref);
-            m = mn;
-            l = l * f + p;
+        for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
+        const float f = exp2_fast(m - ref), p = exp2_fast(s - ref);
+        m = mn;
+        float sum = p;
+#pragma unroll
+        for (int x = 32; x >= 1; x >>= 1) sum += __shfl_xor(sum, x);
+        l = l * f + sum;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) acc[j] *= f;
+        for (uint64_t left = __ballot(held); left; left &= left - 1) {
+            const int x = __builtin_ctzll(left);
+            const float px = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), x));
+            const int64_t hx =
+                static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(
+                                         __builtin_amdgcn_readlane(static_cast<int>(hr >> 32), x)))
+                                     << 32) |
+                static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(hr), x));
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                acc[j] = fmaf(p, element<D, KV>(d.c.v, d.c.v_scale, hr, PER * lane + j), acc[j] * f);
+                acc[j] = fmaf(px, element<D, KV>(d.c.v, d.c.v_scale, hx, PER * lane + j), acc[j]);
         }
     }
 #pragma unroll
@@ -593,6 +645,7 @@ k_paged_rows(PagedDev d) {
             const int x = __builtin_ctz(rows);
             rows &= rows - 1;
             const int rr = r0 + x;
+            if (!stray<D, KV, STEP>(d, table, h, ks, t0, t1, pmin, pmax, p0 + rr / d.group)) continue;
             redo_row<D, Q32, KV, STEP>(d, table, h, ks, t0, t1, sq.q0 + rr / d.group, h * d.group + rr % d.group,
                                        p0 + rr / d.group, o_row(wave, x), &sm_m[wave][x], &sm_l[wave][x]);
         }
@@ -1054,6 +1107,7 @@ k_paged_tiles(PagedDev d) {
             const int x = __builtin_ctz(rows);
             rows &= rows - 1;
             const int rr = r0 + x;
+            if (!stray<D, KV, KEYS>(d, table, h, ks, t0, t1, pmin, pmax, p0 + rr / d.group)) continue;
             redo_row<D, Q32, KV, KEYS>(d, table, h, ks, t0, t1, sq.q0 + rr / d.group,
                                             h * d.group + rr % d.group, p0 + rr / d.group, red, red + D, red + D + 1);
             __builtin_amdgcn_wave_barrier();

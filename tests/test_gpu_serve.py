@@ -271,6 +271,32 @@ def test_attention_of_few_rows(gpu_device, qt, kind, qh, kvh, dim, q_lens):
     c.check(c.run(1 << 30, 0), 1 << 30, 0)
 
 
+@pytest.mark.parametrize("qt,kind", [(F32, "f32"), (F32, "bf16"), (F32, "mxfp4"), (BF16, "bf16"), (BF16, "mxfp4")])
+@pytest.mark.parametrize("qh,kvh,dim,n,kv,window", [(4, 1, 64, 40, 900, 1 << 30), (2, 2, 128, 3, 900, 1 << 30),
+                                                    (2, 1, 64, 30, 700, 333), (8, 1, 128, 2, 700, 250)])
+def test_rows_computed_again(gpu_device, qt, kind, qh, kvh, dim, n, kv, window):
+    """Long rows next to rows that see an infinite value keep their own."""
+    note(f"again {qt} {kind} {qh}/{kvh} {dim} {n} {kv} {window}")
+    c = Case(gpu_device, qt, kind, qh, kvh, dim, 16, [n], [kv], seed=21)
+    j = kv - 2
+    page, off = c.table[0, j // 16], j % 16
+    if kind == "mxfp4":
+        c.cache.v_scale[page, :, off] = 255
+    else:
+        c.cache.v[page, :, off] = -float("inf")
+    got = f64(c.run(window, 5)).reshape(n, qh, dim)
+    assert not np.isfinite(got[n - 2:]).any()
+    if kind == "mxfp4":
+        c.cache.v_scale[page, :, off] = 127
+    else:
+        c.cache.v[page, :, off] = 1.0
+    k, v = held(c.cache)
+    want, mag, prod, seen = oracle.attention(f64(c.q).reshape(n, qh, dim), k, v, c.offs, c.kv_lens, c.table, 16, qh,
+                                             window, 5, 1 / math.sqrt(dim), c.pages)
+    bound = oracle.attention_bound(want, mag, prod, seen, dim, qt, 24 if qt is F32 else 8)
+    assert (np.abs(got - want) <= bound)[:n - 2].all()
+
+
 @pytest.mark.parametrize("qt,kind", [(F32, "bf16"), (F32, "mxfp4"), (BF16, "bf16"), (BF16, "mxfp4")])
 @pytest.mark.parametrize("n,kv", [(4, 40), (3, 1500)])
 def test_unseen_values_of_few_rows(gpu_device, qt, kind, n, kv):
