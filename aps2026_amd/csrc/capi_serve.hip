@@ -76,6 +76,8 @@ int check_paged(const aps::KvCache& c, int64_t rows, int32_t q_heads, int64_t ba
         max_kv_len > kMaxRows)
         return fail(APS_ERR_SHAPE, "%s: rows %lld, batch %lld, max_q_len %lld, max_kv_len %lld", what, (long long)rows,
                     (long long)batch, (long long)max_q_len, (long long)max_kv_len);
+    if (rows * q_heads > int64_t(1) << 40)  // sizes in bytes stay far from 64 bits
+        return fail(APS_ERR_SHAPE, "%s: %lld rows of %d heads", what, (long long)rows, q_heads);
     if (window < 1 || sinks < 0) return fail(APS_ERR_SHAPE, "%s: window %d, sinks %d", what, window, sinks);
     a->rows = rows;
     a->q_heads = q_heads;

@@ -150,8 +150,23 @@ def test_attention_workspace_overlap_is_refused():
         assert "overlap" in capi.last_error()
 
 
-def test_attention_of_too_many_sequences():
+def test_attention_of_too_many_sequences_or_rows():
     assert attend(batch=(1 << 20) + 1) == capi.APS_ERR_SHAPE
+    assert attend(rows=1 << 30, qh=2048, qs=2048 * 128) == capi.APS_ERR_SHAPE
+
+
+def test_workspace_sizes_over_the_range():
+    """Parts of every (row, head) for at most 256 splits, whatever the sizes."""
+    size = capi.lib().aps_attention_paged_workspace_size
+    rng = np.random.default_rng(1)
+    for _ in range(3000):
+        kvh = int(rng.integers(1, 9))
+        qh = kvh * int(rng.integers(1, 40))
+        rows, batch, mq = (int(2 ** rng.uniform(0, e)) for e in (20, 14, 20))
+        mkv, window = (int(2 ** rng.uniform(0, 30)) for _ in range(2))
+        dim = int(rng.choice([64, 128]))
+        got = size(cache(kv_heads=kvh, head_dim=dim), rows, qh, batch, mq, mkv, window, int(rng.integers(0, 9)))
+        assert got % 256 == 0 and got <= 2 * (rows * qh * 256 * (dim + 2) * 4 + 256)
 
 
 def logits(rules=None, rows=1, **kw):
