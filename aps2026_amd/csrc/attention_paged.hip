@@ -64,6 +64,8 @@ struct PagedDev {
     bool tiled;      // k_paged_tiles, else k_paged_rows
     int least, most;  // rows of the sequences that this launch serves
     int64_t max_q;    // the most tokens of one
+    bool by_seq;      // parts stand by (sequence, token), max_q of each, else by row of q
+    int64_t slots;    // (sequence, token)s or rows that have parts
     int waves;       // of a workgroup
     int lds_rows;    // rows of a tile that can be live: LDS keeps those
     int64_t blocks;  // workgroups
@@ -668,14 +670,16 @@ k_paged_rows(PagedDev d) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[j] = fmaf(o_row(w, rc)[dim + j], f, o[j]);
         }
-        const int64_t orow = (sq.q0 + rr / d.group) * d.a.q_heads + h * d.group + rr % d.group;
+        const int head = h * d.group + rr % d.group;
+        const int64_t orow = (sq.q0 + rr / d.group) * d.a.q_heads + head;
         if (d.splits > 1) {
-            const int64_t at = orow * d.splits + split;
+            const int64_t slot = d.by_seq ? b * d.max_q + rr / d.group : sq.q0 + rr / d.group;
+            const int64_t at = (slot * d.a.q_heads + head) * d.splits + split;
             float* po = d.part + at * D + dim;
             *reinterpret_cast<f32x4*>(po) = f32x4{o[0], o[1], o[2], o[3]};
             *reinterpret_cast<f32x4*>(po + 4) = f32x4{o[4], o[5], o[6], o[7]};
             if (dim == 0) {
-                float* ml = d.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+                float* ml = d.part + d.slots * d.a.q_heads * d.splits * D + 2 * at;
                 ml[0] = mm;
                 ml[1] = ll;
             }
@@ -1127,7 +1131,7 @@ k_paged_tiles(PagedDev d) {
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
     const int64_t at = orow * d.splits + split;
     if (d.splits > 1 && hf == 0) {
-        float* ml = d.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+        float* ml = d.part + d.slots * d.a.q_heads * d.splits * D + 2 * at;
         ml[0] = m;
         ml[1] = l;
     }
@@ -1166,8 +1170,8 @@ k_paged_tiles(PagedDev d) {
 
 // out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the splits of one
 // (row, head), a workgroup each.  The row's sequence is looked up, 64 at a time,
-// while its parts are on their way: rows that no sequence of this launch names
-// are left as they were.
+// while its parts are on their way (by_seq: it is known): rows that no sequence
+// of this launch names are left as they were.
 template <int D, bool Q32, int JW>
 __global__ void __launch_bounds__(64 * JW)
 k_paged_join(PagedDev d) {
@@ -1175,9 +1179,11 @@ k_paged_join(PagedDev d) {
     __shared__ float part[JW][D];
     __shared__ float weight[JW][JW == 1 ? 1 : kMaxSplits];  // a wave's own copy
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t orow = blockIdx.x, at = orow * d.splits;
-    const int64_t row = blockIdx.x / static_cast<uint32_t>(d.a.q_heads);
-    const float* ml = d.part + d.a.rows * d.a.q_heads * d.splits * D + 2 * at;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * d.splits;
+    const uint32_t slot = blockIdx.x / static_cast<uint32_t>(d.a.q_heads);
+    const int head = static_cast<int>(blockIdx.x - slot * static_cast<uint32_t>(d.a.q_heads));
+    int64_t row = slot;
+    const float* ml = d.part + d.slots * d.a.q_heads * d.splits * D + 2 * at;
     const float* po = d.part + at * D + PER * lane;
     constexpr int MOST = JW == 1 ? kFewSplits : kMaxSplits, MX = (MOST + 63) / 64;
     // few splits: everything is on its way before the first wait
@@ -1199,7 +1205,13 @@ k_paged_join(PagedDev d) {
         top = fmaxf(top, m[x]);
     }
     bool named = false;
-    for (int64_t b0 = 0; b0 < d.a.batch && !named; b0 += 64) {
+    if (d.by_seq) {
+        const uint32_t b = slot / static_cast<uint32_t>(d.max_q), tok = slot - b * static_cast<uint32_t>(d.max_q);
+        const Seq one = sequence(d, b);
+        row = one.q0 + tok;
+        named = static_cast<int64_t>(tok) * d.group < rows_of(d, one.len);
+    }
+    for (int64_t b0 = 0; b0 < d.a.batch && !named && !d.by_seq; b0 += 64) {
         bool mine = false;
         if (b0 + lane < d.a.batch) {
             const Seq one = clipped(d, d.a.q_offsets[b0 + lane], d.a.q_offsets[b0 + lane + 1], 0);
@@ -1208,6 +1220,7 @@ k_paged_join(PagedDev d) {
         named = __ballot(mine) != 0;
     }
     if (!named) return;
+    const int64_t orow = row * d.a.q_heads + head;
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -1258,8 +1271,9 @@ k_paged_join(PagedDev d) {
     }
 }
 
-// One launch over the sequences of least .. most rows under a key head.
-PagedDev plan_one(const KvCache& c, const PagedArgs& a, int64_t least, int64_t most) {
+// One launch over the sequences of least .. most rows under a key head; `beside`:
+// the short ones next to one that is not.
+PagedDev plan_one(const KvCache& c, const PagedArgs& a, int64_t least, int64_t most, bool beside) {
     PagedDev d;
     d.a = a;
     d.c = c;
@@ -1282,14 +1296,19 @@ PagedDev plan_one(const KvCache& c, const PagedArgs& a, int64_t least, int64_t m
         // the blocks of rows that there can be, and about how many there are; two
         // workgroups a CU and no more (a third round costs what a split saves)
         tiles = std::min<int64_t>(tiles, c.kv_heads * (a.rows * d.group / kBlockRows + a.batch));
-        const int64_t about = std::max<int64_t>(ceil_div(a.rows * a.q_heads, kBlockRows),
+        // (short ones beside them taken for steps of a token)
+        const int64_t long_rows = least > 1 ? std::max<int64_t>(a.rows - a.batch, 1) : a.rows;
+        const int64_t about = std::max<int64_t>(ceil_div(long_rows * a.q_heads, kBlockRows),
                                                 c.kv_heads * (least > 1 ? 1 : a.batch));
         splits = std::min<int64_t>(512 / about, ceil_div(steps, 8));
     } else {
         // four workgroups a CU of a large batch, two where there are few tiles and
         // the parts to join weigh more (us with two / four: 64 x 8192 keys 148 /
         // 145, in 4 bits 99 / 89; 32 x 2051 27 / 31, 1 x 100000 39 / 42)
-        splits = std::min<int64_t>(ceil_div(tiles > 128 ? 1024 : 512, tiles), ceil_div(steps, 2 * kWaves));
+        // (beside chunks: what there is when all but one are steps of a token, not the
+        // two tiles that each could have)
+        const int64_t about = beside ? (a.batch - 1) * c.kv_heads * ceil_div(d.group, kRows) : tiles;
+        splits = std::min<int64_t>(ceil_div(about > 128 ? 1024 : 512, about), ceil_div(steps, 2 * kWaves));
         if (splits > 1 && steps <= 4 * kMostWaves && kMostWaves * d.lds_rows * (c.head_dim + 4) * 4 <= kPlainLds) {
             // short: one larger workgroup instead of a second launch
             d.waves = kMostWaves;
@@ -1298,35 +1317,42 @@ PagedDev plan_one(const KvCache& c, const PagedArgs& a, int64_t least, int64_t m
     }
     d.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits)));
     d.blocks = tiles * d.splits;
+    // the short sequences of a batch with chunks have few of its rows
+    d.by_seq = !d.tiled && a.batch * d.max_q < a.rows;
+    d.slots = d.by_seq ? a.batch * d.max_q : a.rows;
     return d;
 }
 
 int64_t part_floats(const PagedDev& d) {
-    return d.splits > 1 ? ceil_div(d.a.rows * d.a.q_heads * d.splits * (d.c.head_dim + 2), 64) * 64 : 0;
+    return d.splits > 1 ? ceil_div(d.slots * d.a.q_heads * d.splits * (d.c.head_dim + 2), 64) * 64 : 0;
 }
 
-// The launches of a call: long chunks to k_paged_tiles, the rest to
-// k_paged_rows.  Which sequence is which stands on the device; the host goes by
-// the lengths' bound and mean: where all but the longest can only be short, a
-// batch may mix chunks with steps and both are launched, else one serves all.
+// The launches of a call: sequences of kTiledRows rows and more to k_paged_tiles,
+// shorter ones to k_paged_rows, by each one's own rows, so that the bits of its
+// weights are not its neighbours' choice.  Which is which stands on the device; the
+// host launches both unless the sizes leave no room for one kind: max_q_len is
+// short itself, or the rows are too many for a short one beside batch - 1 of
+// max_q_len.  (bf16, 16 heads of 128, us as one launch of k_paged_tiles / as two:
+// 4 prompts of 512 and 60 steps on 8192 keys 296 / 359, one of the steps on 100000
+// 2403 / 547; 2 prompts and 62 steps 267 / 294, in 4 bits 225 / 177.  Where all are
+// prompts, 16 of up to 512, the launch for none costs 3 of 41.)
 struct Plan {
     PagedDev d[2];
     int n;
 };
 Plan plan(const KvCache& c, const PagedArgs& a) {
     Plan p;
-    const int64_t group = a.q_heads / c.kv_heads, longest = a.max_q_len * group;
-    const bool mixed = longest >= kTiledRows && a.batch > 1 &&
-                       (a.rows - a.max_q_len) * group < kTiledRows * (a.batch - 1);
-    p.n = mixed ? 2 : 1;
-    p.d[0] = plan_one(c, a, mixed ? kTiledRows : 1, longest);
-    if (mixed) p.d[1] = plan_one(c, a, 1, kTiledRows - 1);
+    const int64_t group = a.q_heads / c.kv_heads, longest = a.max_q_len * group, few = (kTiledRows - 1) / group;
+    const bool both = longest >= kTiledRows && few > 0 && a.rows <= (a.batch - 1) * a.max_q_len + few;
+    p.n = both ? 2 : 1;
+    p.d[0] = plan_one(c, a, both ? kTiledRows : 1, longest, false);
+    if (both) p.d[1] = plan_one(c, a, 1, kTiledRows - 1, true);
     return p;
 }
 
 template <int D, bool Q32, Kv KV>
 hipError_t launch(const PagedDev& d, hipStream_t s) {
-    const int64_t joins = d.a.rows * d.a.q_heads;
+    const int64_t joins = d.slots * d.a.q_heads;
     if (d.blocks > 0x7FFFFFFF || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
     const dim3 blocks(static_cast<unsigned>(d.blocks)), grid(static_cast<unsigned>(joins));
     if (d.tiled)

@@ -86,8 +86,10 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * kv_heads; query head h reads key head h / (q_heads / kv_heads).
  * q_dtype F32 takes every cache type, BF16 the BF16 and MXFP4 ones.  Products
  * are exact and sums are fp32; with BF16 queries the softmax weights are held
- * to 16 bits for their product with v, and to bf16's 8 in a call whose longest
- * sequence may have more than 32 rows (max_q_len times q_heads / kv_heads).
+ * for their product with v to 16 bits, and of a sequence with more than 32 rows
+ * (tokens times q_heads / kv_heads) to bf16's 8.  (Shorter sequences beside
+ * padding rows share the 8 where max_q_len is past 32 rows and rows >
+ * (batch - 1) max_q_len + 32 / (q_heads / kv_heads): no room but for padding.)
  *
  * All arrays in device memory; q_offsets ascend; batch up to 2^20, max_kv_len up
  * to 2^30.  max_q_len and max_kv_len bound the batch's
