@@ -16,7 +16,7 @@ q [rows, q_heads * 128], k and v [rows, kv_heads * 128], fp32, q_heads =
 """
 from __future__ import annotations
 
-from typing import Dict, Tuple, Union
+from typing import Dict, List, Tuple, Union
 
 import numpy as np
 import torch
@@ -30,7 +30,7 @@ HEAD_DIM = 128             # include/config.h:12
 SLIDING_WINDOW = 2047      # include/config.h:17
 ROPE_THETA = 10000.0       # include/config.h:18
 
-_tables: Dict[Tuple[torch.device, int, int, float], Tuple[torch.Tensor, torch.Tensor]] = {}
+_tables: Dict[Tuple[torch.device, int, float], List[Tuple[torch.Tensor, torch.Tensor]]] = {}
 
 
 def rope_table(max_seq: int, head_dim: int = HEAD_DIM, theta: float = ROPE_THETA) -> Tuple[np.ndarray, np.ndarray]:
@@ -45,14 +45,16 @@ def rope_table(max_seq: int, head_dim: int = HEAD_DIM, theta: float = ROPE_THETA
 
 def _device_table(device: torch.device, max_seq: int, head_dim: int, theta: float):
     """Device copies of the tables, kept per device and grown on demand (the
-    reference keeps one static table, src/tensor.cu:2703-2712)."""
-    key = (device, head_dim, float(theta))
-    have = _tables.get(key)
-    if have is None or have[0].shape[0] < max_seq:
-        c, s = rope_table(max_seq, head_dim, theta)
-        have = (torch.from_numpy(c).to(device), torch.from_numpy(s).to(device))
-        _tables[key] = have
-    return have
+    reference keeps one static table, src/tensor.cu:2703-2712).  The ones
+    outgrown stay, for kernels still under way on another stream and recorded
+    graphs read them; each has at least twice the rows of the one before, so
+    all of them take less than twice the newest's memory."""
+    kept = _tables.setdefault((device, head_dim, float(theta)), [])
+    if not kept or kept[-1][0].shape[0] < max_seq:
+        rows = max(max_seq, 2 * kept[-1][0].shape[0]) if kept else max_seq
+        c, s = rope_table(rows, head_dim, theta)
+        kept.append((torch.from_numpy(c).to(device), torch.from_numpy(s).to(device)))
+    return kept[-1]
 
 
 def _rows_u32(t: Union[torch.Tensor, np.ndarray], device) -> torch.Tensor:
