@@ -331,17 +331,21 @@ class Model:
             self._bufs[rows] = b
         return b
 
-    def prefill(self, plan, on_layer=None, caches: Optional[Sequence[serve.PagedKvCache]] = None) -> torch.Tensor:
+    def prefill(self, plan, on_layer=None, caches: Optional[Sequence[serve.PagedKvCache]] = None,
+                buffers: Optional[Buffers] = None) -> torch.Tensor:
         """logits [batch][vocab] of each prompt's last token; launches only
         (the outputs come from torch's caching allocator).  on_layer(i, b),
         when given, runs after layer i's launches (for example to copy its
         routes out of the shared workspace on the same stream).  With caches
         (one a layer) plan is CachedRows: its tokens join the sequences that
-        the caches hold."""
+        the caches hold.  buffers: the activations' place, of plan.rows rows;
+        the model's own, kept for each row count, unless given."""
         L, dev = capi.lib(), self.emb.device
         stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-        b = self.buffers(plan.rows)
+        b = self.buffers(plan.rows) if buffers is None else buffers
         T, H = plan.rows, self.H
+        if b.rows != T:
+            raise ValueError("prefill: buffers of other rows")
         _call(L.aps_gather_rows(_p(self.emb), self.emb.shape[0], H, _p(plan.node_token), T, _p(b.x), stream))
         for i, layer in enumerate(self.layers):
             layer.forward_carry(b, plan, i > 0, stream, caches[i] if caches is not None else None)
@@ -383,7 +387,8 @@ class Model:
         chosen from: after the penalties, the biases {id: value} and the mask
         ([1] or [batch] rows of int32 words, bit t % 32 of word t / 32 allows
         token t).  Of equal logits the lowest id wins.  One host wait, at the
-        end."""
+        end.  Caches and activations are the call's own, from torch's caching
+        allocator: calls may run side by side on other streams."""
         if len(prompts) == 0:
             raise RuntimeError("generate_decode received an empty input batch")
         if max_new_tokens < 1:
@@ -433,8 +438,11 @@ class Model:
                 rules.update(mask_index=torch.zeros(n_seq, dtype=torch.int32, device=dev))
         out = torch.empty((n_seq, max_new_tokens, V), dtype=torch.float32, device=dev)
         ids = torch.empty((n_seq, max_new_tokens), dtype=torch.int32, device=dev)
+        bufs = None
         for t in range(max_new_tokens):
-            logits = self.prefill(rows, caches=caches)
+            if bufs is None or bufs.rows != rows.rows:
+                bufs = Buffers.allocate(rows.rows, self.H, self.layers[0].w.moe, dev)
+            logits = self.prefill(rows, caches=caches, buffers=bufs)
             if rules:
                 if history is not None:
                     rules["history_lens"] = kv_lens
