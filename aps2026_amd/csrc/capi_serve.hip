@@ -17,6 +17,46 @@ bool overlap(const void* p, size_t np, const void* q, size_t nq) {
     return np && nq && a < b + nq && b < a + np;
 }
 
+// `count` rows of `width` bytes, `stride` bytes apart.
+typedef __int128 wide;
+struct Rows {
+    const void* at;
+    int64_t count, width;
+    wide stride;
+};
+Rows rows_of(const void* p, int64_t rows, int64_t values, int64_t stride, uintptr_t elt) {
+    const int64_t e = static_cast<int64_t>(elt);
+    return {p, p ? rows : 0, values * e, static_cast<wide>(stride) * e};
+}
+// True if a row of a shares a byte with a row of b: of slices of one wider row,
+// which lie between each other, none does.
+bool overlap(const Rows& a, const Rows& b) {
+    if (a.count <= 0 || b.count <= 0 || a.width <= 0 || b.width <= 0) return false;
+    const wide d = static_cast<wide>(reinterpret_cast<uintptr_t>(b.at)) - reinterpret_cast<uintptr_t>(a.at);
+    if (d >= (a.count - 1) * a.stride + a.width ||
+        -d >= (b.count - 1) * b.stride + b.width)
+        return false;
+    if (a.count == 1 && b.count == 1) return true;
+    auto floor_div = [](wide x, wide y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };
+    // the first row of b that ends behind the start of a's row i, from
+    // b.width + d + j stride > i stride; rows of one stride are alike for all i
+    if (a.stride == b.stride || a.count == 1 || b.count == 1) {
+        // (a single row's stride is the other's)
+        const wide s = a.count == 1 ? b.stride : a.stride;
+        const wide first = -(a.count - 1), last = b.count - 1;
+        wide j = floor_div(-d - b.width, s) + 1;
+        if (j < first) j = first;
+        return j <= last && d + j * s < a.width;
+    }
+    for (int64_t i = 0; i < a.count; ++i) {
+        const wide to = i * a.stride;
+        wide j = floor_div(to - d - b.width, b.stride) + 1;
+        if (j < 0) j = 0;
+        if (j < b.count && d + j * b.stride < to + a.width) return true;
+    }
+    return false;
+}
+
 int launched(hipError_t err, const char* what) {
     if (err == hipSuccess) return APS_OK;
     return fail(APS_ERR_HIP, "%s: %s", what, hipGetErrorString(err));
@@ -53,6 +93,12 @@ int check_cache(const aps_kv_cache* d, const char* what, bool arrays, aps::KvCac
     out->head_dim = d->head_dim;
     out->type = static_cast<aps::Kv>(d->dtype);
     return APS_OK;
+}
+
+// Bytes of k, and of v.
+int64_t held_bytes(const aps::KvCache& c) {
+    const int64_t n = (c.num_pages << c.page_shift) * c.kv_heads * c.head_dim;
+    return c.type == aps::Kv::kMx ? n / 2 : c.type == aps::Kv::kBf16 ? 2 * n : 4 * n;
 }
 
 int check_heads(const aps::KvCache& c, int32_t q_heads, const char* what) {
@@ -124,6 +170,14 @@ int aps_kv_append(const aps_kv_cache* cache, const void* k, int64_t k_stride, co
     const uintptr_t elt = src_dtype == APS_DTYPE_F32 ? 4 : 2;
     if (!k || !v || !positions || !slots || (max_pos > 0 && (!cos_table || !sin_table)) || (q && !q_out))
         return fail(APS_ERR_ARG, "%s: NULL pointer", what);
+    // a row is read after others were written
+    const int64_t qd = static_cast<int64_t>(q_heads) * c.head_dim;
+    const Rows to = rows_of(q ? q_out : nullptr, rows, qd, q_out_stride, elt);
+    const int64_t held = held_bytes(c);
+    if ((q != q_out && overlap(to, rows_of(q, rows, qd, q_stride, elt))) ||
+        overlap(to, rows_of(k, rows, kv, k_stride, elt)) || overlap(to, rows_of(v, rows, kv, v_stride, elt)) ||
+        overlap(to, {c.k, 1, held, held}) || overlap(to, {c.v, 1, held, held}))
+        return fail(APS_ERR_ARG, "%s: q_out overlaps another array", what);
     if (mis(k, elt) || mis(v, elt) || mis(q, elt) || mis(q_out, elt) || mis(positions, 4) || mis(slots, 8) ||
         mis(cos_table, 4) || mis(sin_table, 4))
         return fail(APS_ERR_ARG, "%s: arrays must be aligned to their elements", what);
@@ -143,6 +197,12 @@ int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64_t rows,
     if (rows < 0 || rows > kMaxRows) return fail(APS_ERR_SHAPE, "%s: rows %lld", what, (long long)rows);
     if (rows == 0 || (!k_out && !v_out)) return APS_OK;
     if (!slots) return fail(APS_ERR_ARG, "%s: NULL pointer", what);
+    const int64_t kv = static_cast<int64_t>(c.kv_heads) * c.head_dim, held = held_bytes(c);
+    const size_t out_bytes = static_cast<size_t>(rows * kv) * (out_dtype == APS_DTYPE_F32 ? 4 : 2);
+    for (void* to : {k_out, v_out})
+        if (to && (overlap(to, out_bytes, c.k, held) || overlap(to, out_bytes, c.v, held) ||
+                   overlap(to, out_bytes, to == k_out ? v_out : nullptr, v_out ? out_bytes : 0)))
+            return fail(APS_ERR_ARG, "%s: an output overlaps another array", what);
     if (mis(k_out, 16) || mis(v_out, 16) || mis(slots, 8))
         return fail(APS_ERR_ARG, "%s: outputs must be 16-byte, slots 8-byte aligned", what);
     return launched(aps::launch_kv_gather(c, slots, rows, k_out, v_out, out_dtype == APS_DTYPE_F32,

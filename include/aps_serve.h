@@ -54,7 +54,8 @@ typedef struct aps_kv_cache {
  * [head_dim] of src_dtype (F32 or BF16) with row strides in elements, so they
  * may be slices of one projection's rows.  q NULL: keys and values alone; else
  * q_out takes the rotated queries in src_dtype (q_out may be q itself with q's
- * stride; it overlaps nothing else).
+ * stride; its rows overlap nothing else, refused for those of q, k and v and the
+ * cached values).
  * Row r goes to slots[r]; a slot outside the cache (-1: padding) writes no key
  * and no value.  Slots of one call are distinct: of rows that name the same
  * slot either may stay, element by element.  A position outside [0, max_pos)
@@ -70,7 +71,8 @@ APS_API int aps_kv_append(const aps_kv_cache* cache, const void* k, int64_t k_st
 /* Reads cached rows back: k_out, v_out [rows][kv_heads][head_dim] of out_dtype
  * (F32, or BF16 rounded to nearest even; 16-byte aligned), the values that the
  * codes of a 4-bit cache stand for.  Either may be NULL.  A slot outside the
- * cache gives a row of zeros. */
+ * cache gives a row of zeros.  The outputs overlap nothing else (refused for each
+ * other and the cached values). */
 APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64_t rows, void* k_out, void* v_out,
                           int32_t out_dtype, void* stream);
 
