@@ -292,6 +292,9 @@ int aps_logits_process(const void* logits, int64_t logits_stride, int32_t dtype,
     if (logits == out && logits_stride != out_stride)
         return fail(APS_ERR_ARG, "%s: logits changed in place keep their stride", what);
     const uintptr_t elt = dtype == APS_DTYPE_F32 ? 4 : 2;
+    if (logits != out && overlap(rows_of(logits, rows, vocab, logits_stride, elt),
+                                 rows_of(out, rows, vocab, out_stride, elt)))
+        return fail(APS_ERR_ARG, "%s: logits and out overlap", what);
     if (mis(logits, elt) || mis(out, elt) || mis(r.history, 4) || mis(r.history_lens, 4) || mis(r.prompt_lens, 4) ||
         mis(r.repetition, 4) || mis(r.frequency, 4) || mis(r.presence, 4) || mis(r.bias_ids, 4) ||
         mis(r.bias_values, 4) || mis(r.bias_lens, 4) || mis(r.mask, 4) || mis(r.mask_index, 4))

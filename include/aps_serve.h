@@ -141,7 +141,8 @@ typedef struct aps_logits_rules {
 } aps_logits_rules;
 
 /* out[r][t] from x = logits[r][t] (F32 or BF16, row strides in elements; out
- * may be logits itself with its stride), in fp32, rounded once:
+ * may be logits itself with its stride, and overlaps nothing else of the call:
+ * other rows over logits' are refused), in fp32, rounded once:
  *   t anywhere in the history:     x = x > 0 ? x / repetition : x * repetition
  *   t n > 0 times past the prompt: x = x - frequency n, then x - presence
  *   t in the bias list:            x = x + its value

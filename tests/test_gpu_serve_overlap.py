@@ -26,3 +26,15 @@ def test_append_between_the_rows_of_one_buffer(gpu_device):
     for to in (x[:, 1:2 * dim + 1], x[:, 2 * dim:4 * dim], x[:, dim:3 * dim]):
         with pytest.raises(ValueError, match="q_out overlaps"):
             serve.kv_append_gpu(cache, k, v, pos, slots, cos, sin, q=q, q_out=to)
+
+
+def test_logits_beside_their_rows(gpu_device):
+    """Logits and their results as halves of one buffer's rows; a shifted slice."""
+    dev = gpu_device
+    x = torch.randn(7, 2 * 45, device=dev)
+    mask = torch.full((7, 2), 0x5A5A5A5A, dtype=torch.int32, device=dev)
+    want = serve.logits_process_gpu(x[:, :45].contiguous(), mask=mask)
+    out = x[:, 45:]
+    assert serve.logits_process_gpu(x[:, :45], mask=mask, out=out) is out and torch.equal(out, want)
+    with pytest.raises(ValueError, match="overlap"):
+        serve.logits_process_gpu(x[:, :45], mask=mask, out=x[:, 1:46])

@@ -98,3 +98,41 @@ def test_gather():
     for at in (P << 10, P << 11):
         assert gather(at, None) and gather(P, at + held - 16) and gather(at - size + 16, P)
         assert not gather(at + held, None) and not gather(P, at - size)
+
+
+def logits(rows, x, xs, out, os, vocab=100):
+    """True if refused for an overlap (a misaligned list of lengths ends any other call)."""
+    r = capi.LogitsRules(history=P, history_lens=P + 2, history_stride=4)
+    assert capi.lib().aps_logits_process(x, xs, BF16, rows, vocab, ctypes.byref(r), out, os, None) == ARG
+    message = capi.last_error()
+    assert ("overlap" in message) != ("aligned" in message)
+    return "overlap" in message
+
+
+def test_logits():
+    assert not logits(6, P, 100, P, 100) and not logits(6, P, 130, P, 130)           # in place
+    assert logits(6, P, 100, P + 2, 100) and logits(6, P + 2, 100, P, 100)           # shifted by a logit
+    assert logits(6, P, 130, P + 260, 130)                                           # by a row
+    assert not logits(6, P, 230, P + 200, 230) and logits(6, P, 230, P + 198, 230)   # beside each other in a row
+    assert not logits(6, P, 100, P + 1200, 100) and logits(6, P, 100, P + 1198, 100)
+    assert logits(1, P, 100, P + 198, 100) and not logits(1, P, 100, P + 200, 100)
+    assert logits(6, P, 100, P + 600, 300) and not logits(6, P, 100, P + 1200, 300)  # other strides
+
+
+def test_logits_as_sets_of_bytes():
+    rng = np.random.default_rng(5)
+    found = set()
+    for _ in range(2000):
+        rows, vocab = int(rng.integers(1, 7)), 40
+        xs, os = (vocab + int(rng.integers(0, 90)) for _ in range(2))
+        if rng.random() < 0.7:
+            os = xs
+        x, out = (P + 2 * int(rng.integers(0, 900)) for _ in range(2))
+        if x == out:
+            continue
+        spans = [{b for r in range(rows) for b in range(at + 2 * r * st, at + 2 * (r * st + vocab))}
+                 for at, st in ((x, xs), (out, os))]
+        want = bool(spans[0] & spans[1])
+        assert logits(rows, x, xs, out, os, vocab) is want, (rows, x - P, xs, out - P, os)
+        found.add(want)
+    assert found == {True, False}
