@@ -38,8 +38,11 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 
 # A decode step is a row of short launches, so what Python does around them
 # counts: the stream's handle without an object for it, checks on plain numbers.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# A torch that lacks the short ways (one without a GPU backend has neither) gives
+# both by its public calls.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(fn, device: torch.device, *args) -> None:

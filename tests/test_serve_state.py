@@ -1,10 +1,15 @@
 """What the serving path keeps between calls, on the CPU."""
 import gc
+import os
+import subprocess
+import sys
 import weakref
 
 import torch
 
 from aps2026_amd import attention
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def test_outgrown_rotation_tables_stay():
@@ -26,3 +31,14 @@ def test_outgrown_rotation_tables_stay():
     assert torch.equal(c[:9], want[0]) and torch.equal(s[:9], want[1])
     assert all(torch.equal(r(), w) for r, w in zip(held, want))
     attention._tables.pop((dev, 64, theta))
+
+
+def test_import_without_a_gpu_backend():
+    """A torch built without one has none of the functions that ask for the
+    current device and stream."""
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_getCurrent') or n == '_cuda_getDevice']:\n"
+            "    delattr(torch._C, n)\n"
+            "from aps2026_amd import decoder, serve\n"
+            "assert callable(serve._raw_stream) and callable(serve._current_device)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, timeout=300)
