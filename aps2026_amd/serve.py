@@ -2,8 +2,8 @@
 cache, attention over it, and the rules on the logits of the next token.
 
 The reference has no counterpart: its generate_decode computes the whole
-prefix again for every token (src/model.cu:163-204).  decoder.Model.decode
-runs on these.
+prefix again for every token (src/model.cu:163-204).
+decoder.Model.generate_decode runs on these.
 
 A decode step of a batch, on torch's current stream:
 

@@ -1,13 +1,14 @@
 """What the serving path keeps between calls, on the CPU."""
 import gc
 import os
+import re
 import subprocess
 import sys
 import weakref
 
 import torch
 
-from aps2026_amd import attention
+from aps2026_amd import attention, decoder, serve
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -42,3 +43,8 @@ def test_import_without_a_gpu_backend():
             "from aps2026_amd import decoder, serve\n"
             "assert callable(serve._raw_stream) and callable(serve._current_device)\n")
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT, timeout=300)
+
+
+def test_docstrings_name_what_there_is():
+    named = re.findall(r"decoder\.Model\.(\w+)", serve.__doc__)
+    assert named and all(hasattr(decoder.Model, n) for n in named)
