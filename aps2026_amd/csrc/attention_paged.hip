@@ -903,22 +903,19 @@ k_paged_tiles(PagedDev d) {
     if (t0 < t1) fetch(t0, 0);  // on its way while the queries are read
 
     // queries: a lane holds dims 16 s + 8 hf + j of its row; the sign of the
-    // scale goes into them, so that the largest product is the largest score
+    // scale goes into them (exactly), so that the largest product is the largest
+    // score, and of a scale of 0 the zero, or NaN where they are not finite
     bf16x8 qb[FP ? 1 : QT][FP ? 1 : KS];
     f32x4 qf[FP ? KS : 1];
     const float cs = d.scale_log2 == 0.0f ? 1.0f : fabsf(d.scale_log2);
-    const uint32_t flip = d.scale_log2 < 0.0f ? (FP ? 0x80000000u : 0x80008000u) : 0u;
-    const uint32_t keep = d.scale_log2 == 0.0f ? 0u : ~0u;
+    const float qs = d.scale_log2 < 0.0f ? -1.0f : d.scale_log2 == 0.0f ? 0.0f : 1.0f;
     {
         const int64_t qat = (sq.q0 + tok) * d.a.q_stride + static_cast<int64_t>(qh) * D;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int dim = (FP ? 8 : 16) * s + (FP ? 4 : 8) * hf;
             if constexpr (FP) {
-                u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const float*>(d.a.q) + qat + dim);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
-                qf[s] = __builtin_bit_cast(f32x4, w);
+                qf[s] = *reinterpret_cast<const f32x4*>(static_cast<const float*>(d.a.q) + qat + dim) * qs;
                 continue;
             }
             if constexpr (FP) {
@@ -927,7 +924,7 @@ k_paged_tiles(PagedDev d) {
                 const f32x4 x0 = *reinterpret_cast<const f32x4*>(p), x1 = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float x = j < 4 ? x0[j & 3] : x1[j & 3];
+                    float x = (j < 4 ? x0[j & 3] : x1[j & 3]) * qs;
 #pragma unroll
                     for (int t = 0; t < QT; ++t) {
                         const float hi = bf16_round(x);
@@ -936,14 +933,10 @@ k_paged_tiles(PagedDev d) {
                     }
                 }
             } else {
-                qb[0][s] = *reinterpret_cast<const bf16x8*>(static_cast<const bf16_t*>(d.a.q) + qat + dim);
-            }
+                u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const bf16_t*>(d.a.q) + qat + dim);
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                u32x4 w = __builtin_bit_cast(u32x4, qb[t][s]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (w[j] ^ flip) & keep;
-                qb[t][s] = __builtin_bit_cast(bf16x8, w);
+                for (int j = 0; j < 4; ++j) w[j] = pack2_bf16(bf16w_lo(w[j]) * qs, bf16w_hi(w[j]) * qs);
+                qb[0][s] = __builtin_bit_cast(bf16x8, w);
             }
         }
     }

@@ -67,3 +67,19 @@ def test_outputs_of_another_scale_fail(gpu_device, q_lens, kv_lens):
     for got in (c.run(50, 3, scale=0.5), torch.zeros_like(c.q), c.run(50, 3, scale=-0.5) + 1e-2):
         assert (np.abs(f64(got).reshape(want.shape) - want) > bound).mean() > 0.5
     assert math.isfinite(bound.max())
+
+
+@pytest.mark.parametrize("qt,kind", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("q_lens,kv_lens", [([2, 1], [40, 70]), ([40, 33], [90, 200])])
+def test_queries_that_are_not_finite_at_no_scale(gpu_device, qt, kind, value, q_lens, kv_lens):
+    """0 times NaN or an infinity is NaN, also where every score is 0."""
+    note(f"no scale {qt} {kind} {value} {q_lens}")
+    c = Case(gpu_device, qt, kind, 4, 2, 64, 16, q_lens, kv_lens, seed=5)
+    want, bound = exact(c, 50, 3, 0.0)
+    c.q[1, 64 + 7] = value                     # row 1, head 1
+    got = f64(c.run(50, 3, scale=0.0)).reshape(want.shape)
+    assert np.isnan(got[1, 1]).all()
+    rest = np.ones(want.shape[:2], bool)
+    rest[1, 1] = False
+    assert (np.abs(got - want) <= bound)[rest].all()
