@@ -1272,7 +1272,7 @@ PagedDev plan_one(const KvCache& c, const PagedArgs& a, int64_t least, int64_t m
     d.c = c;
     d.page_shift = c.page_shift;
     d.group = a.q_heads / c.kv_heads;
-    d.scale_log2 = a.scale * 1.4426950408889634f;
+    d.scale_log2 = a.scale * kLog2e;
     d.least = static_cast<int>(least);
     d.most = static_cast<int>(most);
     d.max_q = std::min<int64_t>(a.max_q_len, std::max<int64_t>(most / d.group, 1));

@@ -231,7 +231,8 @@ int aps_attention_paged(const aps_kv_cache* cache, const void* q, int64_t q_stri
     if (int rc = check_cache(cache, what, rows > 0 && batch > 0, &c)) return rc;
     if (int rc = check_source(c, q_dtype, what)) return rc;
     if (int rc = check_paged(c, rows, q_heads, batch, max_q_len, max_kv_len, window, sinks, &a)) return rc;
-    if (!(scale == scale) || scale - scale != 0.0f) return fail(APS_ERR_ARG, "%s: scale is not finite", what);
+    const float scale_log2 = scale * aps::kLog2e;  // what the kernels take
+    if (!(scale_log2 - scale_log2 == 0.0f)) return fail(APS_ERR_ARG, "%s: scale is not finite", what);
     const int64_t qd = static_cast<int64_t>(q_heads) * c.head_dim, per = q_dtype == APS_DTYPE_F32 ? 4 : 8;
     if (q_stride < qd || q_stride % per != 0)
         return fail(APS_ERR_SHAPE, "%s: query row stride %lld of %lld values", what, (long long)q_stride,

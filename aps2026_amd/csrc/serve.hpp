@@ -32,6 +32,7 @@ hipError_t launch_kv_append(const KvCache& cache, const KvAppendArgs& a, bool sr
 hipError_t launch_kv_gather(const KvCache& cache, const int64_t* slots, int64_t rows, void* k_out, void* v_out,
                             bool out_f32, hipStream_t s);
 
+constexpr float kLog2e = 1.4426950408889634f;
 struct PagedArgs {
     const void* q;
     int64_t q_stride;

@@ -85,7 +85,8 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * j > p - window or j < sinks: a sliding window and the first tokens.
  *   out = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j), out [rows]
  * [q_heads][head_dim] contiguous, of q's type.  q_heads is a multiple of
- * kv_heads; query head h reads key head h / (q_heads / kv_heads).
+ * kv_heads; query head h reads key head h / (q_heads / kv_heads).  scale log2 e
+ * has to be finite in fp32.
  * q_dtype F32 takes every cache type, BF16 the BF16 and MXFP4 ones.  Products
  * are exact and sums are fp32; with BF16 queries the softmax weights are held
  * for their product with v to 16 bits, and of a sequence with more than 32 rows

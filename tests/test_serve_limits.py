@@ -1,12 +1,14 @@
 """The limits on attention's distances (tests/serve_limits.py), on the CPU: they
 pass the numbers of bits that the kernels state, and fail one term (8 bits of a
 weight or a query) fewer."""
+import ctypes
 import math
 
 import numpy as np
 import pytest
 import torch
 
+from aps2026_amd import capi
 from tests import serve_limits as limits
 from tests import serve_oracle as oracle
 
@@ -43,3 +45,14 @@ def test_limits_tell_the_bits(dim, q_lens, kv_lens, query_type, bits, fewer):
     assert distance(*bits) < limits.LIMIT[bits[1]]
     for less in fewer:
         assert distance(*less) > limits.LIMIT[bits[1]]
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -2.4e38, 3.4e38, float("inf"), float("-inf"), float("nan")])
+def test_scales_without_a_base_2_form_are_refused(scale):
+    """Scores are scaled by scale log2 e, which passes fp32's range from 2.36e38."""
+    p = 1 << 20                                # no array is read
+    cache = capi.KvCacheDesc(p, p, None, None, 8, 16, 4, 128, capi.DTYPE_BF16)
+    # out lies over q, so that a call whose scale is taken is refused as well
+    rc = capi.lib().aps_attention_paged(ctypes.byref(cache), p, 2048, capi.DTYPE_BF16, 4, 16, p, p, p, 4, 2, 1, 64, 64, 0,
+                                        scale, p, None, 0, None)
+    assert rc == capi.APS_ERR_ARG and "scale" in capi.last_error()
