@@ -8,6 +8,7 @@ import torch
 from tests import serve_limits as limits
 from tests import serve_oracle as oracle
 from tests.test_gpu_serve import BF16, F32, Case, f64, held, note
+from tests.test_serve_limits import SHAPES
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,16 @@ def test_rows_of_short_sequences_beside_prompts(gpu_device):
     assert len(left) == 2 and bool((cut[left] == 5.0).all())
     c.check(torch.where(torch.isin(torch.arange(n, device=gpu_device), torch.tensor(keep, device=gpu_device))[:, None],
                         cut, out[2:2 + n]), 1 << 30, 0)
+
+
+@pytest.mark.parametrize("qt,kind", [(F32, "f32"), (F32, "bf16"), (F32, "mxfp4"), (BF16, "bf16"), (BF16, "mxfp4")])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_lens,kv_lens", SHAPES + [([90, 33], [700, 1500])])
+def test_bits_of_every_form(gpu_device, qt, kind, dim, q_lens, kv_lens):
+    """Terms beside each other in the columns (4 rows, of bf16 queries 8), tiles of
+    16 rows, blocks of 128 rows and keys that are split: 24 bits of fp32 queries
+    and their weights, 16 of bf16 queries' weights and past 32 rows 8."""
+    note(f"bits {qt} {kind} {dim} {q_lens}")
+    c = Case(gpu_device, qt, kind, 4, 1, dim, 16, q_lens, kv_lens, seed=23)
+    bits = 24 if qt is F32 else 16 if max(q_lens) <= 8 else 8
+    assert distances(c, 1 << 30, 0, [range(len(q_lens))])[0] < limits.LIMIT[bits]
