@@ -151,7 +151,7 @@ def _rows_of(t: torch.Tensor, width: int, what: str) -> int:
     if len(shape) == 2 and shape[1] == width:
         row, col = t.stride()
         if col == 1 or width == 1:
-            return row if shape[0] > 1 or row > width else width
+            return row if shape[0] > 1 else width   # the stride of a single row says nothing
     raise ValueError(f"{what}: expects rows of {width} neighbouring values")
 
 

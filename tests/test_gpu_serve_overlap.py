@@ -38,3 +38,23 @@ def test_logits_beside_their_rows(gpu_device):
     assert serve.logits_process_gpu(x[:, :45], mask=mask, out=out) is out and torch.equal(out, want)
     with pytest.raises(ValueError, match="overlap"):
         serve.logits_process_gpu(x[:, :45], mask=mask, out=x[:, 1:46])
+
+
+def test_one_row_of_a_wider_buffer(gpu_device):
+    """A single token's queries and logits, taken from rows of odd width."""
+    dev = gpu_device
+    cache = serve.PagedKvCache.allocate(2, 16, 1, 64, torch.bfloat16, dev)
+    cache.k.normal_(), cache.v.normal_()
+    plan = serve.PagedBatch([1], [20], [[1, 0]], 16, dev)
+    wide = torch.randn(3, 2 * 64 + 1, dtype=torch.bfloat16, device=dev)
+    args = (cache, plan.q_offsets, plan.kv_lens, plan.page_table, 1, 20)
+    want = serve.attention_paged_gpu(wide[:1, :128].contiguous(), *args, q_heads=2, window=64)
+    assert torch.equal(serve.attention_paged_gpu(wide[:1, :128], *args, q_heads=2, window=64), want)
+    with pytest.raises(ValueError, match="stride"):
+        serve.attention_paged_gpu(wide[:2, :128], *args, q_heads=2, window=64)
+    x = torch.randn(3, 91, device=dev)
+    y = x[:1, :90]
+    bias = dict(bias_ids=torch.tensor([[5]], dtype=torch.int32, device=dev), bias_values=torch.ones(1, 1, device=dev),
+                bias_lens=torch.ones(1, dtype=torch.int32, device=dev))
+    want = serve.logits_process_gpu(y.contiguous(), **bias)
+    assert torch.equal(serve.logits_process_gpu(y, out=y, **bias), want) and torch.equal(x[:1, :90], want)

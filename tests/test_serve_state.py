@@ -48,3 +48,12 @@ def test_import_without_a_gpu_backend():
 def test_docstrings_name_what_there_is():
     named = re.findall(r"decoder\.Model\.(\w+)", serve.__doc__)
     assert named and all(hasattr(decoder.Model, n) for n in named)
+
+
+def test_a_single_row_has_no_stride():
+    """One row of a wider buffer, whatever its neighbours' distance; more rows keep it."""
+    wide = torch.zeros(5, 2 * 64 + 1)
+    assert serve._rows_of(wide[:1, :64], 64, "x") == 64
+    assert serve._rows_of(wide[2:3, 64:128], 64, "x") == 64
+    assert serve._rows_of(wide[:2, :64], 64, "x") == 129
+    assert serve._rows_of(torch.zeros(1, 64).expand(3, 64), 64, "x") == 0
