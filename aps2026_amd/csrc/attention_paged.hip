@@ -1345,9 +1345,7 @@ Plan plan(const KvCache& c, const PagedArgs& a) {
 
 template <int D, bool Q32, Kv KV>
 hipError_t launch(const PagedDev& d, hipStream_t s) {
-    const int64_t joins = d.slots * d.a.q_heads;
-    if (d.blocks > 0x7FFFFFFF || (d.splits > 1 && joins > 0x7FFFFFFF)) return hipErrorInvalidValue;
-    const dim3 blocks(static_cast<unsigned>(d.blocks)), grid(static_cast<unsigned>(joins));
+    const dim3 blocks(static_cast<unsigned>(d.blocks)), grid(static_cast<unsigned>(d.slots * d.a.q_heads));
     if (d.tiled)
         hipLaunchKernelGGL((k_paged_tiles<D, Q32, KV>), blocks, dim3(64 * kWaves), 0, s, d);
     else if (KV != Kv::kF32 && d.lds_rows <= side_rows(Q32))
@@ -1371,6 +1369,14 @@ hipError_t launch_d(const PagedDev& d, bool q_f32, hipStream_t s) {
 }
 
 }  // namespace
+
+int64_t attention_paged_blocks(const KvCache& cache, const PagedArgs& a) {
+    const Plan p = plan(cache, a);
+    int64_t n = 0;
+    for (int i = 0; i < p.n; ++i)
+        n = std::max({n, p.d[i].blocks, p.d[i].splits > 1 ? p.d[i].slots * a.q_heads : 0});
+    return n;
+}
 
 size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a) {
     const Plan p = plan(cache, a);

@@ -136,6 +136,9 @@ int check_paged(const aps::KvCache& c, int64_t rows, int32_t q_heads, int64_t ba
     if (a->max_q_len * (q_heads / c.kv_heads) > kMaxRows)
         return fail(APS_ERR_SHAPE, "%s: %lld rows under a key head", what,
                     (long long)(a->max_q_len * (q_heads / c.kv_heads)));
+    if (rows == 0 || batch == 0 || a->max_q_len == 0) return APS_OK;
+    const int64_t blocks = aps::attention_paged_blocks(c, *a);
+    if (blocks > 0x7FFFFFFF) return fail(APS_ERR_SHAPE, "%s: %lld workgroups", what, (long long)blocks);
     return APS_OK;
 }
 

@@ -45,7 +45,9 @@ struct PagedArgs {
     void* out;
     float* part;  // partial results of a split key axis
 };
-// Bytes of `part`, and the launch; both follow one plan of the sizes.
+// The most workgroups of a launch, bytes of `part`, and the launches; all follow
+// one plan of the sizes.
+int64_t attention_paged_blocks(const KvCache& cache, const PagedArgs& a);
 size_t attention_paged_part_bytes(const KvCache& cache, const PagedArgs& a);
 hipError_t launch_attention_paged(const KvCache& cache, const PagedArgs& a, bool q_f32, hipStream_t s);
 

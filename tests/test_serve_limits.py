@@ -56,3 +56,17 @@ def test_scales_without_a_base_2_form_are_refused(scale):
     rc = capi.lib().aps_attention_paged(ctypes.byref(cache), p, 2048, capi.DTYPE_BF16, 4, 16, p, p, p, 4, 2, 1, 64, 64, 0,
                                         scale, p, None, 0, None)
     assert rc == capi.APS_ERR_ARG and "scale" in capi.last_error()
+
+
+@pytest.mark.parametrize("kv_heads,max_q", [(2048, 1),    # 2^31 workgroups for 2^20 steps
+                                            (1024, 40)])  # and for the short sequences beside chunks
+def test_more_workgroups_than_a_launch_has_are_refused(kv_heads, max_q):
+    """Before the first launch of the call: nothing is written."""
+    p, L = 1 << 20, capi.lib()
+    cache = capi.KvCacheDesc(p, p, None, None, 8, 16, kv_heads, 64, capi.DTYPE_BF16)
+    sizes = (1 << 20, kv_heads)
+    # out lies over q, so that a call whose sizes are taken is refused as well
+    rc = L.aps_attention_paged(ctypes.byref(cache), p, kv_heads * 64, capi.DTYPE_BF16, *sizes, p, p, p, 4, 1 << 20, max_q,
+                               64, 64, 0, 0.1, p, None, 0, None)
+    assert rc == capi.APS_ERR_SHAPE and "workgroups" in capi.last_error()
+    assert L.aps_attention_paged_workspace_size(ctypes.byref(cache), *sizes, 1 << 20, max_q, 64, 64, 0) == 0
