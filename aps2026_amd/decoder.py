@@ -405,6 +405,8 @@ class Model:
             raise ValueError("token out of vocabulary")
         if not repetition > 0.0:
             raise ValueError("repetition must be positive")
+        if page_size not in (16, 32, 64, 128, 256):
+            raise ValueError("page_size is 16, 32, 64, 128 or 256")
         if mask is not None and (mask.dim() != 2 or mask.shape[0] not in (1, n_seq)):
             raise ValueError("mask: one row of words, or one a prompt")
         # pages for the whole answer, consecutive for each sequence

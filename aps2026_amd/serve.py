@@ -123,6 +123,7 @@ class PagedBatch:
                  device, num_pages: Optional[int] = None):
         q, kv = np.asarray(q_lens, np.int64).reshape(-1), np.asarray(kv_lens, np.int64).reshape(-1)
         _require(q.size == kv.size == len(pages), "paged batch: one length and page list a sequence")
+        _require(page_size >= 1, "paged batch: page size")
         _require(bool(np.all(q >= 0)) and bool(np.all(kv >= q)) and bool(np.all(kv < 1 << 30)) and int(q.sum()) < 1 << 30,
                  "paged batch: 0 <= q_lens <= kv_lens")
         ids = [np.asarray(p, np.int64).reshape(-1) for p in pages]

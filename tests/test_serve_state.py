@@ -6,6 +6,7 @@ import subprocess
 import sys
 import weakref
 
+import pytest
 import torch
 
 from aps2026_amd import attention, decoder, serve
@@ -57,3 +58,14 @@ def test_a_single_row_has_no_stride():
     assert serve._rows_of(wide[2:3, 64:128], 64, "x") == 64
     assert serve._rows_of(wide[:2, :64], 64, "x") == 129
     assert serve._rows_of(torch.zeros(1, 64).expand(3, 64), 64, "x") == 0
+
+
+@pytest.mark.parametrize("page_size", [0, -16, 24, 512])
+def test_page_sizes_that_no_cache_has(page_size):
+    emb = torch.zeros(8, 16)
+    model = decoder.Model(emb, emb[0], emb[0], emb, None, [])
+    with pytest.raises(ValueError, match="page_size is 16"):
+        model.generate_decode([[1, 2]], 2, page_size=page_size)
+    if page_size < 1:
+        with pytest.raises(ValueError, match="page size"):
+            serve.PagedBatch([1], [1], [[0]], page_size, "cpu")
