@@ -265,13 +265,15 @@ class DecoderLayer:
 
     def attention_cached(self, b: Buffers, plan: CachedRows, cache: serve.PagedKvCache, stream) -> None:
         """normed -> att over the paged cache: projections, q and k rotated as
-        k and v go into the cache, attention over what is there."""
+        k and v go into the cache, attention over what is there.  All of it on
+        `stream`, the current one or not."""
         self._project(b, b.normed, (("q_proj", b.q, QD), ("k_proj", b.k, KD), ("v_proj", b.v, KD)), stream)
         p = plan.batch
         c, s = _device_table(b.q.device, p.max_kv_len, HEAD_DIM, ROPE_THETA)
-        serve.kv_append_gpu(cache, b.k, b.v, p.positions, p.slots, c, s, q=b.q, q_out=b.q)
-        serve.attention_paged_gpu(b.q, cache, p.q_offsets, p.kv_lens, p.page_table, p.max_q_len, p.max_kv_len,
-                                  q_heads=NUM_ATTENTION_HEADS, window=plan.window, sinks=plan.sinks, out=b.att)
+        with serve.on_stream(stream, b.q.device):
+            serve.kv_append_gpu(cache, b.k, b.v, p.positions, p.slots, c, s, q=b.q, q_out=b.q)
+            serve.attention_paged_gpu(b.q, cache, p.q_offsets, p.kv_lens, p.page_table, p.max_q_len, p.max_kv_len,
+                                      q_heads=NUM_ATTENTION_HEADS, window=plan.window, sinks=plan.sinks, out=b.att)
 
     def forward_carry(self, b: Buffers, plan, has_carry: bool, stream, cache: Optional[serve.PagedKvCache] = None
                       ) -> None:

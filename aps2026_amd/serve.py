@@ -18,6 +18,7 @@ host).  Wrong shapes, types and layouts raise ValueError.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional, Sequence, Tuple
@@ -55,6 +56,16 @@ def _launch(fn, device: torch.device, *args) -> None:
             rc = fn(*args, _raw_stream(index))
     if rc:
         _call(rc)
+
+
+def on_stream(stream, device: torch.device):
+    """A context whose current stream of device is `stream`: a handle, as an
+    int or a c_void_p (None or 0: the default stream)."""
+    handle = (stream.value if isinstance(stream, ctypes.c_void_p) else stream) or 0
+    if handle == _raw_stream(device.index):
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(handle, device) if handle
+                             else torch.cuda.default_stream(device))
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
