@@ -51,7 +51,15 @@ constexpr int kMostWaves = 8;  // 256 registers a wave
 constexpr int kRows = 16;      // rows of a tile
 constexpr int kMaxSplits = 256, kFewSplits = 8;
 constexpr int kPlainLds = 62 * 1024;  // dynamic LDS that needs no leave: 64 KB less the static part
-constexpr int64_t kTiledRows = 33;  // rows of a sequence under a key head from which k_paged_tiles takes them
+// Rows of a sequence under a key head from which k_paged_tiles takes them.  us in
+// k_paged_rows / k_paged_tiles, of 64 sequences on 1024 keys and of 2 on 8192:
+//   36 rows  bf16 67 / 34, 26 / 18   fp32 on bf16 69 / 50, 29 / 25
+//            4 bits 31 / 30, 16 / 17  fp32 cache 122 / 141, 47 / 48
+//   20 rows  bf16 47 / 31, 15 / 17   fp32 on bf16 49 / 38, 17 / 24
+//            4 bits 23 / 25, 12 / 16  fp32 cache 85 / 84, 25 / 46
+// Below it k_paged_rows is ahead where there are few sequences or few bits, and
+// holds weights to more of them.
+constexpr int64_t kTiledRows = 33;
 
 // What both kernels know of the launch.
 struct PagedDev {
@@ -282,6 +290,7 @@ __device__ void redo_row(const PagedDev& d, const int32_t* table, int h, const K
 // then hold the same weight and take their term of it; O is summed at the end.
 // (One sequence of 131072 4-bit keys, fp32 queries: 27.0 -> 24.7 us; 64 of 16384:
 // 113 -> 94, with BF16 queries 91 -> 89; a bf16 cache is bound by its bytes.)
+// The rows that 16 columns hold beside each other: of four terms, of two.
 constexpr int side_rows(bool q32) { return q32 ? 4 : 8; }
 
 template <int D, bool Q32, Kv KV, bool SIDE>
@@ -719,7 +728,9 @@ k_paged_rows(PagedDev d) {
 // weights keeps 32 bits): a second term would cost half as many MFMAs again.  fp32
 // queries keep three.
 // Bound by the matrix cores and what feeds them: 4 x 2048 tokens on 8192 keys, 16
-// heads of 128, bf16, 358 us = 0.91 PFLOP/s (the library's 8192^3 product 1.16).
+// heads of 128, bf16, 358 to 367 us = 0.91 PFLOP/s (the library's 8192^3 product
+// 1.16); many times over without a pause 411, at the clock that is left then.  fp32
+// queries, three products for one: 858 on a bf16 cache, 874 on 4 bits.
 // LDS rows are one key's D values; 16-byte chunks are permuted so that the lanes
 // served together (16 keys' same chunk for K, 4 keys' 64 bytes for V) lie in
 // different banks.
@@ -758,9 +769,10 @@ k_paged_tiles(PagedDev d) {
     const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
     // Workgroups take the row blocks that there are, sequence by sequence, so
     // that those without one are the last of the grid (left between, they
-    // take their XCD's share: 3 ragged chunks of 500 tokens 59 us, closed up
-    // 35).  Row blocks of one key head go round the XCDs: each L2 reads every
-    // sequence's keys, but no XCD is left with the long ones.
+    // take their XCD's share: 3 ragged chunks of 500 tokens on a 4-bit cache, with
+    // the join, 69 us, closed up 55).  Row blocks of one key head go round the
+    // XCDs: each L2 reads every sequence's keys, but no XCD is left with the long
+    // ones.
     uint32_t id = blockIdx.x;
     const uint32_t per = static_cast<uint32_t>(d.c.kv_heads * d.splits);
     int64_t b = -1;
@@ -1354,6 +1366,9 @@ hipError_t launch(const PagedDev& d, hipStream_t s) {
     else
         hipLaunchKernelGGL((k_paged_rows<D, Q32, KV, false>), blocks, dim3(64 * d.waves),
                            static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4, s, d);
+    // (us of the call with a wave a row / four: 16 x 8192 keys, 8 parts, 45.5 / 46.4;
+    // with four / sixteen: 1 x 131072, 128 parts, 47.6 / 47.0, 1 x 20000, 79 parts,
+    // 16.5 / 15.9)
     if (d.splits > 64) hipLaunchKernelGGL((k_paged_join<D, Q32, 16>), grid, dim3(1024), 0, s, d);
     else if (d.splits > kFewSplits) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
     else if (d.splits > 1) hipLaunchKernelGGL((k_paged_join<D, Q32, 1>), grid, dim3(64), 0, s, d);

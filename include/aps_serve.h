@@ -95,10 +95,11 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * (batch - 1) max_q_len + 32 / (q_heads / kv_heads): no room but for padding.)
  *
  * All arrays in device memory; q_offsets ascend; batch up to 2^20, max_kv_len up
- * to 2^30.  max_q_len and max_kv_len bound the batch's
- * lengths on the host (they shape the launch, so a recorded graph serves any
- * lengths within them): queries past max_q_len of a sequence are left as they
- * were, lengths past max_kv_len or past table_stride pages are cut.
+ * to 2^30 (sizes that take more than 2^31 - 1 workgroups are refused).  max_q_len
+ * and max_kv_len bound the batch's lengths on the host (they shape the launch, so a
+ * recorded graph serves any lengths within them): queries past max_q_len of a
+ * sequence are left as they were, lengths past max_kv_len or past table_stride
+ * pages are cut.
  * Rows of out that no sequence names are left as they were.  A query that sees
  * no key (kv_lens[b] below its queries' number, or 0), or whose every score is
  * -inf, gives zeros.  A page id outside the cache leaves its keys out; entries
@@ -107,8 +108,8 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * see, NaN may stand where the formula has an infinity.
  * workspace: aps_attention_paged_workspace_size bytes (0: none), 256-byte
  * aligned; calls that overlap need one each.  q, out 16-byte aligned, q_stride
- * a multiple of 16 bytes.  out and workspace overlap nothing else of the call (refused
- * for q, out and workspace). */
+ * a multiple of 16 bytes.  out and workspace overlap nothing else of the call
+ * (refused for q, out and workspace). */
 APS_API size_t aps_attention_paged_workspace_size(const aps_kv_cache* cache, int64_t rows, int32_t q_heads,
                                                   int64_t batch, int64_t max_q_len, int64_t max_kv_len,
                                                   int32_t window, int32_t sinks);
