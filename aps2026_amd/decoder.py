@@ -25,6 +25,7 @@ reading fp32 x exactly and the experts a bf16 copy of it).
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -388,7 +389,8 @@ class Model:
         and with eos, and the logits [batch][max_new_tokens][vocab] they were
         chosen from: after the penalties, the biases {id: value} and the mask
         ([1] or [batch] rows of int32 words, bit t % 32 of word t / 32 allows
-        token t).  Of equal logits the lowest id wins.  One host wait, at the
+        token t).  Of equal logits the lowest id wins; NaN never does beside
+        a number, and of none but NaN and -inf id 0.  One host wait, at the
         end.  Caches and activations are the call's own, from torch's caching
         allocator: calls may run side by side on other streams."""
         if len(prompts) == 0:
@@ -452,9 +454,9 @@ class Model:
                     rules["history_lens"] = kv_lens
                 serve.logits_process_gpu(logits, out=logits, **rules)
             out[:, t] = logits
-            # argmax leaves open which of equal logits it takes
-            top = torch.where(logits == logits.amax(1, keepdim=True), torch.arange(V, device=dev), V).amin(1)
-            token = top.clamp(max=V - 1).to(torch.int32)
+            # argmax leaves open which of equal logits it takes, and takes a NaN
+            x = torch.where(logits.isnan(), -math.inf, logits)
+            token = torch.where(x == x.amax(1, keepdim=True), torch.arange(V, device=dev), V).amin(1).to(torch.int32)
             ids[:, t] = token
             if t + 1 == max_new_tokens:
                 break

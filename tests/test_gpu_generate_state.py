@@ -98,3 +98,26 @@ def test_a_layer_runs_on_the_stream_it_is_given(model, gpu_device, as_int):
     assert bool(want[0].abs().sum() > 0)
     for stream, within in ((side, default), (default, side), (side, side)):
         assert all(torch.equal(a, b) for a, b in zip(run(stream, within), want))
+
+
+def test_a_logit_that_is_nan_is_not_chosen(model, gpu_device):
+    """One token's logit is NaN in every step: the choice is the largest of the
+    others; of nothing but NaN it is token 0."""
+    ids, logits = model.generate_decode([[5, 9, 200], [7]], 3, eos=-1)
+    keep = model.head_w.clone()
+    try:
+        model.head_w[ids[0][0]] = float("nan")
+        got, with_nan = model.generate_decode([[5, 9, 200], [7]], 3, eos=-1)
+        assert bool(with_nan[:, :, ids[0][0]].isnan().all())
+        best = torch.where(with_nan.isnan(), -float("inf"), with_nan).amax(2)
+        assert got[0][0] != ids[0][0]
+        for b in range(2):
+            for t in range(3):
+                assert with_nan[b, t, got[b][t]] == best[b, t]
+        second = logits[:, 0].clone()
+        second[:, ids[0][0]] = -float("inf")
+        assert [row[0] for row in got] == second.argmax(1).tolist()
+        model.head_w.fill_(float("nan"))
+        assert model.generate_decode([[5], [7, 8]], 2, eos=-1)[0] == [[0, 0], [0, 0]]
+    finally:
+        model.head_w.copy_(keep)
