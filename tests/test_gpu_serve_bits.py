@@ -31,6 +31,7 @@ def distances(c, window, sinks, parts, **kw):
     ([90, 1, 90, 90] + [1] * 5, [400, 900, 90, 300, 130, 350, 800, 411, 202], 1),    # three prompts beside steps
     ([1, 70, 8, 70], [700, 70, 300, 350], 8),                                        # up to 8 tokens: 32 rows
     ([64, 64, 3], [64, 500, 1900], 3),                                               # keys of the steps are split
+    ([64, 8, 64], [300, 400, 500], 8),                                               # the most rows that leave room for it
 ])
 def test_steps_beside_prompts_keep_their_bits(gpu_device, kind, q_lens, kv_lens, most):
     """Weights of a sequence of up to 32 rows keep 16 bits whatever stands beside
