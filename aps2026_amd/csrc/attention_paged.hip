@@ -728,8 +728,8 @@ k_paged_rows(PagedDev d) {
 // weights keeps 32 bits): a second term would cost half as many MFMAs again.  fp32
 // queries keep three.
 // Bound by the matrix cores and what feeds them: 4 x 2048 tokens on 8192 keys, 16
-// heads of 128, bf16, 358 to 367 us = 0.91 PFLOP/s (the library's 8192^3 product
-// 1.16); many times over without a pause 411, at the clock that is left then.  fp32
+// heads of 128, bf16, 358 to 372 us = 0.88 to 0.91 PFLOP/s (the library's 8192^3
+// product 1.16); many times over without a pause 411, at the clock that is left then.  fp32
 // queries, three products for one: 858 on a bf16 cache, 874 on 4 bits.
 // LDS rows are one key's D values; 16-byte chunks are permuted so that the lanes
 // served together (16 keys' same chunk for K, 4 keys' 64 bytes for V) lie in
