@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libaps_moe.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "aps_moe.h")
 SERVE_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "aps_serve.h")
+DECODE_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "aps_decode.h")
 
 APS_OK = 0
 APS_ERR_SHAPE = -1
@@ -28,6 +29,8 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_E4M3 = 2
 KV_MXFP4 = 3
+ROPE_HALF = 0
+ROPE_PAIRS = 1
 
 _c_vp = ctypes.c_void_p
 _c_vpp = ctypes.POINTER(ctypes.c_void_p)
@@ -69,6 +72,11 @@ class LogitsRules(ctypes.Structure):
                 ("bias_ids", _c_vp), ("bias_values", _c_vp), ("bias_lens", _c_vp), ("bias_stride", ctypes.c_int64),
                 ("mask", _c_vp), ("mask_rows", ctypes.c_int64), ("mask_stride", ctypes.c_int64),
                 ("mask_index", _c_vp)]
+
+
+class Q4WeightDesc(ctypes.Structure):
+    _fields_ = [("codes", _c_vp), ("scales", _c_vp), ("zeros", _c_vp), ("out_features", ctypes.c_int32),
+                ("in_features", ctypes.c_int32), ("group", ctypes.c_int32), ("scale_dtype", ctypes.c_int32)]
 
 
 class ApsError(RuntimeError):
@@ -152,7 +160,20 @@ def lib():
     L.aps_attention_paged.argtypes = [cache, _c_vp, i64, i32, i64, i32, _c_vp, _c_vp, _c_vp, i64, i64, i64, i64, i32,
                                       i32, ctypes.c_float, _c_vp, _c_vp, sz, _c_vp]
     L.aps_logits_process.argtypes = [_c_vp, i64, i32, i64, i64, ctypes.POINTER(LogitsRules), _c_vp, i64, _c_vp]
-    for name in ("aps_kv_append", "aps_kv_gather", "aps_attention_paged", "aps_logits_process"):
+    f32, q4 = ctypes.c_float, ctypes.POINTER(Q4WeightDesc)
+    L.aps_rope.argtypes = [_c_vp, i64, _c_vp, i64, i32, _c_vp, i64, _c_vp, i64, i32, i32, i64, i32, i32, i32, i32, _c_vp,
+                           _c_vp, f32, _c_vp]
+    L.aps_rope_freq_table.argtypes = [_c_vp, i32, i64, i64, f32, _c_vp, _c_vp, _c_vp]
+    L.aps_linear_q4_workspace_size.argtypes = [q4, i64, i32]
+    L.aps_linear_q4_workspace_size.restype = sz
+    L.aps_linear_q4.argtypes = [_c_vp, i64, i32, i64, q4, _c_vp, _c_vp, _c_vp, sz, _c_vp]
+    L.aps_quantise_q4.argtypes = [_c_vp, i32, q4, _c_vp]
+    L.aps_token_logprobs_workspace_size.argtypes = [i64, i64, i32, i32]
+    L.aps_token_logprobs_workspace_size.restype = sz
+    L.aps_token_logprobs.argtypes = [_c_vp, i64, i32, i64, i64, _c_vp, i64, i32, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, sz,
+                                     _c_vp]
+    for name in ("aps_kv_append", "aps_kv_gather", "aps_attention_paged", "aps_logits_process", "aps_rope",
+                 "aps_rope_freq_table", "aps_linear_q4", "aps_quantise_q4", "aps_token_logprobs"):
         getattr(L, name).restype = ctypes.c_int
     for name in ("aps_moe_weights_register", "aps_moe_weights_release", "aps_moe_workspace_layout",
                  "aps_router_logits", "aps_moe_route_top2", "aps_moe_dispatch", "aps_moe_expert_ffn",

@@ -68,6 +68,61 @@ struct LogitsArgs {
 };
 hipError_t launch_logits_process(const LogitsArgs& a, bool f32, hipStream_t s);
 
+struct RopeArgs {
+    const void *q, *k;
+    void *q_out, *k_out;
+    int64_t q_stride, q_out_stride, k_stride, k_out_stride;
+    int64_t rows;
+    int q_heads, k_heads;  // 0 without
+    int head_dim, rotary_dim;
+    bool pairs, inverse;
+    const int32_t* positions;
+    const double* freq;
+    float amplitude;
+};
+hipError_t launch_rope(const RopeArgs& a, bool f32, hipStream_t s);
+hipError_t launch_rope_table(const double* freq, int pairs, int64_t first, int64_t count, float amplitude,
+                             float* cosv, float* sinv, hipStream_t s);
+
+struct LogprobArgs {
+    const void* x;
+    int64_t x_stride, rows, vocab;
+    const int32_t* tokens;
+    int64_t n_tokens;
+    int top;
+    float *logprobs, *entropy;  // entropy may be null
+    int32_t* top_ids;
+    float* top_logprobs;
+    float* part;  // a split row's parts
+};
+constexpr int kLogprobTop = 64;
+constexpr int64_t kLogprobVocab = int64_t(1) << 20;
+int64_t token_logprobs_blocks(int64_t rows, int64_t vocab, bool f32);
+size_t token_logprobs_part_bytes(int64_t rows, int64_t vocab, int top, bool f32);
+hipError_t launch_token_logprobs(const LogprobArgs& a, bool f32, hipStream_t s);
+
+// Weights in 4 bits: w[n][k] = (code - zero) scale, a scale and a zero for each
+// `group` neighbouring k.
+struct Q4 {
+    const uint8_t* codes;
+    const void* scales;
+    const uint8_t* zeros;  // null: 8
+    int out, in, group;
+    bool scales_f32;
+};
+struct LinearQ4Args {
+    Q4 w;
+    const void* x;
+    int64_t x_stride, rows;
+    const float* bias;
+    void* y;          // [rows][out]
+    uint16_t* terms;  // fp32 x in bf16 terms, for many rows
+};
+size_t linear_q4_term_bytes(int64_t rows, int in, int out, bool f32);
+hipError_t launch_linear_q4(const LinearQ4Args& a, bool f32, hipStream_t s);
+hipError_t launch_quantise_q4(const void* w, bool w_f32, int64_t out, int in, int group, uint8_t* codes,
+                              void* scales, bool scales_f32, uint8_t* zeros, hipStream_t s);
+
 // ---- 4-bit blocks ----------------------------------------------------------
 
 // The scale byte of a block from the largest |value| bits in it: with amax =

@@ -1,5 +1,7 @@
-"""Serving operators over the C ABI (include/aps_serve.h): a paged key/value
-cache, attention over it, and the rules on the logits of the next token.
+"""Serving operators over the C ABI (include/aps_serve.h, aps_decode.h): a
+paged key/value cache, attention over it, and the rules on the logits of the
+next token; rotary positions of other layouts and scalings, linear layers with
+weights in 4 bits, and log probabilities of tokens.
 
 The reference has no counterpart: its generate_decode computes the whole
 prefix again for every token (src/model.cu:163-204).
@@ -12,6 +14,13 @@ A decode step of a batch, on torch's current stream:
     out = attention_paged_gpu(q, cache, plan.q_offsets, plan.kv_lens, plan.page_table, plan.max_q_len,
                               plan.max_kv_len, q_heads=16, window=2047, sinks=4)
 
+and around it, for a model with weights in 4 bits:
+
+    w = quantise_q4_gpu(weight, group=128)
+    y = linear_q4_gpu(x, w, bias)
+    q, k = rope_gpu(q, k, plan.positions, freq, head_dim=128, layout="pairs", amplitude=amplitude)
+    scores = token_logprobs_gpu(logits, tokens, top=5)
+
 Calls launch kernels and read nothing back, so they can be captured into a
 graph; index arrays are read on the device (PagedBatch checks its own on the
 host).  Wrong shapes, types and layouts raise ValueError.
@@ -21,7 +30,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -329,3 +338,232 @@ def logits_process_gpu(logits: torch.Tensor, history: Optional[torch.Tensor] = N
     _launch(capi.lib().aps_logits_process, dev, logits.data_ptr(), stride, code, rows, vocab, ctypes.byref(rules),
             out.data_ptr(), _rows_of(out, vocab, what))
     return out
+
+
+# ---- rotary positions ---------------------------------------------------------
+
+_LAYOUT = {"half": capi.ROPE_HALF, "pairs": capi.ROPE_PAIRS}
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                     trained: int = 4096, fast: float = 32.0, slow: float = 1.0,
+                     divisors: Optional[Sequence[float]] = None) -> Tuple[np.ndarray, float]:
+    """(angles per position [rotary_dim / 2] in 64 bits, amplitude) of the pairs
+    theta^(-2 i / rotary_dim), for contexts `factor` times the trained length:
+      "none"    as they are
+      "linear"  all divided by factor: positions between the trained ones
+      "base"    theta times factor^(rotary_dim / (rotary_dim - 2)): the fastest
+                pair stays, the slowest is divided by factor
+      "parts"   pairs that turn `fast` times or more in the trained length stay,
+                those that turn `slow` times or less are divided by factor, in
+                between by parts; amplitude 1 + 0.1 ln factor
+      "divisors" each pair by its own"""
+    _require(rotary_dim >= 2 and rotary_dim % 2 == 0, "rope_frequencies: an even rotary_dim")
+    _require(theta > 0.0 and 0.0 < factor < math.inf, "rope_frequencies: theta and factor are positive")
+    i = np.arange(rotary_dim // 2)
+    if scaling == "base":
+        _require(rotary_dim > 2, "rope_frequencies: a base needs two pairs")
+        return (theta * factor ** (rotary_dim / (rotary_dim - 2))) ** (-2.0 * i / rotary_dim), 1.0
+    freq = float(theta) ** (-2.0 * i / rotary_dim)
+    if scaling == "linear":
+        return freq / factor, 1.0
+    if scaling == "parts":
+        _require(fast > slow and trained >= 1, "rope_frequencies: fast > slow, a trained length")
+        stay = np.clip((trained * freq / (2 * math.pi) - slow) / (fast - slow), 0.0, 1.0)
+        return freq * (stay + (1 - stay) / factor), 1.0 + 0.1 * math.log(factor)
+    if scaling == "divisors":
+        by = np.asarray(divisors if divisors is not None else (), np.float64)
+        _require(by.shape == freq.shape and bool(np.all(by > 0)), "rope_frequencies: a positive divisor for each pair")
+        return freq / by, 1.0
+    _require(scaling == "none", f"rope_frequencies: scaling {scaling!r}")
+    return freq, 1.0
+
+
+def rope_gpu(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freq: torch.Tensor, head_dim: int,
+             layout: str = "half", amplitude: float = 1.0, inverse: bool = False,
+             q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None
+             ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(q, k) [rows, heads * head_dim], fp32 or bf16 with any row stride, turned
+    by positions (int32; a negative one copies its row) times freq (float64, an
+    angle for each pair: the first 2 len(freq) values of a head turn, the rest is
+    copied).  layout: the pairs are (i, i + len(freq)) ("half") or (2 i, 2 i + 1)
+    ("pairs").  inverse turns back: the gradient.  k may be None.  q_out and k_out
+    may be q and k themselves."""
+    what, dev, dt = "rope", q.device, q.dtype
+    code = _CODE.get(dt)
+    if code is None or dev.type != "cuda":
+        raise ValueError("rope: fp32 or bf16 rows on a GPU")
+    if layout not in _LAYOUT:
+        raise ValueError(f"rope: layout {layout!r}")
+    rows, width = q.shape[0], q.shape[-1]
+    q_stride = _rows_of(q, width, what)
+    if head_dim < 2 or width % head_dim or positions.numel() != rows or freq.dim() != 1:
+        raise ValueError("rope shape")
+    if q_out is None:
+        q_out, qo_stride = _like(q), width
+    elif q_out.shape != q.shape or q_out.dtype is not dt or q_out.device != dev:
+        raise ValueError("rope: q_out of q's shape and type")
+    else:
+        qo_stride = _rows_of(q_out, width, what)
+    kp = kop = None
+    k_heads = k_stride = ko_stride = 0
+    if k is not None:
+        k_width = k.shape[-1]
+        k_stride = _rows_of(k, k_width, what)
+        if k.shape[0] != rows or k_width % head_dim or k.dtype is not dt or k.device != dev:
+            raise ValueError("rope: k [rows, heads * head_dim] of q's type")
+        if k_out is None:
+            k_out, ko_stride = _like(k), k_width
+        elif k_out.shape != k.shape or k_out.dtype is not dt or k_out.device != dev:
+            raise ValueError("rope: k_out of k's shape and type")
+        else:
+            ko_stride = _rows_of(k_out, k_width, what)
+        kp, kop, k_heads = k.data_ptr(), k_out.data_ptr(), k_width // head_dim
+    elif k_out is not None:
+        raise ValueError("rope: k_out without k")
+    _launch(capi.lib().aps_rope, dev, q.data_ptr(), q_stride, q_out.data_ptr(), qo_stride, width // head_dim, kp,
+            k_stride, kop, ko_stride, k_heads, code, rows, head_dim, 2 * freq.shape[0], _LAYOUT[layout], inverse,
+            _dev(positions, dev, torch.int32, what), _dev(freq, dev, torch.float64, what), amplitude)
+    return q_out, k_out
+
+
+def rope_table_gpu(freq: torch.Tensor, positions: int, amplitude: float = 1.0, first: int = 0
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin) [positions, len(freq)] fp32 of the positions from `first`, times
+    amplitude: kv_append_gpu's tables from such frequencies."""
+    dev = freq.device
+    if freq.dim() != 1 or dev.type != "cuda" or positions < 0:
+        raise ValueError("rope_table: a vector of frequencies on a GPU")
+    cos = torch.empty((positions, freq.shape[0]), dtype=torch.float32, device=dev)
+    sin = torch.empty_like(cos)
+    _launch(capi.lib().aps_rope_freq_table, dev, _dev(freq, dev, torch.float64, "rope_table"), freq.shape[0], first,
+            positions, amplitude, cos.data_ptr(), sin.data_ptr())
+    return cos, sin
+
+
+# ---- weights in 4 bits --------------------------------------------------------
+
+class Q4Weight:
+    """A weight [out, in] in 4 bits, (code - zero) scale: codes uint8 [out, in /
+    2] (two to a byte, the even input in the low half), scales [out, in / group]
+    fp32 or bf16, zeros uint8 [out, in / group] (None: 8); groups of 32, 64 or
+    128.  The tensors stay the caller's; quantise_q4_gpu makes them."""
+
+    __slots__ = ("codes", "scales", "zeros", "out_features", "in_features", "group", "device", "_desc", "_ref")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None):
+        dev, shape, per = codes.device, codes.shape, scales.shape
+        code = _CODE.get(scales.dtype)
+        if len(shape) != 2 or codes.dtype is not torch.uint8 or dev.type != "cuda" or not codes.is_contiguous():
+            raise ValueError("4-bit weight: codes uint8 [out, in / 2] on a GPU")
+        if len(per) != 2 or per[0] != shape[0] or not per[1] or 2 * shape[1] % per[1] or code is None or \
+                scales.device != dev or not scales.is_contiguous():
+            raise ValueError("4-bit weight: scales [out, in / group], fp32 or bf16")
+        if zeros is not None and (zeros.shape != per or zeros.dtype is not torch.uint8 or zeros.device != dev or
+                                  not zeros.is_contiguous()):
+            raise ValueError("4-bit weight: zeros uint8 [out, in / group]")
+        self.out_features, self.in_features, self.device = shape[0], 2 * shape[1], dev
+        self.group = self.in_features // per[1]
+        if self.group not in (32, 64, 128):
+            raise ValueError(f"4-bit weight: groups of {self.group} (32, 64 or 128)")
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+        self._desc = capi.Q4WeightDesc(codes.data_ptr(), scales.data_ptr(), _p(zeros), self.out_features,
+                                       self.in_features, self.group, code)
+        self._ref = ctypes.byref(self._desc)
+
+
+def quantise_q4_gpu(weight: torch.Tensor, group: int = 128, zeros: bool = True,
+                    scale_dtype: torch.dtype = torch.bfloat16) -> Q4Weight:
+    """weight [out, in] (contiguous, fp32 or bf16) in 4 bits: the codes of each
+    group spread over its range (zeros), or its largest magnitude at 7."""
+    code = _CODE.get(weight.dtype)
+    if weight.dim() != 2 or code is None or weight.device.type != "cuda" or not weight.is_contiguous():
+        raise ValueError("quantise_q4: a contiguous fp32 or bf16 weight [out, in] on a GPU")
+    n, k = weight.shape
+    if group not in (32, 64, 128) or k % group or not k or scale_dtype not in _CODE:
+        raise ValueError("quantise_q4: groups of 32, 64 or 128 that divide the inputs, fp32 or bf16 scales")
+    new = lambda width, dt: torch.empty((n, width), dtype=dt, device=weight.device)  # noqa: E731
+    to = Q4Weight(new(k // 2, torch.uint8), new(k // group, scale_dtype),
+                  new(k // group, torch.uint8) if zeros else None)
+    _launch(capi.lib().aps_quantise_q4, weight.device, weight.data_ptr(), code, to._ref)
+    return to
+
+
+def linear_q4_gpu(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x W^T (+ bias, fp32) of x [rows, in], fp32 or bf16 with any row stride, in
+    x's type.  The workspace is torch's, taken on the current stream, unless one
+    is given (uint8)."""
+    what, dev, dt = "linear_q4", weight.device, x.dtype
+    code = _CODE.get(dt)
+    if code is None or x.device != dev:
+        raise ValueError("linear_q4: fp32 or bf16 rows on the weight's device")
+    stride, rows, n = _rows_of(x, weight.in_features, what), x.shape[0], weight.out_features
+    if out is None:
+        out = torch.empty((rows, n), dtype=dt, device=dev)
+    elif out.shape != (rows, n) or out.dtype is not dt or out.device != dev or not out.is_contiguous():
+        raise ValueError("linear_q4: out [rows, out] of x's type, contiguous")
+    bp = None
+    if bias is not None:
+        if bias.numel() != n:
+            raise ValueError("linear_q4: a bias for each output")
+        bp = _dev(bias, dev, torch.float32, what)
+    lib = capi.lib()
+    wp, wn = None, lib.aps_linear_q4_workspace_size(weight._ref, rows, code)
+    if wn:
+        if workspace is None:
+            workspace = torch.empty(wn, dtype=torch.uint8, device=dev)
+        elif workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("linear_q4: a contiguous workspace on the weight's device")
+        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch(lib.aps_linear_q4, dev, x.data_ptr(), stride, code, rows, weight._ref, bp, out.data_ptr(), wp, wn)
+    return out
+
+
+# ---- log probabilities --------------------------------------------------------
+
+class TokenLogprobs(NamedTuple):
+    """logprobs as the tokens' shape (None without tokens), entropy [rows],
+    top_ids (int32) and top_logprobs [rows, top]."""
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs_gpu(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0,
+                       workspace: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """Log probabilities under logits [rows, vocab], fp32 or bf16 with any row
+    stride: of the given tokens ([rows] or [rows, n] int32; 0 for an id outside
+    the vocabulary), and of the `top` likeliest (up to 64; of equal logits the
+    lower id first), and the rows' entropies, all fp32.  Logits of -inf have the
+    probability 0.  The workspace is torch's, taken on the current stream, unless
+    one is given (uint8)."""
+    what, dev = "token_logprobs", logits.device
+    code = _CODE.get(logits.dtype)
+    if code is None or dev.type != "cuda" or logits.dim() != 2:
+        raise ValueError("token_logprobs: fp32 or bf16 logits [rows, vocab] on a GPU")
+    rows, vocab = logits.shape
+    stride = _rows_of(logits, vocab, what)
+    n, tp, lp, logprobs = 0, None, None, None
+    if tokens is not None:
+        shape = tokens.shape
+        if len(shape) not in (1, 2) or shape[0] != rows:
+            raise ValueError("token_logprobs: tokens [rows] or [rows, n]")
+        n, tp = (shape[1] if len(shape) == 2 else 1), _dev(tokens, dev, torch.int32, what)
+        logprobs = torch.empty(shape, dtype=torch.float32, device=dev)
+        lp = logprobs.data_ptr()
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    top_ids = torch.empty((rows, max(top, 0)), dtype=torch.int32, device=dev)
+    top_logprobs = torch.empty((rows, max(top, 0)), dtype=torch.float32, device=dev)
+    lib = capi.lib()
+    wp, wn = None, lib.aps_token_logprobs_workspace_size(rows, vocab, top, code)
+    if wn:
+        if workspace is None:
+            workspace = torch.empty(wn, dtype=torch.uint8, device=dev)
+        elif workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("token_logprobs: a contiguous workspace on the logits' device")
+        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch(lib.aps_token_logprobs, dev, logits.data_ptr(), stride, code, rows, vocab, tp, n, top, lp,
+            entropy.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(), wp, wn)
+    return TokenLogprobs(logprobs, entropy, top_ids, top_logprobs)
