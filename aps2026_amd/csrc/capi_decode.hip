@@ -141,7 +141,7 @@ size_t aps_linear_q4_workspace_size(const aps_q4_weight* weight, int64_t rows, i
     if (check_q4(weight, "linear_q4", false, &w) || check_dtype(dtype, "linear_q4") ||
         check_linear_q4(w, rows, "linear_q4"))
         return 0;
-    return aps::linear_q4_term_bytes(rows, w.in, w.out, dtype == APS_DTYPE_F32);
+    return aps::linear_q4_bytes(w, rows, dtype == APS_DTYPE_F32);
 }
 
 int aps_linear_q4(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, const aps_q4_weight* weight,
@@ -158,7 +158,7 @@ int aps_linear_q4(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, 
     const uintptr_t elt = dtype == APS_DTYPE_F32 ? 4 : 2;
     if (mis(x, elt) || mis(y, elt) || mis(bias, 4))
         return fail(APS_ERR_ARG, "%s: arrays must be aligned to their elements", what);
-    const size_t need = aps::linear_q4_term_bytes(rows, w.in, w.out, dtype == APS_DTYPE_F32);
+    const size_t need = aps::linear_q4_bytes(w, rows, dtype == APS_DTYPE_F32);
     if (need && (!workspace || workspace_bytes < need))
         return fail(APS_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
     if (need && mis(workspace, 16)) return fail(APS_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", what);

@@ -1,21 +1,20 @@
 // Linear layers with weights in 4 bits (aps_linear_q4): y = x W^T + b with
 // W[n][k] = (code - zero) scale, a scale and a zero for each `group` inputs; and
-// aps_quantise_q4, which makes such weights.
+// aps_quantise_q4, which makes such weights.  Few rows here, many in
+// linear_q4_many.hip.
 //
 // The matrix cores do the products for one row as for many: they take the codes
 // with the fewest instructions.  A code c becomes the bf16 value 1 + c / 16 by
 // putting its bits below an exponent (a shift and an and-or for two), and
 //   sum_k x (c - zero) scale = 16 scale (sum_k x (1 + c / 16) - (1 + zero / 16) sum_k x)
-// over each group, where sum_k x is the product with a matrix of ones, which lies
-// in the accumulators as the other sum does.  All products are exact, sums are
-// fp32.  An offset of 16 + zero codes, not the 128 of codes in the lowest bits,
-// costs the fp32 sums 2 to 3 bits of a group's own sum: about 3e-7 of y where
-// an fp32 chain over the inputs has 5e-7.
+// over each group.  All products are exact, sums are fp32.  An offset of 16 + zero
+// codes, not the 128 of codes in the lowest bits, costs the fp32 sums 2 to 3 bits
+// of a group's own sum: about 2e-7 of y where an fp32 chain over the inputs has
+// 6e-7.
 //
 // fp32 x is the sum of three bf16 terms (8 bits each, cut off one after the
-// other), so its products are exact too.  Up to five rows have their terms side
-// by side as rows of the matrix cores' 16; for more rows a launch before writes
-// the terms to the workspace.
+// other), so its products are exact too.  Up to five rows have their terms below
+// each other as rows of the matrix cores' 16.
 //
 // A lane loads 16 bytes, 32 codes of a row; the four lanes of a row hold 128
 // neighbouring codes, so four swaps between the lanes' quarters (a 4 x 4
@@ -23,284 +22,181 @@
 // smallest group.  Within a lane's word of 8 codes the pairs of a register are
 // (i, i + 4); x is put in the same order.
 //
-// A workgroup's waves share its columns and take the 256-input pieces (a 128-byte
-// line of every row) in turn; their sums are joined in LDS in a fixed order.
-// Bound by the codes' bytes up to some 64 rows.
-#include "serve.hpp"
+// Bound by the codes' bytes up to some 64 rows, with short launches' fixed 4 us.
+#include "q4.hpp"
 
 namespace aps {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+using namespace q4;
 
-constexpr int kPiece = 256;      // inputs of a wave's turn: two loads of codes
 constexpr int kPackRows = 5;     // fp32 rows whose three terms fit in 16
-constexpr int kTermPitch = 272;  // bytes of a row of 128 terms in LDS
+constexpr int kWaves = 16;       // one workgroup of 16 waves on a CU
+constexpr int kFew = 64 * kWaves;
+constexpr int kLds = 156 * 1024;
 
-enum class X { kBf16, kPack, kTerms };
-
-__device__ inline bf16x8 frag(u32x4 w) { return __builtin_bit_cast(bf16x8, w); }
-__device__ inline f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+// LDS of a launch with 2^turns waves along the inputs: x, its sums, the waves'
+// scales and zeros.
+struct FewLds {
+    int pitch;                   // bytes of a row of x
+    int64_t x, sums, scales;     // bytes
+};
+__host__ __device__ inline FewLds few_lds(int rows, int in, int group, int turns, bool scales32) {
+    const int pieces = (in + kPiece - 1) / kPiece, held = ((pieces + (1 << turns) - 1) >> turns) << turns;
+    FewLds l;
+    l.pitch = held * kPiece * 2 + kPad;
+    l.x = static_cast<int64_t>(rows) * l.pitch;
+    l.sums = static_cast<int64_t>(held) * (kPiece / group) * 64;
+    l.scales = kWaves * 16 * (kBlock * (scales32 ? 4 : 2) + kPad + kBlock);
+    return l;
 }
 
-// Register r of the lanes' quarter q <- register q of quarter r.
-__device__ inline u32x4 transpose_quarters(u32x4 w) {
-    const auto a = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false);
-    const auto b = __builtin_amdgcn_permlane16_swap(w[2], w[3], false, false);
-    const auto c = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
-    const auto d = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
-    return u32x4{c[0], d[0], c[1], d[1]};
-}
-
-// Eight codes as bf16 1 + c / 16: (0, 4), (1, 5), (2, 6), (3, 7).
-__device__ inline bf16x8 code_values(uint32_t w) {
-    constexpr uint32_t kMask = 0x00780078u, kOne = 0x3F803F80u;
-    return frag(u32x4{((w << 3) & kMask) | kOne, ((w >> 1) & kMask) | kOne, ((w >> 5) & kMask) | kOne,
-                      ((w >> 9) & kMask) | kOne});
-}
-
-// Eight neighbouring bf16 values in the codes' order.
-__device__ inline u32x4 code_order(u32x4 w) {
-    return u32x4{__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
-                 __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
-}
-
-// The three bf16 terms of eight fp32 values, in the codes' order.
-__device__ inline void terms_of(const float (&x)[8], u32x4 (&t)[3]) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = x[i];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            t[j][i] = __builtin_amdgcn_perm(__float_as_uint(v[i + 4]), __float_as_uint(v[i]), 0x07060302u);
-        if (j < 2) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] - __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
-        }
-    }
-}
-
-__device__ inline void load8(const float* p, bool vec, float (&x)[8]) {
-    if (vec) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = p[i];
-    }
-}
-__device__ inline u32x4 load8(const bf16_t* p, bool vec) {
-    if (vec) return *reinterpret_cast<const u32x4*>(p);
-    u32x4 w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = static_cast<uint32_t>(p[2 * i]) | static_cast<uint32_t>(p[2 * i + 1]) << 16;
-    return w;
-}
-
-// fp32 x [rows][in] -> [3][rows][in] bf16 terms in the codes' order.
-__global__ void __launch_bounds__(256)
-k_q4_terms(const float* __restrict__ x, int64_t stride, int64_t rows, int in, bool vec, bf16_t* __restrict__ to) {
-    const int64_t runs = in / 8, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= rows * runs) return;
-    const int64_t row = i / runs, at = (i - row * runs) * 8;
-    float v[8];
-    u32x4 t[3];
-    load8(x + row * stride + at, vec, v);
-    terms_of(v, t);
-#pragma unroll
-    for (int j = 0; j < 3; ++j) *reinterpret_cast<u32x4*>(to + (j * rows + row) * in + at) = t[j];
-}
-
-template <int MT, int NT, int GROUP, X KIND, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES)
-k_linear_q4(LinearQ4Args a, bool x_vec, int n_blocks, int m_blocks) {
+// 2^columns waves lie side by side, 16 outputs each; the others share the inputs, a
+// run of pieces each.  All of x lies in LDS.
+//
+// Rows of x in LDS: bf16 as they are, up to 16; fp32 a row's three terms below each
+// other, up to five.  Row m of these is row 4 (m % 4) + m / 4 of the matrix cores'
+// 16, so that up to four (NARROW) are register 0 of every lane and the others are
+// not joined.
+//
+// A launch lasts little longer than its code takes to come from memory (10 KB
+// more of it: 2 us), so loops stay loops.
+template <int GROUP, bool F32, bool SCALES32, bool NARROW>
+__global__ void __launch_bounds__(kFew) k_q4_few(LinearQ4Args a, int columns) {
     constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32;  // of a piece; product steps of a group
-    constexpr int TERMS = KIND == X::kTerms ? 3 : 1;
-    constexpr int COLS = 16 * NT, RED = WAVES * 16 * MT * COLS * 4;
-    constexpr int PACK = KIND == X::kPack ? WAVES * 16 * kTermPitch : 0;
-    __shared__ __align__(16) unsigned char lds[RED > PACK ? RED : PACK];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, col = lane & 15, q = lane >> 4;
-    // blocks of the same columns on one XCD (workgroups go round the eight)
-    int nb = blockIdx.x, mb = 0;
-    if (m_blocks > 1) {
-        const int turn = blockIdx.x / 8;
-        nb = (turn / m_blocks) * 8 + (blockIdx.x & 7);
-        mb = turn % m_blocks;
-        if (nb >= n_blocks) return;
-    }
-    const int in = a.w.in, groups = in / GROUP;
-    const int64_t m0 = static_cast<int64_t>(mb) * 16 * MT;
-    const int n0 = nb * COLS;
-    const uint8_t* code_row[NT];
-    int64_t scale_row[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int n = min(n0 + 16 * j + col, a.w.out - 1);
-        code_row[j] = a.w.codes + static_cast<int64_t>(n) * (in / 2) + 16 * q;
-        scale_row[j] = static_cast<int64_t>(n) * groups;
-    }
-    int64_t x_row[MT];  // of the lane's row of each tile
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t m = min(m0 + 16 * i + col, a.rows - 1);
-        x_row[i] = m * (KIND == X::kTerms ? in : a.x_stride);
-    }
-    struct Held { u32x4 code[2][NT]; };
-    auto fetch = [&](int piece) {
-        Held h;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int k = piece * kPiece + 128 * c + 32 * q;
-                h.code[c][j] = u32x4{0u, 0u, 0u, 0u};
-                if (k < in) h.code[c][j] = *reinterpret_cast<const u32x4*>(code_row[j] + (piece * kPiece + 128 * c) / 2);
-            }
-        return h;
+    constexpr int REGS = NARROW ? 1 : 4, BLOCK = kBlock / GROUPS;   // pieces of a block of scales
+    constexpr int AHEAD = F32 ? 2 : 4;   // runs of x that a lane loads at once: 16 registers
+    __shared__ __align__(16) unsigned char lds[kLds];
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid & 63, col = lane & 15, q = lane >> 4;
+    const int wn = wave & ((1 << columns) - 1), wk = wave >> columns, log_turns = 4 - columns;
+    const int in = a.w.in, pieces = (in + kPiece - 1) / kPiece, m_rows = static_cast<int>(a.rows);
+    const int rounds = (pieces + (1 << log_turns) - 1) >> log_turns, rows = F32 ? 3 * m_rows : m_rows;
+    const FewLds l = few_lds(rows, in, GROUP, log_turns, SCALES32);
+    const int x_row = min(4 * (col & 3) + (col >> 2), rows - 1) * l.pitch + 16 * q;
+    float* sums = reinterpret_cast<float*>(lds + l.x);   // [group][16]
+    const CodeBits bits = code_bits();
+
+    // Runs of 8 inputs go to lanes in units of 64 of a row.
+    struct Run {
+        float v[F32 ? 8 : 1];
+        u32x4 w;
     };
-    const f32x4 zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
-    const bf16x8 ones = frag(u32x4{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});
-    f32x4 total[NT][MT];
+    const int runs = (rounds << log_turns) * (kPiece / 8), units = (runs + 63) / 64;
+    auto load_run = [&](int unit) {   // no branch
+        Run r{};
+        const int m = min(unit / units, m_rows - 1), run = unit % units * 64 + lane;
+        const int64_t at = m * a.x_stride + begin_of(run / 32, run & 31, in).k;
+        if constexpr (F32) load8(static_cast<const float*>(a.x) + at, r.v);
+        else r.w = load8(static_cast<const bf16_t*>(a.x) + at);
+        return r;
+    };
+    auto store_run = [&](int unit, Run r) {
+        const int m = unit / units, run = unit % units * 64 + lane;
+        if (m >= m_rows) return;   // the wave's all
+        const Begin b = begin_of(run / 32, run & 31, in);
+        if (b.k < b.at) r = Run{};
+        float sum = 0.0f;
+        if constexpr (F32) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+            for (int i = 0; i < 8; ++i) sum += r.v[i];
+        } else {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) total[j][i] = zero4;
-    const int pieces = (in + kPiece - 1) / kPiece;
-    Held now{};
-    if (wave < pieces) now = fetch(wave);
-    for (int piece = wave; piece < pieces; piece += WAVES) {
-        const int k0 = piece * kPiece;
-        // scales and zeros of the piece's groups: 16 scale, -(1 + zero / 16)
-        float scale[NT][GROUPS], off[NT][GROUPS];
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                scale[j][g] = 0.0f;
-                off[j][g] = -1.5f;
-                if (k0 + g * GROUP < in) {
-                    const int64_t at = scale_row[j] + piece * GROUPS + g;
-                    scale[j][g] = a.w.scales_f32
-                                      ? static_cast<const float*>(a.w.scales)[at]
-                                      : __uint_as_float(static_cast<uint32_t>(static_cast<const bf16_t*>(a.w.scales)[at]) << 16);
-                    if (a.w.zeros) off[j][g] = fmaf(static_cast<float>(a.w.zeros[at]), -0.0625f, -1.0f);
-                }
-            }
-        Held next{};
-        if (piece + WAVES < pieces) next = fetch(piece + WAVES);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int kc = k0 + 128 * c;
-            if (kc >= in) break;
-            unsigned char* mine = lds + wave * 16 * kTermPitch;
-            if constexpr (KIND == X::kPack) {
-                // 16 runs of 8 values a row: their terms into rows 3 m, 3 m + 1, 3 m + 2
-                for (int run = lane; run < static_cast<int>(a.rows) * 16; run += 64) {
-                    const int m = run >> 4, k = kc + 8 * (run & 15);
-                    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                    if (k < in) load8(static_cast<const float*>(a.x) + m * a.x_stride + k, x_vec, v);
-                    u32x4 t[3];
-                    terms_of(v, t);
-#pragma unroll
-                    for (int j = 0; j < 3; ++j)
-                        *reinterpret_cast<u32x4*>(mine + (3 * m + j) * kTermPitch + 16 * (run & 15)) = t[j];
-                }
-                __builtin_amdgcn_wave_barrier();
-            }
-            u32x4 code[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) code[j] = transpose_quarters(now.code[c][j]);
-#pragma unroll
-            for (int g = 0; g < 128 / GROUP; ++g) {
-                f32x4 sum[MT], dot[NT][MT];
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    sum[i] = zero4;
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) dot[j][i] = zero4;
-                }
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    const int t = g * STEPS + s, k = kc + 32 * t;
-                    bf16x8 xs[TERMS][MT];
-#pragma unroll
-                    for (int e = 0; e < TERMS; ++e)
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            u32x4 w = {0u, 0u, 0u, 0u};
-                            if constexpr (KIND == X::kPack) {
-                                w = *reinterpret_cast<const u32x4*>(mine + col * kTermPitch + 64 * t + 16 * q);
-                            } else if (k < in) {
-                                if constexpr (KIND == X::kTerms)
-                                    w = *reinterpret_cast<const u32x4*>(a.terms + e * a.rows * in + x_row[i] + k + 8 * q);
-                                else
-                                    w = code_order(load8(static_cast<const bf16_t*>(a.x) + x_row[i] + k + 8 * q, x_vec));
-                            }
-                            xs[e][i] = frag(w);
-                        }
-#pragma unroll
-                    for (int e = 0; e < TERMS; ++e)
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) sum[i] = mfma(xs[e][i], ones, sum[i]);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const bf16x8 v = code_values(code[j][t]);
-#pragma unroll
-                        for (int e = 0; e < TERMS; ++e)
-#pragma unroll
-                            for (int i = 0; i < MT; ++i) dot[j][i] = mfma(xs[e][i], v, dot[j][i]);
-                    }
-                }
-                const int at = c * (128 / GROUP) + g;
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            total[j][i][r] = fmaf(scale[j][at], fmaf(off[j][at], sum[i][r], dot[j][i][r]), total[j][i][r]);
-            }
-            if constexpr (KIND == X::kPack) __builtin_amdgcn_wave_barrier();
+            for (int i = 0; i < 4; ++i) sum += bf16w_lo(r.w[i]) + bf16w_hi(r.w[i]);
         }
-        now = next;
+        sum = add_lanes<GROUP / 8>(sum);
+        if (run >= runs) return;
+        float* to = sums + run / (GROUP / 8) * 16;
+        auto place = [](int row) { return 4 * (row & 3) + (row >> 2); };
+        if constexpr (F32) {
+            u32x4 t[3];
+            terms_of(r.v, t);
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                *reinterpret_cast<u32x4*>(lds + 16 * run + (3 * m + e) * l.pitch) = t[e];
+                to[place(3 * m + e)] = e ? 0.0f : sum;   // the terms meet at the end
+            }
+        } else {
+            *reinterpret_cast<u32x4*>(lds + 16 * run + m * l.pitch) = code_order(r.w);
+            to[place(m)] = sum;
+        }
+    };
+
+    using Weight = Columns<1, GROUP, SCALES32>;
+    const Weight w(a.w, ((static_cast<int>(blockIdx.x) << columns) + wn) * 16, lane, lds + l.x + l.sums + wave * Weight::LDS);
+    const int first = wk * rounds, last = min(first + rounds, pieces);   // this wave's pieces
+    float total[REGS] = {};
+    // x before the codes, which come in order: it goes to LDS while they are on their way
+    Run ahead[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) ahead[j] = load_run(wave + j * kWaves);
+    Held<1> h0 = w.fetch(min(first, last - 1)), h1 = w.fetch(min(first + 1, last - 1));
+    int block = w.load_scales(first);   // the first group of the scales in LDS
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) store_run(wave + j * kWaves, ahead[j]);
+#pragma unroll 1
+    for (int unit = wave + AHEAD * kWaves; unit < m_rows * units; unit += AHEAD * kWaves) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) ahead[j] = load_run(unit + j * kWaves);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) store_run(unit + j * kWaves, ahead[j]);
     }
-    // join the waves: [wave][row][column]
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(lds);
+    lds_barrier();
+#pragma unroll 1
+    for (int begin = first; begin < last; begin += BLOCK) {
+        if (begin > first) block = w.load_scales(begin);
+        const int end = min(begin + BLOCK, last);
+#pragma unroll 1
+        for (int piece = begin; piece < end; ++piece) {
+            const Held<1> h = h0;
+            h0 = h1;
+            h1 = w.fetch(min(piece + 2, last - 1));
+            const unsigned char* x = lds + x_row + piece * (kPiece * 2);
+            const float* sum = sums + piece * GROUPS * 16 + 4 * q;
+            const auto of = w.scales(w.first_group(piece) - block);
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+            for (int c = 0; c < 2; ++c) {
+                const u32x4 code = to_columns(h.code[c][0], lane);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+                for (int g = c * (128 / GROUP); g < (c + 1) * (128 / GROUP); ++g) {
+                    f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                red[(wave * 16 * MT + 16 * i + 4 * q + r) * COLS + 16 * j + col] = total[j][i][r];
-    __syncthreads();
-    const int64_t left = a.rows - m0;
-    const int m_rows = left < 16 * MT ? static_cast<int>(left) : 16 * MT;
-    for (int e = threadIdx.x; e < m_rows * COLS; e += 64 * WAVES) {
-        const int m = e / COLS, n = n0 + e % COLS;
-        if (n >= a.w.out) continue;
+                    for (int t = g * STEPS; t < (g + 1) * STEPS; ++t)
+                        dot = mfma(frag(*reinterpret_cast<const u32x4*>(x + 64 * t)), code_values(code[t & 3], bits), dot);
+#pragma unroll
+                    for (int r = 0; r < REGS; ++r)
+                        total[r] = fmaf(of.scale(0, g), fmaf(of.off(0, g), sum[16 * g + r], dot[r]), total[r]);
+                }
+            }
+        }
+    }
+    // join the waves of the same columns in a fixed order
+    lds_barrier();
+    float* red = reinterpret_cast<float*>(lds);   // [wave][register][lane]
+#pragma unroll
+    for (int r = 0; r < REGS; ++r) red[(wave * REGS + r) * 64 + lane] = total[r];
+    lds_barrier();
+#pragma unroll 1
+    for (int i = tid; i < m_rows << (columns + 4); i += kFew) {
+        const int m = i >> (columns + 4), c = i & ((16 << columns) - 1);
+        const int at = (static_cast<int>(blockIdx.x) << (columns + 4)) + c;
+        if (at >= a.w.out) continue;
+        // row m lies in register m / 4 of the lanes 16 (m % 4) ..
+        auto of = [&](int wv, int row) { return red[(wv * REGS + (NARROW ? 0 : row >> 2)) * 64 + 16 * (row & 3) + (c & 15)]; };
         float y = 0.0f;
-        for (int w = 0; w < WAVES; ++w) {
-            if constexpr (KIND == X::kPack) {
+#pragma unroll 4
+        for (int wv = c >> 4; wv < kWaves; wv += 1 << columns) {
+            if constexpr (F32) {
 #pragma unroll
-                for (int t = 2; t >= 0; --t) y += red[(w * 16 + 3 * m + t) * COLS + e % COLS];
+                for (int t = 2; t >= 0; --t) y += of(wv, 3 * m + t);
             } else {
-                y += red[(w * 16 * MT + m) * COLS + e % COLS];
+                y += of(wv, m);
             }
         }
         y *= 16.0f;
-        if (a.bias) y += a.bias[n];
-        const int64_t to = (m0 + m) * a.w.out + n;
-        if constexpr (KIND == X::kBf16) static_cast<bf16_t*>(a.y)[to] = static_cast<bf16_t>(pack2_bf16(y, 0.0f) & 0xFFFFu);
-        else static_cast<float*>(a.y)[to] = y;
+        if (a.bias) y += a.bias[at];
+        const int64_t to = static_cast<int64_t>(m) * a.w.out + at;
+        if constexpr (F32) static_cast<float*>(a.y)[to] = y;
+        else static_cast<bf16_t*>(a.y)[to] = static_cast<bf16_t>(pack2_bf16(y, 0.0f) & 0xFFFFu);
     }
 }
 
@@ -315,9 +211,9 @@ k_quantise_q4(const void* __restrict__ w, int64_t runs, int lanes, uint32_t* __r
     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (live) {
         if constexpr (F32) {
-            load8(static_cast<const float*>(w) + 8 * i, true, x);
+            load8(static_cast<const float*>(w) + 8 * i, x);
         } else {
-            const u32x4 v = load8(static_cast<const bf16_t*>(w) + 8 * i, true);
+            const u32x4 v = load8(static_cast<const bf16_t*>(w) + 8 * i);
 #pragma unroll
             for (int k = 0; k < 4; ++k) { x[2 * k] = bf16w_lo(v[k]); x[2 * k + 1] = bf16w_hi(v[k]); }
         }
@@ -357,50 +253,41 @@ k_quantise_q4(const void* __restrict__ w, int64_t runs, int lanes, uint32_t* __r
     }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-template <int MT, int NT, int GROUP, X KIND, int WAVES>
-hipError_t run(const LinearQ4Args& a, hipStream_t s) {
-    const int64_t n_blocks = ceil_div(a.w.out, 16 * NT), m_blocks = ceil_div(a.rows, 16 * MT);
-    const int64_t blocks = m_blocks > 1 ? ceil_div(n_blocks, 8) * 8 * m_blocks : n_blocks;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const bool vec = aligned16(a.x) && a.x_stride % (KIND == X::kBf16 ? 8 : 4) == 0;
-    hipLaunchKernelGGL((k_linear_q4<MT, NT, GROUP, KIND, WAVES>), dim3(static_cast<unsigned>(blocks)),
-                       dim3(64 * WAVES), 0, s, a, vec, static_cast<int>(n_blocks), static_cast<int>(m_blocks));
-    return hipGetLastError();
+// The waves side by side: as many as leave every CU a workgroup (4096 x 32064, one
+// row: 8 of them 18 us, 4 22, 16 30).  -1 where x is too large for this kernel.
+int few_columns(const Q4& w, int64_t rows, bool f32) {
+    if (rows > (f32 ? kPackRows : 16)) return -1;
+    const int64_t tiles = ceil_div(w.out, 16);
+    int columns = 0;
+    while (columns < 4 && 256 << columns < tiles) ++columns;
+    const FewLds l = few_lds(static_cast<int>(f32 ? 3 * rows : rows), w.in, w.group, 4 - columns, w.scales_f32);
+    return l.x + l.sums + l.scales <= kLds ? columns : -1;
 }
 
-template <int GROUP>
-hipError_t by_rows(const LinearQ4Args& a, bool f32, hipStream_t s) {
-    if (f32 && a.rows <= kPackRows) return run<1, 1, GROUP, X::kPack, 8>(a, s);
-    if (f32) {
-        if (a.rows <= 16) return run<1, 2, GROUP, X::kTerms, 8>(a, s);
-        if (a.rows <= 32) return run<2, 2, GROUP, X::kTerms, 8>(a, s);
-        return run<4, 2, GROUP, X::kTerms, 8>(a, s);
-    }
-    if (a.rows <= 16) return run<1, 1, GROUP, X::kBf16, 8>(a, s);
-    if (a.rows <= 32) return run<2, 2, GROUP, X::kBf16, 8>(a, s);
-    return run<4, 2, GROUP, X::kBf16, 8>(a, s);
+template <int GROUP, bool F32>
+hipError_t run_few(const LinearQ4Args& a, int columns, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.w.out, 16 << columns))), block(kFew);
+    const bool narrow = a.rows * (F32 ? 3 : 1) <= 4;
+    if (narrow && a.w.scales_f32) hipLaunchKernelGGL((k_q4_few<GROUP, F32, true, true>), grid, block, 0, s, a, columns);
+    else if (narrow) hipLaunchKernelGGL((k_q4_few<GROUP, F32, false, true>), grid, block, 0, s, a, columns);
+    else if (a.w.scales_f32) hipLaunchKernelGGL((k_q4_few<GROUP, F32, true, false>), grid, block, 0, s, a, columns);
+    else hipLaunchKernelGGL((k_q4_few<GROUP, F32, false, false>), grid, block, 0, s, a, columns);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-size_t linear_q4_term_bytes(int64_t rows, int in, int, bool f32) {
-    return f32 && rows > kPackRows ? static_cast<size_t>(rows) * in * 6 : 0;
+size_t linear_q4_bytes(const Q4& w, int64_t rows, bool f32) {
+    return rows <= 0 || few_columns(w, rows, f32) >= 0 ? 0 : q4_many_bytes(w, rows, f32);
 }
 
 hipError_t launch_linear_q4(const LinearQ4Args& a, bool f32, hipStream_t s) {
     if (a.rows <= 0 || a.w.out <= 0) return hipSuccess;
-    if (a.terms) {
-        const int64_t blocks = ceil_div(a.rows * (a.w.in / 8), 256);
-        if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-        hipLaunchKernelGGL(k_q4_terms, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
-                           static_cast<const float*>(a.x), a.x_stride, a.rows, a.w.in,
-                           aligned16(a.x) && a.x_stride % 4 == 0, a.terms);
-    }
-    if (a.w.group == 32) return by_rows<32>(a, f32, s);
-    if (a.w.group == 64) return by_rows<64>(a, f32, s);
-    return by_rows<128>(a, f32, s);
+    const int columns = few_columns(a.w, a.rows, f32);
+    if (columns < 0) return launch_q4_many(a, f32, s);
+    if (a.w.group == 32) return f32 ? run_few<32, true>(a, columns, s) : run_few<32, false>(a, columns, s);
+    if (a.w.group == 64) return f32 ? run_few<64, true>(a, columns, s) : run_few<64, false>(a, columns, s);
+    return f32 ? run_few<128, true>(a, columns, s) : run_few<128, false>(a, columns, s);
 }
 
 hipError_t launch_quantise_q4(const void* w, bool w_f32, int64_t out, int in, int group, uint8_t* codes,

@@ -1,0 +1,218 @@
+// Linear layers with weights in 4 bits for many rows (and for few whose inputs do
+// not fit the kernel of linear_q4.hip): the same products, in two launches.
+//
+// The first puts x into the order in which the matrix cores take it, fp32 x as
+// three bf16 terms (the workspace holds it):
+//   [16 rows][piece of 256 inputs]: [term][8 steps of 32 inputs][64 lanes][16 bytes],
+//   then 1 KB with the sums of x, [group][16 rows]
+// so that an operand is one load of neighbouring bytes.  In the second a wave
+// multiplies 16 MT rows by 16 NT columns over its share of the pieces, and a
+// workgroup's eight waves are joined in LDS.  x comes from L2 without a stay in
+// LDS: waves beside each other have other inputs, not the same ones.
+//
+// Bound by those reads of x, 64 bytes a cycle and CU (64 rows on 8192 x 8192: 1 MB
+// for every 32 columns), and by the codes' bytes.
+#include "q4.hpp"
+
+namespace aps {
+namespace {
+
+using namespace q4;
+
+constexpr int kWaves = 8;
+constexpr int kMany = 64 * kWaves;
+
+constexpr int piece_bytes(int terms) { return (8 * terms + 1) * 1024; }
+
+// A wave to a group of 16 rows: lane (row, quarter) takes runs of 8 inputs, 32 of
+// them apart.
+template <bool F32>
+__global__ void __launch_bounds__(256) k_q4_arrange(LinearQ4Args a, int64_t waves) {
+    constexpr int TERMS = F32 ? 3 : 1;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
+    if (at >= waves) return;
+    const int lane = threadIdx.x & 63, q = lane >> 4, in = a.w.in, steps = a.w.group / 32;
+    const int pieces = (in + kPiece - 1) / kPiece, groups = pieces * (kPiece / a.w.group);
+    const int64_t tile = at / groups;
+    const int group = static_cast<int>(at - tile * groups), piece = group * a.w.group / kPiece;
+    const int first = group * steps & 7;   // step of the piece
+    const int64_t row = min(tile * 16 + (lane & 15), a.rows - 1);
+    uint8_t* to = reinterpret_cast<uint8_t*>(a.terms) + (tile * pieces + piece) * piece_bytes(TERMS);
+    float sum = 0.0f;
+    for (int i = 0; i < steps; ++i) {
+        const Begin b = begin_of(piece, 4 * (first + i) + q, in);
+        u32x4 t[TERMS];
+        if constexpr (F32) {
+            float v[8];
+            load8(static_cast<const float*>(a.x) + row * a.x_stride + b.k, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = b.k < b.at ? 0.0f : v[e];
+                sum += v[e];
+            }
+            terms_of(v, t);
+        } else {
+            u32x4 v = load8(static_cast<const bf16_t*>(a.x) + row * a.x_stride + b.k);
+            if (b.k < b.at) v = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += bf16w_lo(v[e]) + bf16w_hi(v[e]);
+            t[0] = code_order(v);
+        }
+#pragma unroll
+        for (int e = 0; e < TERMS; ++e) *reinterpret_cast<u32x4*>(to + (8 * e + first + i) * 1024 + 16 * lane) = t[e];
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (lane < 16) reinterpret_cast<float*>(to + 8 * TERMS * 1024)[first / steps * 16 + lane] = sum;
+}
+
+// 2^columns of a workgroup's waves lie side by side, 16 NT outputs each; the others
+// share the inputs, a run of pieces each.
+template <int GROUP, bool F32, int MT, int NT, bool SCALES32>
+__global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, int n_blocks, int m_blocks) {
+    constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32, TERMS = F32 ? 3 : 1, BLOCK = kBlock / GROUPS;
+    using Weight = Columns<NT, GROUP, SCALES32>;
+    constexpr int RED = kWaves * NT * MT * 4 * 64 * 4, SCALE = kWaves * Weight::LDS;
+    __shared__ __align__(16) unsigned char lds[RED > SCALE ? RED : SCALE];
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid & 63, q = lane >> 4;
+    const int wn = wave & ((1 << columns) - 1), wk = wave >> columns, log_turns = 3 - columns;
+    // blocks of the same columns on one XCD (workgroups go round the eight)
+    int nb = blockIdx.x, mb = 0;
+    if (m_blocks > 1) {
+        const int turn = blockIdx.x / 8;
+        nb = (turn / m_blocks) * 8 + (blockIdx.x & 7);
+        mb = turn % m_blocks;
+        if (nb >= n_blocks) return;
+    }
+    const int in = a.w.in, pieces = (in + kPiece - 1) / kPiece, rounds = (pieces + (1 << log_turns) - 1) >> log_turns;
+    const int64_t last_tile = (a.rows - 1) / 16;
+    const uint8_t* x[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+        x[i] = reinterpret_cast<const uint8_t*>(a.terms) +
+               min(static_cast<int64_t>(mb) * MT + i, last_tile) * pieces * piece_bytes(TERMS);
+    const Weight w(a.w, ((nb << columns) + wn) * 16 * NT, lane, lds + wave * Weight::LDS);
+    const CodeBits bits = code_bits();
+    const int first = wk * rounds, last = min(first + rounds, pieces);
+    f32x4 total[NT][MT] = {};
+    if (first < last) {
+        Held<NT> h0 = w.fetch(first), h1 = w.fetch(min(first + 1, last - 1));
+#pragma unroll 1
+        for (int begin = first; begin < last; begin += BLOCK) {
+            const int block = w.load_scales(begin), end = min(begin + BLOCK, last);
+#pragma unroll 1
+            for (int piece = begin; piece < end; ++piece) {
+                const auto of = w.scales(w.first_group(piece) - block);
+                const int64_t at = static_cast<int64_t>(piece) * piece_bytes(TERMS);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    u32x4 code[NT];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) code[j] = to_columns(h0.code[c][j], lane);
+#pragma unroll
+                    for (int g = c * (128 / GROUP); g < (c + 1) * (128 / GROUP); ++g) {
+                        f32x4 dot[NT][MT] = {}, sum[MT];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+                            sum[i] = *reinterpret_cast<const f32x4*>(x[i] + at + 8 * TERMS * 1024 + 64 * g + 16 * q);
+                        // the smallest terms first: what they add is kept under the largest's sums
+#pragma unroll
+                        for (int e = TERMS - 1; e >= 0; --e)
+#pragma unroll
+                            for (int t = g * STEPS; t < (g + 1) * STEPS; ++t) {
+                                bf16x8 xs[MT];
+#pragma unroll
+                                for (int i = 0; i < MT; ++i)
+                                    xs[i] = frag(*reinterpret_cast<const u32x4*>(x[i] + at + (8 * e + t) * 1024 + 16 * lane));
+#pragma unroll
+                                for (int j = 0; j < NT; ++j) {
+                                    const bf16x8 v = code_values(code[j][t & 3], bits);
+#pragma unroll
+                                    for (int i = 0; i < MT; ++i) dot[j][i] = mfma(xs[i], v, dot[j][i]);
+                                }
+                            }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    total[j][i][r] = fmaf(of.scale(j, g), fmaf(of.off(j, g), sum[i][r], dot[j][i][r]), total[j][i][r]);
+                    }
+                }
+                // behind this piece's x: loads come in order
+                h0 = h1;
+                h1 = w.fetch(min(piece + 2, last - 1));
+            }
+        }
+    }
+    // join the waves of the same columns in a fixed order
+    lds_barrier();
+    float* red = reinterpret_cast<float*>(lds);   // [wave][tile][row][column]
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                red[((wave * NT + j) * 16 * MT + 16 * i + 4 * q + r) * 16 + (lane & 15)] = total[j][i][r];
+    lds_barrier();
+    const int64_t m0 = static_cast<int64_t>(mb) * 16 * MT, left = a.rows - m0;
+    const int m_rows = left < 16 * MT ? static_cast<int>(left) : 16 * MT, cols = (16 * NT) << columns;
+#pragma unroll 1
+    for (int i = tid; i < m_rows * cols; i += kMany) {
+        const int m = i / cols, c = i - m * cols, n = nb * cols + c;
+        if (n >= a.w.out) continue;
+        float y = 0.0f;
+        for (int wv = c / (16 * NT); wv < kWaves; wv += 1 << columns)
+            y += red[((wv * NT + c / 16 % NT) * 16 * MT + m) * 16 + (c & 15)];
+        y *= 16.0f;
+        if (a.bias) y += a.bias[n];
+        const int64_t to = (m0 + m) * a.w.out + n;
+        if constexpr (F32) static_cast<float*>(a.y)[to] = y;
+        else static_cast<bf16_t*>(a.y)[to] = static_cast<bf16_t>(pack2_bf16(y, 0.0f) & 0xFFFFu);
+    }
+}
+
+template <int GROUP, bool F32, int MT, int NT>
+hipError_t run(const LinearQ4Args& a, hipStream_t s) {
+    const int64_t pieces = ceil_div(a.w.in, kPiece);
+    int columns = 0;
+    while (columns < 3 && (kWaves >> columns) > pieces) ++columns;
+    const int64_t n_blocks = ceil_div(a.w.out, (16 * NT) << columns), m_blocks = ceil_div(a.rows, 16 * MT);
+    const int64_t blocks = m_blocks > 1 ? ceil_div(n_blocks, 8) * 8 * m_blocks : n_blocks;
+    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(blocks)), block(kMany);
+    const int n = static_cast<int>(n_blocks), m = static_cast<int>(m_blocks);
+    if (a.w.scales_f32) hipLaunchKernelGGL((k_q4_many<GROUP, F32, MT, NT, true>), grid, block, 0, s, a, columns, n, m);
+    else hipLaunchKernelGGL((k_q4_many<GROUP, F32, MT, NT, false>), grid, block, 0, s, a, columns, n, m);
+    return hipGetLastError();
+}
+
+template <int GROUP, bool F32>
+hipError_t by_rows(const LinearQ4Args& a, hipStream_t s) {
+    const int64_t tiles = ceil_div(a.w.out, 16);
+    if (a.rows <= 16) return tiles >= 1024 ? run<GROUP, F32, 1, 4>(a, s) : run<GROUP, F32, 1, 1>(a, s);
+    if constexpr (F32) return run<GROUP, F32, 2, 2>(a, s);
+    else return a.rows <= 32 ? run<GROUP, F32, 2, 2>(a, s) : run<GROUP, F32, 4, 2>(a, s);
+}
+
+}  // namespace
+
+size_t q4_many_bytes(const Q4& w, int64_t rows, bool f32) {
+    return static_cast<size_t>(ceil_div(rows, 16) * ceil_div(w.in, kPiece)) * piece_bytes(f32 ? 3 : 1);
+}
+
+hipError_t launch_q4_many(const LinearQ4Args& a, bool f32, hipStream_t s) {
+    const int64_t waves = ceil_div(a.rows, 16) * ceil_div(a.w.in, kPiece) * (kPiece / a.w.group), blocks = ceil_div(waves, 4);
+    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (f32) hipLaunchKernelGGL(k_q4_arrange<true>, grid, dim3(256), 0, s, a, waves);
+    else hipLaunchKernelGGL(k_q4_arrange<false>, grid, dim3(256), 0, s, a, waves);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (a.w.group == 32) return f32 ? by_rows<32, true>(a, s) : by_rows<32, false>(a, s);
+    if (a.w.group == 64) return f32 ? by_rows<64, true>(a, s) : by_rows<64, false>(a, s);
+    return f32 ? by_rows<128, true>(a, s) : by_rows<128, false>(a, s);
+}
+
+}  // namespace aps

@@ -116,9 +116,9 @@ struct LinearQ4Args {
     int64_t x_stride, rows;
     const float* bias;
     void* y;          // [rows][out]
-    uint16_t* terms;  // fp32 x in bf16 terms, for many rows
+    uint16_t* terms;  // x in the products' order, for many rows
 };
-size_t linear_q4_term_bytes(int64_t rows, int in, int out, bool f32);
+size_t linear_q4_bytes(const Q4& w, int64_t rows, bool f32);
 hipError_t launch_linear_q4(const LinearQ4Args& a, bool f32, hipStream_t s);
 hipError_t launch_quantise_q4(const void* w, bool w_f32, int64_t out, int in, int group, uint8_t* codes,
                               void* scales, bool scales_f32, uint8_t* zeros, hipStream_t s);
