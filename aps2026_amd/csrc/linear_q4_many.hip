@@ -3,8 +3,8 @@
 //
 // The first puts x into the order in which the matrix cores take it, fp32 x as
 // three bf16 terms (the workspace holds it):
-//   [16 rows][piece of 256 inputs]: [term][8 steps of 32 inputs][64 lanes][16 bytes],
-//   then 1 KB with the sums of x, [group][16 rows]
+//   [16 rows][piece of 256 inputs][term][8 steps of 32 inputs][64 lanes][16 bytes],
+//   then the sums of x, [16 rows][group][row]
 // so that an operand is one load of neighbouring bytes.  In the second a wave
 // multiplies 16 MT rows by 16 NT columns over its share of the pieces, and a
 // workgroup's eight waves are joined in LDS.  x comes from L2 without a stay in
@@ -22,48 +22,59 @@ using namespace q4;
 constexpr int kWaves = 8;
 constexpr int kMany = 64 * kWaves;
 
-constexpr int piece_bytes(int terms) { return (8 * terms + 1) * 1024; }
+constexpr int piece_bytes(int terms) { return 8 * terms * 1024; }
+// Groups of a row with those of its last piece that lie past the inputs.
+__host__ __device__ inline int all_groups(int in, int group) { return (in + kPiece - 1) / kPiece * (kPiece / group); }
+__host__ __device__ inline int64_t sums_at(int64_t rows, int in, int terms) {
+    return (rows + 15) / 16 * ((in + kPiece - 1) / kPiece) * piece_bytes(terms);
+}
 
 // A wave to a group of 16 rows: lane (row, quarter) takes runs of 8 inputs, 32 of
-// them apart.
-template <bool F32>
+// them apart, all of them loaded before the first is used.
+template <bool F32, int GROUP>
 __global__ void __launch_bounds__(256) k_q4_arrange(LinearQ4Args a, int64_t waves) {
-    constexpr int TERMS = F32 ? 3 : 1;
+    constexpr int TERMS = F32 ? 3 : 1, STEPS = GROUP / 32;
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
     if (at >= waves) return;
-    const int lane = threadIdx.x & 63, q = lane >> 4, in = a.w.in, steps = a.w.group / 32;
-    const int pieces = (in + kPiece - 1) / kPiece, groups = pieces * (kPiece / a.w.group);
+    const int lane = threadIdx.x & 63, q = lane >> 4, in = a.w.in, groups = all_groups(in, GROUP);
     const int64_t tile = at / groups;
-    const int group = static_cast<int>(at - tile * groups), piece = group * a.w.group / kPiece;
-    const int first = group * steps & 7;   // step of the piece
-    const int64_t row = min(tile * 16 + (lane & 15), a.rows - 1);
-    uint8_t* to = reinterpret_cast<uint8_t*>(a.terms) + (tile * pieces + piece) * piece_bytes(TERMS);
+    const int group = static_cast<int>(at - tile * groups), piece = group * GROUP / kPiece;
+    const int first = group * STEPS & 7;   // step of the piece
+    const int64_t row = min(tile * 16 + (lane & 15), a.rows - 1) * a.x_stride;
+    uint8_t* to = reinterpret_cast<uint8_t*>(a.terms) + (tile * ((in + kPiece - 1) / kPiece) + piece) * piece_bytes(TERMS);
+    float v[F32 ? STEPS : 1][8];
+    u32x4 w[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        const int k = begin_of(piece, 4 * (first + i) + q, in).k;
+        if constexpr (F32) load8(static_cast<const float*>(a.x) + row + k, v[i]);
+        else w[i] = load8(static_cast<const bf16_t*>(a.x) + row + k);
+    }
     float sum = 0.0f;
-    for (int i = 0; i < steps; ++i) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
         const Begin b = begin_of(piece, 4 * (first + i) + q, in);
-        u32x4 t[TERMS];
+        u32x4 t[3];
         if constexpr (F32) {
-            float v[8];
-            load8(static_cast<const float*>(a.x) + row * a.x_stride + b.k, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = b.k < b.at ? 0.0f : v[e];
-                sum += v[e];
+                v[i][e] = b.k < b.at ? 0.0f : v[i][e];
+                sum += v[i][e];
             }
-            terms_of(v, t);
+            terms_of(v[i], t);
         } else {
-            u32x4 v = load8(static_cast<const bf16_t*>(a.x) + row * a.x_stride + b.k);
-            if (b.k < b.at) v = u32x4{0u, 0u, 0u, 0u};
+            if (b.k < b.at) w[i] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += bf16w_lo(v[e]) + bf16w_hi(v[e]);
-            t[0] = code_order(v);
+            for (int e = 0; e < 4; ++e) sum += bf16w_lo(w[i][e]) + bf16w_hi(w[i][e]);
+            t[0] = code_order(w[i]);
         }
 #pragma unroll
         for (int e = 0; e < TERMS; ++e) *reinterpret_cast<u32x4*>(to + (8 * e + first + i) * 1024 + 16 * lane) = t[e];
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (lane < 16) reinterpret_cast<float*>(to + 8 * TERMS * 1024)[first / steps * 16 + lane] = sum;
+    float* sums = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.terms) + sums_at(a.rows, in, TERMS));
+    if (lane < 16) sums[at * 16 + lane] = sum;
 }
 
 // 2^columns of a workgroup's waves lie side by side, 16 NT outputs each; the others
@@ -72,7 +83,9 @@ template <int GROUP, bool F32, int MT, int NT, bool SCALES32>
 __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, int n_blocks, int m_blocks) {
     constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32, TERMS = F32 ? 3 : 1, BLOCK = kBlock / GROUPS;
     using Weight = Columns<NT, GROUP, SCALES32>;
-    constexpr int RED = kWaves * NT * MT * 4 * 64 * 4, SCALE = kWaves * Weight::LDS;
+    // a wave's scales and zeros, and its rows' sums: [tile][group of the block][row]
+    constexpr int OWN = Weight::LDS + MT * kBlock * 64;
+    constexpr int RED = kWaves * NT * MT * 4 * 64 * 4, SCALE = kWaves * OWN;
     __shared__ __align__(16) unsigned char lds[RED > SCALE ? RED : SCALE];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid & 63, q = lane >> 4;
     const int wn = wave & ((1 << columns) - 1), wk = wave >> columns, log_turns = 3 - columns;
@@ -91,7 +104,10 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
     for (int i = 0; i < MT; ++i)
         x[i] = reinterpret_cast<const uint8_t*>(a.terms) +
                min(static_cast<int64_t>(mb) * MT + i, last_tile) * pieces * piece_bytes(TERMS);
-    const Weight w(a.w, ((nb << columns) + wn) * 16 * NT, lane, lds + wave * Weight::LDS);
+    const Weight w(a.w, ((nb << columns) + wn) * 16 * NT, lane, lds + wave * OWN);
+    float* own_sums = reinterpret_cast<float*>(lds + wave * OWN + Weight::LDS);
+    const float* sums = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.terms) + sums_at(a.rows, in, TERMS));
+    const int groups = all_groups(in, GROUP);
     const CodeBits bits = code_bits();
     const int first = wk * rounds, last = min(first + rounds, pieces);
     f32x4 total[NT][MT] = {};
@@ -100,6 +116,13 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
 #pragma unroll 1
         for (int begin = first; begin < last; begin += BLOCK) {
             const int block = w.load_scales(begin), end = min(begin + BLOCK, last);
+            // 16 groups of 16 rows, the last of them again past a row's end
+            const int mine = min(begin * GROUPS + (lane >> 2), groups - 1) * 16 + 4 * (lane & 3);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                reinterpret_cast<f32x4*>(own_sums)[64 * i + lane] =
+                    *reinterpret_cast<const f32x4*>(sums + min(static_cast<int64_t>(mb) * MT + i, last_tile) * groups * 16 + mine);
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
             for (int piece = begin; piece < end; ++piece) {
                 const auto of = w.scales(w.first_group(piece) - block);
@@ -114,7 +137,7 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
                         f32x4 dot[NT][MT] = {}, sum[MT];
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
-                            sum[i] = *reinterpret_cast<const f32x4*>(x[i] + at + 8 * TERMS * 1024 + 64 * g + 16 * q);
+                            sum[i] = *reinterpret_cast<const f32x4*>(own_sums + (i * kBlock + (piece - begin) * GROUPS + g) * 16 + 4 * q);
                         // the smallest terms first: what they add is kept under the largest's sums
 #pragma unroll
                         for (int e = TERMS - 1; e >= 0; --e)
@@ -160,17 +183,20 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
     const int64_t m0 = static_cast<int64_t>(mb) * 16 * MT, left = a.rows - m0;
     const int m_rows = left < 16 * MT ? static_cast<int>(left) : 16 * MT, cols = (16 * NT) << columns;
 #pragma unroll 1
-    for (int i = tid; i < m_rows * cols; i += kMany) {
-        const int m = i / cols, c = i - m * cols, n = nb * cols + c;
-        if (n >= a.w.out) continue;
-        float y = 0.0f;
+    for (int i = tid; i < m_rows * cols / 4; i += kMany) {
+        const int m = i / (cols / 4), c = (i - m * (cols / 4)) * 4, n = nb * cols + c;
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int wv = c / (16 * NT); wv < kWaves; wv += 1 << columns)
-            y += red[((wv * NT + c / 16 % NT) * 16 * MT + m) * 16 + (c & 15)];
-        y *= 16.0f;
-        if (a.bias) y += a.bias[n];
-        const int64_t to = (m0 + m) * a.w.out + n;
-        if constexpr (F32) static_cast<float*>(a.y)[to] = y;
-        else static_cast<bf16_t*>(a.y)[to] = static_cast<bf16_t>(pack2_bf16(y, 0.0f) & 0xFFFFu);
+            y += *reinterpret_cast<const f32x4*>(red + ((wv * NT + c / 16 % NT) * 16 * MT + m) * 16 + (c & 15));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (n + e >= a.w.out) break;
+            float v = y[e] * 16.0f;
+            if (a.bias) v += a.bias[n + e];
+            const int64_t to = (m0 + m) * a.w.out + n + e;
+            if constexpr (F32) static_cast<float*>(a.y)[to] = v;
+            else static_cast<bf16_t*>(a.y)[to] = static_cast<bf16_t>(pack2_bf16(v, 0.0f) & 0xFFFFu);
+        }
     }
 }
 
@@ -200,19 +226,23 @@ hipError_t by_rows(const LinearQ4Args& a, hipStream_t s) {
 }  // namespace
 
 size_t q4_many_bytes(const Q4& w, int64_t rows, bool f32) {
-    return static_cast<size_t>(ceil_div(rows, 16) * ceil_div(w.in, kPiece)) * piece_bytes(f32 ? 3 : 1);
+    return static_cast<size_t>(sums_at(rows, w.in, f32 ? 3 : 1) + ceil_div(rows, 16) * all_groups(w.in, w.group) * 64);
+}
+
+template <int GROUP>
+static hipError_t launch(const LinearQ4Args& a, bool f32, hipStream_t s) {
+    const int64_t waves = ceil_div(a.rows, 16) * all_groups(a.w.in, GROUP), blocks = ceil_div(waves, 4);
+    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (f32) hipLaunchKernelGGL((k_q4_arrange<true, GROUP>), grid, dim3(256), 0, s, a, waves);
+    else hipLaunchKernelGGL((k_q4_arrange<false, GROUP>), grid, dim3(256), 0, s, a, waves);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    return f32 ? by_rows<GROUP, true>(a, s) : by_rows<GROUP, false>(a, s);
 }
 
 hipError_t launch_q4_many(const LinearQ4Args& a, bool f32, hipStream_t s) {
-    const int64_t waves = ceil_div(a.rows, 16) * ceil_div(a.w.in, kPiece) * (kPiece / a.w.group), blocks = ceil_div(waves, 4);
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (f32) hipLaunchKernelGGL(k_q4_arrange<true>, grid, dim3(256), 0, s, a, waves);
-    else hipLaunchKernelGGL(k_q4_arrange<false>, grid, dim3(256), 0, s, a, waves);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    if (a.w.group == 32) return f32 ? by_rows<32, true>(a, s) : by_rows<32, false>(a, s);
-    if (a.w.group == 64) return f32 ? by_rows<64, true>(a, s) : by_rows<64, false>(a, s);
-    return f32 ? by_rows<128, true>(a, s) : by_rows<128, false>(a, s);
+    if (a.w.group == 32) return launch<32>(a, f32, s);
+    return a.w.group == 64 ? launch<64>(a, f32, s) : launch<128>(a, f32, s);
 }
 
 }  // namespace aps
