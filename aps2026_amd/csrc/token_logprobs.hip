@@ -17,6 +17,10 @@
 // nothing.  A row of one slice ends there; others leave maxima, sums and their
 // `top` keys in the workspace, and a second launch joins a row's slices in the
 // same way.
+//
+// Bound by the logits' bytes where workgroups are small enough that some load
+// while others compute (4096 x 32064 fp32: 178 us with one of 1024 threads on a
+// CU, 120 with four slices of 256).
 #include "serve.hpp"
 
 namespace aps {
@@ -26,6 +30,7 @@ constexpr int kMost = 1024;   // keys collected in LDS
 constexpr int kGroups = 64;   // and the largest `top`
 constexpr int kMaxSlices = 32;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
 
 template <bool F32>
@@ -40,6 +45,7 @@ __device__ inline u64 key_of(float x, uint32_t id) {
     const uint32_t up = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
     return static_cast<u64>(up) << 32 | (0xFFFFFFFFu - id);
 }
+// (+0 for -0, and -inf for a NaN, whose row's sums are NaN)
 __device__ inline float key_value(u64 key) {
     const uint32_t up = static_cast<uint32_t>(key >> 32);
     return __uint_as_float(up & 0x80000000u ? up ^ 0x80000000u : ~up);
@@ -56,8 +62,8 @@ __device__ inline float shrink(float from, float to) {
     return from == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((from - to) * kLog2e);
 }
 template <typename Get>
-__device__ inline Sums join(int n, Get get) {
-    Sums all = {-INFINITY, 0.0f, 0.0f};
+__device__ inline Sums join(int n, Get get, float m = -INFINITY) {
+    Sums all = {m, 0.0f, 0.0f};
     for (int i = 0; i < n; ++i) all.m = fmaxf(all.m, get(i).m);
     for (int i = 0; i < n; ++i) {
         const Sums p = get(i);
@@ -90,7 +96,7 @@ __device__ inline void write_row(const LogprobArgs& a, int64_t row, Sums t, cons
     }
     for (int j = tid; j < a.top; j += threads) {
         a.top_ids[row * a.top + j] = static_cast<int32_t>(key_id(top[j]));
-        a.top_logprobs[row * a.top + j] = load1<F32>(a.x, row * a.x_stride + key_id(top[j])) - o.m - o.log_s;
+        a.top_logprobs[row * a.top + j] = key_value(top[j]) - o.m - o.log_s;
     }
 }
 
@@ -99,6 +105,7 @@ __device__ inline void rank(const u64* keys, int n, u64* best, int top, int tid,
     for (int i = tid; i < n; i += threads) {
         const u64 mine = keys[i];
         int above = 0;
+#pragma unroll 4
         for (int j = 0; j < n; ++j) above += keys[j] > mine;
         if (above < top) best[above] = mine;
     }
@@ -109,43 +116,48 @@ __device__ inline void rank(const u64* keys, int n, u64* best, int top, int tid,
 // first slice.
 template <bool F32, int T, int N>
 __global__ void __launch_bounds__(T) k_logprobs(LogprobArgs a, int slices) {
-    constexpr int U = F32 ? 4 : 8, WAVES = T / kWave, SPAN = T / kGroups;
+    constexpr int U = F32 ? 4 : 8, WAVES = T / kWave, SPAN = T / kGroups, kSize = F32 ? 4 : 2;
     __shared__ Sums part[WAVES];
-    __shared__ u64 group[kGroups], keys[kMost], best[kGroups], floor_key;
-    __shared__ int count;
+    __shared__ __align__(16) float group[kGroups];
+    __shared__ float floor_value;
+    __shared__ u64 keys[kMost], best[kGroups];
+    __shared__ uint16_t hit[T * N];
+    __shared__ int count, hits;
     const int64_t row = blockIdx.x / slices;
-    const int slice = static_cast<int>(blockIdx.x - row * slices), tid = threadIdx.x;
-    const char* x = static_cast<const char*>(a.x) + row * a.x_stride * (F32 ? 4 : 2);
-    constexpr int kSize = F32 ? 4 : 2;
+    const int slice = static_cast<int>(blockIdx.x - row * slices), tid = threadIdx.x, top = a.top;
+    const char* x = static_cast<const char*>(a.x) + row * a.x_stride * kSize;
     const int off = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / kSize;
-    const int head = off < a.vocab ? off : static_cast<int>(a.vocab);
-    const int vocab = static_cast<int>(a.vocab), body = (vocab - head) / U;  // whole accesses
-    const int tail = vocab - head - body * U;
+    const int vocab = static_cast<int>(a.vocab), head = off < vocab ? off : vocab;
+    const int body = (vocab - head) / U, tail = vocab - head - body * U;   // whole accesses, and what is behind them
     const int v0 = slice * T * N + tid;
     const u32x4* in = reinterpret_cast<const u32x4*>(x + static_cast<int64_t>(head) * kSize);
     constexpr uint32_t kNone = F32 ? 0xFF800000u : 0xFF80FF80u;  // -inf
-    u32x4 w[N];
+    u32x4 w[N];   // the row's values stay in registers
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int v = v0 + n * T;
         w[n] = u32x4{kNone, kNone, kNone, kNone};
-        if (v < body) w[n] = in[v];
+        if (v0 + n * T < body) w[n] = in[v0 + n * T];
     }
     float extra = -INFINITY;
-    uint32_t extra_id = 0x40000000u + tid;  // ids past the vocabulary stand for nothing
+    uint32_t extra_id = 0x40000000u;   // past the vocabulary: nothing
     if (slice == 0 && tid < head + tail) {
         extra_id = static_cast<uint32_t>(tid < head ? tid : vocab - tail + (tid - head));
         extra = load1<F32>(x, extra_id);
     }
+    if (tid == 0) count = hits = 0;
+    if (tid < top) best[tid] = 0;
     auto value = [&](int n, int u) {
         if constexpr (F32) return __uint_as_float(w[n][u]);
         else return (u & 1) ? bf16w_hi(w[n][u / 2]) : bf16w_lo(w[n][u / 2]);
     };
-    auto id_of = [&](int n, int u) {
-        const int v = v0 + n * T;
-        return static_cast<uint32_t>(head + v * U + u) + (v < body ? 0u : 0x40000000u);
+    // a phase takes the values from their words again rather than hold both
+    auto phase = [&]() {
+        if constexpr (!F32) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) asm("" : "+v"(w[n]));
+        }
     };
-    // maximum of what is a number, of the thread and of the wave
+    // the largest number of the thread and of the wave (a NaN is none)
     float mine = fmaxf(extra, -INFINITY);
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -153,15 +165,19 @@ __global__ void __launch_bounds__(T) k_logprobs(LogprobArgs a, int slices) {
         for (int u = 0; u < U; ++u) mine = fmaxf(mine, value(n, u));
     float m = mine;
 #pragma unroll
-    for (int by = 1; by < kWave; by *= 2) m = fmaxf(m, __shfl_xor(m, by));
+    for (int by = 1; by < kWave; by *= 2) {
+        if (by == SPAN && top > 1 && tid % SPAN == 0) group[tid / SPAN] = m;
+        m = fmaxf(m, __shfl_xor(m, by));
+    }
     const float base = m == -INFINITY ? 0.0f : m;
     float s = 0.0f, t = 0.0f;
     auto add = [&](float v) {
-        const float d = base - v;                       // >= 0, inf for -inf, NaN
-        const float e = __builtin_amdgcn_exp2f(d * -kLog2e);
+        const float d = v - base;                                  // <= 0, -inf, or NaN
+        const float e = __builtin_amdgcn_exp2f(d * kLog2e);
         s += e;
-        t = fmaf(e, fminf(d, 1e4f), t);                 // e is 0 long before (NaN stays in s)
+        t = fmaf(e, fmaxf(d, -1e4f), t);                           // e is 0 long before (NaN stays in s)
     };
+    phase();
     add(extra);
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -172,83 +188,83 @@ __global__ void __launch_bounds__(T) k_logprobs(LogprobArgs a, int slices) {
         s += __shfl_xor(s, by);
         t += __shfl_xor(t, by);
     }
-    if ((tid & 63) == 0) part[tid / kWave] = {m, s, t};
-    if (a.top > 0) {
-        // the thread's first largest, then its group's
-        uint32_t id = 0x40000000u + extra_id;
-#pragma unroll
-        for (int n = N - 1; n >= 0; --n)
-#pragma unroll
-            for (int u = U - 1; u >= 0; --u) {
-                if (fmaxf(value(n, u), -INFINITY) == mine) id = id_of(n, u);
-            }
-        if (fmaxf(extra, -INFINITY) == mine && extra_id < id) id = extra_id;
-        u64 k = key_of(mine, id);
-#pragma unroll
-        for (int by = 1; by < SPAN; by *= 2) k = max64(k, shfl_xor64(k, by));
-        if (tid % SPAN == 0) group[tid / SPAN] = k;
-        if (tid == 0) count = 0;
-    }
+    if ((tid & 63) == 0) part[tid / kWave] = {m, s, -t};
     __syncthreads();
     const Sums all = join(WAVES, [&](int i) { return part[i]; });
-    if (a.top == 1) {
-        if (tid < kGroups) {
-            u64 k = group[tid];
+    if (top > 0) {
+        if (top > 1) {
+            if (tid < kGroups) {
+                const float g = group[tid];
+                int above = 0, least = 0;
 #pragma unroll
-            for (int by = 1; by < kWave; by *= 2) k = max64(k, shfl_xor64(k, by));
-            if (tid == 0) best[0] = k;
+                for (int j = 0; j < kGroups; j += 4) {
+                    const f32x4 of = *reinterpret_cast<const f32x4*>(group + j);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        above += of[i] > g;
+                        least += of[i] >= g;
+                    }
+                }
+                if (above < top && least >= top) floor_value = g;   // equal ones write the same
+            }
+            __syncthreads();
         }
-        __syncthreads();
-    } else if (a.top > 1) {
-        if (tid < kGroups) {
-            const u64 k = group[tid];
-            int above = 0;
-            for (int j = 0; j < kGroups; ++j) above += group[j] > k;
-            if (above == a.top - 1) floor_key = k;
-        }
-        __syncthreads();
-        const u64 least = floor_key;
-        const float low = key_value(least);
+        const float low = top > 1 ? floor_value : all.m;
+        // Fewer than `top` groups with a number: all numbers, and of the others the
+        // slice's first `top` ids hold as many as can be wanted.
+        const uint32_t window = slice == 0 ? 0u : static_cast<uint32_t>(head + slice * T * N * U);
         auto keep = [&](float v, uint32_t id) {
             v = fmaxf(v, -INFINITY);
-            if (v < low) return;
-            const u64 k = key_of(v, id);
-            if (k < least) return;
+            if (!(v >= low) || (low == -INFINITY && v == low && id - window >= static_cast<uint32_t>(top))) return;
             const int at = atomicAdd(&count, 1);
-            if (at < kMost) keys[at] = k;
+            if (at < kMost) keys[at] = key_of(v, id);
         };
+        // the accesses that hold one, then their values: a wave whose every access has
+        // some lane's value would else go through all of them
+        phase();
         keep(extra, extra_id);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; ++u) most = fmaxf(most, value(n, u));
+            if (most >= low && v0 + n * T < body) hit[atomicAdd(&hits, 1)] = static_cast<uint16_t>(n * T + tid);
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = tid; i < hits; i += T) {
+            const int at = slice * T * N + hit[i];
+            const u32x4 v = in[at];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                keep(value(n, u), id_of(n, u));
+                if constexpr (F32) keep(__uint_as_float(v[u]), head + at * U + u);
+                else keep((u & 1) ? bf16w_hi(v[u / 2]) : bf16w_lo(v[u / 2]), head + at * U + u);
             }
+        }
         __syncthreads();
         if (count <= kMost) {
-            rank(keys, count, best, a.top, tid, T);
+            rank(keys, count, best, top, tid, T);
         } else {
-            // too many reach the floor (large logits all in a few groups): one at a time
+            // too many reach the floor (equal logits, or large ones all in a few
+            // groups): one at a time
             u64 last = ~0ull;
-            for (int j = 0; j < a.top; ++j) {
+#pragma unroll 1
+            for (int j = 0; j < top; ++j) {
                 u64 k = 0;
                 auto next = [&](float v, uint32_t id) {
                     const u64 c = key_of(fmaxf(v, -INFINITY), id);
                     if (c < last) k = max64(k, c);
                 };
                 next(extra, extra_id);
-#pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                                next(value(n, u), id_of(n, u));
-                    }
+                const int first = head + slice * T * N * U, end = head + min(body, (slice + 1) * T * N) * U;
+#pragma unroll 1
+                for (int id = first + tid; id < end; id += T) next(load1<F32>(x, id), id);
 #pragma unroll
                 for (int by = 1; by < kWave; by *= 2) k = max64(k, shfl_xor64(k, by));
-                if ((tid & 63) == 0) group[tid / kWave] = k;
+                if ((tid & 63) == 0) keys[tid / kWave] = k;
                 __syncthreads();
-                k = group[0];
-                for (int i = 1; i < WAVES; ++i) k = max64(k, group[i]);
+                k = keys[0];
+                for (int i = 1; i < WAVES; ++i) k = max64(k, keys[i]);
                 last = k;
                 if (tid == 0) best[j] = k;
                 __syncthreads();
@@ -266,35 +282,58 @@ __global__ void __launch_bounds__(T) k_logprobs(LogprobArgs a, int slices) {
             to[1] = all.s;
             to[2] = all.w;
         }
-        u64* to = reinterpret_cast<u64*>(a.part + 4 * a.rows * slices) + at * a.top;
-        for (int j = tid; j < a.top; j += T) to[j] = best[j];
+        u64* to = reinterpret_cast<u64*>(a.part + 4 * a.rows * slices) + at * top;
+        for (int j = tid; j < top; j += T) to[j] = best[j];
     }
 }
 
+// A wave to a row; what it reads is on its way before anything waits.
 template <bool F32>
-__global__ void __launch_bounds__(256) k_logprobs_join(LogprobArgs a, int slices) {
-    __shared__ u64 keys[kMaxSlices * kGroups], best[kGroups], floor_key;
+__global__ void __launch_bounds__(kWave) k_logprobs_join(LogprobArgs a, int slices) {
+    __shared__ u64 keys[kMaxSlices * kGroups], best[kGroups];
     __shared__ int count;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x;
-    const float* part = a.part + 4 * row * slices;
-    const Sums all = join(slices, [&](int i) { return Sums{part[4 * i], part[4 * i + 1], part[4 * i + 2]}; });
+    Sums p = {-INFINITY, 0.0f, 0.0f};
+    if (tid < slices) {
+        const float* part = a.part + 4 * (row * slices + tid);
+        p = {part[0], part[1], part[2]};
+    }
+    const u64* from = reinterpret_cast<const u64*>(a.part + 4 * a.rows * slices) + row * slices * a.top;
+    // `top` keys at least reach the largest of the slices' last ones
+    u64 floor_key = a.top > 0 && tid < slices ? from[tid * a.top + a.top - 1] : 0;
+    if (tid == 0) count = 0;
+    if (tid < a.top) best[tid] = 0;
+    Sums all = {p.m, 0.0f, 0.0f};
+#pragma unroll
+    for (int by = 1; by < kMaxSlices; by *= 2) {
+        all.m = fmaxf(all.m, __shfl_xor(all.m, by));
+        floor_key = max64(floor_key, shfl_xor64(floor_key, by));
+    }
+    if (tid < slices) {
+        const Sums one = join(1, [&](int) { return p; }, all.m);
+        all.s = one.s;
+        all.w = one.w;
+    }
+#pragma unroll
+    for (int by = 1; by < kMaxSlices; by *= 2) {
+        all.s += __shfl_xor(all.s, by);
+        all.w += __shfl_xor(all.w, by);
+    }
+    // (slices are in the first 32 lanes: the others have their own)
+    all = {__shfl(all.m, 0), __shfl(all.s, 0), __shfl(all.w, 0)};
+    floor_key = static_cast<u64>(__shfl(static_cast<long long>(floor_key), 0));
+    __syncthreads();
     if (a.top > 0) {
-        const u64* from = reinterpret_cast<const u64*>(a.part + 4 * a.rows * slices) + row * slices * a.top;
-        // `top` keys at least reach the largest of the slices' last ones
-        if (tid == 0) { floor_key = 0; count = 0; }
-        __syncthreads();
-        for (int i = tid; i < slices; i += 256) atomicMax(&floor_key, from[static_cast<int64_t>(i) * a.top + a.top - 1]);
-        __syncthreads();
-        for (int i = tid; i < slices * a.top; i += 256) {
+        for (int i = tid; i < slices * a.top; i += kWave) {
             const u64 k = from[i];
             if (k >= floor_key) keys[atomicAdd(&count, 1)] = k;
         }
         __syncthreads();
-        rank(keys, count, best, a.top, tid, 256);
+        rank(keys, count, best, a.top, tid, kWave);
         __syncthreads();
     }
-    write_row<F32>(a, row, all, best, tid, 256);
+    write_row<F32>(a, row, all, best, tid, kWave);
 }
 
 // The slices of a row: T threads hold N accesses of 16 bytes.
@@ -302,10 +341,11 @@ struct Plan {
     int threads, slices;
 };
 constexpr int kN = 8;
+constexpr int64_t kFewRows = 64;
 Plan plan_of(int64_t rows, int64_t vocab, bool f32) {
     const int64_t accesses = vocab / (f32 ? 4 : 8);
     auto slices = [&](int t) { return static_cast<int>(accesses > 0 ? ceil_div(accesses, int64_t(t) * kN) : 1); };
-    if (slices(1024) == 1 || slices(256) > kMaxSlices) return {1024, slices(1024)};
+    if ((rows < kFewRows && slices(1024) == 1) || slices(256) > kMaxSlices) return {1024, slices(1024)};
     return {256, slices(256)};
 }
 
@@ -335,8 +375,8 @@ hipError_t launch_token_logprobs(const LogprobArgs& a, bool f32, hipStream_t s) 
     }
     if (p.slices > 1) {
         const dim3 grid(static_cast<unsigned>(a.rows));
-        if (f32) hipLaunchKernelGGL(k_logprobs_join<true>, grid, dim3(256), 0, s, a, p.slices);
-        else hipLaunchKernelGGL(k_logprobs_join<false>, grid, dim3(256), 0, s, a, p.slices);
+        if (f32) hipLaunchKernelGGL(k_logprobs_join<true>, grid, dim3(kWave), 0, s, a, p.slices);
+        else hipLaunchKernelGGL(k_logprobs_join<false>, grid, dim3(kWave), 0, s, a, p.slices);
     }
     return hipGetLastError();
 }
