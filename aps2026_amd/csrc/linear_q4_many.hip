@@ -200,6 +200,109 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
     }
 }
 
+// Up to 16 rows on a wide weight: 16 waves, kSide of them side by side with 16
+// outputs each, which share x through LDS.  Two pieces of it (one for each of the
+// two shares of the inputs) are copied there while the two before are multiplied.
+// A wave that loaded x for itself would read 8 or 24 KB from L2 for every 2 KB of
+// codes (16 fp32 rows on 4096 x 32064: 47 us, even 64 outputs to a wave).
+constexpr int kSide = 8, kWide = 1024, kWideOut = 16384;
+
+template <int GROUP, bool F32, bool SCALES32>
+__global__ void __launch_bounds__(kWide) k_q4_wide(LinearQ4Args a) {
+    constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32, TERMS = F32 ? 3 : 1, BLOCK = kBlock / GROUPS;
+    using Weight = Columns<1, GROUP, SCALES32>;
+    constexpr int OWN = Weight::LDS + kBlock * 64, STAGE = 2 * piece_bytes(TERMS), COPIES = STAGE / 1024 / 16;
+    __shared__ __align__(1024) unsigned char lds[2 * STAGE];
+    __shared__ __align__(16) unsigned char owns[16 * OWN];
+    const int tid = threadIdx.x, wave = tid / 64, lane = tid & 63, q = lane >> 4, wn = wave % kSide, wk = wave / kSide;
+    const int in = a.w.in, pieces = (in + kPiece - 1) / kPiece, rounds = (pieces + 1) / 2, groups = all_groups(in, GROUP);
+    const uint8_t* x = reinterpret_cast<const uint8_t*>(a.terms);
+    const float* sums = reinterpret_cast<const float*>(x + sums_at(a.rows, in, TERMS));
+    const Weight w(a.w, (static_cast<int>(blockIdx.x) * kSide + wn) * 16, lane, owns + wave * OWN);
+    float* own_sums = reinterpret_cast<float*>(owns + wave * OWN + Weight::LDS);
+    const CodeBits bits = code_bits();
+    const int first = wk * rounds, last = min(first + rounds, pieces);
+    // round `round`'s two pieces, 1 KB a copy (past the last piece the last again)
+    auto copy = [&](int round) {
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+            const int at = (i * 16 + wave) * 1024, half = at / piece_bytes(TERMS);
+            const int piece = min(half * rounds + min(round, rounds - 1), pieces - 1);
+            const uint8_t* from = x + static_cast<int64_t>(piece) * piece_bytes(TERMS) + at % piece_bytes(TERMS) + 16 * lane;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)(lds + (round & 1) * STAGE + at), 16, 0, 0);
+        }
+    };
+    f32x4 total = {0.0f, 0.0f, 0.0f, 0.0f};
+    copy(0);
+    Held<1> h0 = w.fetch(min(first, last - 1)), h1 = w.fetch(min(first + 1, last - 1));
+    int block = 0, begin = first;
+#pragma unroll 1
+    for (int round = 0; round < rounds; ++round) {
+        const int piece = first + round;
+        if (round % BLOCK == 0) {
+            block = w.load_scales(piece);
+            begin = piece;
+            const int mine = min(begin * GROUPS + (lane >> 2), groups - 1) * 16 + 4 * (lane & 3);
+            reinterpret_cast<f32x4*>(own_sums)[lane] = *reinterpret_cast<const f32x4*>(sums + mine);
+            __builtin_amdgcn_wave_barrier();
+        }
+        // this round's copies, which were issued before the two loads of codes in flight
+        __builtin_amdgcn_s_waitcnt(0x0F70 | 2);
+        lds_barrier();
+        copy(round + 1);
+        const Held<1> h = h0;
+        h0 = h1;
+        h1 = w.fetch(min(piece + 2, last - 1));
+        if (piece < last) {
+            const unsigned char* xs = lds + (round & 1) * STAGE + wk * piece_bytes(TERMS) + 16 * lane;
+            const auto of = w.scales(w.first_group(piece) - block);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const u32x4 code = to_columns(h.code[c][0], lane);
+#pragma unroll
+                for (int g = c * (128 / GROUP); g < (c + 1) * (128 / GROUP); ++g) {
+                    f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f};
+                    // the smallest terms first: what they add is kept under the largest's sums
+#pragma unroll
+                    for (int e = TERMS - 1; e >= 0; --e)
+#pragma unroll
+                        for (int t = g * STEPS; t < (g + 1) * STEPS; ++t)
+                            dot = mfma(frag(*reinterpret_cast<const u32x4*>(xs + (8 * e + t) * 1024)), code_values(code[t & 3], bits), dot);
+                    const f32x4 sum = *reinterpret_cast<const f32x4*>(own_sums + ((piece - begin) * GROUPS + g) * 16 + 4 * q);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) total[r] = fmaf(of.scale(0, g), fmaf(of.off(0, g), sum[r], dot[r]), total[r]);
+                }
+            }
+        }
+    }
+    // the copies past the last round, then the two shares of a column joined
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    lds_barrier();
+    float* red = reinterpret_cast<float*>(lds);   // [wave][row][column]
+#pragma unroll
+    for (int r = 0; r < 4; ++r) red[(wave * 16 + 4 * q + r) * 16 + (lane & 15)] = total[r];
+    lds_barrier();
+#pragma unroll 1
+    for (int i = tid; i < static_cast<int>(a.rows) * kSide * 16; i += kWide) {
+        const int m = i / (kSide * 16), c = i % (kSide * 16), n = static_cast<int>(blockIdx.x) * kSide * 16 + c;
+        if (n >= a.w.out) continue;
+        float y = (red[((c / 16) * 16 + m) * 16 + c % 16] + red[((c / 16 + kSide) * 16 + m) * 16 + c % 16]) * 16.0f;
+        if (a.bias) y += a.bias[n];
+        const int64_t to = static_cast<int64_t>(m) * a.w.out + n;
+        if constexpr (F32) static_cast<float*>(a.y)[to] = y;
+        else static_cast<bf16_t*>(a.y)[to] = static_cast<bf16_t>(pack2_bf16(y, 0.0f) & 0xFFFFu);
+    }
+}
+
+template <int GROUP, bool F32>
+hipError_t run_wide(const LinearQ4Args& a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.w.out, 16 * kSide))), block(kWide);
+    if (a.w.scales_f32) hipLaunchKernelGGL((k_q4_wide<GROUP, F32, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_q4_wide<GROUP, F32, false>), grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
 template <int GROUP, bool F32, int MT, int NT>
 hipError_t run(const LinearQ4Args& a, hipStream_t s) {
     const int64_t pieces = ceil_div(a.w.in, kPiece);
@@ -217,8 +320,7 @@ hipError_t run(const LinearQ4Args& a, hipStream_t s) {
 
 template <int GROUP, bool F32>
 hipError_t by_rows(const LinearQ4Args& a, hipStream_t s) {
-    const int64_t tiles = ceil_div(a.w.out, 16);
-    if (a.rows <= 16) return tiles >= 1024 ? run<GROUP, F32, 1, 4>(a, s) : run<GROUP, F32, 1, 1>(a, s);
+    if (a.rows <= 16) return a.w.out >= kWideOut ? run_wide<GROUP, F32>(a, s) : run<GROUP, F32, 1, 1>(a, s);
     if constexpr (F32) return run<GROUP, F32, 2, 2>(a, s);
     else return a.rows <= 32 ? run<GROUP, F32, 2, 2>(a, s) : run<GROUP, F32, 4, 2>(a, s);
 }
