@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(kWide) k_q4_wide(LinearQ4Args a) {
     constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32, TERMS = F32 ? 3 : 1, BLOCK = kBlock / GROUPS;
     using Weight = Columns<1, GROUP, SCALES32>;
     constexpr int OWN = Weight::LDS + kBlock * 64, STAGE = 2 * piece_bytes(TERMS), COPIES = STAGE / 1024 / 16;
-    __shared__ __align__(1024) unsigned char lds[2 * STAGE];
+    // two arrays: a read of one need not wait for copies into the other
+    __shared__ __align__(1024) unsigned char even[STAGE], odd[STAGE];
     __shared__ __align__(16) unsigned char owns[16 * OWN];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid & 63, q = lane >> 4, wn = wave % kSide, wk = wave / kSide;
     const int in = a.w.in, pieces = (in + kPiece - 1) / kPiece, rounds = (pieces + 1) / 2, groups = all_groups(in, GROUP);
@@ -223,63 +224,70 @@ __global__ void __launch_bounds__(kWide) k_q4_wide(LinearQ4Args a) {
     const CodeBits bits = code_bits();
     const int first = wk * rounds, last = min(first + rounds, pieces);
     // round `round`'s two pieces, 1 KB a copy (past the last piece the last again)
-    auto copy = [&](int round) {
+    auto copy = [&](int round, unsigned char* to) {
 #pragma unroll
         for (int i = 0; i < COPIES; ++i) {
             const int at = (i * 16 + wave) * 1024, half = at / piece_bytes(TERMS);
             const int piece = min(half * rounds + min(round, rounds - 1), pieces - 1);
             const uint8_t* from = x + static_cast<int64_t>(piece) * piece_bytes(TERMS) + at % piece_bytes(TERMS) + 16 * lane;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                             (__attribute__((address_space(3))) void*)(lds + (round & 1) * STAGE + at), 16, 0, 0);
+            // Written out, for the compiler would let every read of LDS wait for it; it has
+            // no result in registers, and the waits below count it.
+            const uint32_t base = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
+                reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)(to + at))));
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(base), "v"(from) : "memory", "m0");
         }
     };
     f32x4 total = {0.0f, 0.0f, 0.0f, 0.0f};
-    copy(0);
+    copy(0, even);
     Held<1> h0 = w.fetch(min(first, last - 1)), h1 = w.fetch(min(first + 1, last - 1));
     int block = 0, begin = first;
-#pragma unroll 1
-    for (int round = 0; round < rounds; ++round) {
+    auto step = [&](int round, const unsigned char* here, unsigned char* next, Held<1>& h) {
         const int piece = first + round;
-        if (round % BLOCK == 0) {
-            block = w.load_scales(piece);
-            begin = piece;
-            const int mine = min(begin * GROUPS + (lane >> 2), groups - 1) * 16 + 4 * (lane & 3);
-            reinterpret_cast<f32x4*>(own_sums)[lane] = *reinterpret_cast<const f32x4*>(sums + mine);
-            __builtin_amdgcn_wave_barrier();
-        }
         // this round's copies, which were issued before the two loads of codes in flight
-        __builtin_amdgcn_s_waitcnt(0x0F70 | 2);
-        lds_barrier();
-        copy(round + 1);
-        const Held<1> h = h0;
-        h0 = h1;
-        h1 = w.fetch(min(piece + 2, last - 1));
-        if (piece < last) {
-            const unsigned char* xs = lds + (round & 1) * STAGE + wk * piece_bytes(TERMS) + 16 * lane;
-            const auto of = w.scales(w.first_group(piece) - block);
+        // (vmcnt 2, lgkmcnt 0; a fence would wait for those too)
+        __builtin_amdgcn_s_waitcnt(0x0070 | 2);
+        asm volatile("s_barrier" ::: "memory");
+        copy(round + 1, next);
+        const u32x4 codes[2] = {to_columns(h.code[0][0], lane), to_columns(h.code[1][0], lane)};
+        h = w.fetch(min(piece + 2, last - 1));
+        if (piece >= last) return;
+        const unsigned char* xs = here + wk * piece_bytes(TERMS) + 16 * lane;
+        const auto of = w.scales(w.first_group(piece) - block);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const u32x4 code = to_columns(h.code[c][0], lane);
+        for (int g = 0; g < GROUPS; ++g) {
+            f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f};
+            // the smallest terms first: what they add is kept under the largest's sums
 #pragma unroll
-                for (int g = c * (128 / GROUP); g < (c + 1) * (128 / GROUP); ++g) {
-                    f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f};
-                    // the smallest terms first: what they add is kept under the largest's sums
+            for (int e = TERMS - 1; e >= 0; --e)
 #pragma unroll
-                    for (int e = TERMS - 1; e >= 0; --e)
+                for (int t = g * STEPS; t < (g + 1) * STEPS; ++t)
+                    dot = mfma(frag(*reinterpret_cast<const u32x4*>(xs + (8 * e + t) * 1024)), code_values(codes[t / 4][t & 3], bits), dot);
+            const f32x4 sum = *reinterpret_cast<const f32x4*>(own_sums + ((piece - begin) * GROUPS + g) * 16 + 4 * q);
 #pragma unroll
-                        for (int t = g * STEPS; t < (g + 1) * STEPS; ++t)
-                            dot = mfma(frag(*reinterpret_cast<const u32x4*>(xs + (8 * e + t) * 1024)), code_values(code[t & 3], bits), dot);
-                    const f32x4 sum = *reinterpret_cast<const f32x4*>(own_sums + ((piece - begin) * GROUPS + g) * 16 + 4 * q);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) total[r] = fmaf(of.scale(0, g), fmaf(of.off(0, g), sum[r], dot[r]), total[r]);
-                }
-            }
+            for (int r = 0; r < 4; ++r) total[r] = fmaf(of.scale(0, g), fmaf(of.off(0, g), sum[r], dot[r]), total[r]);
+        }
+    };
+#pragma unroll 1
+    for (int round = 0; round < rounds;) {
+        begin = first + round;
+        block = w.load_scales(begin);
+        const int mine = min(begin * GROUPS + (lane >> 2), groups - 1) * 16 + 4 * (lane & 3);
+        reinterpret_cast<f32x4*>(own_sums)[lane] = *reinterpret_cast<const f32x4*>(sums + mine);
+        __builtin_amdgcn_wave_barrier();
+        const int end = min(round + BLOCK, rounds);   // BLOCK is even: the arrays stay in turn
+#pragma unroll 1
+        for (;;) {
+            step(round, even, odd, h0);
+            if (++round == end) break;
+            step(round, odd, even, h1);
+            if (++round == end) break;
         }
     }
     // the copies past the last round, then the two shares of a column joined
     __builtin_amdgcn_s_waitcnt(0x0F70);
     lds_barrier();
-    float* red = reinterpret_cast<float*>(lds);   // [wave][row][column]
+    float* red = reinterpret_cast<float*>(owns);   // [wave][row][column]
+    static_assert(OWN >= 16 * 16 * 4, "a wave's own LDS holds its sums");
 #pragma unroll
     for (int r = 0; r < 4; ++r) red[(wave * 16 + 4 * q + r) * 16 + (lane & 15)] = total[r];
     lds_barrier();
