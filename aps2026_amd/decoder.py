@@ -26,7 +26,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -37,6 +37,7 @@ from .attention import HEAD_DIM, NUM_ATTENTION_HEADS, NUM_KV_HEADS, ROPE_THETA, 
 from .moe import NORM_EPS, MoeWeights, _call, register_moe_weights_gpu
 
 EOS_TOKEN_ID = 32000                  # reference include/config.h:25
+Q4_GROUP = 128                        # inputs that share a scale and a zero, Model(tc="q4")
 QD = NUM_ATTENTION_HEADS * HEAD_DIM   # 2048: q and attention-output width
 KD = NUM_KV_HEADS * HEAD_DIM          # 512: k and v width
 
@@ -208,13 +209,18 @@ class DecoderLayer:
     tc_terms: None for the fp32 projections (the reference's default build);
     3 or 4 for the split-bf16 Linear on the q/k/v/o projections (the
     reference's USE_TC / USE_TC_ALL tensor-core path, src/layer.cu:16-27,
-    src/tensor.cu:514-584), whose weights are packed here once."""
+    src/tensor.cu:514-584), whose weights are packed here once.  q4_group: the
+    projections in 4 bits instead, quantised here once in groups of so many
+    inputs (the reference has no such path)."""
 
-    def __init__(self, w: LayerWeights, tc_terms: Optional[int] = None):
+    def __init__(self, w: LayerWeights, tc_terms: Optional[int] = None, q4_group: Optional[int] = None):
         self.w = w
         self.H = w.in_w.numel()
         self.tc_terms = tc_terms
         self.tc = {}
+        self.q4: Dict[str, serve.Q4Weight] = {}
+        if q4_group is not None:
+            self.q4 = {nm: serve.quantise_q4_gpu(wt, q4_group) for nm, (wt, _) in w.proj.items()}
         if tc_terms is not None:
             from .attention import linear_tc_prepare
             self.tc = {nm: linear_tc_prepare(wt) for nm, (wt, _) in w.proj.items()}
@@ -223,7 +229,11 @@ class DecoderLayer:
         """The projections of one input: fp32 chains, or the split products
         (x split once for all of them)."""
         L, T, K = capi.lib(), b.rows, src.shape[1]
-        if self.tc:
+        if self.q4:
+            with serve.on_stream(stream, src.device):
+                for nm, dst, _ in names:
+                    serve.linear_q4_gpu(src, self.q4[nm], self.w.proj[nm][1], out=dst)
+        elif self.tc:
             # every output of the input in one launch (their column blocks share the grid)
             xs = b.split(src, stream)
             cnt = len(names)
@@ -309,16 +319,19 @@ class Model:
                  tc: str = "off"):
         """tc: "off" (fp32 projections, the reference's default build), "tc"
         (the split-bf16 Linear, three products, for the LM head and layer
-        31's attention projections: the reference's USE_TC) or "all" (four
+        31's attention projections: the reference's USE_TC), "all" (four
         products, the LM head and every layer's attention projections:
-        USE_TC_ALL)."""
-        if tc not in ("off", "tc", "all"):
-            raise ValueError("tc is 'off', 'tc' or 'all'")
+        USE_TC_ALL) or "q4" (those in 4 bits, quantised here in groups of 128
+        inputs with zeros; activations stay fp32.  The weights given are not
+        needed for them any more)."""
+        if tc not in ("off", "tc", "all", "q4"):
+            raise ValueError("tc is 'off', 'tc', 'all' or 'q4'")
         self.emb, self.norm_w, self.norm_b = embeddings, norm_w, norm_b
         self.head_w, self.head_b = lm_head_w, lm_head_b
-        terms = None if tc == "off" else (4 if tc == "all" else 3)
-        self.layers = [DecoderLayer(w, terms if (tc == "all" or (tc == "tc" and i == 31)) else None)
-                       for i, w in enumerate(layers)]
+        terms = {"off": None, "q4": None, "tc": 3, "all": 4}[tc]
+        self.layers = [DecoderLayer(w, terms if (tc == "all" or (tc == "tc" and i == 31)) else None,
+                                    Q4_GROUP if tc == "q4" else None) for i, w in enumerate(layers)]
+        self.head_q4 = serve.quantise_q4_gpu(lm_head_w, Q4_GROUP) if tc == "q4" else None
         self.head_terms = terms
         self.head_tc = None
         if terms is not None:
@@ -363,6 +376,8 @@ class Model:
         batch = plan.last_rows.shape[0]
         rows_out = torch.empty((batch, H), dtype=torch.float32, device=dev)
         _call(L.aps_gather_rows(_p(b.normed), T, H, _p(plan.last_rows), batch, _p(rows_out), stream))
+        if self.head_q4 is not None:
+            return serve.linear_q4_gpu(rows_out, self.head_q4, self.head_b)
         V = self.head_w.shape[0]
         logits = torch.empty((batch, V), dtype=torch.float32, device=dev)
         if self.head_tc is not None:
@@ -377,11 +392,40 @@ class Model:
     def generate(self, prompts: Sequence[Sequence[int]]) -> torch.Tensor:
         return self.prefill(RowPlan.from_prompts(prompts, self.emb.device))
 
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[serve.TokenLogprobs]:
+        """What the model gives each prompt's tokens after the first: for prompt
+        p the len(p) - 1 log probabilities of p[i + 1] behind p[: i + 1], the
+        entropies there and the `top` likeliest tokens (serve.TokenLogprobs).
+        One prefill of all rows; their logits take rows * vocabulary * 4
+        bytes."""
+        if len(prompts) == 0:
+            raise RuntimeError("score received an empty input batch")
+        lens = [len(p) for p in prompts]
+        if min(lens) == 0:
+            raise ValueError("empty input")
+        if max(lens) > prefix.MAX_POSITION_EMBEDDINGS:
+            raise ValueError("sequence is too long")
+        flat = np.concatenate([np.asarray(p, np.int64).reshape(-1) for p in prompts])
+        if flat.min() < 0 or flat.max() >= self.emb.shape[0]:
+            raise ValueError("token out of vocabulary")
+        if not 0 <= top <= min(serve.MAX_TOP, self.head_w.shape[0]):
+            raise ValueError("top is a number of tokens")
+        dev, V = self.emb.device, self.head_w.shape[0]
+        rows = np.delete(np.arange(flat.size), np.cumsum(lens) - 1)   # those with a token behind them
+        if rows.size == 0:
+            logits = torch.empty((0, V), dtype=torch.float32, device=dev)
+        else:
+            plan = replace(RowPlan.packed(prompts, dev), last_rows=torch.from_numpy(rows.astype(np.int32)).to(dev))
+            logits = self.prefill(plan, buffers=Buffers.allocate(plan.rows, self.H, self.layers[0].w.moe, dev))
+        r = serve.token_logprobs_gpu(logits, torch.from_numpy(flat[rows + 1].astype(np.int32)).to(dev), top)
+        at = np.cumsum([0] + [n - 1 for n in lens])
+        return [serve.TokenLogprobs(*(t[b:e] for t in r)) for b, e in zip(at[:-1], at[1:])]
+
     def generate_decode(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, kv_dtype=torch.float32,
                         page_size: int = 16, window: int = SLIDING_WINDOW, sinks: int = 0,
                         repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
                         bias: Optional[Dict[int, float]] = None, mask: Optional[torch.Tensor] = None,
-                        eos: int = EOS_TOKEN_ID) -> Tuple[List[List[int]], torch.Tensor]:
+                        eos: int = EOS_TOKEN_ID, logprobs: Optional[int] = None) -> Tuple:
         """Greedy decoding of a prompt batch on paged caches (kv_dtype:
         torch.float32, torch.bfloat16 or "mxfp4"): each token is computed once,
         where the reference's generate_decode runs the whole prefix again for
@@ -390,8 +434,10 @@ class Model:
         chosen from: after the penalties, the biases {id: value} and the mask
         ([1] or [batch] rows of int32 words, bit t % 32 of word t / 32 allows
         token t).  Of equal logits the lowest id wins; NaN never does beside
-        a number, and of none but NaN and -inf id 0.  One host wait, at the
-        end.  Caches and activations are the call's own, from torch's caching
+        a number, and of none but NaN and -inf id 0.  With logprobs also the
+        chosen tokens' log probabilities, the entropies and so many likeliest
+        tokens under those logits: a serve.TokenLogprobs of [batch]
+        [max_new_tokens] (and [logprobs]) tensors.  One host wait, at the end.  Caches and activations are the call's own, from torch's caching
         allocator: calls may run side by side on other streams."""
         if len(prompts) == 0:
             raise RuntimeError("generate_decode received an empty input batch")
@@ -409,6 +455,8 @@ class Model:
             raise ValueError("token out of vocabulary")
         if not repetition > 0.0:
             raise ValueError("repetition must be positive")
+        if logprobs is not None and not 0 <= logprobs <= min(serve.MAX_TOP, V):
+            raise ValueError("logprobs is a number of tokens")
         if page_size not in (16, 32, 64, 128, 256):
             raise ValueError("page_size is 16, 32, 64, 128 or 256")
         if mask is not None and (mask.dim() != 2 or mask.shape[0] not in (1, n_seq)):
@@ -444,6 +492,7 @@ class Model:
                 rules.update(mask_index=torch.zeros(n_seq, dtype=torch.int32, device=dev))
         out = torch.empty((n_seq, max_new_tokens, V), dtype=torch.float32, device=dev)
         ids = torch.empty((n_seq, max_new_tokens), dtype=torch.int32, device=dev)
+        scores = []
         bufs = None
         for t in range(max_new_tokens):
             if bufs is None or bufs.rows != rows.rows:
@@ -458,6 +507,8 @@ class Model:
             x = torch.where(logits.isnan(), -math.inf, logits)
             token = torch.where(x == x.amax(1, keepdim=True), torch.arange(V, device=dev), V).amin(1).to(torch.int32)
             ids[:, t] = token
+            if logprobs is not None:
+                scores.append(serve.token_logprobs_gpu(logits, token, logprobs))
             if t + 1 == max_new_tokens:
                 break
             if history is not None:
@@ -471,4 +522,6 @@ class Model:
         done = []
         for row in ids.cpu().tolist():
             done.append(row[:row.index(eos) + 1] if eos in row else row)
-        return done, out
+        if logprobs is None:
+            return done, out
+        return done, out, serve.TokenLogprobs(*(torch.stack(parts, 1) for parts in zip(*scores)))

@@ -522,6 +522,9 @@ def linear_q4_gpu(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor
 
 # ---- log probabilities --------------------------------------------------------
 
+MAX_TOP = 64   # likeliest tokens of a row
+
+
 class TokenLogprobs(NamedTuple):
     """logprobs as the tokens' shape (None without tokens), entropy [rows],
     top_ids (int32) and top_logprobs [rows, top]."""
