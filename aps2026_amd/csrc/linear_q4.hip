@@ -95,27 +95,26 @@ __global__ void __launch_bounds__(kFew) k_q4_few(LinearQ4Args a, int columns) {
         if (m >= m_rows) return;   // the wave's all
         const Begin b = begin_of(run / 32, run & 31, in);
         if (b.k < b.at) r = Run{};
-        float sum = 0.0f;
-        if constexpr (F32) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += r.v[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum += bf16w_lo(r.w[i]) + bf16w_hi(r.w[i]);
-        }
-        sum = add_lanes<GROUP / 8>(sum);
-        if (run >= runs) return;
         float* to = sums + run / (GROUP / 8) * 16;
         auto place = [](int row) { return 4 * (row & 3) + (row >> 2); };
         if constexpr (F32) {
             u32x4 t[3];
-            terms_of(r.v, t);
+            float sum[3];
+            terms_of(r.v, t, sum);
+#pragma unroll
+            for (int e = 0; e < 3; ++e) sum[e] = add_lanes<GROUP / 8>(sum[e]);
+            if (run >= runs) return;
 #pragma unroll
             for (int e = 0; e < 3; ++e) {
                 *reinterpret_cast<u32x4*>(lds + 16 * run + (3 * m + e) * l.pitch) = t[e];
-                to[place(3 * m + e)] = e ? 0.0f : sum;   // the terms meet at the end
+                to[place(3 * m + e)] = sum[e];
             }
         } else {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += bf16w_lo(r.w[i]) + bf16w_hi(r.w[i]);
+            sum = add_lanes<GROUP / 8>(sum);
+            if (run >= runs) return;
             *reinterpret_cast<u32x4*>(lds + 16 * run + m * l.pitch) = code_order(r.w);
             to[place(m)] = sum;
         }

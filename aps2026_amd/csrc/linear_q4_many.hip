@@ -4,7 +4,8 @@
 // The first puts x into the order in which the matrix cores take it, fp32 x as
 // three bf16 terms (the workspace holds it):
 //   [16 rows][piece of 256 inputs][term][8 steps of 32 inputs][64 lanes][16 bytes],
-//   then the sums of x, [16 rows][group][row]
+//   then the sums of x, [16 rows][group][row], of fp32 x those of the first term
+//   and those of the other two
 // so that an operand is one load of neighbouring bytes.  In the second a wave
 // multiplies 16 MT rows by 16 NT columns over its share of the pieces, and a
 // workgroup's eight waves are joined in LDS.  x comes from L2 without a stay in
@@ -50,18 +51,18 @@ __global__ void __launch_bounds__(256) k_q4_arrange(LinearQ4Args a, int64_t wave
         if constexpr (F32) load8(static_cast<const float*>(a.x) + row + k, v[i]);
         else w[i] = load8(static_cast<const bf16_t*>(a.x) + row + k);
     }
-    float sum = 0.0f;
+    float sum = 0.0f, low = 0.0f;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
         const Begin b = begin_of(piece, 4 * (first + i) + q, in);
         u32x4 t[3];
         if constexpr (F32) {
+            float of[3];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[i][e] = b.k < b.at ? 0.0f : v[i][e];
-                sum += v[i][e];
-            }
-            terms_of(v[i], t);
+            for (int e = 0; e < 8; ++e) v[i][e] = b.k < b.at ? 0.0f : v[i][e];
+            terms_of(v[i], t, of);
+            sum += of[0];
+            low += of[1] + of[2];
         } else {
             if (b.k < b.at) w[i] = u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
@@ -75,6 +76,11 @@ __global__ void __launch_bounds__(256) k_q4_arrange(LinearQ4Args a, int64_t wave
     sum += __shfl_xor(sum, 32);
     float* sums = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.terms) + sums_at(a.rows, in, TERMS));
     if (lane < 16) sums[at * 16 + lane] = sum;
+    if constexpr (F32) {
+        low += __shfl_xor(low, 16);
+        low += __shfl_xor(low, 32);
+        if (lane < 16) sums[(waves + at) * 16 + lane] = low;
+    }
 }
 
 // 2^columns of a workgroup's waves lie side by side, 16 NT outputs each; the others
@@ -84,7 +90,7 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
     constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32, TERMS = F32 ? 3 : 1, BLOCK = kBlock / GROUPS;
     using Weight = Columns<NT, GROUP, SCALES32>;
     // a wave's scales and zeros, and its rows' sums: [tile][group of the block][row]
-    constexpr int OWN = Weight::LDS + MT * kBlock * 64;
+    constexpr int KINDS = F32 ? 2 : 1, OWN = Weight::LDS + KINDS * MT * kBlock * 64;   // sums of the first term, of the others
     constexpr int RED = kWaves * NT * MT * 4 * 64 * 4, SCALE = kWaves * OWN;
     __shared__ __align__(16) unsigned char lds[RED > SCALE ? RED : SCALE];
     const int tid = threadIdx.x, wave = tid / 64, lane = tid & 63, q = lane >> 4;
@@ -119,9 +125,10 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
             // 16 groups of 16 rows, the last of them again past a row's end
             const int mine = min(begin * GROUPS + (lane >> 2), groups - 1) * 16 + 4 * (lane & 3);
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-                reinterpret_cast<f32x4*>(own_sums)[64 * i + lane] =
-                    *reinterpret_cast<const f32x4*>(sums + min(static_cast<int64_t>(mb) * MT + i, last_tile) * groups * 16 + mine);
+            for (int i = 0; i < KINDS * MT; ++i) {
+                const int64_t tile = min(static_cast<int64_t>(mb) * MT + i % MT, last_tile) + i / MT * (last_tile + 1);
+                reinterpret_cast<f32x4*>(own_sums)[64 * i + lane] = *reinterpret_cast<const f32x4*>(sums + tile * groups * 16 + mine);
+            }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
             for (int piece = begin; piece < end; ++piece) {
@@ -134,13 +141,12 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
                     for (int j = 0; j < NT; ++j) code[j] = to_columns(h0.code[c][j], lane);
 #pragma unroll
                     for (int g = c * (128 / GROUP); g < (c + 1) * (128 / GROUP); ++g) {
-                        f32x4 dot[NT][MT] = {}, sum[MT];
+                        f32x4 dot[NT][MT][KINDS] = {}, sum[MT][KINDS];
 #pragma unroll
-                        for (int i = 0; i < MT; ++i)
-                            sum[i] = *reinterpret_cast<const f32x4*>(own_sums + (i * kBlock + (piece - begin) * GROUPS + g) * 16 + 4 * q);
-                        // the smallest terms first: what they add is kept under the largest's sums
+                        for (int i = 0; i < MT * KINDS; ++i)
+                            sum[i % MT][i / MT] = *reinterpret_cast<const f32x4*>(own_sums + (i * kBlock + (piece - begin) * GROUPS + g) * 16 + 4 * q);
 #pragma unroll
-                        for (int e = TERMS - 1; e >= 0; --e)
+                        for (int e = 0; e < TERMS; ++e)
 #pragma unroll
                             for (int t = g * STEPS; t < (g + 1) * STEPS; ++t) {
                                 bf16x8 xs[MT];
@@ -151,7 +157,7 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
                                 for (int j = 0; j < NT; ++j) {
                                     const bf16x8 v = code_values(code[j][t & 3], bits);
 #pragma unroll
-                                    for (int i = 0; i < MT; ++i) dot[j][i] = mfma(xs[i], v, dot[j][i]);
+                                    for (int i = 0; i < MT; ++i) dot[j][i][e > 0] = mfma(xs[i], v, dot[j][i][e > 0]);
                                 }
                             }
 #pragma unroll
@@ -159,8 +165,11 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
 #pragma unroll
                             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    total[j][i][r] = fmaf(of.scale(j, g), fmaf(of.off(j, g), sum[i][r], dot[j][i][r]), total[j][i][r]);
+                                for (int r = 0; r < 4; ++r) {
+                                    float v = fmaf(of.off(j, g), sum[i][0][r], dot[j][i][0][r]);
+                                    if constexpr (F32) v += fmaf(of.off(j, g), sum[i][1][r], dot[j][i][1][r]);
+                                    total[j][i][r] = fmaf(of.scale(j, g), v, total[j][i][r]);
+                                }
                     }
                 }
                 // behind this piece's x: loads come in order
@@ -211,7 +220,7 @@ template <int GROUP, bool F32, bool SCALES32>
 __global__ void __launch_bounds__(kWide) k_q4_wide(LinearQ4Args a) {
     constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32, TERMS = F32 ? 3 : 1, BLOCK = kBlock / GROUPS;
     using Weight = Columns<1, GROUP, SCALES32>;
-    constexpr int OWN = Weight::LDS + kBlock * 64, STAGE = 2 * piece_bytes(TERMS), COPIES = STAGE / 1024 / 16;
+    constexpr int KINDS = F32 ? 2 : 1, OWN = Weight::LDS + KINDS * kBlock * 64, STAGE = 2 * piece_bytes(TERMS), COPIES = STAGE / 1024 / 16;
     // two arrays: a read of one need not wait for copies into the other
     __shared__ __align__(1024) unsigned char even[STAGE], odd[STAGE];
     __shared__ __align__(16) unsigned char owns[16 * OWN];
@@ -255,16 +264,20 @@ __global__ void __launch_bounds__(kWide) k_q4_wide(LinearQ4Args a) {
         const auto of = w.scales(w.first_group(piece) - block);
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-            f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f};
-            // the smallest terms first: what they add is kept under the largest's sums
+            f32x4 dot[KINDS] = {};
 #pragma unroll
-            for (int e = TERMS - 1; e >= 0; --e)
+            for (int e = 0; e < TERMS; ++e)
 #pragma unroll
                 for (int t = g * STEPS; t < (g + 1) * STEPS; ++t)
-                    dot = mfma(frag(*reinterpret_cast<const u32x4*>(xs + (8 * e + t) * 1024)), code_values(codes[t / 4][t & 3], bits), dot);
-            const f32x4 sum = *reinterpret_cast<const f32x4*>(own_sums + ((piece - begin) * GROUPS + g) * 16 + 4 * q);
+                    dot[e > 0] = mfma(frag(*reinterpret_cast<const u32x4*>(xs + (8 * e + t) * 1024)),
+                                      code_values(codes[t / 4][t & 3], bits), dot[e > 0]);
+            const float* sum = own_sums + ((piece - begin) * GROUPS + g) * 16 + 4 * q;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) total[r] = fmaf(of.scale(0, g), fmaf(of.off(0, g), sum[r], dot[r]), total[r]);
+            for (int r = 0; r < 4; ++r) {
+                float v = fmaf(of.off(0, g), sum[r], dot[0][r]);
+                if constexpr (F32) v += fmaf(of.off(0, g), sum[16 * kBlock + r], dot[1][r]);
+                total[r] = fmaf(of.scale(0, g), v, total[r]);
+            }
         }
     };
 #pragma unroll 1
@@ -272,7 +285,9 @@ __global__ void __launch_bounds__(kWide) k_q4_wide(LinearQ4Args a) {
         begin = first + round;
         block = w.load_scales(begin);
         const int mine = min(begin * GROUPS + (lane >> 2), groups - 1) * 16 + 4 * (lane & 3);
-        reinterpret_cast<f32x4*>(own_sums)[lane] = *reinterpret_cast<const f32x4*>(sums + mine);
+#pragma unroll
+        for (int i = 0; i < KINDS; ++i)
+            reinterpret_cast<f32x4*>(own_sums)[64 * i + lane] = *reinterpret_cast<const f32x4*>(sums + i * groups * 16 + mine);
         __builtin_amdgcn_wave_barrier();
         const int end = min(round + BLOCK, rounds);   // BLOCK is even: the arrays stay in turn
 #pragma unroll 1
@@ -336,7 +351,7 @@ hipError_t by_rows(const LinearQ4Args& a, hipStream_t s) {
 }  // namespace
 
 size_t q4_many_bytes(const Q4& w, int64_t rows, bool f32) {
-    return static_cast<size_t>(sums_at(rows, w.in, f32 ? 3 : 1) + ceil_div(rows, 16) * all_groups(w.in, w.group) * 64);
+    return static_cast<size_t>(sums_at(rows, w.in, f32 ? 3 : 1) + ceil_div(rows, 16) * all_groups(w.in, w.group) * (f32 ? 128 : 64));
 }
 
 template <int GROUP>

@@ -73,8 +73,11 @@ __device__ inline u32x4 code_order(u32x4 w) {
                  __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
 }
 
-// The three bf16 terms of eight fp32 values, in the codes' order.
-__device__ inline void terms_of(const float (&x)[8], u32x4 (&t)[3]) {
+// The three bf16 terms of eight fp32 values, in the codes' order, and the sum of
+// each term's.  The first term's values have 8 bits, so their sums, and those of
+// their products with codes, are all but exact: kept apart from the others' they
+// leave the result's own rounding (one sum for all: 3 times the error).
+__device__ inline void terms_of(const float (&x)[8], u32x4 (&t)[3], float (&sum)[3]) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = x[i];
@@ -83,9 +86,12 @@ __device__ inline void terms_of(const float (&x)[8], u32x4 (&t)[3]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             t[j][i] = __builtin_amdgcn_perm(__float_as_uint(v[i + 4]), __float_as_uint(v[i]), 0x07060302u);
-        if (j < 2) {
+        sum[j] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] - __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
+        for (int i = 0; i < 8; ++i) {
+            const float cut = j < 2 ? __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u) : v[i];
+            sum[j] += cut;
+            v[i] -= cut;
         }
     }
 }

@@ -145,11 +145,11 @@ def test_bad_weights(kw, code):
     (dict(dt=capi.DTYPE_E4M3), DTYPE), (dict(rows=-1), SHAPE), (dict(rows=(1 << 30) + 1), SHAPE),
     (dict(rows=1 << 30, w="wide"), SHAPE), (dict(xs=255), SHAPE), (dict(x=None), ARG), (dict(y=None), ARG),
     (dict(x=P + 1), ARG), (dict(y=4 * FAR + 1), ARG), (dict(bias=P + 2), ARG),
-    (dict(dt=F32, rows=64), WORKSPACE), (dict(dt=F32, rows=64, ws=5 * FAR, wb=4 * 24704 - 1), WORKSPACE),
-    (dict(dt=F32, rows=64, ws=5 * FAR + 8, wb=4 * 24704), WORKSPACE),
+    (dict(dt=F32, rows=64), WORKSPACE), (dict(dt=F32, rows=64, ws=5 * FAR, wb=4 * 24832 - 1), WORKSPACE),
+    (dict(dt=F32, rows=64, ws=5 * FAR + 8, wb=4 * 24832), WORKSPACE),
     (dict(y=P + 2 * 256), ARG), (dict(y=FAR), ARG), (dict(y=2 * FAR), ARG), (dict(y=3 * FAR), ARG),
     (dict(bias=4 * FAR + 4), ARG),
-    (dict(dt=F32, rows=64, ws=P, wb=4 * 24704), ARG), (dict(dt=F32, rows=64, ws=4 * FAR, wb=4 * 24704), ARG),
+    (dict(dt=F32, rows=64, ws=P, wb=4 * 24832), ARG), (dict(dt=F32, rows=64, ws=4 * FAR, wb=4 * 24832), ARG),
 ])
 def test_linear_refusals(kw, code):
     if kw.get("w") == "wide":
@@ -162,9 +162,9 @@ def test_linear_of_nothing_and_workspace():
     assert linear(rows=0, x=None, y=None) == capi.APS_OK
     assert capi.lib().aps_linear_q4(P, 256, BF16, 1, None, None, P, None, 0, None) == ARG
     size = capi.lib().aps_linear_q4_workspace_size
-    # tiles of 16 rows: pieces of 256 inputs, three terms (bf16: one) of 8 KB, and 64 bytes of sums a group
-    assert size(weight(), 64, F32) == 4 * (3 * 8192 + 2 * 64) and size(weight(), 17, BF16) == 2 * (8192 + 2 * 64)
-    assert size(weight(in_features=384), 6, F32) == 2 * 3 * 8192 + 4 * 64
+    # tiles of 16 rows: pieces of 256 inputs, three terms (bf16: one) of 8 KB, and 64 bytes of sums a group (fp32: twice)
+    assert size(weight(), 64, F32) == 4 * (3 * 8192 + 2 * 128) and size(weight(), 17, BF16) == 2 * (8192 + 2 * 64)
+    assert size(weight(in_features=384), 6, F32) == 2 * 3 * 8192 + 4 * 128
     assert size(weight(), 16, BF16) == 0 and size(weight(), 5, F32) == 0 and size(weight(), 0, F32) == 0
     assert size(weight(in_features=16384), 16, BF16) == 64 * 8192 + 128 * 64     # x past what one CU holds
     assert size(weight(), -1, F32) == 0 and size(weight(group=3), 64, F32) == 0 and size(weight(), 64, 9) == 0
