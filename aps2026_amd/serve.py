@@ -500,7 +500,7 @@ def linear_q4_gpu(x: torch.Tensor, weight: Q4Weight, bias: Optional[torch.Tensor
         raise ValueError("linear_q4: fp32 or bf16 rows on the weight's device")
     stride, rows, n = _rows_of(x, weight.in_features, what), x.shape[0], weight.out_features
     if out is None:
-        out = torch.empty((rows, n), dtype=dt, device=dev)
+        out = torch.empty_strided((rows, n), (n, 1), dtype=dt, device=dev)   # (cheaper than empty)
     elif out.shape != (rows, n) or out.dtype is not dt or out.device != dev or not out.is_contiguous():
         raise ValueError("linear_q4: out [rows, out] of x's type, contiguous")
     bp = None
@@ -554,11 +554,14 @@ def token_logprobs_gpu(logits: torch.Tensor, tokens: Optional[torch.Tensor] = No
         if len(shape) not in (1, 2) or shape[0] != rows:
             raise ValueError("token_logprobs: tokens [rows] or [rows, n]")
         n, tp = (shape[1] if len(shape) == 2 else 1), _dev(tokens, dev, torch.int32, what)
-        logprobs = torch.empty(shape, dtype=torch.float32, device=dev)
+        logprobs = torch.empty_like(tokens, dtype=torch.float32)
         lp = logprobs.data_ptr()
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    top_ids = torch.empty((rows, max(top, 0)), dtype=torch.int32, device=dev)
-    top_logprobs = torch.empty((rows, max(top, 0)), dtype=torch.float32, device=dev)
+    if top < 0:
+        raise ValueError("token_logprobs: top is a number of tokens")
+    f32, wide = torch.float32, ((rows, top), (top, 1))
+    entropy = torch.empty(rows, dtype=f32, device=dev)
+    top_ids = torch.empty_strided(*wide, dtype=torch.int32, device=dev)   # (cheaper than empty)
+    top_logprobs = torch.empty_strided(*wide, dtype=f32, device=dev)
     lib = capi.lib()
     wp, wn = None, lib.aps_token_logprobs_workspace_size(rows, vocab, top, code)
     if wn:
