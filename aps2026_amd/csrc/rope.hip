@@ -11,14 +11,19 @@
 // Products and sums are fp32: results are off by about 2^-23 of the pair's norm.
 //
 // Bound by the bytes of q and k.  A thread computes the angles of its V pairs
-// once and turns them in several heads of the row, 16 bytes of each half at a
+// once and turns them in one or two heads of the row, 16 bytes of each half at a
 // time, so the trigonometry (some 30 instructions a pair) hides behind the loads.
+// 65536 bf16 rows of 20 heads of 128 take 116 us (5.8 TB/s; a large copy has
+// 4.9), 8192 rows of which half of each head turns 15.7, one row 3.3.
+#include <algorithm>
+
 #include "serve.hpp"
 
 namespace aps {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kCus = 256;
 constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -179,6 +184,13 @@ hipError_t launch(const RopeArgs& a, hipStream_t s) {
     const int heads = a.q_heads + a.k_heads, places = p.turning + p.still;
     p.spread = heads;
     p.rows_a_block = static_cast<int>(kThreads / (places * p.spread));
+    // Two heads a thread where one would give every CU a workgroup and more: 65536 rows
+    // 145 us with one, 116 with two (three 116, four 121), 8192 rows 21 and 15.7; 512
+    // rows 4.4 either way, 64 rows 3.75 with one and 4.1 with two.
+    if (a.rows > kCus * std::max(p.rows_a_block, 1)) {
+        p.spread = static_cast<int>(ceil_div(heads, 2));
+        p.rows_a_block = static_cast<int>(kThreads / (places * p.spread));
+    }
     if (p.rows_a_block < 1) p.rows_a_block = 1;
     const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, p.rows_a_block)));
     if (a.pairs) hipLaunchKernelGGL((k_rope<F32, V, true>), grid, dim3(kThreads), 0, s, a, p);

@@ -49,6 +49,10 @@ ROPE = [
     ("f32", 40, 40, 128, 2, "pairs", 4, "odd"),
     ("f32", 1, 1, 1024, 1024, "half", 3, "plain"),
     ("bf16", 16, 4, 128, 128, "pairs", 3000, "odd"),
+    # two heads a thread, of an odd number
+    ("bf16", 4, 1, 128, 128, "half", 1701, "in_place"),
+    ("f32", 40, 41, 128, 96, "half", 259, "plain"),
+    ("f32", 1, 0, 32, 32, "pairs", 16500, "no_k"),
 ]
 
 
