@@ -253,12 +253,17 @@ k_quantise_q4(const void* __restrict__ w, int64_t runs, int lanes, uint32_t* __r
 }
 
 // The waves side by side: as many as leave every CU a workgroup (4096 x 32064, one
-// row: 8 of them 18 us, 4 22, 16 30).  -1 where x is too large for this kernel.
+// row: 8 of them 15.7 us, 4 19.6, 16 23.7; 4096 x 6400: 2 7.3 us, 1 10.7, 4 9.1).
+// -1, the other kernels, where x is too large for this one, and with bf16 rows past
+// eight where x stays the longer part: a wave alone on its columns (16 rows on
+// 2048 x 4096: 8.9 us here, 7.5 there; 12 on 4096 x 4096 9.0 either way; on
+// 4096 x 8192 11.1 here, 12.1 there).  fp32 rows take 10 to 28 us there for 6 to 18.
 int few_columns(const Q4& w, int64_t rows, bool f32) {
     if (rows > (f32 ? kPackRows : 16)) return -1;
     const int64_t tiles = ceil_div(w.out, 16);
     int columns = 0;
     while (columns < 4 && 256 << columns < tiles) ++columns;
+    if (!f32 && rows > 8 && columns == 0) return -1;
     const FewLds l = few_lds(static_cast<int>(f32 ? 3 * rows : rows), w.in, w.group, 4 - columns, w.scales_f32);
     return l.x + l.sums + l.scales <= kLds ? columns : -1;
 }

@@ -21,6 +21,7 @@ namespace {
 using namespace q4;
 
 constexpr int kWaves = 8;
+constexpr int64_t kCus = 256;
 constexpr int kMany = 64 * kWaves;
 
 constexpr int piece_bytes(int terms) { return 8 * terms * 1024; }
@@ -341,11 +342,20 @@ hipError_t run(const LinearQ4Args& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Up to 16 rows: k_q4_wide past kWideOut outputs.  More: the largest tile whose
+// workgroups reach the CUs.  bf16 in us with tiles of 64 rows, 32, 16 (the last of 16
+// columns, the others of 32; 64 and 32 need 256 and 128 outputs a CU and row tile):
+//   64 rows on 8192 x 8192   25.2  27.4  37.9     64 rows on 4096 x 4096   15.1  12.0  15.6
+//   256 on 2048 x 4096       18.9  21.9  33.8     32 on 4096 x 4096        14.4  11.6  10.9
+// fp32, whose terms leave no room for 64 rows:
+//   64 rows on 4096 x 4096         25.8  27.4     17 on 4096 x 4096              24.6  17.0
 template <int GROUP, bool F32>
 hipError_t by_rows(const LinearQ4Args& a, hipStream_t s) {
-    if (a.rows <= 16) return a.w.out >= kWideOut ? run_wide<GROUP, F32>(a, s) : run<GROUP, F32, 1, 1>(a, s);
-    if constexpr (F32) return run<GROUP, F32, 2, 2>(a, s);
-    else return a.rows <= 32 ? run<GROUP, F32, 2, 2>(a, s) : run<GROUP, F32, 4, 2>(a, s);
+    if (a.rows <= 16 && a.w.out >= kWideOut) return run_wide<GROUP, F32>(a, s);
+    const auto fills = [&](int mt) { return a.rows > 8 * mt && ceil_div(a.rows, 16 * mt) * ceil_div(a.w.out, 32) >= kCus; };
+    if constexpr (!F32)
+        if (fills(4)) return run<GROUP, F32, 4, 2>(a, s);
+    return fills(2) ? run<GROUP, F32, 2, 2>(a, s) : run<GROUP, F32, 1, 1>(a, s);
 }
 
 }  // namespace

@@ -20,7 +20,7 @@
 //
 // Bound by the logits' bytes where workgroups are small enough that some load
 // while others compute (4096 x 32064 fp32: 178 us with one of 1024 threads on a
-// CU, 120 with four slices of 256).
+// CU, 98 with four slices of 256: 5.4 TB/s).
 #include "serve.hpp"
 
 namespace aps {
@@ -336,16 +336,23 @@ __global__ void __launch_bounds__(kWave) k_logprobs_join(LogprobArgs a, int slic
     write_row<F32>(a, row, all, best, tid, kWave);
 }
 
-// The slices of a row: T threads hold N accesses of 16 bytes.
+// The slices of a row: T threads hold kN accesses of 16 bytes.  256 threads, where
+// some load while others compute and nothing waits for the slowest of 16 waves, but
+// 1024 while no CU has two rows and that spares a row its second launch.  Rows of
+// 32064 fp32 in us, 1024 threads and 256: one row 8.4 and 8.7, 256 rows 10.7 and 13.6,
+// 300 rows 18.0 and 14.4; bf16, which need half as many slices: one row of 32064 11.0
+// and 9.5, 256 rows 12.4 and 12.3, 256 of 50000 13.4 and 17.6.  A row in one slice of
+// 256 threads takes 5.8 where 1024 take 8.1.
 struct Plan {
     int threads, slices;
 };
 constexpr int kN = 8;
-constexpr int64_t kFewRows = 64;
+constexpr int64_t kCus = 256;
 Plan plan_of(int64_t rows, int64_t vocab, bool f32) {
     const int64_t accesses = vocab / (f32 ? 4 : 8);
     auto slices = [&](int t) { return static_cast<int>(accesses > 0 ? ceil_div(accesses, int64_t(t) * kN) : 1); };
-    if ((rows < kFewRows && slices(1024) == 1) || slices(256) > kMaxSlices) return {1024, slices(1024)};
+    const bool one = rows <= kCus && slices(256) > (f32 ? 1 : 2) && slices(1024) == 1;
+    if (one || slices(256) > kMaxSlices) return {1024, slices(1024)};
     return {256, slices(256)};
 }
 
