@@ -214,7 +214,10 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
 // outputs each, which share x through LDS.  Two pieces of it (one for each of the
 // two shares of the inputs) are copied there while the two before are multiplied.
 // A wave that loaded x for itself would read 8 or 24 KB from L2 for every 2 KB of
-// codes (16 fp32 rows on 4096 x 32064: 47 us, even 64 outputs to a wave).
+// codes (16 fp32 rows on 4096 x 32064: 40 us, 30 here, of which 5 for putting x in
+// order).  What bounds it is neither HBM (15 us) nor copies (without them 2 us less)
+// but a round's own length, products after reads of LDS; two tiles of columns to a
+// wave, which halve those reads, measure the same (31).
 constexpr int kSide = 8, kWide = 1024, kWideOut = 16384;
 
 template <int GROUP, bool F32, bool SCALES32>
@@ -330,8 +333,19 @@ hipError_t run_wide(const LinearQ4Args& a, hipStream_t s) {
 template <int GROUP, bool F32, int MT, int NT>
 hipError_t run(const LinearQ4Args& a, hipStream_t s) {
     const int64_t pieces = ceil_div(a.w.in, kPiece);
+    // No wave without a piece; beyond that the columns whose rounds of workgroups take
+    // the least, in pieces: those of a wave and what a workgroup's start and end take.
+    // In us with 1, 2, 4, 8 waves side by side: 256 bf16 rows on 2048 x 4096 19.8, 15.9,
+    // 21.5, 32.1; 64 on 8192 x 8192 26.4, 34.3, 57, 102; 64 on 4096 x 32064 54.8, 42.1,
+    // 37.1, 60.6; 32 fp32 rows on 4096 x 12000 44.7, 40.5, 68.5, 122.
     int columns = 0;
     while (columns < 3 && (kWaves >> columns) > pieces) ++columns;
+    int64_t least = INT64_MAX;
+    for (int c = columns; c <= 3; ++c) {
+        const int64_t blocks = ceil_div(a.w.out, (16 * NT) << c) * ceil_div(a.rows, 16 * MT);
+        const int64_t cost = ceil_div(blocks, (MT > 1 ? 1 : 2) * kCus) * (ceil_div(pieces, kWaves >> c) + (F32 ? 1 : 2));
+        if (cost < least) least = cost, columns = c;
+    }
     const int64_t n_blocks = ceil_div(a.w.out, (16 * NT) << columns), m_blocks = ceil_div(a.rows, 16 * MT);
     const int64_t blocks = m_blocks > 1 ? ceil_div(n_blocks, 8) * 8 * m_blocks : n_blocks;
     if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
@@ -342,7 +356,9 @@ hipError_t run(const LinearQ4Args& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Up to 16 rows: k_q4_wide past kWideOut outputs.  More: the largest tile whose
+// Up to 16 rows: k_q4_wide past kWideOut outputs (16 fp32 rows on 4096 x 16384 27.0 us
+// there, 24.3 here; on 4096 x 20000 27.5 and 34.4; bf16 on 8192 x 16384 30.4 and 25.6,
+// on 8192 x 24000 33.3 and 41.5).  More rows: the largest tile whose
 // workgroups reach the CUs.  bf16 in us with tiles of 64 rows, 32, 16 (the last of 16
 // columns, the others of 32; 64 and 32 need 256 and 128 outputs a CU and row tile):
 //   64 rows on 8192 x 8192   25.2  27.4  37.9     64 rows on 4096 x 4096   15.1  12.0  15.6
@@ -351,7 +367,7 @@ hipError_t run(const LinearQ4Args& a, hipStream_t s) {
 //   64 rows on 4096 x 4096         25.8  27.4     17 on 4096 x 4096              24.6  17.0
 template <int GROUP, bool F32>
 hipError_t by_rows(const LinearQ4Args& a, hipStream_t s) {
-    if (a.rows <= 16 && a.w.out >= kWideOut) return run_wide<GROUP, F32>(a, s);
+    if (a.rows <= 16 && a.w.out > kWideOut) return run_wide<GROUP, F32>(a, s);
     const auto fills = [&](int mt) { return a.rows > 8 * mt && ceil_div(a.rows, 16 * mt) * ceil_div(a.w.out, 32) >= kCus; };
     if constexpr (!F32)
         if (fills(4)) return run<GROUP, F32, 4, 2>(a, s);

@@ -221,6 +221,13 @@ LINEAR = [
     ("f32", 9, 1312, 16390, 32, "f32", "small", True),      # x shared by waves side by side
     ("bf16", 12, 9088, 16385, 64, "bf16", "none", True),
     ("f32", 16, 224, 16500, 32, "bf16", "small", False),
+    ("bf16", 70, 288, 4210, 32, "bf16", "small", True),     # the larger tiles, where they fill the CUs
+    ("bf16", 33, 640, 8210, 64, "f32", "bytes", False),
+    ("bf16", 129, 2432, 2750, 128, "bf16", "none", True),
+    ("bf16", 20, 192, 8190, 64, "bf16", "small", True),
+    ("f32", 70, 416, 2745, 32, "bf16", "bytes", True),
+    ("f32", 33, 2304, 4100, 128, "f32", "small", False),
+    ("bf16", 9, 224, 60, 32, "bf16", "bytes", True),
 ]
 
 
@@ -415,6 +422,9 @@ LOGPROBS = [
     ("bf16", 1, 1 << 20, 3, 64, (0, 0)),
     ("f32", 600, 2053, 1, 3, (0, 0)),
     ("bf16", 300, 33000, 1, 7, (0, 1)),
+    ("f32", 256, 9001, 1, 12, (1, 0)),
+    ("f32", 257, 9001, 1, 12, (0, 2)),
+    ("bf16", 70, 40001, 2, 3, (0, 0)),
 ]
 
 
