@@ -12,7 +12,9 @@
 // LDS: waves beside each other have other inputs, not the same ones.
 //
 // Bound by those reads of x, 64 bytes a cycle and CU (64 rows on 8192 x 8192: 1 MB
-// for every 32 columns), and by the codes' bytes.
+// for every 32 columns, 6.8 us), and by the codes' bytes (7.6); a workgroup's start
+// and end take as long as one to two of its pieces, the first launch and the way to
+// the second 5 us: 24.3 in all, 353 TFLOP/s.
 #include "q4.hpp"
 
 namespace aps {
@@ -358,20 +360,25 @@ hipError_t run(const LinearQ4Args& a, hipStream_t s) {
 
 // Up to 16 rows: k_q4_wide past kWideOut outputs (16 fp32 rows on 4096 x 16384 27.0 us
 // there, 24.3 here; on 4096 x 20000 27.5 and 34.4; bf16 on 8192 x 16384 30.4 and 25.6,
-// on 8192 x 24000 33.3 and 41.5).  More rows: the largest tile whose
-// workgroups reach the CUs.  bf16 in us with tiles of 64 rows, 32, 16 (the last of 16
-// columns, the others of 32; 64 and 32 need 256 and 128 outputs a CU and row tile):
-//   64 rows on 8192 x 8192   25.2  27.4  37.9     64 rows on 4096 x 4096   15.1  12.0  15.6
-//   256 on 2048 x 4096       18.9  21.9  33.8     32 on 4096 x 4096        14.4  11.6  10.9
-// fp32, whose terms leave no room for 64 rows:
-//   64 rows on 4096 x 4096         25.8  27.4     17 on 4096 x 4096              24.6  17.0
+// on 8192 x 24000 33.3 and 41.5).  More rows: 16 rows by 16 columns a wave with fp32 x,
+// whose loads and products are thrice as many; with bf16 two or four times the rows and
+// twice the columns where enough workgroups are left for the CUs.  In us with 64, 32 and
+// 16 rows a tile, bf16:
+//   64 rows on 4096 x 32064   37.1  41.1  61.7     64 rows on 4096 x 4096   15.1  12.7  14.2
+//   256 on 2048 x 4096        15.4  15.6  18.4     64 rows on 8192 x 8192   25.1  24.0  30.7
+//   256 on 2048 x 2048        12.2  11.4  12.8     32 rows on 4096 x 1024   13.3  10.4   7.9
+// fp32 with 32 and 16:
+//   64 rows on 4096 x 4096           25.8  23.6     17 rows on 4096 x 4096        24.3  17.1
+//   256 on 2048 x 4096               42.9  37.3     32 rows on 4096 x 32064       73.8  67.1
 template <int GROUP, bool F32>
 hipError_t by_rows(const LinearQ4Args& a, hipStream_t s) {
     if (a.rows <= 16 && a.w.out > kWideOut) return run_wide<GROUP, F32>(a, s);
-    const auto fills = [&](int mt) { return a.rows > 8 * mt && ceil_div(a.rows, 16 * mt) * ceil_div(a.w.out, 32) >= kCus; };
-    if constexpr (!F32)
-        if (fills(4)) return run<GROUP, F32, 4, 2>(a, s);
-    return fills(2) ? run<GROUP, F32, 2, 2>(a, s) : run<GROUP, F32, 1, 1>(a, s);
+    if constexpr (!F32) {
+        const auto workgroups = [&](int mt) { return ceil_div(a.rows, 16 * mt) * ceil_div(a.w.out, 32); };
+        if (a.rows > 32 && workgroups(4) >= 2 * kCus) return run<GROUP, F32, 4, 2>(a, s);
+        if (a.rows > 16 && workgroups(2) >= kCus) return run<GROUP, F32, 2, 2>(a, s);
+    }
+    return run<GROUP, F32, 1, 1>(a, s);
 }
 
 }  // namespace

@@ -224,6 +224,9 @@ LINEAR = [
     ("bf16", 70, 288, 4210, 32, "bf16", "small", True),     # the larger tiles, where they fill the CUs
     ("bf16", 33, 640, 8210, 64, "f32", "bytes", False),
     ("bf16", 129, 2432, 2750, 128, "bf16", "none", True),
+    ("bf16", 36, 512, 16500, 32, "f32", "small", True),
+    ("bf16", 100, 1088, 8200, 64, "bf16", "bytes", True),
+    ("bf16", 40, 384, 16400, 128, "bf16", "none", False),
     ("bf16", 20, 192, 8190, 64, "bf16", "small", True),
     ("f32", 70, 416, 2745, 32, "bf16", "bytes", True),
     ("f32", 33, 2304, 4100, 128, "f32", "small", False),
