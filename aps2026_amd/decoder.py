@@ -437,7 +437,8 @@ class Model:
         a number, and of none but NaN and -inf id 0.  With logprobs also the
         chosen tokens' log probabilities, the entropies and so many likeliest
         tokens under those logits: a serve.TokenLogprobs of [batch]
-        [max_new_tokens] (and [logprobs]) tensors.  One host wait, at the end.  Caches and activations are the call's own, from torch's caching
+        [max_new_tokens] (and [logprobs]) tensors.  One host wait, at the end.
+        Caches and activations are the call's own, from torch's caching
         allocator: calls may run side by side on other streams."""
         if len(prompts) == 0:
             raise RuntimeError("generate_decode received an empty input batch")

@@ -68,10 +68,12 @@ typedef struct aps_q4_weight {
  * codes and then over the groups; y is rounded once.  A row with an infinity or a
  * NaN gives NaN where the formula may have an infinity.  Any alignment of x and y
  * to their elements (16-byte reads where x allows them).
- * Weights are read once for up to 64 rows, the codes once for each 64 rows more.
+ * The kernel, and with it the order of the sums and the last bits of a row, goes by
+ * the number of rows and the weight's sizes: a row alone and the same row in a batch
+ * may differ by that rounding.  Equal calls give equal bits.
  * rows * in_features and rows * out_features up to 2^38.
- * workspace: aps_linear_q4_workspace_size bytes (0: none), 16-byte aligned; calls
- * that overlap need one each.  y and workspace overlap nothing else of the call
+ * workspace: aps_linear_q4_workspace_size bytes (0 for few rows), 16-byte aligned;
+ * calls that overlap need one each.  y and workspace overlap nothing else of the call
  * (refused). */
 APS_API size_t aps_linear_q4_workspace_size(const aps_q4_weight* weight, int64_t rows, int32_t dtype);
 APS_API int aps_linear_q4(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, const aps_q4_weight* weight,
@@ -96,6 +98,8 @@ APS_API int aps_quantise_q4(const void* w, int32_t dtype, const aps_q4_weight* w
  * Logits of -inf (a mask's) have the probability 0 and the log probability -inf;
  * a row of nothing else has these for all, and the entropy 0.  A row with NaN or
  * +inf gives NaN (but its top_ids).  top up to 64 and vocab, vocab up to 2^20.
+ * The order of the sums goes by rows, vocab, dtype and where a row begins within 16
+ * bytes; equal calls on equally aligned rows give equal bits.
  * workspace: aps_token_logprobs_workspace_size bytes (0: none), 16-byte aligned;
  * calls that overlap need one each. */
 APS_API size_t aps_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int32_t top, int32_t dtype);

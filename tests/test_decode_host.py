@@ -165,7 +165,8 @@ def test_linear_of_nothing_and_workspace():
     # tiles of 16 rows: pieces of 256 inputs, three terms (bf16: one) of 8 KB, and 64 bytes of sums a group (fp32: twice)
     assert size(weight(), 64, F32) == 4 * (3 * 8192 + 2 * 128) and size(weight(), 17, BF16) == 2 * (8192 + 2 * 64)
     assert size(weight(in_features=384), 6, F32) == 2 * 3 * 8192 + 4 * 128
-    assert size(weight(), 16, BF16) == 0 and size(weight(), 5, F32) == 0 and size(weight(), 0, F32) == 0
+    assert size(weight(), 8, BF16) == 0 and size(weight(), 5, F32) == 0 and size(weight(), 0, F32) == 0
+    assert size(weight(out_features=4097), 16, BF16) == 0
     assert size(weight(in_features=16384), 16, BF16) == 64 * 8192 + 128 * 64     # x past what one CU holds
     assert size(weight(), -1, F32) == 0 and size(weight(group=3), 64, F32) == 0 and size(weight(), 64, 9) == 0
 
