@@ -13,7 +13,8 @@
 // 6e-7.
 //
 // fp32 x is the sum of three bf16 terms (8 bits each, cut off one after the
-// other), so its products are exact too.  Up to five rows have their terms below
+// other), so its products are exact too.  A group's sums are below
+// 128 (1 + 255 / 16) of its largest x: finite up to 2^116.  Up to five rows have their terms below
 // each other as rows of the matrix cores' 16.
 //
 // A lane loads 16 bytes, 32 codes of a row; the four lanes of a row hold 128

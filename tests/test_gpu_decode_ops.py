@@ -251,6 +251,20 @@ def test_linear_q4(gpu_device, dtype, rows, k, n, group, scales, zeros, bias):
         assert np.linalg.norm(f64(got) - want) <= 1e-6 * np.linalg.norm(want)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,k,n", [(1, 4096, 200), (16, 512, 16500), (70, 416, 4210)])
+def test_linear_q4_of_large_and_small_inputs(gpu_device, dtype, rows, k, n):
+    """A power of two on x scales every term, product and sum exactly, so it
+    scales the result's bits, up to the 2^116 that a group's sums allow."""
+    note(f"linear_q4 magnitudes {dtype} {rows} x {k} -> {n}")
+    dev, rng = gpu_device, np.random.default_rng(rows)
+    w, _ = q4_weight(n, k, 32, "f32", "bytes", dev, rng)
+    x = to_dev(rng.uniform(0.5, 2.0, (rows, k)) * rng.choice([-1.0, 1.0], (rows, k)), dev, TYPES[dtype])
+    plain = serve.linear_q4_gpu(x, w)
+    for e in (115, -60):
+        assert torch.equal(serve.linear_q4_gpu(x * 2.0 ** e, w).double(), plain.double() * 2.0 ** e)
+
+
 @pytest.mark.parametrize("dtype,rows,k,n,group,scales,zeros,bias", LINEAR)
 def test_linear_q4_exact(gpu_device, dtype, rows, k, n, group, scales, zeros, bias):
     """Small whole inputs and scales that are powers of two: every sum is exact
