@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kWide) k_q4_wide(LinearQ4Args a) {
     int block = 0, begin = first;
     auto step = [&](int round, const unsigned char* here, unsigned char* next, Held<1>& h) {
         const int piece = first + round;
-        // this round's copies, which were issued before the two loads of codes in flight
+        // the copies of these two pieces, which were issued before the two loads of codes in flight
         // (vmcnt 2, lgkmcnt 0; a fence would wait for those too)
         __builtin_amdgcn_s_waitcnt(0x0070 | 2);
         asm volatile("s_barrier" ::: "memory");
