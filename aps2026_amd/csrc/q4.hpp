@@ -142,7 +142,7 @@ __device__ inline u32x4 to_columns(u32x4 loaded, int lane) {
 //
 // The last piece, if it is not whole, covers the last 256 inputs (x is 0 there for
 // those that the piece before has); with fewer than 256 in all, a row's last codes
-// are read again in their place (x is 0 there too).
+// are read again in their place (x is 0 there too, and so are the scales).
 template <int NT, int GROUP, bool SCALES32>
 struct Columns {
     static constexpr int GROUPS = kPiece / GROUP, SIZE = SCALES32 ? 4 : 2, EACH = kBlock / 4;
@@ -184,7 +184,9 @@ struct Columns {
         const int group = first_group(piece);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int64_t at = scale_at[j] + group, left = static_cast<int64_t>(w.out) * (w.in / GROUP) - at;
+            // those that there are: of the weight, or of a short row
+            const int64_t at = scale_at[j] + group, end = static_cast<int64_t>(w.out) * (w.in / GROUP);
+            const int left = w.in < kPiece ? w.in / GROUP - EACH * (lane & 3) : static_cast<int>(min(end - at, static_cast<int64_t>(EACH)));
             const uint8_t* sp = static_cast<const uint8_t*>(w.scales) + at * SIZE;
             unsigned char* to = lds + (16 * j + (lane >> 2)) * ROW;
             unsigned char *scale_to = to + EACH * SIZE * (lane & 3), *zero_to = to + kBlock * SIZE + kPad + EACH * (lane & 3);
@@ -193,10 +195,12 @@ struct Columns {
                 if (w.zeros) *reinterpret_cast<Packed<EACH>*>(zero_to) = *reinterpret_cast<const Packed<EACH>*>(w.zeros + at);
             } else {
 #pragma unroll 1
-                for (int i = 0; i < left; ++i) {   // the weight's end
-                    if constexpr (SCALES32) reinterpret_cast<uint32_t*>(scale_to)[i] = reinterpret_cast<const uint32_t*>(sp)[i];
-                    else reinterpret_cast<uint16_t*>(scale_to)[i] = reinterpret_cast<const uint16_t*>(sp)[i];
-                    if (w.zeros) zero_to[i] = w.zeros[at + i];
+                for (int i = 0; i < EACH; ++i) {
+                    // x is 0 past them, and 0 has to be what it is multiplied with too: 0 times
+                    // an infinity or a NaN of the next rows, or of what LDS held, is not
+                    if constexpr (SCALES32) reinterpret_cast<uint32_t*>(scale_to)[i] = i < left ? reinterpret_cast<const uint32_t*>(sp)[i] : 0u;
+                    else reinterpret_cast<uint16_t*>(scale_to)[i] = i < left ? reinterpret_cast<const uint16_t*>(sp)[i] : uint16_t(0);
+                    if (w.zeros && i < left) zero_to[i] = w.zeros[at + i];
                 }
             }
         }

@@ -67,8 +67,9 @@ typedef struct aps_q4_weight {
  * contiguous of x's type.  Products are exact, sums are fp32, over each group's
  * codes and then over the groups; y is rounded once.  A row with an infinity or a
  * NaN gives NaN where the formula may have an infinity, and so may one with a
- * magnitude past 2^116, of which a group's sum need not be finite.  Any alignment of x and y
- * to their elements (16-byte reads where x allows them).
+ * magnitude past 2^116, of which a group's sum need not be finite.  A scale that is
+ * not finite makes its own output's values NaN or infinite, and no other's.  Any
+ * alignment of x and y to their elements (16-byte reads where x allows them).
  * The kernel, and with it the order of the sums and the last bits of a row, goes by
  * the number of rows and the weight's sizes: a row alone and the same row in a batch
  * may differ by that rounding.  Equal calls give equal bits.
