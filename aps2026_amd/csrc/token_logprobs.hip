@@ -21,6 +21,8 @@
 // Bound by the logits' bytes where workgroups are small enough that some load
 // while others compute (4096 x 32064 fp32: 178 us with one of 1024 threads on a
 // CU, 98 with four slices of 256: 5.4 TB/s).
+#include <algorithm>
+
 #include "serve.hpp"
 
 namespace aps {
@@ -363,6 +365,15 @@ void slice(const LogprobArgs& a, int slices, hipStream_t s) {
     hipLaunchKernelGGL((k_logprobs<F32, T, kN>), dim3(static_cast<unsigned>(a.rows * slices)), dim3(T), 0, s, a, slices);
 }
 
+template <bool F32>
+hipError_t run(const LogprobArgs& a, Plan p, hipStream_t s) {
+    if (p.threads == 1024) slice<F32, 1024>(a, p.slices, s);
+    else slice<F32, 256>(a, p.slices, s);
+    if (p.slices > 1)
+        hipLaunchKernelGGL(k_logprobs_join<F32>, dim3(static_cast<unsigned>(a.rows)), dim3(kWave), 0, s, a, p.slices);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 int64_t token_logprobs_blocks(int64_t rows, int64_t vocab, bool f32) { return rows * plan_of(rows, vocab, f32).slices; }
@@ -375,19 +386,17 @@ size_t token_logprobs_part_bytes(int64_t rows, int64_t vocab, int top, bool f32)
 hipError_t launch_token_logprobs(const LogprobArgs& a, bool f32, hipStream_t s) {
     if (a.rows <= 0) return hipSuccess;
     const Plan p = plan_of(a.rows, a.vocab, f32);
-    if (f32) {
-        if (p.threads == 1024) slice<true, 1024>(a, p.slices, s);
-        else slice<true, 256>(a, p.slices, s);
-    } else {
-        if (p.threads == 1024) slice<false, 1024>(a, p.slices, s);
-        else slice<false, 256>(a, p.slices, s);
+    const int64_t most = most_blocks(p.threads) / p.slices;
+    for (int64_t first = 0; first < a.rows; first += most) {   // the workspace serves one launch's rows after the other's
+        LogprobArgs part = a;
+        part.rows = std::min(most, a.rows - first);
+        part.x = static_cast<const char*>(a.x) + first * a.x_stride * (f32 ? 4 : 2);
+        if (a.n_tokens > 0) part.tokens = a.tokens + first * a.n_tokens, part.logprobs = a.logprobs + first * a.n_tokens;
+        if (a.entropy) part.entropy = a.entropy + first;
+        if (a.top > 0) part.top_ids = a.top_ids + first * a.top, part.top_logprobs = a.top_logprobs + first * a.top;
+        if (const hipError_t e = f32 ? run<true>(part, p, s) : run<false>(part, p, s); e != hipSuccess) return e;
     }
-    if (p.slices > 1) {
-        const dim3 grid(static_cast<unsigned>(a.rows));
-        if (f32) hipLaunchKernelGGL(k_logprobs_join<true>, grid, dim3(kWave), 0, s, a, p.slices);
-        else hipLaunchKernelGGL(k_logprobs_join<false>, grid, dim3(kWave), 0, s, a, p.slices);
-    }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace aps
