@@ -192,10 +192,24 @@ hipError_t launch(const RopeArgs& a, hipStream_t s) {
         p.rows_a_block = static_cast<int>(kThreads / (places * p.spread));
     }
     if (p.rows_a_block < 1) p.rows_a_block = 1;
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, p.rows_a_block)));
-    if (a.pairs) hipLaunchKernelGGL((k_rope<F32, V, true>), grid, dim3(kThreads), 0, s, a, p);
-    else hipLaunchKernelGGL((k_rope<F32, V, false>), grid, dim3(kThreads), 0, s, a, p);
-    return hipGetLastError();
+    const int64_t most = most_blocks(kThreads) * p.rows_a_block;
+    for (int64_t first = 0; first < a.rows; first += most) {
+        constexpr int64_t kSize = F32 ? 4 : 2;
+        RopeArgs part = a;
+        part.rows = std::min(most, a.rows - first);
+        part.positions += first;
+        part.q = static_cast<const char*>(a.q) + first * a.q_stride * kSize;
+        part.q_out = static_cast<char*>(a.q_out) + first * a.q_out_stride * kSize;
+        if (a.k_heads > 0) {
+            part.k = static_cast<const char*>(a.k) + first * a.k_stride * kSize;
+            part.k_out = static_cast<char*>(a.k_out) + first * a.k_out_stride * kSize;
+        }
+        const dim3 grid(static_cast<unsigned>(ceil_div(part.rows, p.rows_a_block)));
+        if (a.pairs) hipLaunchKernelGGL((k_rope<F32, V, true>), grid, dim3(kThreads), 0, s, part, p);
+        else hipLaunchKernelGGL((k_rope<F32, V, false>), grid, dim3(kThreads), 0, s, part, p);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -215,9 +229,15 @@ hipError_t launch_rope(const RopeArgs& a, bool f32, hipStream_t s) {
 hipError_t launch_rope_table(const double* freq, int pairs, int64_t first, int64_t count, float amplitude,
                              float* cosv, float* sinv, hipStream_t s) {
     if (count <= 0 || pairs <= 0) return hipSuccess;
-    const dim3 grid(static_cast<unsigned>(ceil_div(count * pairs, kThreads)));
-    hipLaunchKernelGGL(k_rope_table, grid, dim3(kThreads), 0, s, freq, pairs, first, count, amplitude, cosv, sinv);
-    return hipGetLastError();
+    const int64_t most = most_blocks(kThreads) * kThreads / pairs;   // positions of a launch
+    for (int64_t at = 0; at < count; at += most) {
+        const int64_t n = std::min(most, count - at);
+        const dim3 grid(static_cast<unsigned>(ceil_div(n * pairs, kThreads)));
+        hipLaunchKernelGGL(k_rope_table, grid, dim3(kThreads), 0, s, freq, pairs, first + at, n, amplitude,
+                           cosv + at * pairs, sinv + at * pairs);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace aps

@@ -48,3 +48,26 @@ def test_logprobs_of_many_rows(gpu_device):
     got = serve.token_logprobs_gpu(repeated(few, rows), repeated(tokens, rows), 2)
     for g, w in zip(got, want):
         assert_repeats(g, w)
+
+
+def test_rope_of_many_rows(gpu_device):
+    """Rows of which each fills a workgroup: 514 values, two to a thread."""
+    rows = (1 << 24) + 3
+    note(f"rope of {rows} rows")
+    few = torch.randn(1009, 514, device=gpu_device).to(BF16)
+    pos = torch.randint(-1, 1 << 20, (1009,), dtype=torch.int32, device=gpu_device)
+    freq = torch.ones(1, dtype=torch.float64, device=gpu_device)
+    want, _ = serve.rope_gpu(few, None, pos, freq, 514)
+    x = repeated(few, rows)
+    got, _ = serve.rope_gpu(x, None, repeated(pos, rows), freq, 514, q_out=x)
+    assert_repeats(got, want)
+
+
+def test_rope_table_of_many_positions(gpu_device):
+    count, pairs = (1 << 23) + 2, 512
+    note(f"rope table of {count} positions")
+    freq = torch.from_numpy(serve.rope_frequencies(2 * pairs)[0]).to(gpu_device)
+    for got, name in zip(serve.rope_table_gpu(freq, count, 1.5), (0, 1)):
+        for first in (0, (1 << 23) - 2, (1 << 23) - 1, (1 << 23)):
+            n = min(5, count - first)
+            assert torch.equal(got[first:first + n], serve.rope_table_gpu(freq, n, 1.5, first)[name]), first
