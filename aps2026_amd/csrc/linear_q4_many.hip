@@ -15,6 +15,8 @@
 // for every 32 columns, 6.8 us), and by the codes' bytes (7.6); a workgroup's start
 // and end take as long as one to two of its pieces, the first launch and the way to
 // the second 5 us: 24.3 in all, 353 TFLOP/s.
+#include <algorithm>
+
 #include "q4.hpp"
 
 namespace aps {
@@ -36,9 +38,9 @@ __host__ __device__ inline int64_t sums_at(int64_t rows, int in, int terms) {
 // A wave to a group of 16 rows: lane (row, quarter) takes runs of 8 inputs, 32 of
 // them apart, all of them loaded before the first is used.
 template <bool F32, int GROUP>
-__global__ void __launch_bounds__(256) k_q4_arrange(LinearQ4Args a, int64_t waves) {
+__global__ void __launch_bounds__(256) k_q4_arrange(LinearQ4Args a, int64_t first_wave, int64_t waves) {
     constexpr int TERMS = F32 ? 3 : 1, STEPS = GROUP / 32;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
+    const int64_t at = first_wave + static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
     if (at >= waves) return;
     const int lane = threadIdx.x & 63, q = lane >> 4, in = a.w.in, groups = all_groups(in, GROUP);
     const int64_t tile = at / groups;
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(256) k_q4_arrange(LinearQ4Args a, int64_t wave
 // 2^columns of a workgroup's waves lie side by side, 16 NT outputs each; the others
 // share the inputs, a run of pieces each.
 template <int GROUP, bool F32, int MT, int NT, bool SCALES32>
-__global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, int n_blocks, int m_blocks) {
+__global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, int n_blocks, int first_m, int m_blocks) {
     constexpr int GROUPS = kPiece / GROUP, STEPS = GROUP / 32, TERMS = F32 ? 3 : 1, BLOCK = kBlock / GROUPS;
     using Weight = Columns<NT, GROUP, SCALES32>;
     // a wave's scales and zeros, and its rows' sums: [tile][group of the block][row]
@@ -99,11 +101,11 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
     const int tid = threadIdx.x, wave = tid / 64, lane = tid & 63, q = lane >> 4;
     const int wn = wave & ((1 << columns) - 1), wk = wave >> columns, log_turns = 3 - columns;
     // blocks of the same columns on one XCD (workgroups go round the eight)
-    int nb = blockIdx.x, mb = 0;
+    int nb = blockIdx.x, mb = first_m;
     if (m_blocks > 1) {
         const int turn = blockIdx.x / 8;
         nb = (turn / m_blocks) * 8 + (blockIdx.x & 7);
-        mb = turn % m_blocks;
+        mb += turn % m_blocks;
         if (nb >= n_blocks) return;
     }
     const int in = a.w.in, pieces = (in + kPiece - 1) / kPiece, rounds = (pieces + (1 << log_turns) - 1) >> log_turns;
@@ -349,13 +351,15 @@ hipError_t run(const LinearQ4Args& a, hipStream_t s) {
         if (cost < least) least = cost, columns = c;
     }
     const int64_t n_blocks = ceil_div(a.w.out, (16 * NT) << columns), m_blocks = ceil_div(a.rows, 16 * MT);
-    const int64_t blocks = m_blocks > 1 ? ceil_div(n_blocks, 8) * 8 * m_blocks : n_blocks;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks)), block(kMany);
-    const int n = static_cast<int>(n_blocks), m = static_cast<int>(m_blocks);
-    if (a.w.scales_f32) hipLaunchKernelGGL((k_q4_many<GROUP, F32, MT, NT, true>), grid, block, 0, s, a, columns, n, m);
-    else hipLaunchKernelGGL((k_q4_many<GROUP, F32, MT, NT, false>), grid, block, 0, s, a, columns, n, m);
-    return hipGetLastError();
+    const int64_t across = ceil_div(n_blocks, 8) * 8, most = most_blocks(kMany) / across;
+    for (int64_t first = 0; first < m_blocks; first += most) {
+        const int n = static_cast<int>(n_blocks), f = static_cast<int>(first), m = static_cast<int>(std::min(most, m_blocks - first));
+        const dim3 grid(static_cast<unsigned>(m > 1 ? across * m : n_blocks)), block(kMany);
+        if (a.w.scales_f32) hipLaunchKernelGGL((k_q4_many<GROUP, F32, MT, NT, true>), grid, block, 0, s, a, columns, n, f, m);
+        else hipLaunchKernelGGL((k_q4_many<GROUP, F32, MT, NT, false>), grid, block, 0, s, a, columns, n, f, m);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // Up to 16 rows: k_q4_wide past kWideOut outputs (16 fp32 rows on 4096 x 16384 27.0 us
@@ -389,12 +393,13 @@ size_t q4_many_bytes(const Q4& w, int64_t rows, bool f32) {
 
 template <int GROUP>
 static hipError_t launch(const LinearQ4Args& a, bool f32, hipStream_t s) {
-    const int64_t waves = ceil_div(a.rows, 16) * all_groups(a.w.in, GROUP), blocks = ceil_div(waves, 4);
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (f32) hipLaunchKernelGGL((k_q4_arrange<true, GROUP>), grid, dim3(256), 0, s, a, waves);
-    else hipLaunchKernelGGL((k_q4_arrange<false, GROUP>), grid, dim3(256), 0, s, a, waves);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const int64_t waves = ceil_div(a.rows, 16) * all_groups(a.w.in, GROUP), most = most_blocks(256) * 4;
+    for (int64_t first = 0; first < waves; first += most) {
+        const dim3 grid(static_cast<unsigned>(ceil_div(std::min(most, waves - first), 4)));
+        if (f32) hipLaunchKernelGGL((k_q4_arrange<true, GROUP>), grid, dim3(256), 0, s, a, first, waves);
+        else hipLaunchKernelGGL((k_q4_arrange<false, GROUP>), grid, dim3(256), 0, s, a, first, waves);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
     return f32 ? by_rows<GROUP, true>(a, s) : by_rows<GROUP, false>(a, s);
 }
 

@@ -71,3 +71,18 @@ def test_rope_table_of_many_positions(gpu_device):
         for first in (0, (1 << 23) - 2, (1 << 23) - 1, (1 << 23)):
             n = min(5, count - first)
             assert torch.equal(got[first:first + n], serve.rope_table_gpu(freq, n, 1.5, first)[name]), first
+
+
+@pytest.mark.parametrize("dtype,rows", [(F32, (1 << 24) + 40), (BF16, (1 << 27) + 40)])
+def test_linear_q4_of_many_rows(gpu_device, dtype, rows):
+    """Whole inputs and scales of 1: every result is exact.  bf16: past what a launch
+    that puts x in order holds too."""
+    note(f"linear_q4 of {rows} rows")
+    dev, rng = gpu_device, np.random.default_rng(rows)
+    codes = rng.integers(0, 256, (1, 16), dtype=np.uint8)
+    w = serve.Q4Weight(torch.from_numpy(codes).to(dev), torch.ones(1, 1, device=dev))
+    few = rng.integers(-2, 3, (1013, 32)).astype(np.float32)
+    values = np.stack((codes & 15, codes >> 4), -1).reshape(32).astype(np.float32) - 8
+    want = torch.from_numpy(few @ values[:, None]).to(dev, dtype)   # whole and below 2^9: bf16's 8 bits round once
+    got = serve.linear_q4_gpu(repeated(torch.from_numpy(few).to(dev, dtype), rows), w)
+    assert_repeats(got, want)
