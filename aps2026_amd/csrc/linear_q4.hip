@@ -24,6 +24,8 @@
 // (i, i + 4); x is put in the same order.
 //
 // Bound by the codes' bytes up to some 64 rows, with short launches' fixed 4 us.
+#include <algorithm>
+
 #include "q4.hpp"
 
 namespace aps {
@@ -295,19 +297,29 @@ hipError_t launch_linear_q4(const LinearQ4Args& a, bool f32, hipStream_t s) {
     return f32 ? run_few<128, true>(a, columns, s) : run_few<128, false>(a, columns, s);
 }
 
+template <bool F32, bool ZEROS>
+static void quantise(const void* w, int64_t runs, int lanes, uint32_t* codes, void* scales, bool scales_f32,
+                     uint8_t* zeros, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(runs, 256))), block(256);
+    hipLaunchKernelGGL((k_quantise_q4<F32, ZEROS>), grid, block, 0, s, w, runs, lanes, codes, scales, scales_f32, zeros);
+}
+
 hipError_t launch_quantise_q4(const void* w, bool w_f32, int64_t out, int in, int group, uint8_t* codes,
                               void* scales, bool scales_f32, uint8_t* zeros, hipStream_t s) {
-    const int64_t runs = out * (in / 8), blocks = ceil_div(runs, 256);
-    if (runs <= 0) return hipSuccess;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks)), block(256);
-    uint32_t* to = reinterpret_cast<uint32_t*>(codes);
     const int lanes = group / 8;
-    if (w_f32 && zeros) hipLaunchKernelGGL((k_quantise_q4<true, true>), grid, block, 0, s, w, runs, lanes, to, scales, scales_f32, zeros);
-    else if (w_f32) hipLaunchKernelGGL((k_quantise_q4<true, false>), grid, block, 0, s, w, runs, lanes, to, scales, scales_f32, zeros);
-    else if (zeros) hipLaunchKernelGGL((k_quantise_q4<false, true>), grid, block, 0, s, w, runs, lanes, to, scales, scales_f32, zeros);
-    else hipLaunchKernelGGL((k_quantise_q4<false, false>), grid, block, 0, s, w, runs, lanes, to, scales, scales_f32, zeros);
-    return hipGetLastError();
+    const int64_t runs = out * (in / 8), most = most_blocks(256) * 256;   // whole groups to a launch
+    for (int64_t first = 0; first < runs; first += most) {
+        const int64_t n = std::min(most, runs - first), groups = first / lanes;
+        const void* from = static_cast<const char*>(w) + first * (w_f32 ? 32 : 16);
+        uint32_t* to = reinterpret_cast<uint32_t*>(codes) + first;
+        void* sc = static_cast<char*>(scales) + groups * (scales_f32 ? 4 : 2);
+        if (w_f32 && zeros) quantise<true, true>(from, n, lanes, to, sc, scales_f32, zeros + groups, s);
+        else if (w_f32) quantise<true, false>(from, n, lanes, to, sc, scales_f32, nullptr, s);
+        else if (zeros) quantise<false, true>(from, n, lanes, to, sc, scales_f32, zeros + groups, s);
+        else quantise<false, false>(from, n, lanes, to, sc, scales_f32, nullptr, s);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace aps

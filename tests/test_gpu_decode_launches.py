@@ -86,3 +86,13 @@ def test_linear_q4_of_many_rows(gpu_device, dtype, rows):
     want = torch.from_numpy(few @ values[:, None]).to(dev, dtype)   # whole and below 2^9: bf16's 8 bits round once
     got = serve.linear_q4_gpu(repeated(torch.from_numpy(few).to(dev, dtype), rows), w)
     assert_repeats(got, want)
+
+
+def test_quantise_q4_of_a_large_weight(gpu_device):
+    n, k = (1 << 21) + 1, 1 << 14
+    note(f"quantise_q4 of {n} x {k}")
+    few = torch.randn(61, k, device=gpu_device).to(BF16)
+    want = serve.quantise_q4_gpu(few, 128)
+    got = serve.quantise_q4_gpu(repeated(few, n), 128)
+    for name in ("codes", "scales", "zeros"):
+        assert_repeats(getattr(got, name), getattr(want, name))
