@@ -1355,6 +1355,12 @@ Plan plan(const KvCache& c, const PagedArgs& a) {
     return p;
 }
 
+// The waves that join a row's parts.
+// (us of the call with a wave a row / four: 16 x 8192 keys, 8 parts, 45.5 / 46.4;
+// with four / sixteen: 1 x 131072, 128 parts, 47.6 / 47.0, 1 x 20000, 79 parts,
+// 16.5 / 15.9)
+int join_waves(const PagedDev& d) { return d.splits > 64 ? 16 : d.splits > kFewSplits ? 4 : 1; }
+
 template <int D, bool Q32, Kv KV>
 hipError_t launch(const PagedDev& d, hipStream_t s) {
     const dim3 blocks(static_cast<unsigned>(d.blocks)), grid(static_cast<unsigned>(d.slots * d.a.q_heads));
@@ -1366,11 +1372,8 @@ hipError_t launch(const PagedDev& d, hipStream_t s) {
     else
         hipLaunchKernelGGL((k_paged_rows<D, Q32, KV, false>), blocks, dim3(64 * d.waves),
                            static_cast<unsigned>(d.waves) * d.lds_rows * (D + 4) * 4, s, d);
-    // (us of the call with a wave a row / four: 16 x 8192 keys, 8 parts, 45.5 / 46.4;
-    // with four / sixteen: 1 x 131072, 128 parts, 47.6 / 47.0, 1 x 20000, 79 parts,
-    // 16.5 / 15.9)
-    if (d.splits > 64) hipLaunchKernelGGL((k_paged_join<D, Q32, 16>), grid, dim3(1024), 0, s, d);
-    else if (d.splits > kFewSplits) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
+    if (d.splits > 1 && join_waves(d) == 16) hipLaunchKernelGGL((k_paged_join<D, Q32, 16>), grid, dim3(1024), 0, s, d);
+    else if (d.splits > 1 && join_waves(d) == 4) hipLaunchKernelGGL((k_paged_join<D, Q32, 4>), grid, dim3(256), 0, s, d);
     else if (d.splits > 1) hipLaunchKernelGGL((k_paged_join<D, Q32, 1>), grid, dim3(64), 0, s, d);
     return hipGetLastError();
 }
@@ -1385,11 +1388,13 @@ hipError_t launch_d(const PagedDev& d, bool q_f32, hipStream_t s) {
 
 }  // namespace
 
-int64_t attention_paged_blocks(const KvCache& cache, const PagedArgs& a) {
+int64_t attention_paged_threads(const KvCache& cache, const PagedArgs& a) {
     const Plan p = plan(cache, a);
     int64_t n = 0;
-    for (int i = 0; i < p.n; ++i)
-        n = std::max({n, p.d[i].blocks, p.d[i].splits > 1 ? p.d[i].slots * a.q_heads : 0});
+    for (int i = 0; i < p.n; ++i) {
+        const PagedDev& d = p.d[i];
+        n = std::max({n, d.blocks * 64 * (d.tiled ? kWaves : d.waves), d.splits > 1 ? d.slots * a.q_heads * 64 * join_waves(d) : 0});
+    }
     return n;
 }
 

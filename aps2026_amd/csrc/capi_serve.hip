@@ -86,8 +86,9 @@ int check_paged(const aps::KvCache& c, int64_t rows, int32_t q_heads, int64_t ba
         return fail(APS_ERR_SHAPE, "%s: %lld rows under a key head", what,
                     (long long)(a->max_q_len * (q_heads / c.kv_heads)));
     if (rows == 0 || batch == 0 || a->max_q_len == 0) return APS_OK;
-    const int64_t blocks = aps::attention_paged_blocks(c, *a);
-    if (blocks > 0x7FFFFFFF) return fail(APS_ERR_SHAPE, "%s: %lld workgroups", what, (long long)blocks);
+    const int64_t threads = aps::attention_paged_threads(c, *a);
+    if (threads > aps::most_blocks(1))
+        return fail(APS_ERR_SHAPE, "%s: workgroups of %lld threads in one launch", what, (long long)threads);
     return APS_OK;
 }
 

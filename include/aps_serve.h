@@ -95,7 +95,7 @@ APS_API int aps_kv_gather(const aps_kv_cache* cache, const int64_t* slots, int64
  * (batch - 1) max_q_len + 32 / (q_heads / kv_heads): no room but for padding.)
  *
  * All arrays in device memory; q_offsets ascend; batch up to 2^20, max_kv_len up
- * to 2^30 (sizes that take more than 2^31 - 1 workgroups are refused).  max_q_len
+ * to 2^30 (sizes that take 2^32 threads and more in a launch are refused).  max_q_len
  * and max_kv_len bound the batch's lengths on the host (they shape the launch, so a
  * recorded graph serves any lengths within them): queries past max_q_len of a
  * sequence are left as they were, lengths past max_kv_len or past table_stride
