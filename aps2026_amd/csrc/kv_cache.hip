@@ -13,6 +13,8 @@
 // D / 16 threads take one head of one row, 8 values of each half: 16-byte
 // accesses (bf16), both halves of every pair in one thread, and the 32 values
 // of a 4-bit block in four neighbouring lanes.
+#include <algorithm>
+
 #include "serve.hpp"
 
 namespace aps {
@@ -191,20 +193,33 @@ void append(const KvCache& c, const KvAppendArgs& a, unsigned blocks, bool vec, 
 }
 
 template <int D>
-hipError_t append_d(const KvCache& c, const KvAppendArgs& a, bool src_f32, hipStream_t s) {
-    const int64_t blocks = ceil_div(a.rows * (2 * c.kv_heads + a.q_heads) * (D / 16), kThreads);
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const unsigned n = static_cast<unsigned>(blocks);
+hipError_t append_d(const KvCache& c, const KvAppendArgs& all, bool src_f32, hipStream_t s) {
     const int64_t per = src_f32 ? 4 : 8;  // elements of 16 bytes
-    const bool vec = aligned16(a.k) && aligned16(a.v) && aligned16(a.q) && aligned16(a.q_out) && aligned16(a.cosv) &&
-                     aligned16(a.sinv) && a.k_stride % per == 0 && a.v_stride % per == 0 &&
-                     (a.q_heads == 0 || (a.q_stride % per == 0 && a.q_out_stride % per == 0));
-    if (c.type == Kv::kF32) append<D, true, Kv::kF32>(c, a, n, vec, s);
-    else if (c.type == Kv::kBf16 && src_f32) append<D, true, Kv::kBf16>(c, a, n, vec, s);
-    else if (c.type == Kv::kBf16) append<D, false, Kv::kBf16>(c, a, n, vec, s);
-    else if (src_f32) append<D, true, Kv::kMx>(c, a, n, vec, s);
-    else append<D, false, Kv::kMx>(c, a, n, vec, s);
-    return hipGetLastError();
+    const bool vec = aligned16(all.k) && aligned16(all.v) && aligned16(all.q) && aligned16(all.q_out) &&
+                     aligned16(all.cosv) && aligned16(all.sinv) && all.k_stride % per == 0 && all.v_stride % per == 0 &&
+                     (all.q_heads == 0 || (all.q_stride % per == 0 && all.q_out_stride % per == 0));
+    const int64_t threads = static_cast<int64_t>(2 * c.kv_heads + all.q_heads) * (D / 16);   // of a row
+    const int64_t most = most_blocks(kThreads) * kThreads / threads, size = src_f32 ? 4 : 2;
+    for (int64_t first = 0; first < all.rows; first += most) {
+        KvAppendArgs a = all;
+        a.rows = std::min(most, all.rows - first);
+        a.positions += first;
+        a.slots += first;
+        a.k = static_cast<const char*>(all.k) + first * all.k_stride * size;
+        a.v = static_cast<const char*>(all.v) + first * all.v_stride * size;
+        if (all.q_heads > 0) {
+            a.q = static_cast<const char*>(all.q) + first * all.q_stride * size;
+            a.q_out = static_cast<char*>(all.q_out) + first * all.q_out_stride * size;
+        }
+        const unsigned n = static_cast<unsigned>(ceil_div(a.rows * threads, kThreads));
+        if (c.type == Kv::kF32) append<D, true, Kv::kF32>(c, a, n, vec, s);
+        else if (c.type == Kv::kBf16 && src_f32) append<D, true, Kv::kBf16>(c, a, n, vec, s);
+        else if (c.type == Kv::kBf16) append<D, false, Kv::kBf16>(c, a, n, vec, s);
+        else if (src_f32) append<D, true, Kv::kMx>(c, a, n, vec, s);
+        else append<D, false, Kv::kMx>(c, a, n, vec, s);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 template <int D, Kv KV>
@@ -215,14 +230,20 @@ void gather(const KvCache& c, const int64_t* slots, int64_t rows, void* k, void*
 }
 
 template <int D>
-hipError_t gather_d(const KvCache& c, const int64_t* slots, int64_t rows, void* k, void* v, bool f32, hipStream_t s) {
-    const int64_t blocks = ceil_div(rows * c.kv_heads * (D / 8), kThreads);
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const unsigned n = static_cast<unsigned>(blocks);
-    if (c.type == Kv::kF32) gather<D, Kv::kF32>(c, slots, rows, k, v, f32, n, s);
-    else if (c.type == Kv::kBf16) gather<D, Kv::kBf16>(c, slots, rows, k, v, f32, n, s);
-    else gather<D, Kv::kMx>(c, slots, rows, k, v, f32, n, s);
-    return hipGetLastError();
+hipError_t gather_d(const KvCache& c, const int64_t* slots, int64_t all, void* k_out, void* v_out, bool f32, hipStream_t s) {
+    const int64_t threads = static_cast<int64_t>(c.kv_heads) * (D / 8);   // of a row
+    const int64_t most = most_blocks(kThreads) * kThreads / threads, bytes = static_cast<int64_t>(c.kv_heads) * D * (f32 ? 4 : 2);
+    for (int64_t first = 0; first < all; first += most, slots += most) {
+        const int64_t rows = std::min(most, all - first);
+        void* k = k_out ? static_cast<char*>(k_out) + first * bytes : nullptr;
+        void* v = v_out ? static_cast<char*>(v_out) + first * bytes : nullptr;
+        const unsigned n = static_cast<unsigned>(ceil_div(rows * threads, kThreads));
+        if (c.type == Kv::kF32) gather<D, Kv::kF32>(c, slots, rows, k, v, f32, n, s);
+        else if (c.type == Kv::kBf16) gather<D, Kv::kBf16>(c, slots, rows, k, v, f32, n, s);
+        else gather<D, Kv::kMx>(c, slots, rows, k, v, f32, n, s);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace

@@ -9,6 +9,8 @@
 // whatever the order.  Then it passes over the slice's logits once.  Bound by
 // the logits' bytes; every slice reads the whole history, from L2 after the
 // first.
+#include <algorithm>
+
 #include "serve.hpp"
 
 namespace aps {
@@ -159,6 +161,30 @@ k_logits_process(LogitsArgs a, uint32_t slices, uint32_t deal) {
     }
 }
 
+// `rows` of the rows from `first` on.
+LogitsArgs rows_from(LogitsArgs a, int64_t first, int64_t rows, int64_t size) {
+    auto skip = [&](auto& p, int64_t values) { if (p) p += first * values; };
+    a.rows = rows;
+    a.x = static_cast<const char*>(a.x) + first * a.x_stride * size;
+    a.out = static_cast<char*>(a.out) + first * a.out_stride * size;
+    skip(a.history, a.history_stride);
+    skip(a.history_lens, 1);
+    skip(a.prompt_lens, 1);
+    skip(a.repetition, 1);
+    skip(a.frequency, 1);
+    skip(a.presence, 1);
+    skip(a.bias_ids, a.bias_stride);
+    skip(a.bias_values, a.bias_stride);
+    skip(a.bias_lens, 1);
+    if (a.mask_index) {
+        a.mask_index += first;
+    } else if (a.mask) {
+        a.mask += first * a.mask_stride;
+        a.mask_rows -= first;
+    }
+    return a;
+}
+
 template <bool F32, int SLICE>
 hipError_t launch(const LogitsArgs& a, bool vec, hipStream_t s) {
     // workgroups go round the XCDs: rows dealt the same way keep the slices of one
@@ -166,13 +192,16 @@ hipError_t launch(const LogitsArgs& a, bool vec, hipStream_t s) {
     // 47.8 -> 35.7 MB, 20.7 -> 18.6 us).  Of 8 to 128 rows either order takes the
     // same to within 0.2 us, and fewer than 8 would leave XCDs idle.
     const int64_t deal = a.rows >= 64 ? 8 : 1;
-    const int64_t slices = ceil_div(a.vocab, SLICE), blocks = ceil_div(a.rows, deal) * deal * slices;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
+    const int64_t slices = ceil_div(a.vocab, SLICE), most = most_blocks(kThreads) / slices / deal * deal;
     const uint32_t n = static_cast<uint32_t>(slices), m = static_cast<uint32_t>(deal);
-    if (vec) hipLaunchKernelGGL((k_logits_process<F32, true, SLICE>), grid, block, 0, s, a, n, m);
-    else hipLaunchKernelGGL((k_logits_process<F32, false, SLICE>), grid, block, 0, s, a, n, m);
-    return hipGetLastError();
+    for (int64_t first = 0; first < a.rows; first += most) {
+        const LogitsArgs part = rows_from(a, first, std::min(most, a.rows - first), F32 ? 4 : 2);
+        const dim3 grid(static_cast<unsigned>(ceil_div(part.rows, deal) * deal * slices)), block(kThreads);
+        if (vec) hipLaunchKernelGGL((k_logits_process<F32, true, SLICE>), grid, block, 0, s, part, n, m);
+        else hipLaunchKernelGGL((k_logits_process<F32, false, SLICE>), grid, block, 0, s, part, n, m);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
