@@ -482,6 +482,8 @@ def quantise_q4_gpu(weight: torch.Tensor, group: int = 128, zeros: bool = True,
     n, k = weight.shape
     if group not in (32, 64, 128) or k % group or not k or scale_dtype not in _CODE:
         raise ValueError("quantise_q4: groups of 32, 64 or 128 that divide the inputs, fp32 or bf16 scales")
+    if weight.data_ptr() % 16:   # the kernel reads 16 bytes at a time
+        weight = weight.clone()
     new = lambda width, dt: torch.empty((n, width), dtype=dt, device=weight.device)  # noqa: E731
     to = Q4Weight(new(k // 2, torch.uint8), new(k // group, scale_dtype),
                   new(k // group, torch.uint8) if zeros else None)
