@@ -54,7 +54,7 @@ class LayerWeights:
     in_b: torch.Tensor
     post_w: torch.Tensor
     post_b: torch.Tensor
-    proj: Dict[str, Tuple[torch.Tensor, torch.Tensor]]   # q_proj, k_proj, v_proj, o_proj: (weight, bias)
+    proj: Dict[str, Tuple[Optional[torch.Tensor], torch.Tensor]]   # q_proj, k_proj, v_proj, o_proj: (weight, bias)
     gate: torch.Tensor
     moe: MoeWeights
 
@@ -203,6 +203,13 @@ class Buffers:
                        e(rows, QD), e(rows, H), ws)
 
 
+def _held_in_4_bits(weight: torch.Tensor, group: int) -> serve.Q4Weight:
+    """weight in 4 bits; the caller may free it from here on, whatever stream it came from."""
+    q4 = serve.quantise_q4_gpu(weight, group)
+    weight.record_stream(torch.cuda.current_stream(weight.device))
+    return q4
+
+
 class DecoderLayer:
     """PhiDecoderLayer over the C ABI (reference include/layer.h:77-95).
 
@@ -211,7 +218,7 @@ class DecoderLayer:
     reference's USE_TC / USE_TC_ALL tensor-core path, src/layer.cu:16-27,
     src/tensor.cu:514-584), whose weights are packed here once.  q4_group: the
     projections in 4 bits instead, quantised here once in groups of so many
-    inputs (the reference has no such path)."""
+    inputs (the reference has no such path); the layer keeps their biases alone."""
 
     def __init__(self, w: LayerWeights, tc_terms: Optional[int] = None, q4_group: Optional[int] = None):
         self.w = w
@@ -220,7 +227,8 @@ class DecoderLayer:
         self.tc = {}
         self.q4: Dict[str, serve.Q4Weight] = {}
         if q4_group is not None:
-            self.q4 = {nm: serve.quantise_q4_gpu(wt, q4_group) for nm, (wt, _) in w.proj.items()}
+            self.q4 = {nm: _held_in_4_bits(wt, q4_group) for nm, (wt, _) in w.proj.items()}
+            self.w = replace(w, proj={nm: (None, b) for nm, (_, b) in w.proj.items()})
         if tc_terms is not None:
             from .attention import linear_tc_prepare
             self.tc = {nm: linear_tc_prepare(wt) for nm, (wt, _) in w.proj.items()}
@@ -322,16 +330,17 @@ class Model:
         31's attention projections: the reference's USE_TC), "all" (four
         products, the LM head and every layer's attention projections:
         USE_TC_ALL) or "q4" (those in 4 bits, quantised here in groups of 128
-        inputs with zeros; activations stay fp32.  The weights given are not
-        needed for them any more)."""
+        inputs with zeros; activations stay fp32.  The model keeps none of the
+        weights that were given for them)."""
         if tc not in ("off", "tc", "all", "q4"):
             raise ValueError("tc is 'off', 'tc', 'all' or 'q4'")
         self.emb, self.norm_w, self.norm_b = embeddings, norm_w, norm_b
-        self.head_w, self.head_b = lm_head_w, lm_head_b
+        self.vocab = lm_head_w.shape[0]
+        self.head_w, self.head_b = None if tc == "q4" else lm_head_w, lm_head_b
         terms = {"off": None, "q4": None, "tc": 3, "all": 4}[tc]
         self.layers = [DecoderLayer(w, terms if (tc == "all" or (tc == "tc" and i == 31)) else None,
                                     Q4_GROUP if tc == "q4" else None) for i, w in enumerate(layers)]
-        self.head_q4 = serve.quantise_q4_gpu(lm_head_w, Q4_GROUP) if tc == "q4" else None
+        self.head_q4 = _held_in_4_bits(lm_head_w, Q4_GROUP) if tc == "q4" else None
         self.head_terms = terms
         self.head_tc = None
         if terms is not None:
@@ -378,7 +387,7 @@ class Model:
         _call(L.aps_gather_rows(_p(b.normed), T, H, _p(plan.last_rows), batch, _p(rows_out), stream))
         if self.head_q4 is not None:
             return serve.linear_q4_gpu(rows_out, self.head_q4, self.head_b)
-        V = self.head_w.shape[0]
+        V = self.vocab
         logits = torch.empty((batch, V), dtype=torch.float32, device=dev)
         if self.head_tc is not None:
             xs = torch.empty(2 * batch * H, dtype=torch.int16, device=dev)
@@ -408,9 +417,9 @@ class Model:
         flat = np.concatenate([np.asarray(p, np.int64).reshape(-1) for p in prompts])
         if flat.min() < 0 or flat.max() >= self.emb.shape[0]:
             raise ValueError("token out of vocabulary")
-        if not 0 <= top <= min(serve.MAX_TOP, self.head_w.shape[0]):
+        if not 0 <= top <= min(serve.MAX_TOP, self.vocab):
             raise ValueError("top is a number of tokens")
-        dev, V = self.emb.device, self.head_w.shape[0]
+        dev, V = self.emb.device, self.vocab
         rows = np.delete(np.arange(flat.size), np.cumsum(lens) - 1)   # those with a token behind them
         if rows.size == 0:
             logits = torch.empty((0, V), dtype=torch.float32, device=dev)
@@ -445,7 +454,7 @@ class Model:
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
         dev, n_seq = self.emb.device, len(prompts)
-        V = self.head_w.shape[0]
+        V = self.vocab
         lens = [len(p) for p in prompts]
         flat = np.concatenate([np.asarray(p, np.int64).reshape(-1) for p in prompts])
         if min(lens) == 0:
