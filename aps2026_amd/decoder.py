@@ -421,6 +421,8 @@ class Model:
             raise ValueError("top is a number of tokens")
         dev, V = self.emb.device, self.vocab
         rows = np.delete(np.arange(flat.size), np.cumsum(lens) - 1)   # those with a token behind them
+        if rows.size and flat[rows + 1].max() >= V:   # a narrower head has no logit for it
+            raise ValueError("token out of vocabulary")
         if rows.size == 0:
             logits = torch.empty((0, V), dtype=torch.float32, device=dev)
         else:
