@@ -18,9 +18,10 @@ constexpr int kPiece = 256;   // inputs of a wave's turn: a 128-byte line of a r
 constexpr int kBlock = 16;    // groups whose scales and zeros a wave holds in LDS
 constexpr int kPad = 16;      // bytes behind a row in LDS: other banks for the next
 
-// Bytes at any address, in words.
+// Bytes at any address, in words; what is written as one number of them is read as
+// another, so they may be aliases of anything.
 template <int BYTES>
-struct __attribute__((packed, aligned(1))) Packed {
+struct __attribute__((packed, aligned(1), may_alias)) Packed {
     uint32_t w[(BYTES + 3) / 4];
     __device__ uint32_t get4(int i) const { return w[i]; }
     __device__ uint32_t get2(int i) const { return (w[i / 2] >> (16 * (i & 1))) & 0xFFFFu; }
@@ -30,7 +31,7 @@ struct __attribute__((packed, aligned(1))) Packed {
     __device__ void set1(int i, uint32_t v) { w[i / 4] = (i & 3) ? w[i / 4] | v << (8 * (i & 3)) : v; }
 };
 template <>
-struct __attribute__((packed, aligned(1))) Packed<2> {
+struct __attribute__((packed, aligned(1), may_alias)) Packed<2> {
     uint16_t w;
     __device__ uint32_t get1(int i) const { return (w >> (8 * i)) & 0xFFu; }
     __device__ void set1(int i, uint32_t v) { w = static_cast<uint16_t>(i ? w | v << 8 : v); }
@@ -198,8 +199,7 @@ struct Columns {
                 for (int i = 0; i < EACH; ++i) {
                     // x is 0 past them, and 0 has to be what it is multiplied with too: 0 times
                     // an infinity or a NaN of the next rows, or of what LDS held, is not
-                    if constexpr (SCALES32) reinterpret_cast<uint32_t*>(scale_to)[i] = i < left ? reinterpret_cast<const uint32_t*>(sp)[i] : 0u;
-                    else reinterpret_cast<uint16_t*>(scale_to)[i] = i < left ? reinterpret_cast<const uint16_t*>(sp)[i] : uint16_t(0);
+                    *reinterpret_cast<Packed<SIZE>*>(scale_to + i * SIZE) = i < left ? *reinterpret_cast<const Packed<SIZE>*>(sp + i * SIZE) : Packed<SIZE>{};
                     if (w.zeros && i < left) zero_to[i] = w.zeros[at + i];
                 }
             }
