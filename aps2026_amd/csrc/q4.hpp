@@ -10,7 +10,6 @@ namespace aps {
 namespace q4 {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
@@ -26,15 +25,11 @@ struct __attribute__((packed, aligned(1), may_alias)) Packed {
     __device__ uint32_t get4(int i) const { return w[i]; }
     __device__ uint32_t get2(int i) const { return (w[i / 2] >> (16 * (i & 1))) & 0xFFFFu; }
     __device__ uint32_t get1(int i) const { return (w[i / 4] >> (8 * (i & 3))) & 0xFFu; }
-    __device__ void set4(int i, uint32_t v) { w[i] = v; }
-    __device__ void set2(int i, uint32_t v) { w[i / 2] = (i & 1) ? (w[i / 2] & 0xFFFFu) | v << 16 : v; }
-    __device__ void set1(int i, uint32_t v) { w[i / 4] = (i & 3) ? w[i / 4] | v << (8 * (i & 3)) : v; }
 };
 template <>
 struct __attribute__((packed, aligned(1), may_alias)) Packed<2> {
     uint16_t w;
     __device__ uint32_t get1(int i) const { return (w >> (8 * i)) & 0xFFu; }
-    __device__ void set1(int i, uint32_t v) { w = static_cast<uint16_t>(i ? w | v << 8 : v); }
 };
 
 __device__ inline bf16x8 frag(u32x4 w) { return __builtin_bit_cast(bf16x8, w); }
