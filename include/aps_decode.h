@@ -67,7 +67,8 @@ typedef struct aps_q4_weight {
  * contiguous of x's type.  Products are exact, sums are fp32, over each group's
  * codes and then over the groups; y is rounded once.  A row with an infinity or a
  * NaN gives NaN where the formula may have an infinity, and so may one with a
- * magnitude past 2^116, of which a group's sum need not be finite.  A scale that is
+ * magnitude past 2^116, of which a group's sum need not be finite.  Of fp32 x the bits
+ * below 2^-133, bf16's smallest number, are left out.  A scale that is
  * not finite makes its own output's values NaN or infinite, and no other's.  Any
  * alignment of x and y to their elements (16-byte reads where x allows them).
  * The kernel, and with it the order of the sums and the last bits of a row, goes by
