@@ -14,7 +14,11 @@
 // Bound by those reads of x, 64 bytes a cycle and CU (64 rows on 8192 x 8192: 1 MB
 // for every 32 columns, 6.8 us), and by the codes' bytes (7.6); a workgroup's start
 // and end take as long as one to two of its pieces, the first launch and the way to
-// the second 5 us: 24.3 in all, 353 TFLOP/s.
+// the second 5 us: 23.5 in all, 366 TFLOP/s.  Of a prompt's rows every 32 columns
+// read x again, of fp32 x, whose terms are three times the bytes and products, every
+// 16: 10240 rows on 4096 x 2048 take 291 us in bf16 (591 TFLOP/s) and 1438 in fp32
+// (119, of the result's); a library's product with weights held in the same type
+// 179 and 1155.
 #include <algorithm>
 
 #include "q4.hpp"
@@ -218,7 +222,7 @@ __global__ void __launch_bounds__(kMany) k_q4_many(LinearQ4Args a, int columns, 
 // outputs each, which share x through LDS.  Two pieces of it (one for each of the
 // two shares of the inputs) are copied there while the two before are multiplied.
 // A wave that loaded x for itself would read 8 or 24 KB from L2 for every 2 KB of
-// codes (16 fp32 rows on 4096 x 32064: 40 us, 30 here, of which 5 for putting x in
+// codes (16 fp32 rows on 4096 x 32064: 40 us, 27.7 here, of which 5 for putting x in
 // order).  What bounds it is neither HBM (15 us) nor copies (without them 2 us less)
 // but a round's own length, products after reads of LDS; two tiles of columns to a
 // wave, which halve those reads, measure the same (31).

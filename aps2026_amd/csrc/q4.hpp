@@ -131,8 +131,8 @@ __device__ inline u32x4 to_columns(u32x4 loaded, int lane) {
 //
 // Four neighbouring lanes read 64 neighbouring bytes of a row: a load takes a
 // cycle for each line that such four touch, and a lane of its own row each, as the
-// products want them, takes four times as many (4096 x 32064, one row: 24 us
-// where this has 20).  The words go to their lanes through LDS's crossbar.  Scales
+// products want them, takes four times as many (this alone took one row on 4096 x
+// 32064 from 24 us to 20).  The words go to their lanes through LDS's crossbar.  Scales
 // and zeros come 16 groups at a time into LDS of the wave's own, for the same
 // reason.
 //

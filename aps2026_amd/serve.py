@@ -542,7 +542,8 @@ def token_logprobs_gpu(logits: torch.Tensor, tokens: Optional[torch.Tensor] = No
     stride: of the given tokens ([rows] or [rows, n] int32; 0 for an id outside
     the vocabulary), and of the `top` likeliest (up to 64; of equal logits the
     lower id first), and the rows' entropies, all fp32.  Logits of -inf have the
-    probability 0.  The workspace is torch's, taken on the current stream, unless
+    probability 0 (as a mask they are quicker than a finite value, whose ties the
+    likeliest tokens are then picked from one by one).  The workspace is torch's, taken on the current stream, unless
     one is given (uint8)."""
     what, dev = "token_logprobs", logits.device
     code = _CODE.get(logits.dtype)

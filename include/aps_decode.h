@@ -100,7 +100,9 @@ APS_API int aps_quantise_q4(const void* w, int32_t dtype, const aps_q4_weight* w
  *     first, of equal logits the lower id; a NaN counts as -inf.
  * Logits of -inf (a mask's) have the probability 0 and the log probability -inf;
  * a row of nothing else has these for all, and the entropy 0.  A row with NaN or
- * +inf gives NaN (but its top_ids).  top up to 64 and vocab, vocab up to 2^20.
+ * +inf gives NaN (but its top_ids).  Masks of -inf cost nothing; under one of a finite
+ * value that leaves a row few tokens, as with many equal logits at the top, each of
+ * the `top` tokens costs a pass over the row.  top up to 64 and vocab, vocab up to 2^20.
  * The order of the sums goes by rows, vocab, dtype and where a row begins within 16
  * bytes; equal calls on equally aligned rows give equal bits.
  * workspace: aps_token_logprobs_workspace_size bytes (0: none), 16-byte aligned;
