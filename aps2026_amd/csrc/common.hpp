@@ -23,6 +23,9 @@ constexpr int kF32BN = 64;          // fp32 chain kernels cols per tile
 using bf16_t = uint16_t;            // raw bfloat16 bits in memory
 
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// The most workgroups of a launch: a grid's threads are counted in 32 bits, and one of
+// more runs in part, without an error.
+constexpr int64_t most_blocks(int threads) { return 0xFFFFFFFFll / threads; }
 
 // Two fp32 -> packed bf16, round to nearest even (one v_cvt_pk_bf16_f32).
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));

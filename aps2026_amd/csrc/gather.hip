@@ -71,15 +71,17 @@ hipError_t launch_gather_rows(const float* x, int64_t x_rows, int64_t hidden, co
     const bool vec = hidden % 4 == 0 &&
                      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
     const int64_t spans = ceil_div(hidden, vec ? gather_span<true>() : gather_span<false>());
-    const int64_t blocks = count * spans;
-    if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
-    if (vec)
-        hipLaunchKernelGGL(k_gather_rows<true>, dim3(static_cast<unsigned>(blocks)), dim3(kGatherThreads), 0, s, x,
-                           x_rows, hidden, rows, out, spans);
-    else
-        hipLaunchKernelGGL(k_gather_rows<false>, dim3(static_cast<unsigned>(blocks)), dim3(kGatherThreads), 0, s, x,
-                           x_rows, hidden, rows, out, spans);
-    return hipGetLastError();
+    const int64_t most = most_blocks(kGatherThreads) / spans;   // rows of a launch
+    if (most < 1) return hipErrorInvalidValue;
+    for (int64_t first = 0; first < count; first += most) {
+        const dim3 grid(static_cast<unsigned>((count - first < most ? count - first : most) * spans));
+        const uint32_t* from = rows + first;
+        float* to = out + first * hidden;
+        if (vec) hipLaunchKernelGGL(k_gather_rows<true>, grid, dim3(kGatherThreads), 0, s, x, x_rows, hidden, from, to, spans);
+        else hipLaunchKernelGGL(k_gather_rows<false>, grid, dim3(kGatherThreads), 0, s, x, x_rows, hidden, from, to, spans);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace aps

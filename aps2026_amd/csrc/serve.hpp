@@ -6,10 +6,6 @@
 
 namespace aps {
 
-// The most workgroups of a launch: a grid's threads are counted in 32 bits, and one of
-// more runs in part, without an error.
-constexpr int64_t most_blocks(int threads) { return 0xFFFFFFFFll / threads; }
-
 enum class Kv { kF32 = 0, kBf16 = 1, kMx = 3 };
 
 struct KvCache {
