@@ -92,47 +92,62 @@ __global__ void __launch_bounds__(256) k_zero1(float* __restrict__ x, int64_t n)
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-dim3 grid_for(int64_t n) { return dim3(static_cast<unsigned>(ceil_div(n, 256))); }
+// launch(grid, first, n) over n threads in as many launches as that takes; a
+// launch's threads are a multiple of `of`.
+template <typename Launch>
+hipError_t in_launches(int64_t n, int64_t of, Launch launch) {
+    const int64_t most = most_blocks(256) * 256 / of * of;
+    for (int64_t first = 0; first < n; first += most) {
+        const int64_t part = n - first < most ? n - first : most;
+        launch(dim3(static_cast<unsigned>(ceil_div(part, 256))), first, part);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+v4f* fours(float* p) { return reinterpret_cast<v4f*>(p); }
+const v4f* fours(const float* p) { return reinterpret_cast<const v4f*>(p); }
 
 }  // namespace
 
 hipError_t launch_add_inplace(float* a, const float* b, int64_t n, hipStream_t s) {
-    if (n <= 0) return hipSuccess;
     if (n % 4 == 0 && aligned16(a) && aligned16(b))
-        hipLaunchKernelGGL(k_add4, grid_for(n / 4), dim3(256), 0, s, reinterpret_cast<v4f*>(a),
-                           reinterpret_cast<const v4f*>(b), n / 4);
-    else
-        hipLaunchKernelGGL(k_add1, grid_for(n), dim3(256), 0, s, a, b, n);
-    return hipGetLastError();
+        return in_launches(n / 4, 1, [&](dim3 grid, int64_t i, int64_t m) {
+            hipLaunchKernelGGL(k_add4, grid, dim3(256), 0, s, fours(a) + i, fours(b) + i, m);
+        });
+    return in_launches(n, 1, [&](dim3 grid, int64_t i, int64_t m) {
+        hipLaunchKernelGGL(k_add1, grid, dim3(256), 0, s, a + i, b + i, m);
+    });
 }
 
 hipError_t launch_add_bias(float* a, const float* bias, int64_t n, int h, hipStream_t s) {
-    if (n <= 0) return hipSuccess;
     if (h % 4 == 0 && n % 4 == 0 && aligned16(a) && aligned16(bias))
-        hipLaunchKernelGGL(k_add_bias4, grid_for(n / 4), dim3(256), 0, s, reinterpret_cast<v4f*>(a), bias, n / 4,
-                           h / 4);
-    else
-        hipLaunchKernelGGL(k_add_bias1, grid_for(n), dim3(256), 0, s, a, bias, n, h);
-    return hipGetLastError();
+        return in_launches(n / 4, h / 4, [&](dim3 grid, int64_t i, int64_t m) {
+            hipLaunchKernelGGL(k_add_bias4, grid, dim3(256), 0, s, fours(a) + i, bias, m, h / 4);
+        });
+    return in_launches(n, h, [&](dim3 grid, int64_t i, int64_t m) {
+        hipLaunchKernelGGL(k_add_bias1, grid, dim3(256), 0, s, a + i, bias, m, h);
+    });
 }
 
 hipError_t launch_silu_mul(const float* g, const float* u, float* out, int64_t n, hipStream_t s) {
-    if (n <= 0) return hipSuccess;
     if (n % 4 == 0 && aligned16(g) && aligned16(u) && aligned16(out))
-        hipLaunchKernelGGL(k_silu_mul4, grid_for(n / 4), dim3(256), 0, s, reinterpret_cast<const v4f*>(g),
-                           reinterpret_cast<const v4f*>(u), reinterpret_cast<v4f*>(out), n / 4);
-    else
-        hipLaunchKernelGGL(k_silu_mul1, grid_for(n), dim3(256), 0, s, g, u, out, n);
-    return hipGetLastError();
+        return in_launches(n / 4, 1, [&](dim3 grid, int64_t i, int64_t m) {
+            hipLaunchKernelGGL(k_silu_mul4, grid, dim3(256), 0, s, fours(g) + i, fours(u) + i, fours(out) + i, m);
+        });
+    return in_launches(n, 1, [&](dim3 grid, int64_t i, int64_t m) {
+        hipLaunchKernelGGL(k_silu_mul1, grid, dim3(256), 0, s, g + i, u + i, out + i, m);
+    });
 }
 
 hipError_t launch_zero(float* x, int64_t n, hipStream_t s) {
-    if (n <= 0) return hipSuccess;
     if (n % 4 == 0 && aligned16(x))
-        hipLaunchKernelGGL(k_zero4, grid_for(n / 4), dim3(256), 0, s, reinterpret_cast<v4f*>(x), n / 4);
-    else
-        hipLaunchKernelGGL(k_zero1, grid_for(n), dim3(256), 0, s, x, n);
-    return hipGetLastError();
+        return in_launches(n / 4, 1, [&](dim3 grid, int64_t i, int64_t m) {
+            hipLaunchKernelGGL(k_zero4, grid, dim3(256), 0, s, fours(x) + i, m);
+        });
+    return in_launches(n, 1, [&](dim3 grid, int64_t i, int64_t m) {
+        hipLaunchKernelGGL(k_zero1, grid, dim3(256), 0, s, x + i, m);
+    });
 }
 
 }  // namespace aps

@@ -24,3 +24,24 @@ def test_gather_of_many_rows(gpu_device):
         out = torch.empty(count, width, device=gpu_device)
         call("aps_gather_rows", few, 1013, width, repeated(at, count), count, out)
         assert_repeats(out, few[at.long()])
+
+
+def test_elementwise_of_many_values(gpu_device):
+    """Arrays off 16 bytes, where a thread has one value."""
+    n, h = (1 << 32) + 12, 4
+    note(f"elementwise of {n} values")
+    a, b = (torch.empty(n + 1, device=gpu_device)[1:] for _ in range(2))
+    bias = torch.arange(1, h + 1, dtype=F32, device=gpu_device)
+    rows = lambda t: t.view(-1, h)  # noqa: E731
+    for t, scale in ((a, 1.0), (b, 3.0)):
+        t.fill_(7.0)
+        call("aps_zero", t, n)
+        call("aps_add_bias_inplace", t, scale * bias, n, h)
+        assert_repeats(rows(t), scale * bias[None])
+    call("aps_add_inplace", a, b, n)
+    assert_repeats(rows(a), 4 * bias[None])
+    few = torch.empty(h + 1, device=gpu_device)[1:]
+    call("aps_silu_mul", (4 * bias).contiguous(), (3 * bias).contiguous(), few, h)
+    out = torch.empty(n + 1, device=gpu_device)[1:]
+    call("aps_silu_mul", a, b, out, n)
+    assert_repeats(rows(out), few[None])
