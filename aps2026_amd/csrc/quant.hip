@@ -56,16 +56,16 @@ hipError_t launch_quant_rows_e4m3(const bf16_t* src, int64_t src_stride, int n, 
     if (rows <= 0) return hipSuccess;
     if (n % 8 != 0 || dst_stride % 8 != 0 || dst_stride < n) return hipErrorInvalidValue;
     const int chunks = static_cast<int>(ceil_div(dst_stride, 8));
-    const dim3 grid(static_cast<unsigned>(rows));
-    if (chunks <= 64)
-        hipLaunchKernelGGL(k_quant_rows<1>, grid, dim3(64), 0, s, src, src_stride, n, dst, dst_stride, scale, rows);
-    else if (chunks <= 512)
-        hipLaunchKernelGGL(k_quant_rows<8>, grid, dim3(64), 0, s, src, src_stride, n, dst, dst_stride, scale, rows);
-    else if (chunks <= 1024)
-        hipLaunchKernelGGL(k_quant_rows<16>, grid, dim3(64), 0, s, src, src_stride, n, dst, dst_stride, scale, rows);
-    else
-        return hipErrorInvalidValue;
-    return hipGetLastError();
+    if (chunks > 1024) return hipErrorInvalidValue;
+    auto kern = chunks <= 64 ? k_quant_rows<1> : chunks <= 512 ? k_quant_rows<8> : k_quant_rows<16>;
+    const int64_t most = most_blocks(64);
+    for (int64_t first = 0; first < rows; first += most) {
+        const int64_t m = rows - first < most ? rows - first : most;
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(m)), dim3(64), 0, s, src + first * src_stride, src_stride, n,
+                           dst + first * dst_stride, dst_stride, scale + first, m);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_pack_w13_e4m3(const void* const* w1, const void* const* w3, uint8_t* dst, int experts, int ffn,

@@ -45,3 +45,17 @@ def test_elementwise_of_many_values(gpu_device):
     out = torch.empty(n + 1, device=gpu_device)[1:]
     call("aps_silu_mul", a, b, out, n)
     assert_repeats(rows(out), few[None])
+
+
+def test_quantise_rows_of_many_rows(gpu_device):
+    rows = (1 << 26) + 3
+    note(f"quantise_rows_e4m3 of {rows} rows")
+    few = torch.randn(1009, 16, device=gpu_device).to(BF16)
+
+    def quantised(x):
+        out, scale = torch.empty(len(x), 16, dtype=torch.uint8, device=gpu_device), torch.empty(len(x), 1, device=gpu_device)
+        call("aps_quantise_rows_e4m3", x, 16, 16, out, 16, scale, len(x))
+        return out, scale
+
+    for got, want in zip(quantised(repeated(few, rows)), quantised(few)):
+        assert_repeats(got, want)
