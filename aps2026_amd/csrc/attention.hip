@@ -726,8 +726,6 @@ k_attention_tree(const float* __restrict__ q, const float* __restrict__ k, const
 // keys w = tid, tid + 128, ...; only the denominator is a serial sum.  Keys
 // are the rows seg_offset[row] + begin .. seg_offset[row] + pos of the row's
 // own sequence, begin = max(0, pos + 1 - window).  Dynamic LDS: wmax scores.
-constexpr int kAnyThreads = 128;
-
 __global__ void __launch_bounds__(kAnyThreads)
 k_attention_any(const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v,
                 float* __restrict__ out, const uint32_t* __restrict__ seg_offset, const uint32_t* __restrict__ seg_pos,
@@ -854,6 +852,7 @@ hipError_t launch_attention_tree(const float* q, const float* k, const float* v,
                            q, k, v, out, row_pos, anc, anc_stride, rows, q_heads, kv_heads, wmax, scale, sw);
         return hipGetLastError();
     }
+    if (rows * kv_heads > most_blocks(kAttnThreads)) return hipErrorInvalidValue;
     const size_t lds = static_cast<size_t>(wmax) * (kGroup * sizeof(float) + sizeof(uint32_t));
     // dynamic LDS past 64 KB needs the function's limit raised first
     auto kern = packed ? &k_attention_tree<true> : &k_attention_tree<false>;
@@ -872,7 +871,7 @@ hipError_t launch_attention_any(const float* q, const float* k, const float* v, 
                                 int head_dim, int window_max, hipStream_t s) {
     if (rows <= 0) return hipSuccess;
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 || head_dim > kAnyThreads ||
-        max_seq <= 0 || window_max <= 0 || rows * q_heads > 0x7FFFFFFFll)
+        max_seq <= 0 || window_max <= 0 || rows * q_heads > most_blocks(kAnyThreads))
         return hipErrorInvalidValue;
     const int64_t keys = max_seq < window_max ? max_seq : window_max;
     if (keys > kAttnMaxWindow) return hipErrorInvalidValue;

@@ -850,7 +850,7 @@ int aps_attention_packed(const float* q, const float* k, const float* v, float* 
         if ((max_seq < window ? max_seq : window) > aps::kAttnMaxWindow)
             return fail(APS_ERR_SHAPE, "attention: a window of %lld keys exceeds the %d that fit in LDS",
                         (long long)(max_seq < window ? max_seq : window), aps::kAttnMaxWindow);
-        if (rows * q_heads > 0x7FFFFFFFll)
+        if (rows * q_heads > aps::most_blocks(aps::kAnyThreads))
             return fail(APS_ERR_SHAPE, "attention: %lld rows x %d heads", (long long)rows, q_heads);
         if (rows == 0) return APS_OK;
         if (!q || !k || !v || !out || !seg_offset || !seg_pos) return fail(APS_ERR_ARG, "attention: NULL pointer");

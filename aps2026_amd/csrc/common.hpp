@@ -278,6 +278,7 @@ hipError_t launch_rope_tree(float* q, float* k, const uint32_t* row_pos, int64_t
 // the key's row index) next to 2 KB of its own: windows up to kAttnMaxWindow
 // keys fit gfx950's 160 KB of LDS per workgroup.
 constexpr int kAttnMaxWindow = 7936;
+constexpr int kAnyThreads = 128;    // of a row's head in layouts other than GQA-4
 hipError_t launch_attention_tree(const float* q, const float* k, const float* v, float* out, const uint32_t* row_pos,
                                  const uint32_t* anc, int64_t anc_stride, int64_t rows, int q_heads, int kv_heads,
                                  int head_dim, int window_max, bool packed, hipStream_t s);
