@@ -233,14 +233,14 @@ template <int D>
 hipError_t gather_d(const KvCache& c, const int64_t* slots, int64_t all, void* k_out, void* v_out, bool f32, hipStream_t s) {
     const int64_t threads = static_cast<int64_t>(c.kv_heads) * (D / 8);   // of a row
     const int64_t most = most_blocks(kThreads) * kThreads / threads, bytes = static_cast<int64_t>(c.kv_heads) * D * (f32 ? 4 : 2);
-    for (int64_t first = 0; first < all; first += most, slots += most) {
-        const int64_t rows = std::min(most, all - first);
+    for (int64_t first = 0; first < all; first += most) {
+        const int64_t rows = std::min(most, all - first), *at = slots + first;
         void* k = k_out ? static_cast<char*>(k_out) + first * bytes : nullptr;
         void* v = v_out ? static_cast<char*>(v_out) + first * bytes : nullptr;
         const unsigned n = static_cast<unsigned>(ceil_div(rows * threads, kThreads));
-        if (c.type == Kv::kF32) gather<D, Kv::kF32>(c, slots, rows, k, v, f32, n, s);
-        else if (c.type == Kv::kBf16) gather<D, Kv::kBf16>(c, slots, rows, k, v, f32, n, s);
-        else gather<D, Kv::kMx>(c, slots, rows, k, v, f32, n, s);
+        if (c.type == Kv::kF32) gather<D, Kv::kF32>(c, at, rows, k, v, f32, n, s);
+        else if (c.type == Kv::kBf16) gather<D, Kv::kBf16>(c, at, rows, k, v, f32, n, s);
+        else gather<D, Kv::kMx>(c, at, rows, k, v, f32, n, s);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     return hipSuccess;
